@@ -21,6 +21,9 @@ FL_E_CAPACITY = -3
 
 HEAD_DIM = 128
 GROUP = 64
+MX_BLOCK = 32
+MX_PAD = 128
+MX_MAX_K = 1 << 20
 
 
 class FlCacheView(C.Structure):
@@ -109,6 +112,13 @@ SIGNATURES = {
     "fl_prefill_attention_workspace": (_SZ, [_I32, _I32, _I32]),
     "fl_rope_store": (_I32, [_P, _P, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _P]),
     "fl_swiglu": (_I32, [_P, _P, _P, _I64, _P]),
+    "fl_mx_quantize": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
+    "fl_mx_dequantize": (_I32, [_P, _P, _I64, _I32, _I32, _P, _I64, _P]),
+    "fl_norm_chain_mx": (_I32, [_I32, _I32, _F64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "fl_mx_gemv": (_I32, [_P, _I32, _I64, _I32, _I32, _PP, _PP, _I32, _I32, _PP, _I64, _P, _I64, _P, _P, _I32, _P]),
+    "fl_mx_gemv_chain": (_I32, [_I32, _I32, _F32, _P, _P, _P, _P, _P, _P, _I64, _PP, _PP, _I32, _I32, _PP, _I64, _P,
+                                _I64, _P, _P, _I32, _P]),
+    "fl_mx_matmul": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I64, _P]),
 }
 
 _lib: C.CDLL | None = None

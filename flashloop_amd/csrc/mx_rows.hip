@@ -1,0 +1,395 @@
+// Rows in microscaled formats: quantisation of bf16 or f32 rows to 4 or 8 bits, the values back as
+// bf16, and the residual / RMSNorm chain between two products with its last norm in 8 bits.
+//
+// Quantisation moves 2 or 4 bytes a value in and 1 or 1/2 out, with a maximum over 32 neighbours and a
+// conversion that the hardware has, so it is bound by HBM.  A thread holds 8 neighbouring values (one
+// 16-byte load of bf16), a block of 32 lies in a quad of lanes, whose maximum is two DPP moves.
+#include "mx_common.h"
+
+namespace fl {
+namespace {
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ uint32_t quad_max_u(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(dpp_i<kDppXor1>(static_cast<int>(v))));
+  return max(v, static_cast<uint32_t>(dpp_i<kDppXor2>(static_cast<int>(v))));
+}
+
+struct QuantArgs {
+  const void* x;
+  int64_t x_stride;  // elements between rows
+  int64_t pieces;    // rows * (padded K / 8)
+  int k, per_row;    // pieces of a row
+  int rows_are_vectors;  // rows 16-byte aligned
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = bf16lo_to_f32(w[i]);
+    f[2 * i + 1] = bf16hi_to_f32(w[i]);
+  }
+}
+
+// values [8 c, 8 c + 8) of a row, zero from k on
+template <bool F32>
+__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, float* f) {
+  const int64_t at = row * a.x_stride + 8 * static_cast<int64_t>(c);
+  const int left = a.k - 8 * c;
+  if (a.rows_are_vectors && left >= 8) {
+    if constexpr (F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + at);
+      const float4 u = p[0], v = p[1];
+      f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+    } else {
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + at), f);
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f[e] = 0.0f;
+    if (e < left)
+      f[e] = F32 ? static_cast<const float*>(a.x)[at + e] : bf16_to_f32(static_cast<const uint16_t*>(a.x)[at + e]);
+  }
+}
+
+template <int BITS, bool F32>
+__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(QuantArgs a) {
+  // rows are whole quads of pieces, so a block's lanes are all inside or all past the end
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+  const int64_t row0 = first / a.per_row;  // (uniform)
+  const uint32_t in = static_cast<uint32_t>(first - row0 * a.per_row) + threadIdx.x;
+  const uint32_t over = in / static_cast<uint32_t>(a.per_row);
+  const int64_t piece = first + threadIdx.x;
+  if (piece >= a.pieces) return;
+  float f[8];
+  load8<F32>(a, row0 + over, static_cast<int>(in - over * static_cast<uint32_t>(a.per_row)), f);
+  uint32_t peak = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+  peak = quad_max_u(peak);
+  const uint32_t code = mx_scale_code<BITS>(peak);
+  const float s = mx_scale(code);
+  if constexpr (BITS == 4) {
+    const uint32_t q = mx_encode4(f, s);
+    reinterpret_cast<uint32_t*>(a.codes)[piece] = code == 255u ? 0u : q;
+  } else {
+    const uint2 q = mx_encode8(f, s);
+    reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
+  }
+  if ((threadIdx.x & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+}
+
+struct DequantArgs {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  uint16_t* out;
+  int64_t out_stride, pieces;
+  int k, per_row;
+  int rows_are_vectors;
+};
+
+template <int BITS>
+__global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(DequantArgs a) {
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
+  const int64_t row0 = first / a.per_row;
+  const uint32_t in = static_cast<uint32_t>(first - row0 * a.per_row) + threadIdx.x;
+  const uint32_t over = in / static_cast<uint32_t>(a.per_row);
+  const int64_t piece = first + threadIdx.x;
+  if (piece >= a.pieces) return;
+  const int c = static_cast<int>(in - over * static_cast<uint32_t>(a.per_row));
+  const int left = a.k - 8 * c;
+  if (left <= 0) return;
+  const float s = mx_scale(a.scales[piece >> 2]);
+  uint4 v;
+  if constexpr (BITS == 4)
+    v = mx_decode4(reinterpret_cast<const uint32_t*>(a.codes)[piece], s);
+  else
+    v = mx_decode8(reinterpret_cast<const uint2*>(a.codes)[piece], s);
+  uint16_t* out = a.out + (row0 + over) * a.out_stride + 8 * static_cast<int64_t>(c);
+  if (a.rows_are_vectors && left >= 8) {
+    *reinterpret_cast<uint4*>(out) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) out[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+}
+
+// ---------------------------------------------------------------------------------
+// h = r + norm_a(x), optionally h = norm_f(h), rounded to bf16; z = norm_b(h) in 8 bits, with
+// norm_w(v) = w * v / sqrt(mean(v^2) + eps).
+//
+// A value of z that lies next to a border of e4m3 must not be moved over it by the rounding of what
+// came before (a step of e4m3 is 1/16 of the value), so the sums and the products are in 64 bits: h
+// becomes bf16 as torch converts a 64-bit value (by way of f32), and z, from that h, e4m3 in one
+// rounding.  (A 64-bit FMA costs here what a 32-bit one does.)  The order of the sums shows in no output.
+struct NormMxArgs {
+  int64_t rows, stride;
+  int d, per_row;  // values; 8-value pieces of a padded row
+  double eps;
+  const uint16_t* x;
+  const uint16_t* r;
+  const uint16_t* wa;
+  const uint16_t* wf;
+  const uint16_t* wb;
+  uint16_t* h_out;
+  uint8_t* codes;
+  uint8_t* scales;
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(dpp_i<CTRL>(static_cast<int>(u)));
+  const uint32_t hi = static_cast<uint32_t>(dpp_i<CTRL>(static_cast<int>(u >> 32)));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double lane64(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u), lane));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<kDppXor1>(v);
+  v += dpp64<kDppXor2>(v);
+  v += dpp64<kDppHalfMirror>(v);
+  v += dpp64<kDppMirror>(v);
+  return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+
+// sum over the lanes of a row: one wave, or the workgroup (two LDS buffers in turn, one barrier a sum)
+template <int W>
+struct RowSum64 {
+  double (*red)[4];
+  int phase;
+  __device__ __forceinline__ double operator()(double v) {
+    v = wave_sum64(v);
+    if constexpr (W == 1) return v;
+    double* r = red[phase & 1];
+    ++phase;
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+    lds_barrier();
+    return (r[0] + r[1]) + (r[2] + r[3]);
+  }
+};
+
+__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = static_cast<uint32_t>(f32_to_bf16_rne(f[2 * i])) | static_cast<uint32_t>(f32_to_bf16_rne(f[2 * i + 1])) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// W waves share a row, each lane holds its pieces t, t + 64 W, ... (NC of them).
+template <int NC, int W>
+__global__ __launch_bounds__(kThreads) void norm_chain_mx_kernel(NormMxArgs a) {
+  __shared__ double red[2][4];
+  constexpr int kLanes = 64 * W;
+  const int t = threadIdx.x % kLanes;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (row >= a.rows) return;  // (whole waves; with W = 4 every row has its workgroup)
+  const int nq = a.d / 8;
+  const int64_t base = row * a.stride;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  RowSum64<W> sum{red, 0};
+  uint4 rr[NC], xr[NC], wa[NC], wf[NC], wb[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = t + i * kLanes;
+    const bool in = c < nq;
+    rr[i] = in ? reinterpret_cast<const uint4*>(a.r + base)[c] : zero;
+    xr[i] = in && a.x ? reinterpret_cast<const uint4*>(a.x + base)[c] : zero;
+    wa[i] = in && a.x ? reinterpret_cast<const uint4*>(a.wa)[c] : zero;
+    wf[i] = in && a.wf ? reinterpret_cast<const uint4*>(a.wf)[c] : zero;
+    wb[i] = in ? reinterpret_cast<const uint4*>(a.wb)[c] : zero;
+  }
+  const double d = static_cast<double>(a.d);
+  const auto inv_rms = [&](double ss) { return 1.0 / sqrt(sum(ss) / d + a.eps); };
+  const auto squares = [&](const uint4(&v)[NC]) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      float f[8];
+      unpack_bf16x8(v[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ss);
+    }
+    return ss;
+  };
+  if (a.x != nullptr || a.wf != nullptr) {
+    const double ia = a.x != nullptr ? inv_rms(squares(xr)) : 0.0;
+    const auto sum_of = [&](int i, double* h) {  // r + norm_a(x) of piece i
+      float fr[8], fx[8], fw[8];
+      unpack_bf16x8(rr[i], fr);
+      unpack_bf16x8(xr[i], fx);
+      unpack_bf16x8(wa[i], fw);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[e] = static_cast<double>(fr[e]);
+        if (a.x != nullptr) h[e] = fma(static_cast<double>(fw[e]) * static_cast<double>(fx[e]), ia, h[e]);
+      }
+    };
+    double fi = 1.0;
+    if (a.wf != nullptr) {
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        double h[8];
+        sum_of(i, h);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fma(h[e], h[e], ss);
+      }
+      fi = inv_rms(ss);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      double h[8];
+      float o[8], fw[8];
+      sum_of(i, h);
+      unpack_bf16x8(wf[i], fw);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(a.wf != nullptr ? static_cast<double>(fw[e]) * h[e] * fi : h[e]);
+      rr[i] = pack_bf16x8(o);
+    }
+  }
+  if (a.h_out != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (t + i * kLanes < nq) reinterpret_cast<uint4*>(a.h_out + base)[t + i * kLanes] = rr[i];
+  }
+  const double ib = inv_rms(squares(rr));
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = t + i * kLanes;
+    float fh[8], fw[8], z[8];
+    unpack_bf16x8(rr[i], fh);
+    unpack_bf16x8(wb[i], fw);
+    uint32_t peak = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // (0 past the row, also where the row's statistics are not finite)
+      z[e] = c < nq ? round_odd(static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * ib) : 0.0f;
+      peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
+    }
+    peak = quad_max_u(peak);
+    if (c >= a.per_row) continue;  // (whole quads)
+    const uint32_t code = mx_scale_code<8>(peak);
+    const uint2 q = mx_encode8(z, mx_scale(code));
+    const int64_t piece = row * a.per_row + c;
+    reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
+    if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+  }
+}
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+}  // namespace fl
+
+extern "C" int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_stride, int64_t rows, int32_t k,
+                                  int32_t bits, uint8_t* codes, uint8_t* scales, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(x && codes && scales, "fl_mx_quantize: null pointer");
+  FL_REQUIRE(bits == 4 || bits == 8, "fl_mx_quantize: bits must be 4 or 8");
+  FL_REQUIRE(rows >= 0 && k > 0 && k <= FL_MX_MAX_K && x_stride >= 0, "fl_mx_quantize: bad sizes");
+  FL_REQUIRE(aligned(x, x_is_f32 ? 4 : 2), "fl_mx_quantize: x is not aligned to its elements");
+  FL_REQUIRE(aligned(codes, 16), "fl_mx_quantize: codes must be 16-byte aligned");
+  if (rows == 0) return FL_OK;
+  QuantArgs a{};
+  a.x = x;
+  a.x_stride = x_stride;
+  a.k = k;
+  a.per_row = static_cast<int>(mx_padded(k) / 8);
+  FL_REQUIRE(rows <= INT64_MAX / 2 / a.per_row, "fl_mx_quantize: too many rows");
+  a.pieces = rows * a.per_row;
+  a.rows_are_vectors = aligned(x, 16) && (x_stride * (x_is_f32 ? 4 : 2)) % 16 == 0;
+  a.codes = codes;
+  a.scales = scales;
+  const int64_t blocks = (a.pieces + kThreads - 1) / kThreads;
+  FL_REQUIRE(blocks <= 0xFFFFFFFFll / kThreads, "fl_mx_quantize: grid too large");
+  const dim3 g(static_cast<unsigned>(blocks)), t(kThreads);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (bits == 4) {
+    if (x_is_f32)
+      hipLaunchKernelGGL((mx_quantize_kernel<4, true>), g, t, 0, st, a);
+    else
+      hipLaunchKernelGGL((mx_quantize_kernel<4, false>), g, t, 0, st, a);
+  } else {
+    if (x_is_f32)
+      hipLaunchKernelGGL((mx_quantize_kernel<8, true>), g, t, 0, st, a);
+    else
+      hipLaunchKernelGGL((mx_quantize_kernel<8, false>), g, t, 0, st, a);
+  }
+  FL_LAUNCH_CHECK("fl_mx_quantize");
+  return FL_OK;
+}
+
+extern "C" int32_t fl_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t k, int32_t bits,
+                                    uint16_t* out, int64_t out_stride, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(codes && scales && out, "fl_mx_dequantize: null pointer");
+  FL_REQUIRE(bits == 4 || bits == 8, "fl_mx_dequantize: bits must be 4 or 8");
+  FL_REQUIRE(rows >= 0 && k > 0 && k <= FL_MX_MAX_K && out_stride >= k, "fl_mx_dequantize: bad sizes");
+  FL_REQUIRE(aligned(codes, 16), "fl_mx_dequantize: codes must be 16-byte aligned");
+  FL_REQUIRE(aligned(out, 2), "fl_mx_dequantize: out is not aligned to its elements");
+  if (rows == 0) return FL_OK;
+  DequantArgs a{};
+  a.codes = codes;
+  a.scales = scales;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.k = k;
+  a.per_row = static_cast<int>(mx_padded(k) / 8);
+  FL_REQUIRE(rows <= INT64_MAX / 2 / a.per_row, "fl_mx_dequantize: too many rows");
+  a.pieces = rows * a.per_row;
+  a.rows_are_vectors = aligned(out, 16) && out_stride % 8 == 0;
+  const int64_t blocks = (a.pieces + kThreads - 1) / kThreads;
+  FL_REQUIRE(blocks <= 0xFFFFFFFFll / kThreads, "fl_mx_dequantize: grid too large");
+  const dim3 g(static_cast<unsigned>(blocks)), t(kThreads);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (bits == 4)
+    hipLaunchKernelGGL(mx_dequantize_kernel<4>, g, t, 0, st, a);
+  else
+    hipLaunchKernelGGL(mx_dequantize_kernel<8>, g, t, 0, st, a);
+  FL_LAUNCH_CHECK("fl_mx_dequantize");
+  return FL_OK;
+}
+
+extern "C" int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, const uint16_t* r,
+                                    const uint16_t* w_a, const uint16_t* w_f, const uint16_t* w_b, uint16_t* h_out,
+                                    uint8_t* z_codes, uint8_t* z_scales, int64_t stride, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(m >= 0 && d > 0 && d % 8 == 0 && d <= 8192 && stride >= d && stride % 8 == 0,
+             "fl_norm_chain_mx: d must be a multiple of 8 up to 8192 and the row stride a multiple of 8");
+  FL_REQUIRE(r && w_b && z_codes && z_scales, "fl_norm_chain_mx: r, w_b and the outputs of z are required");
+  FL_REQUIRE(x == nullptr || w_a != nullptr, "fl_norm_chain_mx: x needs its norm weight");
+  for (const void* p : {static_cast<const void*>(x), static_cast<const void*>(r), static_cast<const void*>(w_a),
+                        static_cast<const void*>(w_f), static_cast<const void*>(w_b),
+                        static_cast<const void*>(h_out), static_cast<const void*>(z_codes)})
+    FL_REQUIRE(aligned(p, 16), "fl_norm_chain_mx: every tensor must be 16-byte aligned");
+  if (m == 0) return FL_OK;
+  const int per_row = static_cast<int>(mx_padded(d) / 8);
+  const NormMxArgs a{m, stride, d, per_row, eps, x, r, w_a, w_f, w_b, h_out, z_codes, z_scales};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 t(kThreads);
+  if (per_row <= 256)
+    hipLaunchKernelGGL((norm_chain_mx_kernel<1, 4>), dim3(m), t, 0, st, a);
+  else if (per_row <= 512)
+    hipLaunchKernelGGL((norm_chain_mx_kernel<2, 4>), dim3(m), t, 0, st, a);
+  else
+    hipLaunchKernelGGL((norm_chain_mx_kernel<4, 4>), dim3(m), t, 0, st, a);
+  FL_LAUNCH_CHECK("fl_norm_chain_mx");
+  return FL_OK;
+}

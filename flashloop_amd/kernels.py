@@ -7,13 +7,15 @@ flashloop/engine.py:346-498, flashloop/prefill.py:158-237).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
+from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import GROUP, HEAD_DIM, check, load, ptr_array
+from ._lib import GROUP, HEAD_DIM, MX_BLOCK, MX_MAX_K, MX_PAD, check, load, ptr_array
 
 
 def _stream() -> int:
@@ -676,3 +678,233 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     out = torch.empty_like(gate)
     check(load().fl_swiglu(gate.data_ptr(), up.data_ptr(), out.data_ptr(), gate.numel(), _stream()), "fl_swiglu")
     return out
+
+
+# ---------------------------------------------------------------------------- microscaled rows and weights
+@dataclass(frozen=True)
+class MXTensor:
+    """A matrix ``[rows, cols]`` in a microscaled format (include/flashloop_amd.h): ``codes`` u8
+    ``[rows, Kp * bits / 8]`` and ``scales`` u8 ``[rows, Kp / 32]``, ``Kp`` being ``cols`` padded with
+    zeros to a multiple of 128.  ``bits``: 4 (e2m1, two values a byte) or 8 (e4m3)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    cols: int
+    bits: int
+
+    def __post_init__(self) -> None:
+        if self.bits not in (4, 8):
+            raise ValueError(f"bits must be 4 or 8, got {self.bits}")
+        if not 0 < self.cols <= MX_MAX_K:
+            raise ValueError(f"cols must be 1..{MX_MAX_K}, got {self.cols}")
+        kp = -(-self.cols // MX_PAD) * MX_PAD
+        for t, width, name in ((self.codes, kp * self.bits // 8, "codes"), (self.scales, kp // MX_BLOCK, "scales")):
+            if t.dtype != torch.uint8 or t.ndim != 2 or t.shape[1] != width or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous uint8 [rows, {width}], got {t.dtype} {tuple(t.shape)}")
+        if self.codes.shape[0] != self.scales.shape[0] or self.codes.device != self.scales.device:
+            raise ValueError("codes and scales must have the same rows and device")
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (self.rows, self.cols)
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def _launch_on(device: torch.device):
+    """The tensors' device as the current one while a kernel is launched (on its current stream)."""
+    if device.type != "cuda":
+        raise RuntimeError("tensors must be on the device")
+    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+
+def _same_device(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors lie on different devices ({t.device}, {device})")
+
+
+def _mx_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` as rows [.., K] that follow each other at one stride, values next to each other."""
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError("x needs at least one value a row")
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"x must be bfloat16 or float32, got {x.dtype}")
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) < 0:
+        x2 = x2.contiguous()
+    return x2
+
+
+def mx_quantize(x: torch.Tensor, bits: int = 8) -> MXTensor:
+    """``x`` [.., K] (bf16 or f32) in a microscaled format of 8 or 4 bits (``fl_mx_quantize``): its
+    leading dimensions become the rows.  A block of 32 values that holds a NaN or an infinity reads
+    as NaN."""
+    if bits not in (4, 8):
+        raise ValueError(f"bits must be 4 or 8, got {bits}")
+    x2 = _mx_rows(x)
+    rows, k = x2.shape
+    if k > MX_MAX_K:
+        raise ValueError(f"rows of more than {MX_MAX_K} values")
+    kp = -(-k // MX_PAD) * MX_PAD
+    with _launch_on(x2.device):
+        codes = torch.empty(rows, kp * bits // 8, dtype=torch.uint8, device=x2.device)
+        scales = torch.empty(rows, kp // MX_BLOCK, dtype=torch.uint8, device=x2.device)
+        if rows:
+            check(load().fl_mx_quantize(x2.data_ptr(), int(x2.dtype == torch.float32), x2.stride(0), rows, k, bits,
+                                        codes.data_ptr(), scales.data_ptr(), _stream()), "fl_mx_quantize")
+    return MXTensor(codes, scales, k, bits)
+
+
+def mx_dequantize(t: MXTensor) -> torch.Tensor:
+    """The values of ``t`` as bf16 ``[rows, cols]`` (``fl_mx_dequantize``)."""
+    with _launch_on(t.device):
+        out = torch.empty(t.rows, t.cols, dtype=torch.bfloat16, device=t.device)
+        if t.rows:
+            check(load().fl_mx_dequantize(t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.cols, t.bits,
+                                          out.data_ptr(), t.cols, _stream()), "fl_mx_dequantize")
+    return out
+
+
+def _chain_operands(r, x, w_a, w_f, w_b):
+    """The chain's rows as contiguous bf16 [M, D], its gains checked."""
+    r2 = _rows2d(r, "r")
+    x2 = None if x is None else _rows2d(x, "x")
+    d = r2.shape[1]
+    if x2 is not None and x2.shape != r2.shape:
+        raise ValueError("x must have the shape of r")
+    if x2 is not None and w_a is None:
+        raise ValueError("x needs its norm weight w_a")
+    for t, name in ((r2, "r"), (x2, "x")):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise ValueError(f"{name} must be bf16")
+    for t, name in ((w_a, "w_a"), (w_f, "w_f"), (w_b, "w_b")):
+        if t is not None:
+            _require(t, torch.bfloat16, name)
+            if t.numel() != d:
+                raise ValueError(f"{name} must have {d} values")
+    _same_device(r2.device, x2, w_a, w_f, w_b)
+    return r2, x2
+
+
+def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.Tensor | None = None,
+                  w_f: torch.Tensor | None = None, w_b: torch.Tensor, eps: float, want_h: bool = True):
+    """``norm_chain`` with its ``z`` as the 8-bit rows that ``mx_matmul`` takes (``fl_norm_chain_mx``):
+    ``h = r + RMSNorm_a(x)`` (or ``r``), through ``RMSNorm_f`` where given, and ``z = RMSNorm_b(h)``.
+    Returns (h bf16 [M, D] or None, z)."""
+    r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
+    if w_b is None:
+        raise ValueError("w_b is required")
+    m, d = r2.shape
+    kp = -(-d // MX_PAD) * MX_PAD
+    with _launch_on(r2.device):
+        h = torch.empty(m, d, dtype=torch.bfloat16, device=r2.device) if want_h else None
+        codes = torch.empty(m, kp, dtype=torch.uint8, device=r2.device)
+        scales = torch.empty(m, kp // MX_BLOCK, dtype=torch.uint8, device=r2.device)
+        check(load().fl_norm_chain_mx(m, d, float(eps), _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), w_b.data_ptr(), _p(h),
+                                      codes.data_ptr(), scales.data_ptr(), d, _stream()) if m else 0, "fl_norm_chain_mx")
+    return h, MXTensor(codes, scales, d, 8)
+
+
+def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out):
+    """Outputs, pointer arrays and checked operands of the 4-bit GEMVs."""
+    if epilogue not in (EPI_PLAIN, EPI_F32, EPI_ADD, EPI_SWIGLU, EPI_ROPE):
+        raise ValueError(f"unknown epilogue {epilogue}")
+    need = {EPI_SWIGLU: 2, EPI_ROPE: 3}.get(epilogue, 1)
+    if len(weights) != need:
+        raise ValueError(f"the epilogue takes {need} weight(s), got {len(weights)}")
+    n = weights[0].rows
+    for w in weights:
+        if w.bits != 4 or w.cols != k or w.rows != n:
+            raise ValueError(f"weights must be 4-bit [{n}, {k}], got {w.bits}-bit {w.shape}")
+        _same_device(device, w.codes)
+    if not n:
+        raise ValueError("weights have no rows")
+    dt = torch.float32 if epilogue == EPI_F32 else torch.bfloat16
+    nout = 3 if epilogue == EPI_ROPE else 1
+    if out is None:
+        outs = [torch.empty(m, n, dtype=dt, device=device) for _ in range(nout)]
+    else:
+        _require(out, dt, "out")
+        if nout != 1 or out.shape != (m, n):
+            raise ValueError(f"out must be one [{m}, {n}] tensor")
+        outs = [out]
+    add = cos = sin = None
+    if epilogue == EPI_ADD:
+        if addend is None:
+            raise ValueError("the epilogue takes an addend")
+        add = addend.reshape(m, n)
+        _require(add, torch.bfloat16, "addend")
+    if epilogue == EPI_ROPE:
+        if rope is None:
+            raise ValueError("the epilogue takes rope tables")
+        cos, sin = (t.reshape(m, head_dim).contiguous() for t in rope)
+        _require(cos, torch.bfloat16, "rope cos")
+        _require(sin, torch.bfloat16, "rope sin")
+    _same_device(device, add, cos, sin, *outs)
+    args = (_ptrs([w.codes for w in weights]), _ptrs([w.scales for w in weights]), n, int(epilogue), _ptrs(outs), n,
+            _p(add), n, _p(cos), _p(sin), int(head_dim))
+    return outs, args, (add, cos, sin)  # (the tensors live until the launch)
+
+
+def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torch.Tensor | None = None,
+            rope: tuple[torch.Tensor, torch.Tensor] | None = None, head_dim: int = HEAD_DIM,
+            out: torch.Tensor | None = None):
+    """``gemv`` with 4-bit weights (``fl_mx_gemv``): ``x`` [.., K] of 1 to 8 bf16 rows (f32 is rounded
+    to bf16 first), ``weights`` a list of 4-bit ``MXTensor`` [N, K].  Sums and epilogues are fp32 and
+    rounded once; EPI_F32 returns the sums.  Returns [M, N], or (q, k, v) for EPI_ROPE."""
+    x2 = _rows2d(x, "x")
+    m, k = x2.shape
+    if not 1 <= m <= 8:
+        raise ValueError(f"mx_gemv takes 1 to 8 rows, got {m}")
+    with _launch_on(x2.device):
+        outs, args, held = _mx_gemv_operands(x2.device, m, k, weights, epilogue, addend, rope, head_dim, out)
+        check(load().fl_mx_gemv(x2.data_ptr(), int(x2.dtype == torch.float32), k, m, k, *args, _stream()), "fl_mx_gemv")
+    return tuple(outs) if epilogue == EPI_ROPE else outs[0]
+
+
+def mx_gemv_chain(r: torch.Tensor, weights, *, x: torch.Tensor | None = None, w_a: torch.Tensor | None = None,
+                  w_f: torch.Tensor | None = None, w_b: torch.Tensor | None = None, eps: float, want_h: bool = True,
+                  epilogue: int = EPI_PLAIN, addend: torch.Tensor | None = None,
+                  rope: tuple[torch.Tensor, torch.Tensor] | None = None, head_dim: int = HEAD_DIM,
+                  out: torch.Tensor | None = None):
+    """The chain of ``norm_chain_mx`` with ``z`` in bf16, followed by ``mx_gemv`` of it (of h without
+    ``w_b``), in one launch (``fl_mx_gemv_chain``).  Returns (h or None, the output as ``mx_gemv``
+    returns it)."""
+    r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
+    m, d = r2.shape
+    if not 1 <= m <= 8:
+        raise ValueError(f"mx_gemv_chain takes 1 to 8 rows, got {m}")
+    with _launch_on(r2.device):
+        outs, args, held = _mx_gemv_operands(r2.device, m, d, weights, epilogue, addend, rope, head_dim, out)
+        h = torch.empty(m, d, dtype=torch.bfloat16, device=r2.device) if want_h else None
+        check(load().fl_mx_gemv_chain(m, d, float(eps), _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), _p(w_b), _p(h), d, *args,
+                                      _stream()), "fl_mx_gemv_chain")
+    return h, (tuple(outs) if epilogue == EPI_ROPE else outs[0])
+
+
+def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x @ weight.T`` of 8-bit rows [M, K] and 4-bit weights [N, K] (``fl_mx_matmul``): fp32 sums,
+    returned as bf16 or f32 [M, N].  Any number of rows."""
+    if x.bits != 8 or weight.bits != 4 or x.cols != weight.cols:
+        raise ValueError(f"takes 8-bit rows and 4-bit weights of one K, got {x.bits}-bit {x.shape}, {weight.bits}-bit {weight.shape}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
+    _same_device(x.device, weight.codes)
+    with _launch_on(x.device):
+        y = torch.empty(x.rows, weight.rows, dtype=out_dtype, device=x.device)
+        if y.numel():
+            check(load().fl_mx_matmul(x.codes.data_ptr(), x.scales.data_ptr(), x.rows, x.cols, weight.codes.data_ptr(),
+                                      weight.scales.data_ptr(), weight.rows, y.data_ptr(), int(out_dtype == torch.float32),
+                                      weight.rows, _stream()), "fl_mx_matmul")
+    return y

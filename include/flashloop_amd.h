@@ -37,6 +37,9 @@ extern "C" {
 #define FL_HEAD_DIM 128
 #define FL_GROUP 64
 #define FL_MAX_LOOPS 4
+#define FL_MX_BLOCK 32         /* values that share a scale in a microscaled row */
+#define FL_MX_PAD 128          /* stored rows are padded to a multiple of this many values */
+#define FL_MX_MAX_K (1 << 20)  /* longest row */
 
 /*
  * One layer's packed cross-loop KV cache for a batch of sequences, in HBM.
@@ -535,6 +538,58 @@ int32_t fl_rope_store(const uint16_t* q, const uint16_t* k, const uint16_t* v, i
                       const uint16_t* rope_cos, const uint16_t* rope_sin, const int32_t* positions,
                       int32_t n, int32_t heads, int32_t rows, void* stream);
 int32_t fl_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64_t count, void* stream);
+
+/*
+ * Microscaled (MX) rows and weights: values of 4 bits (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) or 8 bits (e4m3, no infinities) with a power-of-two scale for every FL_MX_BLOCK of
+ * them along K.  A matrix [rows, K] is stored as
+ *   codes   u8 [rows, Kp * bits / 8]  Kp = K padded with zeros to a multiple of FL_MX_PAD; byte j
+ *                                     of a 4-bit row holds value 2j in its low nibble; 16-byte aligned
+ *   scales  u8 [rows, Kp / 32]        exponent + 127 (1..254); 255: the block's values are NaN
+ * The reference has no such weights (its Linear layers are bf16, flashloop/engine.py:396-537); a
+ * looped model reads every weight once per loop, so they are most of a decode step's bytes.
+ *
+ * fl_mx_quantize: rows of bf16 (or f32) values, `x_stride` elements apart.  A block's scale is the
+ * smallest power of two (from 2^-126) with which no value lies past the format's largest, so
+ * nothing saturates; values are rounded to the nearest, ties to the even code.  A block with a NaN
+ * or an infinity gets scale 255 and codes of zero.
+ * fl_mx_dequantize: the values as bf16 (exact, but for results under 2^-126 or past the range).
+ * fl_norm_chain_mx: the chain of fl_norm_chain with z in 8 bits: h = x ? r + RMSNorm_a(x) : r; if
+ * w_f: h = RMSNorm_f(h); h_out (optional) = bf16(h); z = RMSNorm_b(bf16(h)), quantised as above from
+ * its unrounded value.  Sums and products are in 64 bits and only h and z are rounded (fl_norm_chain
+ * rounds every norm and the sum to bf16, as the modules do).  bf16
+ * tensors with row stride `stride`, d % 8 == 0, d <= 8192, 16-byte aligned; w_b is required.
+ */
+int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_stride, int64_t rows, int32_t k,
+                       int32_t bits, uint8_t* codes, uint8_t* scales, void* stream);
+int32_t fl_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t k, int32_t bits,
+                         uint16_t* out, int64_t out_stride, void* stream);
+int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, const uint16_t* r,
+                         const uint16_t* w_a, const uint16_t* w_f, const uint16_t* w_b, uint16_t* h_out,
+                         uint8_t* z_codes, uint8_t* z_scales, int64_t stride, void* stream);
+/*
+ * fl_mx_gemv: y[m, n] = sum_k bf16(x[m, k]) * W[n, k] for the 1..8 rows of a decode step and 4-bit
+ * weights, with the arguments and epilogues of fl_gemv_bf16 (codes / scales in place of weights).
+ * Sums and epilogues are fp32 and each output is rounded once (the bf16 Linear's rounding in
+ * between has no counterpart here); epilogue 1 gives the fp32 sums.  K % 8 == 0, any N (RoPE: a
+ * multiple of head_dim, itself a multiple of 8).  x rows 16-byte aligned.
+ * fl_mx_gemv_chain: the chain of fl_norm_chain_mx, in fp32 and with z rounded to bf16, then
+ * fl_mx_gemv of z (h when w_b is NULL), in one launch; K <= 4096.
+ * fl_mx_matmul: y[m, n] = sum_k X[m, k] * W[n, k] for 8-bit rows X and 4-bit weights W, any m, n
+ * and k, fp32 sums, y bf16 or f32 [m, n] with row stride y_stride.
+ */
+int32_t fl_mx_gemv(const void* x, int32_t x_is_f32, int64_t x_stride, int32_t m, int32_t k,
+                   const uint8_t* const* codes, const uint8_t* const* scales, int32_t n, int32_t epilogue,
+                   void* const* outputs, int64_t out_stride, const uint16_t* addend, int64_t addend_stride,
+                   const uint16_t* rope_cos, const uint16_t* rope_sin, int32_t head_dim, void* stream);
+int32_t fl_mx_gemv_chain(int32_t m, int32_t k, float eps, const uint16_t* x, const uint16_t* r,
+                         const uint16_t* w_a, const uint16_t* w_f, const uint16_t* w_b, uint16_t* h_out,
+                         int64_t stride, const uint8_t* const* codes, const uint8_t* const* scales, int32_t n,
+                         int32_t epilogue, void* const* outputs, int64_t out_stride, const uint16_t* addend,
+                         int64_t addend_stride, const uint16_t* rope_cos, const uint16_t* rope_sin,
+                         int32_t head_dim, void* stream);
+int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m, int32_t k, const uint8_t* w_codes,
+                     const uint8_t* w_scales, int32_t n, void* y, int32_t y_is_f32, int64_t y_stride, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,8 @@ Modules
                (``flashloop_torch/attention_utils.py``, ``flashloop/engine.py``).
 ``tokens``     token-sparse prefill selection and row gather/scatter
                (``flashloop_torch/token_updates.py``, ``flashloop/selection.py``).
+``mx``         microscaled rows and weights of 4 and 8 bits, by search over the formats' values (no
+               counterpart in the reference).
 
 Pinning status of each function is stated in its docstring ("pinned by: ...").
 """
