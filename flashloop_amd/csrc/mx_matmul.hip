@@ -10,13 +10,18 @@
 // f32 results: every code is exact in bf16, so the operands are widened in registers and
 // v_mfma_f32_16x16x32_bf16 sums exact products in fp32 (a quarter of the rate).
 //
-// mx_matmul_tile_kernel: a workgroup's tile of BN rows of W by BM rows of X, K in steps of 128 through
-// LDS.  The operands go from memory to LDS without passing registers, two steps ahead, in three
-// buffers (one barrier a step); 16-byte pieces of a row are stored at a place that depends on the row, so
-// that the 16 lanes of a read phase meet all banks.  Scales come four steps at a time (a row's 16
-// bytes).  Rows past the matrix read as zeros.
-// mx_matmul_rows_kernel: few rows of X.  A wave takes 16 rows of W by up to 64 rows of X straight from
-// memory, the waves of a workgroup divide K.
+// A workgroup's tile is BN rows of W by BM rows of X, K in steps of 128 through LDS.  The operands go from
+// memory to LDS without passing registers, two steps ahead, in three buffers (one barrier a step);
+// 16-byte pieces of a row are stored at a place that depends on the row, so that the 16 lanes of a read
+// phase meet all banks.  Scales come four steps at a time (a row's 16 bytes).  Rows past the matrix read
+// as zeros.  The largest tile takes the LDS of a CU: its eight waves alternate between reading and
+// multiplying, and it goes on to further tiles, whose first steps are on their way while it stores.
+//
+// Bound by the matrix cores' power: with operands in registers the instruction reaches 3500-3750 TFLOP/s on
+// random codes (4700 on zeros), 8192^3 here 2990, 8192 x 2048 -> 5632 2350 (80 us; 704 tiles in
+// three rounds of 256), 8192 x 5632 -> 2048 2660.  The bf16 library product of the same sizes: 1390, 1050, 1410.
+#include <algorithm>
+
 #include "mx_common.h"
 
 namespace fl {
@@ -66,7 +71,7 @@ __device__ __forceinline__ int x_piece(int g, int half) {
 
 // four neighbouring outputs of row m from n on
 template <bool F32>
-__device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const float* v) {
+__device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const mx_f32x4_t& v) {
   if (m >= a.m || n >= a.n) return;
   const int64_t o = m * a.y_stride + n;
   if constexpr (F32) {
@@ -93,6 +98,29 @@ __device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const 
   }
 }
 
+// The same of two groups of 16 n side by side (v, u): the odd rows of 16 lanes change their v for the u of
+// the even ones, so that a lane holds eight neighbours of one group and the four lanes of an m 32.
+__device__ __forceinline__ void store8(const MmArgs& a, int64_t m, int n, int g, const mx_f32x4_t& v, const mx_f32x4_t& u) {
+  const auto pair = [](float lo, float hi) {
+    typedef float f32x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t f = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, mx_bf16x2_t));
+  };
+  const auto p = __builtin_amdgcn_permlane16_swap(pair(v[0], v[1]), pair(u[0], u[1]), false, false);
+  const auto q = __builtin_amdgcn_permlane16_swap(pair(v[2], v[3]), pair(u[2], u[3]), false, false);
+  const uint32_t w[4] = {p[0], q[0], p[1], q[1]};
+  n += 16 * (g & 1) + 8 * (g >> 1);
+  if (m >= a.m || n >= a.n) return;
+  uint16_t* y = static_cast<uint16_t*>(a.y) + m * a.y_stride + n;
+  if (n + 8 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
+    *reinterpret_cast<uint4*>(y) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < a.n) y[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+  }
+}
+
 // ---------------------------------------------------------------------------------
 // A raw buffer over `bytes` bytes at p (wave-uniform): what a load finds past the end is zero.  Word 3
 // is the gfx9 raw-buffer format.
@@ -116,26 +144,30 @@ __device__ __forceinline__ void to_lds(mx_i32x4_t r, uint32_t voff, uint32_t sof
                  : "memory");
 }
 
-template <int BN, int BM, int WN, int WM>
+template <int BN, int BM, int WN, int WM, int KS>
 struct TileGeom {
-  static constexpr int kWaves = WN * WM;
-  static constexpr int kThreads = kWaves * kWave;
+  static constexpr int kWaves = WN * WM;  // of one of the KS groups that divide K
+  static constexpr int kThreads = KS * kWaves * kWave;
   static constexpr int kFN = BN / WN / 16, kFM = BM / WM / 16;  // 16-row groups of a wave
   static constexpr int kWBytes = BN * 64, kXBytes = BM * 128;   // of a step
   static constexpr int kBuffer = kWBytes + kXBytes;
-  static constexpr int kScales = (BN + BM) * 16;                // of four steps
-  static constexpr int kLds = 3 * kBuffer + 2 * kScales;
+  static constexpr int kSRows = (BN + BM + 16 * kWaves - 1) / (16 * kWaves) * (16 * kWaves);
+  static constexpr int kScales = kSRows * 16;                   // of four steps
+  static constexpr int kGroup = 3 * kBuffer + 2 * kScales;      // LDS of a group
+  static constexpr int kLds = KS * kGroup;
   // wave-wide transfers a wave makes
   static constexpr int kWLoads = kWBytes / 1024 / kWaves, kXLoads = kXBytes / 1024 / kWaves;
   static constexpr int kSLoads = kScales / 256 / kWaves;
-  static_assert(kWLoads * 1024 * kWaves == kWBytes && kXLoads * 1024 * kWaves == kXBytes && kSLoads * 256 * kWaves == kScales);
+  static_assert(kWLoads * 1024 * kWaves == kWBytes && kXLoads * 1024 * kWaves == kXBytes && BN % 16 == 0);
   static_assert(kLds <= 160 * 1024);
+  // the groups' sums meet in the LDS of the steps
+  static_assert(KS == 1 || (KS - 1) * kWaves * kFN * kFM * kWave * 16 <= kLds);
 };
 
 // XCD-aware order: workgroups go to the 8 XCDs in turn, so XCD d takes the d-th stretch of the tiles; a
 // stretch walks groups of 8 tile rows of X, whose operands an XCD's L2 then holds.
-__device__ __forceinline__ void tile_of(const MmArgs& a, int* tn, int64_t* tm) {
-  const int total = gridDim.x, id = blockIdx.x;
+__device__ __forceinline__ void tile_of(const MmArgs& a, int id, int* tn, int64_t* tm) {
+  const int total = a.tiles_n * a.tiles_m;
   const int d = id & 7, per = total >> 3, more = total & 7;
   const int t = d * per + min(d, more) + (id >> 3);
   const int group = 8 * a.tiles_n, g = t / group, in = t - g * group;
@@ -144,25 +176,25 @@ __device__ __forceinline__ void tile_of(const MmArgs& a, int* tn, int64_t* tm) {
   *tm = 8 * g + in - *tn * rows;
 }
 
-template <int BN, int BM, int WN, int WM, bool F32>
-__global__ __launch_bounds__(WN* WM* kWave) void mx_matmul_tile_kernel(MmArgs a) {
-  using G = TileGeom<BN, BM, WN, WM>;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[G::kLds];
-  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds));
+template <int BN, int BM, int WN, int WM, int KS, bool F32, bool TURNS>
+__global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArgs a) {
+  using G = TileGeom<BN, BM, WN, WM, KS>;
+  static_assert(KS == 1 || !TURNS);
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_all[G::kLds];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = KS == 1 ? all_waves : all_waves % G::kWaves, part = KS == 1 ? 0 : all_waves / G::kWaves;
+  uint8_t* const lds = lds_all + part * G::kGroup;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds_all)) + part * G::kGroup;
   const int i = lane & 15, g = lane >> 4;
   const int wn = wave % WN, wm = wave / WN;
-  int tn;
-  int64_t tm;
-  tile_of(a, &tn, &tm);
-  const int n0 = tn * BN;
-  const int64_t m0 = tm * BM;
   const int64_t blocks = static_cast<int64_t>(a.steps) * 4;  // of a row
-  const mx_i32x4_t wr = raw_buffer(a.w + n0 * blocks * 16, (a.n - n0) * blocks * 16);
-  const mx_i32x4_t xr = raw_buffer(a.x + m0 * blocks * 32, (a.m - m0) * blocks * 32);
-  const mx_i32x4_t wsr = raw_buffer(a.ws + n0 * blocks, (a.n - n0) * blocks);
-  const mx_i32x4_t xsr = raw_buffer(a.xs + m0 * blocks, (a.m - m0) * blocks);
+  // this workgroup's tiles: blockIdx.x, + gridDim.x, ... (TURNS; else the one); their steps are counted through
+  const int tiles =
+      TURNS ? (a.tiles_n * a.tiles_m - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x) : 1;
+  // this group's steps: all, or the part-th stretch of them
+  const int per = (a.steps + KS - 1) / KS, first_step = KS == 1 ? 0 : part * per;
+  const int total = KS == 1 ? tiles * a.steps : max(0, min(per, a.steps - first_step));
   // what this lane moves: piece p of the tile's step lies at LDS 16 p
   uint32_t wv[G::kWLoads], xv[G::kXLoads], sv[G::kSLoads];
 #pragma unroll
@@ -179,54 +211,68 @@ __global__ __launch_bounds__(WN* WM* kWave) void mx_matmul_tile_kernel(MmArgs a)
   for (int j = 0; j < G::kSLoads; ++j) {
     const int p = (wave * G::kSLoads + j) * 64 + lane, row = p / 4;
     sv[j] = static_cast<uint32_t>(row < BN ? row : row - BN) * static_cast<uint32_t>(blocks) + 4u * (p & 3);
+    if (row >= BN + BM) sv[j] = 0x80000000u;  // (past every buffer)
   }
-  const auto request = [&](int s) __attribute__((always_inline)) {
-    if ((s & 3) == 0) {
-      const uint32_t at = lds0 + 3 * G::kBuffer + (s / 4 & 1) * G::kScales;
+  // the next step to request: tile, step in it, buffer, buffer of its scales
+  mx_i32x4_t wr{}, xr{}, wsr{}, xsr{};
+  int rtile = blockIdx.x, rs = 0, rbuf = 0, rscale = 1;
+  const auto request = [&]() __attribute__((always_inline)) {
+    if (rs == 0) {
+      int tn;
+      int64_t tm;
+      tile_of(a, rtile, &tn, &tm);
+      const int64_t n0 = static_cast<int64_t>(tn) * BN, m0 = tm * BM;
+      wr = raw_buffer(a.w + n0 * blocks * 16, (a.n - n0) * blocks * 16);
+      xr = raw_buffer(a.x + m0 * blocks * 32, (a.m - m0) * blocks * 32);
+      wsr = raw_buffer(a.ws + n0 * blocks, (a.n - n0) * blocks);
+      xsr = raw_buffer(a.xs + m0 * blocks, (a.m - m0) * blocks);
+    }
+    if ((rs & 3) == 0) {
+      rscale ^= 1;
+      const uint32_t at = lds0 + 3 * G::kBuffer + rscale * G::kScales;
 #pragma unroll
       for (int j = 0; j < G::kSLoads; ++j) {
         const int first = (wave * G::kSLoads + j) * 16;  // (16 rows a transfer: all of W or all of X)
         if (first < BN)
-          to_lds<4>(wsr, sv[j], 4u * s, at + 256u * (wave * G::kSLoads + j));
+          to_lds<4>(wsr, sv[j], 4u * (first_step + rs), at + 256u * (wave * G::kSLoads + j));
         else
-          to_lds<4>(xsr, sv[j], 4u * s, at + 256u * (wave * G::kSLoads + j));
+          to_lds<4>(xsr, sv[j], 4u * (first_step + rs), at + 256u * (wave * G::kSLoads + j));
       }
     }
-    const uint32_t at = lds0 + s % 3 * G::kBuffer;
+    const uint32_t at = lds0 + rbuf * G::kBuffer;
 #pragma unroll
-    for (int j = 0; j < G::kWLoads; ++j) to_lds<16>(wr, wv[j], 64u * s, at + 1024u * (wave * G::kWLoads + j));
+    for (int j = 0; j < G::kWLoads; ++j) to_lds<16>(wr, wv[j], 64u * (first_step + rs), at + 1024u * (wave * G::kWLoads + j));
 #pragma unroll
     for (int j = 0; j < G::kXLoads; ++j)
-      to_lds<16>(xr, xv[j], 128u * s, at + G::kWBytes + 1024u * (wave * G::kXLoads + j));
+      to_lds<16>(xr, xv[j], 128u * (first_step + rs), at + G::kWBytes + 1024u * (wave * G::kXLoads + j));
+    rbuf = rbuf == 2 ? 0 : rbuf + 1;
+    if (++rs == a.steps) {
+      rs = 0;
+      rtile += gridDim.x;
+    }
   };
 
   mx_f32x4_t acc[G::kFN][G::kFM];
+  const auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int n = 0; n < G::kFN; ++n)
+    for (int n = 0; n < G::kFN; ++n)
 #pragma unroll
-    for (int m = 0; m < G::kFM; ++m) acc[n][m] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int m = 0; m < G::kFM; ++m) acc[n][m] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  };
   const int wrow = wn * (BN / WN) + i, xrow = wm * (BM / WM) + i;
   const uint8_t* wl = lds + wrow * 64 + 16 * (g ^ ((i >> 2) & 3));
   const uint8_t* xl0 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 0) ^ ((i >> 1) & 7));
   const uint8_t* xl1 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 1) ^ ((i >> 1) & 7));
   const uint8_t* sl = lds + 3 * G::kBuffer + g;
 
-  request(0);
-  if (a.steps > 1) request(1);
-  constexpr int kStep = G::kWLoads + G::kXLoads;  // transfers of a step, its scales aside (they are made first)
-  for (int s = 0; s < a.steps; ++s) {
-    // step s has landed (of step s + 1 at most its own transfers are under way), for every wave, and
-    // no wave reads step s - 1 any more, whose buffer the next request fills
-    if (s + 1 < a.steps)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kStep) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (s + 2 < a.steps) request(s + 2);
-    const uint32_t at = s % 3 * G::kBuffer, sat = (s / 4 & 1) * G::kScales + 4 * (s & 3);
-    uint4 w[G::kFN];
-    uint32_t ws[G::kFN];
+  uint4 w[G::kFN], x0[G::kFM], x1[G::kFM];
+  uint32_t ws[G::kFN], xs[G::kFM];
+  // the step in hand: tile, step in it, buffer, buffer of its scales
+  int ctile = blockIdx.x, cs = 0, cbuf = 0, cscale = 1;
+  const auto read_step = [&]() __attribute__((always_inline)) {
+    if ((cs & 3) == 0) cscale ^= 1;
+    const uint32_t at = cbuf * G::kBuffer, sat = cscale * G::kScales + 4 * (cs & 3);
+    cbuf = cbuf == 2 ? 0 : cbuf + 1;
 #pragma unroll
     for (int n = 0; n < G::kFN; ++n) {
       w[n] = *reinterpret_cast<const uint4*>(wl + at + n * 1024);
@@ -234,95 +280,149 @@ __global__ __launch_bounds__(WN* WM* kWave) void mx_matmul_tile_kernel(MmArgs a)
     }
 #pragma unroll
     for (int m = 0; m < G::kFM; ++m) {
-      const uint4 x0 = *reinterpret_cast<const uint4*>(xl0 + at + m * 2048);
-      const uint4 x1 = *reinterpret_cast<const uint4*>(xl1 + at + m * 2048);
-      const uint32_t xs = sl[sat + (BN + xrow + 16 * m) * 16];
-#pragma unroll
-      for (int n = 0; n < G::kFN; ++n) acc[n][m] = mx_step<F32>(w[n], ws[n], x0, x1, xs, acc[n][m]);
+      x0[m] = *reinterpret_cast<const uint4*>(xl0 + at + m * 2048);
+      x1[m] = *reinterpret_cast<const uint4*>(xl1 + at + m * 2048);
+      xs[m] = sl[sat + (BN + xrow + 16 * m) * 16];
     }
+  };
+  const auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < G::kFM; ++m)
+#pragma unroll
+      for (int n = 0; n < G::kFN; ++n) acc[n][m] = mx_step<F32>(w[n], ws[n], x0[m], x1[m], xs[m], acc[n][m]);
+  };
+  constexpr int kStep = G::kWLoads + G::kXLoads;  // transfers of a step, its scales aside (they are made first)
+  // this wave's transfers of step s have landed (those of step s + 1, if made, may be under way)
+  const auto landed = [&](int s) __attribute__((always_inline)) {
+    if (s + 1 < total)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kStep) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  const auto barrier = [&]() __attribute__((always_inline)) {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+  };
+
+  // after a tile's last step: its results, while the next tile's first steps are on their way
+  const auto finish = [&]() __attribute__((always_inline)) {
+    int tn;
+    int64_t tm;
+    tile_of(a, ctile, &tn, &tm);
+    ctile += gridDim.x;
+#pragma unroll
+    for (int m = 0; m < G::kFM; ++m)
+#pragma unroll
+      for (int n = 0; n < G::kFN; n += 2) {
+        const int64_t row = tm * BM + xrow + 16 * m;
+        const int col = tn * BN + wn * (BN / WN) + 16 * n;
+        if constexpr (F32) {
+          store4<F32>(a, row, col + 4 * g, acc[n][m]);
+          store4<F32>(a, row, col + 16 + 4 * g, acc[n + 1][m]);
+        } else {
+          store8(a, row, col, g, acc[n][m], acc[n + 1][m]);
+        }
+      }
+  };
+
+  clear();
+  if (KS == 1 || total > 0) request();
+  if (total > 1) request();
+  if constexpr (TURNS) {
+    // The waves of a SIMD take turns: four waves read a step from LDS while the other four multiply the one
+    // that they hold, a barrier between the turns.  Waves 0..3 read step s in turn 2 s, waves 4..7 in turn
+    // 2 s + 1.  Step s + 1 has landed for every wave before the barrier that ends turn 2 s + 1, and the
+    // buffer that step s + 2 fills was last read in turn 2 s - 1, before a barrier that follows that read.
+    const bool second = wave >= G::kWaves / 2;
+    landed(0);
+    barrier();
+    if (second) barrier();
+    for (int s = 0; s < total; ++s) {
+      if (s + 2 < total) request();
+      read_step();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (second && s + 1 < total) landed(s + 1);
+      barrier();
+      multiply();
+      if (!second && s + 1 < total) landed(s + 1);
+      if (++cs == a.steps) {
+        cs = 0;
+        finish();
+        clear();
+      }
+      barrier();
+    }
+    if (!second) barrier();
+  } else {
+    for (int s = 0; s < (KS == 1 ? total : per); ++s) {
+      // step s has landed for every wave, and no wave reads step s - 1 any more, whose buffer the next
+      // request fills
+      landed(s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      barrier();
+      if (s + 2 < total) request();
+      if (KS == 1 || s < total) {
+        read_step();
+        multiply();
+      }
+      ++cs;
+    }
+    if constexpr (KS > 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      barrier();
+      mx_f32x4_t* sums = reinterpret_cast<mx_f32x4_t*>(lds_all);
+      const auto at = [&](int p, int n, int m) { return (((p - 1) * G::kWaves + wave) * G::kFN * G::kFM + n * G::kFM + m) * kWave + lane; };
+      if (part > 0) {
+#pragma unroll
+        for (int n = 0; n < G::kFN; ++n)
+#pragma unroll
+          for (int m = 0; m < G::kFM; ++m) sums[at(part, n, m)] = acc[n][m];
+      }
+      __syncthreads();
+      if (part > 0) return;
+#pragma unroll
+      for (int p = 1; p < KS; ++p)
+#pragma unroll
+        for (int n = 0; n < G::kFN; ++n)
+#pragma unroll
+          for (int m = 0; m < G::kFM; ++m) acc[n][m] += sums[at(p, n, m)];
+    }
+    finish();
   }
-#pragma unroll
-  for (int m = 0; m < G::kFM; ++m)
-#pragma unroll
-    for (int n = 0; n < G::kFN; ++n) {
-      const float v[4] = {acc[n][m][0], acc[n][m][1], acc[n][m][2], acc[n][m][3]};
-      store4<F32>(a, m0 + xrow + 16 * m, n0 + wn * (BN / WN) + 16 * n + 4 * g, v);
-    }
 }
 
-template <int BN, int BM, int WN, int WM, bool F32>
+template <int BN, int BM, int WN, int WM, int KS, bool F32, bool TURNS>
 void launch_tiles(MmArgs a, hipStream_t st) {
   a.tiles_n = (a.n + BN - 1) / BN;
   a.tiles_m = static_cast<int>((a.m + BM - 1) / BM);
-  hipLaunchKernelGGL((mx_matmul_tile_kernel<BN, BM, WN, WM, F32>), dim3(a.tiles_n * a.tiles_m), dim3(WN * WM * kWave), 0, st, a);
+  // A workgroup takes further tiles where all CUs are in use (one workgroup each).  The two buffers of scales
+  // then want no stretch of four steps that ends after one.
+  const int tiles = a.tiles_n * a.tiles_m, grid = TURNS && a.steps % 4 != 1 ? std::min(tiles, 256) : tiles;
+  hipLaunchKernelGGL((mx_matmul_tile_kernel<BN, BM, WN, WM, KS, F32, TURNS>), dim3(grid), dim3(KS * WN * WM * kWave), 0, st, a);
 }
 
-// ---------------------------------------------------------------------------------
-constexpr int kRowWaves = 4;
-
-template <int MB, bool F32>  // MB: groups of 16 rows of X
-__global__ __launch_bounds__(kRowWaves* kWave) void mx_matmul_rows_kernel(MmArgs a) {
-  __shared__ mx_f32x4_t red[kRowWaves][MB][kWave];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int i = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * (16 * MB);
-  const int64_t kb = static_cast<int64_t>(a.steps) * 4;  // blocks of a row
-  const int64_t wrow = min(n0 + i, a.n - 1);
-  const uint8_t* w = a.w + wrow * kb * 16 + 16 * g;
-  const uint8_t* ws = a.ws + wrow * kb + g;
-  const uint8_t* x[MB];
-  const uint8_t* xs[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b) {
-    const int64_t xrow = min(m0 + 16 * b + i, a.m - 1);
-    x[b] = a.x + xrow * kb * 32;
-    xs[b] = a.xs + xrow * kb + g;
-  }
-  mx_f32x4_t acc[MB];
-#pragma unroll
-  for (int b = 0; b < MB; ++b) acc[b] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = wave; s < a.steps; s += kRowWaves) {
-    const uint4 wv = *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(s) * 64);
-    const uint32_t wsv = ws[s * 4];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) {
-      const uint4 x0 = *reinterpret_cast<const uint4*>(x[b] + static_cast<int64_t>(s) * 128 + 16 * x_piece<F32>(g, 0));
-      const uint4 x1 = *reinterpret_cast<const uint4*>(x[b] + static_cast<int64_t>(s) * 128 + 16 * x_piece<F32>(g, 1));
-      acc[b] = mx_step<F32>(wv, wsv, x0, x1, xs[b][s * 4], acc[b]);
-    }
-  }
-#pragma unroll
-  for (int b = 0; b < MB; ++b) red[wave][b][lane] = acc[b];
-  __syncthreads();
-  for (int b = wave; b < MB; b += kRowWaves) {
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int p = 0; p < kRowWaves; ++p) {
-      const mx_f32x4_t r = red[p][b][lane];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += r[e];
-    }
-    store4<F32>(a, m0 + 16 * b + i, n0 + 4 * g, v);
-  }
-}
-
-template <int MB, bool F32>
-void launch_rows(const MmArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((mx_matmul_rows_kernel<MB, F32>), dim3((a.n + 15) / 16, static_cast<unsigned>((a.m + 16 * MB - 1) / (16 * MB))),
-                     dim3(kRowWaves * kWave), 0, st, a);
-}
-
+// The larger the tile, the less LDS traffic a product needs; the more workgroups, the more CUs work, and where
+// a CU has few of them KS groups of waves divide K, so that its steps do not follow one another.  Measured, us,
+// bf16 results, m x n x k (tile of n by m, groups):
+//   8192 x 5632 x 2048: 256 x 256 80.5, 128 x 128 129; 8192^3: 367, 656
+//   820 x 5632 x 2048: 128 x 128 18.6, 64 x 64 18.9; 64 x 49152 x 2048: 64 x 64 14.4, two groups 16.0
+//   820 x 2048 x 2048: 64 x 64 in two groups 9.7, one 9.8; 512 x 2048 x 2048: 7.4, 8.5; 32 x 32 in four 10.2
+//   128 x 2048 x 2048: 32 x 32 in four groups 5.0, 64 x 64 in one, two, four 8.1, 7.0, 7.1
+//   256 x 2048 x 2048: 6.4, 64 x 64 in two 7.1; 128 x 5632 x 2048: 8.7, 7.2
+//   32 x 49152 x 2048: 64 x 32 11.2, 64 x 64 12.6, 32 x 32 in four groups 15.2
 template <bool F32>
 void launch_matmul(const MmArgs& a, hipStream_t st) {
   const auto tiles = [&](int64_t bn, int64_t bm) { return ((a.n + bn - 1) / bn) * ((a.m + bm - 1) / bm); };
-  if (a.m <= 16) return launch_rows<1, F32>(a, st);
-  if (a.m <= 32) return launch_rows<2, F32>(a, st);
-  if (a.m <= 64) return launch_rows<4, F32>(a, st);
+  if (tiles(32, 32) <= 512) return launch_tiles<32, 32, 1, 2, 4, F32, false>(a, st);
+  if (a.m <= 32) return launch_tiles<64, 32, 2, 2, 1, F32, false>(a, st);
+  if (tiles(64, 64) <= 512) return launch_tiles<64, 64, 2, 2, 2, F32, false>(a, st);
   if constexpr (!F32)
-    if (tiles(256, 256) >= 256) return launch_tiles<256, 256, 2, 4, F32>(a, st);
-  if (tiles(128, 128) >= 256) return launch_tiles<128, 128, 2, 2, F32>(a, st);
-  launch_tiles<64, 64, 2, 2, F32>(a, st);
+    if (tiles(256, 256) >= 256) return launch_tiles<256, 256, 2, 4, 1, F32, true>(a, st);
+  if (tiles(128, 128) >= 256) return launch_tiles<128, 128, 2, 2, 1, F32, false>(a, st);
+  launch_tiles<64, 64, 2, 2, 1, F32, false>(a, st);
 }
 
 }  // namespace

@@ -10,6 +10,7 @@ namespace fl {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kNormGrid = 256 * 5;  // workgroups of a norm: what the CUs hold at once
 
 __device__ __forceinline__ uint32_t quad_max_u(uint32_t v) {
   v = max(v, static_cast<uint32_t>(dpp_i<kDppXor1>(static_cast<int>(v))));
@@ -165,128 +166,160 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
 }
 
-// sum over the lanes of a row: one wave, or the workgroup (two LDS buffers in turn, one barrier a sum)
+// sum over the lanes of a row: W waves (two LDS buffers in turn, one barrier a sum)
 template <int W>
 struct RowSum64 {
-  double (*red)[4];
+  double (*red)[W < 4 ? 4 : W];
   int phase;
   __device__ __forceinline__ double operator()(double v) {
     v = wave_sum64(v);
     if constexpr (W == 1) return v;
     double* r = red[phase & 1];
     ++phase;
-    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) r[wave] = v;
     lds_barrier();
-    return (r[0] + r[1]) + (r[2] + r[3]);
+    double s = r[first];
+#pragma unroll
+    for (int i = 1; i < W; ++i) s += r[first + i];
+    return s;
   }
 };
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = static_cast<uint32_t>(f32_to_bf16_rne(f[2 * i])) | static_cast<uint32_t>(f32_to_bf16_rne(f[2 * i + 1])) << 16;
+  for (int i = 0; i < 4; ++i) {
+    const f32x2_t v = {f[2 * i], f[2 * i + 1]};
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_bf16x2_t));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// W waves share a row, each lane holds its pieces t, t + 64 W, ... (NC of them).
-template <int NC, int W>
-__global__ __launch_bounds__(kThreads) void norm_chain_mx_kernel(NormMxArgs a) {
-  __shared__ double red[2][4];
-  constexpr int kLanes = 64 * W;
-  const int t = threadIdx.x % kLanes;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / kLanes) + threadIdx.x / kLanes;
-  if (row >= a.rows) return;  // (whole waves; with W = 4 every row has its workgroup)
-  const int nq = a.d / 8;
-  const int64_t base = row * a.stride;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  RowSum64<W> sum{red, 0};
-  uint4 rr[NC], xr[NC], wa[NC], wf[NC], wb[NC];
+// Eight 64-bit values as f32 that round on to e4m3 as the 64-bit ones do.  The nearest f32 does unless it
+// has reached a border (between two codes, or two scales: its last 19 bits are zero there), where the
+// value rounded to odd takes its place.
+typedef float f32x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x8_t round8_for_codes(const double (&v)[8]) {
+  f32x8_t f;
+  uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = t + i * kLanes;
-    const bool in = c < nq;
-    rr[i] = in ? reinterpret_cast<const uint4*>(a.r + base)[c] : zero;
-    xr[i] = in && a.x ? reinterpret_cast<const uint4*>(a.x + base)[c] : zero;
-    wa[i] = in && a.x ? reinterpret_cast<const uint4*>(a.wa)[c] : zero;
-    wf[i] = in && a.wf ? reinterpret_cast<const uint4*>(a.wf)[c] : zero;
-    wb[i] = in ? reinterpret_cast<const uint4*>(a.wb)[c] : zero;
+  for (int e = 0; e < 8; ++e) {
+    f[e] = static_cast<float>(v[e]);
+    least = min(least, __float_as_uint(f[e]) & 0x7FFFFu);
   }
-  const double d = static_cast<double>(a.d);
-  const auto inv_rms = [&](double ss) { return 1.0 / sqrt(sum(ss) / d + a.eps); };
-  const auto squares = [&](const uint4(&v)[NC]) {
+  if (least == 0) f = f32x8_t{round_odd(v[0]), round_odd(v[1]), round_odd(v[2]), round_odd(v[3]),
+                              round_odd(v[4]), round_odd(v[5]), round_odd(v[6]), round_odd(v[7])};
+  return f;
+}
+
+// W waves share a row, a lane holds one piece of it.  A workgroup takes one row, or as many as 4 waves
+// hold, and goes on to further ones, whose r and x are requested before the sums of the ones in hand.
+template <int W>
+constexpr int kNormThreads = W < 4 ? 256 : 64 * W;
+
+template <int W, bool ADD, bool FINAL>
+__global__ __launch_bounds__(kNormThreads<W>) void norm_chain_mx_kernel(NormMxArgs a) {
+  __shared__ double red[2][W < 4 ? 4 : W];
+  constexpr int kLanes = 64 * W, kRows = kNormThreads<W> / kLanes;
+  const int t = threadIdx.x % kLanes, nq = a.d / 8;
+  RowSum64<W> sum{red, 0};
+  uint4 r, x;
+  const bool in = t < nq;
+  const uint4 wa = ADD && in ? reinterpret_cast<const uint4*>(a.wa)[t] : make_uint4(0, 0, 0, 0);
+  const uint4 wf = FINAL && in ? reinterpret_cast<const uint4*>(a.wf)[t] : make_uint4(0, 0, 0, 0);
+  const uint4 wb = in ? reinterpret_cast<const uint4*>(a.wb)[t] : make_uint4(0, 0, 0, 0);
+  const double inv_d = 1.0 / static_cast<double>(a.d);
+  const auto inv_rms = [&](double ss) { return rsqrt(fma(sum(ss), inv_d, a.eps)); };
+  const auto request = [&](int64_t row, uint4& rr, uint4& xx) {
+    const int64_t base = row * a.stride;
+    rr = in ? reinterpret_cast<const uint4*>(a.r + base)[t] : make_uint4(0, 0, 0, 0);
+    if constexpr (ADD) xx = in ? reinterpret_cast<const uint4*>(a.x + base)[t] : make_uint4(0, 0, 0, 0);
+  };
+  const auto squares = [&](const uint4& v) {
     double ss = 0.0;
+    float f[8];
+    unpack_bf16x8(v, f);
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      float f[8];
-      unpack_bf16x8(v[i], f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ss);
-    }
+    for (int e = 0; e < 8; ++e) ss = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ss);
     return ss;
   };
-  if (a.x != nullptr || a.wf != nullptr) {
-    const double ia = a.x != nullptr ? inv_rms(squares(xr)) : 0.0;
-    const auto sum_of = [&](int i, double* h) {  // r + norm_a(x) of piece i
-      float fr[8], fx[8], fw[8];
-      unpack_bf16x8(rr[i], fr);
-      unpack_bf16x8(xr[i], fx);
-      unpack_bf16x8(wa[i], fw);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
+  request(min(row, a.rows - 1), r, x);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kRows; first < a.rows; first += step, row += step) {
+    const bool live = row < a.rows;  // (a row past the last is the last again, not stored)
+    uint4 nr, nx;
+    if (first + step < a.rows) request(min(row + step, a.rows - 1), nr, nx);
+    if constexpr (ADD || FINAL) {
+      const double ia = ADD ? inv_rms(squares(x)) : 0.0;
+      double h[8];  // r + norm_a(x)
+      float f[8], w[8], o[8];
+      unpack_bf16x8(r, f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[e] = static_cast<double>(fr[e]);
-        if (a.x != nullptr) h[e] = fma(static_cast<double>(fw[e]) * static_cast<double>(fx[e]), ia, h[e]);
+      for (int e = 0; e < 8; ++e) h[e] = static_cast<double>(f[e]);
+      if constexpr (ADD) {
+        unpack_bf16x8(x, f);
+        unpack_bf16x8(wa, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = fma(static_cast<double>(w[e]) * static_cast<double>(f[e]), ia, h[e]);
       }
-    };
-    double fi = 1.0;
-    if (a.wf != nullptr) {
-      double ss = 0.0;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        double h[8];
-        sum_of(i, h);
+      if constexpr (FINAL) {
+        double ss = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fma(h[e], h[e], ss);
+        const double fi = inv_rms(ss);
+        unpack_bf16x8(wf, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] *= static_cast<double>(w[e]) * fi;
       }
-      fi = inv_rms(ss);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(h[e]);
+      r = pack_bf16x8(o);
     }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      double h[8];
-      float o[8], fw[8];
-      sum_of(i, h);
-      unpack_bf16x8(wf[i], fw);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(a.wf != nullptr ? static_cast<double>(fw[e]) * h[e] * fi : h[e]);
-      rr[i] = pack_bf16x8(o);
-    }
-  }
-  if (a.h_out != nullptr) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-      if (t + i * kLanes < nq) reinterpret_cast<uint4*>(a.h_out + base)[t + i * kLanes] = rr[i];
-  }
-  const double ib = inv_rms(squares(rr));
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = t + i * kLanes;
+    if (a.h_out != nullptr && live && in) reinterpret_cast<uint4*>(a.h_out + row * a.stride)[t] = r;
+    // (0 past the row, also where the row's statistics are not finite)
+    const double ib = inv_rms(squares(r)), scale = in ? ib : 0.0;
     float fh[8], fw[8], z[8];
-    unpack_bf16x8(rr[i], fh);
-    unpack_bf16x8(wb[i], fw);
+    double v[8];
+    unpack_bf16x8(r, fh);
+    unpack_bf16x8(wb, fw);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * scale;
+    const f32x8_t rounded = round8_for_codes(v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[e] = rounded[e];
     uint32_t peak = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // (0 past the row, also where the row's statistics are not finite)
-      z[e] = c < nq ? round_odd(static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * ib) : 0.0f;
-      peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
-    }
+    for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
     peak = quad_max_u(peak);
-    if (c >= a.per_row) continue;  // (whole quads)
-    const uint32_t code = mx_scale_code<8>(peak);
-    const uint2 q = mx_encode8(z, mx_scale(code));
-    const int64_t piece = row * a.per_row + c;
-    reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
-    if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+    if (t < a.per_row && live) {  // (whole quads)
+      const uint32_t code = mx_scale_code<8>(peak);
+      const uint2 q = mx_encode8(z, mx_scale(code));
+      const int64_t piece = row * a.per_row + t;
+      reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
+      if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+    }
+    r = nr;
+    if constexpr (ADD) x = nx;
+  }
+}
+
+template <int W>
+void launch_norm(const NormMxArgs& a, hipStream_t st) {
+  constexpr int kRows = kNormThreads<W> / (64 * W);
+  const int64_t groups = (a.rows + kRows - 1) / kRows, most = kNormGrid * 256 / kNormThreads<W>;
+  const dim3 g(static_cast<unsigned>(groups < most ? groups : most)), t(kNormThreads<W>);
+  if (a.x != nullptr) {
+    if (a.wf != nullptr)
+      hipLaunchKernelGGL((norm_chain_mx_kernel<W, true, true>), g, t, 0, st, a);
+    else
+      hipLaunchKernelGGL((norm_chain_mx_kernel<W, true, false>), g, t, 0, st, a);
+  } else if (a.wf != nullptr) {
+    hipLaunchKernelGGL((norm_chain_mx_kernel<W, false, true>), g, t, 0, st, a);
+  } else {
+    hipLaunchKernelGGL((norm_chain_mx_kernel<W, false, false>), g, t, 0, st, a);
   }
 }
 
@@ -383,13 +416,16 @@ extern "C" int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint
   const int per_row = static_cast<int>(mx_padded(d) / 8);
   const NormMxArgs a{m, stride, d, per_row, eps, x, r, w_a, w_f, w_b, h_out, z_codes, z_scales};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 t(kThreads);
-  if (per_row <= 256)
-    hipLaunchKernelGGL((norm_chain_mx_kernel<1, 4>), dim3(m), t, 0, st, a);
+  if (per_row <= 64)
+    launch_norm<1>(a, st);
+  else if (per_row <= 128)
+    launch_norm<2>(a, st);
+  else if (per_row <= 256)
+    launch_norm<4>(a, st);
   else if (per_row <= 512)
-    hipLaunchKernelGGL((norm_chain_mx_kernel<2, 4>), dim3(m), t, 0, st, a);
+    launch_norm<8>(a, st);
   else
-    hipLaunchKernelGGL((norm_chain_mx_kernel<4, 4>), dim3(m), t, 0, st, a);
+    launch_norm<16>(a, st);
   FL_LAUNCH_CHECK("fl_norm_chain_mx");
   return FL_OK;
 }

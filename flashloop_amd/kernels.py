@@ -7,10 +7,8 @@ flashloop/engine.py:346-498, flashloop/prefill.py:158-237).
 
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
-from dataclasses import dataclass
 
 import torch
 
@@ -681,51 +679,67 @@ def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------- microscaled rows and weights
-@dataclass(frozen=True)
+# (The decode step's calls take a few microseconds on the GPU, so these functions are kept to few Python
+# operations: torch.cuda.current_stream alone costs 2.6 us, an allocation 1.1, a launch 2.)
 class MXTensor:
     """A matrix ``[rows, cols]`` in a microscaled format (include/flashloop_amd.h): ``codes`` u8
     ``[rows, Kp * bits / 8]`` and ``scales`` u8 ``[rows, Kp / 32]``, ``Kp`` being ``cols`` padded with
     zeros to a multiple of 128.  ``bits``: 4 (e2m1, two values a byte) or 8 (e4m3)."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    cols: int
-    bits: int
+    __slots__ = ("codes", "scales", "cols", "bits", "rows", "device")
 
-    def __post_init__(self) -> None:
-        if self.bits not in (4, 8):
-            raise ValueError(f"bits must be 4 or 8, got {self.bits}")
-        if not 0 < self.cols <= MX_MAX_K:
-            raise ValueError(f"cols must be 1..{MX_MAX_K}, got {self.cols}")
-        kp = -(-self.cols // MX_PAD) * MX_PAD
-        for t, width, name in ((self.codes, kp * self.bits // 8, "codes"), (self.scales, kp // MX_BLOCK, "scales")):
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int, bits: int) -> None:
+        if bits != 4 and bits != 8:
+            raise ValueError(f"bits must be 4 or 8, got {bits}")
+        if not 0 < cols <= MX_MAX_K:
+            raise ValueError(f"cols must be 1..{MX_MAX_K}, got {cols}")
+        kp = -(-cols // MX_PAD) * MX_PAD
+        rows = codes.shape[0] if codes.ndim == 2 else -1
+        for t, width, name in ((codes, kp * bits // 8, "codes"), (scales, kp // MX_BLOCK, "scales")):
             if t.dtype != torch.uint8 or t.ndim != 2 or t.shape[1] != width or not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous uint8 [rows, {width}], got {t.dtype} {tuple(t.shape)}")
-        if self.codes.shape[0] != self.scales.shape[0] or self.codes.device != self.scales.device:
+        if scales.shape[0] != rows or codes.device != scales.device:
             raise ValueError("codes and scales must have the same rows and device")
+        self.codes, self.scales, self.cols, self.bits = codes, scales, cols, bits
+        self.rows, self.device = rows, codes.device
 
-    @property
-    def rows(self) -> int:
-        return self.codes.shape[0]
+    @classmethod
+    def _empty(cls, rows: int, cols: int, bits: int, device) -> "MXTensor":
+        t = cls.__new__(cls)
+        kp = -(-cols // MX_PAD) * MX_PAD
+        t.codes = torch.empty((rows, kp * bits // 8), dtype=torch.uint8, device=device)
+        t.scales = torch.empty((rows, kp // MX_BLOCK), dtype=torch.uint8, device=device)
+        t.cols, t.bits, t.rows, t.device = cols, bits, rows, device
+        return t
 
     @property
     def shape(self) -> tuple[int, int]:
         return (self.rows, self.cols)
 
     @property
-    def device(self) -> torch.device:
-        return self.codes.device
-
-    @property
     def nbytes(self) -> int:
         return self.codes.numel() + self.scales.numel()
 
+    def __repr__(self) -> str:
+        return f"MXTensor({self.rows}x{self.cols}, {self.bits} bits, {self.device})"
 
-def _launch_on(device: torch.device):
-    """The tensors' device as the current one while a kernel is launched (on its current stream)."""
+
+def _launch(device: torch.device, what: str, call, *args) -> None:
+    """``call(*args, stream)`` on the current stream of the tensors' device, which is made the current one."""
     if device.type != "cuda":
-        raise RuntimeError("tensors must be on the device")
-    return contextlib.nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+        raise RuntimeError(f"{what}: tensors must be on the device")
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
+
+
+def _pointers(tensors) -> C.Array:
+    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
 def _same_device(device: torch.device, *tensors) -> None:
@@ -734,66 +748,55 @@ def _same_device(device: torch.device, *tensors) -> None:
             raise ValueError(f"tensors lie on different devices ({t.device}, {device})")
 
 
-def _mx_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as rows [.., K] that follow each other at one stride, values next to each other."""
-    if x.ndim == 0 or x.shape[-1] == 0:
-        raise ValueError("x needs at least one value a row")
-    if x.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"x must be bfloat16 or float32, got {x.dtype}")
-    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.stride(0) < 0:
-        x2 = x2.contiguous()
-    return x2
-
-
 def mx_quantize(x: torch.Tensor, bits: int = 8) -> MXTensor:
     """``x`` [.., K] (bf16 or f32) in a microscaled format of 8 or 4 bits (``fl_mx_quantize``): its
     leading dimensions become the rows.  A block of 32 values that holds a NaN or an infinity reads
     as NaN."""
-    if bits not in (4, 8):
+    if bits != 4 and bits != 8:
         raise ValueError(f"bits must be 4 or 8, got {bits}")
-    x2 = _mx_rows(x)
+    if x.ndim == 0 or not 0 < x.shape[-1] <= MX_MAX_K:
+        raise ValueError(f"x needs at least one value a row, and at most {MX_MAX_K}")
+    f32 = x.dtype == torch.float32
+    if not f32 and x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bfloat16 or float32, got {x.dtype}")
+    x2 = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1:  # (rows may lie at any distance, their values next to each other)
+        x2 = x2.contiguous()
     rows, k = x2.shape
-    if k > MX_MAX_K:
-        raise ValueError(f"rows of more than {MX_MAX_K} values")
-    kp = -(-k // MX_PAD) * MX_PAD
-    with _launch_on(x2.device):
-        codes = torch.empty(rows, kp * bits // 8, dtype=torch.uint8, device=x2.device)
-        scales = torch.empty(rows, kp // MX_BLOCK, dtype=torch.uint8, device=x2.device)
-        if rows:
-            check(load().fl_mx_quantize(x2.data_ptr(), int(x2.dtype == torch.float32), x2.stride(0), rows, k, bits,
-                                        codes.data_ptr(), scales.data_ptr(), _stream()), "fl_mx_quantize")
-    return MXTensor(codes, scales, k, bits)
+    t = MXTensor._empty(rows, k, bits, x2.device)
+    if rows:
+        _launch(t.device, "fl_mx_quantize", load().fl_mx_quantize, x2.data_ptr(), f32, x2.stride(0), rows, k, bits,
+                t.codes.data_ptr(), t.scales.data_ptr())
+    return t
 
 
 def mx_dequantize(t: MXTensor) -> torch.Tensor:
     """The values of ``t`` as bf16 ``[rows, cols]`` (``fl_mx_dequantize``)."""
-    with _launch_on(t.device):
-        out = torch.empty(t.rows, t.cols, dtype=torch.bfloat16, device=t.device)
-        if t.rows:
-            check(load().fl_mx_dequantize(t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.cols, t.bits,
-                                          out.data_ptr(), t.cols, _stream()), "fl_mx_dequantize")
+    out = torch.empty((t.rows, t.cols), dtype=torch.bfloat16, device=t.device)
+    if t.rows:
+        _launch(t.device, "fl_mx_dequantize", load().fl_mx_dequantize, t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.cols,
+                t.bits, out.data_ptr(), t.cols)
     return out
 
 
 def _chain_operands(r, x, w_a, w_f, w_b):
     """The chain's rows as contiguous bf16 [M, D], its gains checked."""
     r2 = _rows2d(r, "r")
-    x2 = None if x is None else _rows2d(x, "x")
-    d = r2.shape[1]
-    if x2 is not None and x2.shape != r2.shape:
-        raise ValueError("x must have the shape of r")
-    if x2 is not None and w_a is None:
-        raise ValueError("x needs its norm weight w_a")
-    for t, name in ((r2, "r"), (x2, "x")):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise ValueError(f"{name} must be bf16")
-    for t, name in ((w_a, "w_a"), (w_f, "w_f"), (w_b, "w_b")):
-        if t is not None:
-            _require(t, torch.bfloat16, name)
-            if t.numel() != d:
-                raise ValueError(f"{name} must have {d} values")
-    _same_device(r2.device, x2, w_a, w_f, w_b)
+    device, d = r2.device, r2.shape[1]
+    if r2.dtype != torch.bfloat16:
+        raise ValueError("r must be bf16")
+    x2 = None
+    if x is not None:
+        x2 = _rows2d(x, "x")
+        if x2.shape != r2.shape or x2.dtype != torch.bfloat16:
+            raise ValueError("x must be bf16 of the shape of r")
+        if w_a is None:
+            raise ValueError("x needs its norm weight w_a")
+        if x2.device != device:
+            raise ValueError("x and r lie on different devices")
+    for w in (w_a, w_f, w_b):
+        if w is not None and (w.dtype != torch.bfloat16 or w.numel() != d or w.device != device or not w.is_contiguous()):
+            raise ValueError(f"norm weights must be {d} contiguous bf16 values on the rows' device")
     return r2, x2
 
 
@@ -802,59 +805,53 @@ def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.
     """``norm_chain`` with its ``z`` as the 8-bit rows that ``mx_matmul`` takes (``fl_norm_chain_mx``):
     ``h = r + RMSNorm_a(x)`` (or ``r``), through ``RMSNorm_f`` where given, and ``z = RMSNorm_b(h)``.
     Returns (h bf16 [M, D] or None, z)."""
-    r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
     if w_b is None:
         raise ValueError("w_b is required")
+    r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
     m, d = r2.shape
-    kp = -(-d // MX_PAD) * MX_PAD
-    with _launch_on(r2.device):
-        h = torch.empty(m, d, dtype=torch.bfloat16, device=r2.device) if want_h else None
-        codes = torch.empty(m, kp, dtype=torch.uint8, device=r2.device)
-        scales = torch.empty(m, kp // MX_BLOCK, dtype=torch.uint8, device=r2.device)
-        check(load().fl_norm_chain_mx(m, d, float(eps), _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), w_b.data_ptr(), _p(h),
-                                      codes.data_ptr(), scales.data_ptr(), d, _stream()) if m else 0, "fl_norm_chain_mx")
-    return h, MXTensor(codes, scales, d, 8)
+    h = torch.empty_like(r2) if want_h else None
+    z = MXTensor._empty(m, d, 8, r2.device)
+    if m:
+        _launch(z.device, "fl_norm_chain_mx", load().fl_norm_chain_mx, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f),
+                w_b.data_ptr(), _p(h), z.codes.data_ptr(), z.scales.data_ptr(), d)
+    return h, z
 
 
 def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out):
-    """Outputs, pointer arrays and checked operands of the 4-bit GEMVs."""
-    if epilogue not in (EPI_PLAIN, EPI_F32, EPI_ADD, EPI_SWIGLU, EPI_ROPE):
-        raise ValueError(f"unknown epilogue {epilogue}")
-    need = {EPI_SWIGLU: 2, EPI_ROPE: 3}.get(epilogue, 1)
-    if len(weights) != need:
-        raise ValueError(f"the epilogue takes {need} weight(s), got {len(weights)}")
+    """(outputs, what the caller holds until the launch, arguments) of the 4-bit GEMVs, checked."""
+    need = 3 if epilogue == EPI_ROPE else (2 if epilogue == EPI_SWIGLU else 1)
+    if not EPI_PLAIN <= epilogue <= EPI_ROPE or len(weights) != need:
+        raise ValueError(f"epilogue {epilogue} with {len(weights)} weight(s)")
     n = weights[0].rows
     for w in weights:
-        if w.bits != 4 or w.cols != k or w.rows != n:
-            raise ValueError(f"weights must be 4-bit [{n}, {k}], got {w.bits}-bit {w.shape}")
-        _same_device(device, w.codes)
-    if not n:
-        raise ValueError("weights have no rows")
+        if w.bits != 4 or w.cols != k or w.rows != n or not n or w.device != device:
+            raise ValueError(f"weights must be 4-bit [{n or 'N'}, {k}] on {device}, got {w}")
     dt = torch.float32 if epilogue == EPI_F32 else torch.bfloat16
-    nout = 3 if epilogue == EPI_ROPE else 1
-    if out is None:
-        outs = [torch.empty(m, n, dtype=dt, device=device) for _ in range(nout)]
-    else:
+    if out is not None:
         _require(out, dt, "out")
-        if nout != 1 or out.shape != (m, n):
-            raise ValueError(f"out must be one [{m}, {n}] tensor")
-        outs = [out]
+        if need == 3 or out.shape != (m, n) or out.device != device:
+            raise ValueError(f"out must be one [{m}, {n}] tensor on {device}")
+        outs = (out,)
+    elif need == 3:
+        outs = torch.empty((3, m, n), dtype=dt, device=device).unbind(0)
+    else:
+        outs = (torch.empty((m, n), dtype=dt, device=device),)
     add = cos = sin = None
     if epilogue == EPI_ADD:
         if addend is None:
             raise ValueError("the epilogue takes an addend")
         add = addend.reshape(m, n)
         _require(add, torch.bfloat16, "addend")
-    if epilogue == EPI_ROPE:
+        _same_device(device, add)
+    elif need == 3:
         if rope is None:
             raise ValueError("the epilogue takes rope tables")
         cos, sin = (t.reshape(m, head_dim).contiguous() for t in rope)
         _require(cos, torch.bfloat16, "rope cos")
         _require(sin, torch.bfloat16, "rope sin")
-    _same_device(device, add, cos, sin, *outs)
-    args = (_ptrs([w.codes for w in weights]), _ptrs([w.scales for w in weights]), n, int(epilogue), _ptrs(outs), n,
-            _p(add), n, _p(cos), _p(sin), int(head_dim))
-    return outs, args, (add, cos, sin)  # (the tensors live until the launch)
+        _same_device(device, cos, sin)
+    return outs, (add, cos, sin), (_pointers([w.codes for w in weights]), _pointers([w.scales for w in weights]), n, epilogue,
+                                   _pointers(outs), n, _p(add), n, _p(cos), _p(sin), head_dim)
 
 
 def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torch.Tensor | None = None,
@@ -867,10 +864,10 @@ def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torc
     m, k = x2.shape
     if not 1 <= m <= 8:
         raise ValueError(f"mx_gemv takes 1 to 8 rows, got {m}")
-    with _launch_on(x2.device):
-        outs, args, held = _mx_gemv_operands(x2.device, m, k, weights, epilogue, addend, rope, head_dim, out)
-        check(load().fl_mx_gemv(x2.data_ptr(), int(x2.dtype == torch.float32), k, m, k, *args, _stream()), "fl_mx_gemv")
-    return tuple(outs) if epilogue == EPI_ROPE else outs[0]
+    device = x2.device
+    outs, held, args = _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out)
+    _launch(device, "fl_mx_gemv", load().fl_mx_gemv, x2.data_ptr(), x2.dtype == torch.float32, k, m, k, *args)
+    return outs if epilogue == EPI_ROPE else outs[0]
 
 
 def mx_gemv_chain(r: torch.Tensor, weights, *, x: torch.Tensor | None = None, w_a: torch.Tensor | None = None,
@@ -885,26 +882,27 @@ def mx_gemv_chain(r: torch.Tensor, weights, *, x: torch.Tensor | None = None, w_
     m, d = r2.shape
     if not 1 <= m <= 8:
         raise ValueError(f"mx_gemv_chain takes 1 to 8 rows, got {m}")
-    with _launch_on(r2.device):
-        outs, args, held = _mx_gemv_operands(r2.device, m, d, weights, epilogue, addend, rope, head_dim, out)
-        h = torch.empty(m, d, dtype=torch.bfloat16, device=r2.device) if want_h else None
-        check(load().fl_mx_gemv_chain(m, d, float(eps), _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), _p(w_b), _p(h), d, *args,
-                                      _stream()), "fl_mx_gemv_chain")
-    return h, (tuple(outs) if epilogue == EPI_ROPE else outs[0])
+    device = r2.device
+    outs, held, args = _mx_gemv_operands(device, m, d, weights, epilogue, addend, rope, head_dim, out)
+    h = torch.empty_like(r2) if want_h else None
+    _launch(device, "fl_mx_gemv_chain", load().fl_mx_gemv_chain, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), _p(w_b),
+            _p(h), d, *args)
+    return h, (outs if epilogue == EPI_ROPE else outs[0])
 
 
 def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ weight.T`` of 8-bit rows [M, K] and 4-bit weights [N, K] (``fl_mx_matmul``): fp32 sums,
     returned as bf16 or f32 [M, N].  Any number of rows."""
     if x.bits != 8 or weight.bits != 4 or x.cols != weight.cols:
-        raise ValueError(f"takes 8-bit rows and 4-bit weights of one K, got {x.bits}-bit {x.shape}, {weight.bits}-bit {weight.shape}")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"takes 8-bit rows and 4-bit weights of one K, got {x} and {weight}")
+    f32 = out_dtype == torch.float32
+    if not f32 and out_dtype != torch.bfloat16:
         raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
-    _same_device(x.device, weight.codes)
-    with _launch_on(x.device):
-        y = torch.empty(x.rows, weight.rows, dtype=out_dtype, device=x.device)
-        if y.numel():
-            check(load().fl_mx_matmul(x.codes.data_ptr(), x.scales.data_ptr(), x.rows, x.cols, weight.codes.data_ptr(),
-                                      weight.scales.data_ptr(), weight.rows, y.data_ptr(), int(out_dtype == torch.float32),
-                                      weight.rows, _stream()), "fl_mx_matmul")
+    device, m, n = x.device, x.rows, weight.rows
+    if weight.device != device:
+        raise ValueError(f"x and weight lie on different devices ({device}, {weight.device})")
+    y = torch.empty((m, n), dtype=out_dtype, device=device)
+    if m and n:
+        _launch(device, "fl_mx_matmul", load().fl_mx_matmul, x.codes.data_ptr(), x.scales.data_ptr(), m, x.cols,
+                weight.codes.data_ptr(), weight.scales.data_ptr(), n, y.data_ptr(), f32, n)
     return y
