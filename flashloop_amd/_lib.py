@@ -115,9 +115,10 @@ SIGNATURES = {
     "fl_mx_quantize": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
     "fl_mx_dequantize": (_I32, [_P, _P, _I64, _I32, _I32, _P, _I64, _P]),
     "fl_norm_chain_mx": (_I32, [_I32, _I32, _F64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
-    "fl_mx_gemv": (_I32, [_P, _I32, _I64, _I32, _I32, _PP, _PP, _I32, _I32, _PP, _I64, _P, _I64, _P, _P, _I32, _P]),
-    "fl_mx_gemv_chain": (_I32, [_I32, _I32, _F32, _P, _P, _P, _P, _P, _P, _I64, _PP, _PP, _I32, _I32, _PP, _I64, _P,
-                                _I64, _P, _P, _I32, _P]),
+    # (the pointer arrays of these two as addresses: one array holds all three)
+    "fl_mx_gemv": (_I32, [_P, _I32, _I64, _I32, _I32, _P, _P, _I32, _I32, _P, _I64, _P, _I64, _P, _P, _I32, _P]),
+    "fl_mx_gemv_chain": (_I32, [_I32, _I32, _F32, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _P, _I64,
+                                _P, _P, _I32, _P]),
     "fl_mx_matmul": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I64, _P]),
 }
 

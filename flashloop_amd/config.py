@@ -17,6 +17,7 @@ class FlashLoopConfig:
     enable_sparse_decode: bool = True
     quantize_cross_loop_kv: bool = True
     decode_capacity: int = 4096  # packed-prefix room reserved for decode tokens
+    weight_bits: int = 16  # Linear weights: bf16, or a microscaled copy of 4 bits
 
     def __post_init__(self) -> None:
         if not 0.0 < self.prefill_fraction_loop4 <= self.prefill_fraction_loop3 <= 1.0:
@@ -34,6 +35,8 @@ class FlashLoopConfig:
         for name in ("enable_token_sparse_prefill", "enable_sparse_decode"):
             if not isinstance(getattr(self, name), bool):
                 raise TypeError(f"{name} takes True or False, got {getattr(self, name)!r}")
+        if self.weight_bits not in (4, 16):
+            raise ValueError(f"weight_bits={self.weight_bits}: Linear weights are bf16 (16) or microscaled (4)")
         if self.decode_capacity < 0:
             raise ValueError(f"decode_capacity={self.decode_capacity} is negative")
 

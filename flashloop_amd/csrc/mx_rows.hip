@@ -229,7 +229,7 @@ __global__ __launch_bounds__(kNormThreads<W>) void norm_chain_mx_kernel(NormMxAr
   const bool in = t < nq;
   const uint4 wa = ADD && in ? reinterpret_cast<const uint4*>(a.wa)[t] : make_uint4(0, 0, 0, 0);
   const uint4 wf = FINAL && in ? reinterpret_cast<const uint4*>(a.wf)[t] : make_uint4(0, 0, 0, 0);
-  const uint4 wb = in ? reinterpret_cast<const uint4*>(a.wb)[t] : make_uint4(0, 0, 0, 0);
+  const uint4 wb = in && a.wb ? reinterpret_cast<const uint4*>(a.wb)[t] : make_uint4(0, 0, 0, 0);
   const double inv_d = 1.0 / static_cast<double>(a.d);
   const auto inv_rms = [&](double ss) { return rsqrt(fma(sum(ss), inv_d, a.eps)); };
   const auto request = [&](int64_t row, uint4& rr, uint4& xx) {
@@ -279,27 +279,29 @@ __global__ __launch_bounds__(kNormThreads<W>) void norm_chain_mx_kernel(NormMxAr
       r = pack_bf16x8(o);
     }
     if (a.h_out != nullptr && live && in) reinterpret_cast<uint4*>(a.h_out + row * a.stride)[t] = r;
-    // (0 past the row, also where the row's statistics are not finite)
-    const double ib = inv_rms(squares(r)), scale = in ? ib : 0.0;
-    float fh[8], fw[8], z[8];
-    double v[8];
-    unpack_bf16x8(r, fh);
-    unpack_bf16x8(wb, fw);
+    if (a.wb != nullptr) {
+      // (0 past the row, also where the row's statistics are not finite)
+      const double ib = inv_rms(squares(r)), scale = in ? ib : 0.0;
+      float fh[8], fw[8], z[8];
+      double v[8];
+      unpack_bf16x8(r, fh);
+      unpack_bf16x8(wb, fw);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * scale;
-    const f32x8_t rounded = round8_for_codes(v);
+      for (int e = 0; e < 8; ++e) v[e] = static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * scale;
+      const f32x8_t rounded = round8_for_codes(v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = rounded[e];
-    uint32_t peak = 0;
+      for (int e = 0; e < 8; ++e) z[e] = rounded[e];
+      uint32_t peak = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
-    peak = quad_max_u(peak);
-    if (t < a.per_row && live) {  // (whole quads)
-      const uint32_t code = mx_scale_code<8>(peak);
-      const uint2 q = mx_encode8(z, mx_scale(code));
-      const int64_t piece = row * a.per_row + t;
-      reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
-      if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+      for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
+      peak = quad_max_u(peak);
+      if (t < a.per_row && live) {  // (whole quads)
+        const uint32_t code = mx_scale_code<8>(peak);
+        const uint2 q = mx_encode8(z, mx_scale(code));
+        const int64_t piece = row * a.per_row + t;
+        reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
+        if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+      }
     }
     r = nr;
     if constexpr (ADD) x = nx;
@@ -406,7 +408,9 @@ extern "C" int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint
   clear_error();
   FL_REQUIRE(m >= 0 && d > 0 && d % 8 == 0 && d <= 8192 && stride >= d && stride % 8 == 0,
              "fl_norm_chain_mx: d must be a multiple of 8 up to 8192 and the row stride a multiple of 8");
-  FL_REQUIRE(r && w_b && z_codes && z_scales, "fl_norm_chain_mx: r, w_b and the outputs of z are required");
+  FL_REQUIRE(r != nullptr, "fl_norm_chain_mx: null residual/input");
+  FL_REQUIRE(w_b == nullptr || (z_codes && z_scales), "fl_norm_chain_mx: z needs its outputs");
+  FL_REQUIRE(w_b || h_out, "fl_norm_chain_mx: nothing to write");
   FL_REQUIRE(x == nullptr || w_a != nullptr, "fl_norm_chain_mx: x needs its norm weight");
   for (const void* p : {static_cast<const void*>(x), static_cast<const void*>(r), static_cast<const void*>(w_a),
                         static_cast<const void*>(w_f), static_cast<const void*>(w_b),

@@ -15,6 +15,11 @@ on this build's HIP kernels:
 The prefill's contractions with the weights are library GEMMs (hipBLASLt); its attention
 (``fl_prefill_attention``), rotary embedding and K/V placement (``fl_rope_store``), norms and
 residuals (``fl_norm_chain``) and SwiGLU (``fl_swiglu``) are HIP kernels.
+
+With ``FlashLoopConfig(weight_bits=4)`` every Linear layer runs on a microscaled 4-bit copy of its
+weights (a looped model reads each weight once per loop): prompt rows, and decode steps of more than
+8 sequences, in 8 bits through ``fl_norm_chain_mx``, ``fl_mx_quantize`` and ``fl_mx_matmul``, smaller
+decode steps in bf16 through ``fl_mx_gemv[_chain]``.
 """
 
 from __future__ import annotations
@@ -54,6 +59,31 @@ def _is_plain(m: torch.nn.Module, kind: type) -> bool:
     """Whether calling ``m`` runs the ``forward`` that ``kind`` was defined with and nothing else: no
     subclass, no ``forward`` replaced on the instance or the class, no hook on it or on every module."""
     return _is_bare(m, kind) and _calls_are_plain()
+
+
+def _mx_rows_gemv(x, weights, *, epilogue=kernels.EPI_PLAIN, addend=None, rope=None, head_dim=kernels.HEAD_DIM, out=None):
+    """``kernels.mx_gemv`` for any number of rows (``x``: rows, or an 8-bit ``MXTensor``): 8-bit rows and
+    ``mx_matmul``."""
+    if not isinstance(x, kernels.MXTensor):
+        x = kernels.mx_quantize(x, 8)
+    if epilogue == kernels.EPI_F32:
+        y = kernels.mx_matmul(x, weights[0], out_dtype=torch.float32)
+        return y if out is None else out.copy_(y)
+    ys = [kernels.mx_matmul(x, w) for w in weights]
+    if epilogue == kernels.EPI_ADD:
+        return ys[0] + addend.reshape(ys[0].shape)
+    if epilogue == kernels.EPI_SWIGLU:
+        return kernels.swiglu(*ys) if ys[0].numel() % 8 == 0 else F.silu(ys[0]) * ys[1]
+    if epilogue == kernels.EPI_ROPE:
+        q, k, v = (y.view(y.shape[0], -1, 1, head_dim) for y in ys)
+        return (*(t.reshape(ys[0].shape) for t in apply_rope(q, k, *(t[:, None] for t in rope))), ys[2])
+    return ys[0]
+
+
+def _mx_rows_gemv_chain(r, weights, *, x=None, w_a=None, w_f=None, w_b=None, eps, want_h=True, **gemv):
+    """``kernels.mx_gemv_chain`` for any number of rows."""
+    h, z = kernels.norm_chain_mx(r, x=x, w_a=w_a, w_f=w_f, w_b=w_b, eps=eps, want_h=want_h or w_b is None)
+    return h, _mx_rows_gemv(h if z is None else z, weights, **gemv)
 
 
 @dataclass(frozen=True)
@@ -243,6 +273,50 @@ class FlashLoopEngine:
         # consumes it (False: separate fl_norm_chain launches; same results bit for bit)
         self.fused_chain = True
         self._wcache = None
+        self._mx = None  # weight_bits=4: (per layer, norm and lm_head) as _fused_weights gives them
+        if self.config.weight_bits == 4:
+            self.quantize_weights()
+
+    def quantize_weights(self) -> None:
+        """Make the 4-bit copies of the Linear weights that this engine runs on (``weight_bits=4``), anew
+        after the model's weights have changed.  The model keeps its own."""
+        if self.config.weight_bits != 4:
+            raise ValueError("quantize_weights needs FlashLoopConfig(weight_bits=4)")
+
+        def linear(m):
+            if not _is_plain(m, torch.nn.Linear) or m.bias is not None:
+                raise ValueError("weight_bits=4 needs plain Linear layers without a bias")
+            return kernels.mx_quantize(m.weight.detach(), 4)
+
+        def norm(m):
+            w = m.weight.detach() if _is_plain(m, RMSNorm) else None
+            if (w is None or w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16
+                    or m.eps != self.backbone.norm.eps):
+                raise ValueError("weight_bits=4 needs plain bf16 RMSNorm layers of one eps")
+            return w
+
+        hidden = self.backbone.norm.weight.numel()
+        if hidden % 8 or hidden > 8192 or any(l.mlp.up_proj.weight.shape[0] % 8 for l in self.layers):
+            raise ValueError("weight_bits=4 needs a hidden width up to 8192 and an MLP width, multiples of 8")
+        layers = []
+        for layer in self.layers:
+            a, m = layer.self_attn, layer.mlp
+            if not _is_bare(m, MLP):
+                raise ValueError("weight_bits=4 needs plain MLP modules")
+            layers.append(dict(q=linear(a.q_proj), k=linear(a.k_proj), v=linear(a.v_proj), o=linear(a.o_proj),
+                               gate=linear(m.gate_proj), up=linear(m.up_proj), down=linear(m.down_proj),
+                               ln1=norm(layer.input_layernorm), ln2=norm(layer.input_layernorm_2),
+                               ln3=norm(layer.post_attention_layernorm), ln4=norm(layer.post_attention_layernorm_2)))
+        self._mx = (layers, dict(norm=norm(self.backbone.norm), lm_head=linear(self.model.lm_head)))
+        self._runner.reset()  # (captured steps hold the old copies)
+
+    def _lm_head(self, h: torch.Tensor) -> torch.Tensor:
+        """Logits f32 of hidden rows [.., hidden]."""
+        if self._mx is None:
+            return self.model.lm_head(h).float()
+        rows = h.reshape(-1, h.shape[-1])
+        product = kernels.mx_gemv if rows.shape[0] <= 8 else _mx_rows_gemv
+        return product(rows, [self._mx[1]["lm_head"]], epilogue=kernels.EPI_F32).view(*h.shape[:-1], -1)
 
     @classmethod
     def from_pretrained(cls, model_path: str, *, config: FlashLoopConfig | None = None,
@@ -332,6 +406,19 @@ class FlashLoopEngine:
             layers.append(w)
         return (layers, float(eps.pop())) if len(eps) == 1 else None
 
+    def _mx_layer_rows(self, w, hid, z, rope, kv, positions, eps, w_next, w_final):
+        """``_layer_rows`` on 4-bit weights; ``z`` and the input norm that it returns are 8-bit rows."""
+        q, k, v = (kernels.mx_matmul(z, w[n]) for n in ("q", "k", "v"))
+        kernels.rope_store(q, k, v, rope, kv[0], kv[1], positions)
+        heads = kv[0].shape[0]
+        o = kernels.prefill_attention(q.view(q.shape[0], heads, -1).transpose(0, 1), kv[0], kv[1],
+                                      kv[0].shape[-1] ** -0.5, positions)
+        x = kernels.mx_matmul(kernels.mx_quantize(o, 8), w["o"])
+        hid, z = kernels.norm_chain_mx(hid, x=x, w_a=w["ln2"], w_b=w["ln3"], eps=eps)
+        act = kernels.swiglu(kernels.mx_matmul(z, w["gate"]), kernels.mx_matmul(z, w["up"]))
+        y = kernels.mx_matmul(kernels.mx_quantize(act, 8), w["down"])
+        return kernels.norm_chain_mx(hid, x=y, w_a=w["ln4"], w_f=w_final, w_b=w_next, eps=eps)
+
     def _layer_rows(self, weights, hid, z, rope, kv, positions, eps, w_next, w_final):
         """One prefill layer over rows ``hid`` [n, hidden] whose input norm is ``z``: K/V rows into
         ``kv`` ([H, T, 128] each, at ``positions`` or 0..n-1), attention up to each row's own
@@ -351,6 +438,14 @@ class FlashLoopEngine:
     def _rows_loop(self, weights, rows, rope, kv, positions):
         """Every layer over ``rows`` [n, hidden], then the final norm."""
         layers, eps = weights
+        if self._mx is not None:
+            layers = self._mx[0]
+            hid, (_, z) = rows, kernels.norm_chain_mx(rows, w_b=layers[0]["ln1"], eps=eps, want_h=False)
+            for li, w in enumerate(layers):
+                last = li == len(layers) - 1
+                hid, z = self._mx_layer_rows(w, hid, z, rope, kv[li], positions, eps, None if last else layers[li + 1]["ln1"],
+                                             self._mx[1]["norm"] if last else None)
+            return hid
         hid, (_, z) = rows, kernels.norm_chain(rows, w_b=layers[0][7], eps=eps, want_h=False)
         for li, w in enumerate(layers):
             last = li == len(layers) - 1
@@ -358,10 +453,16 @@ class FlashLoopEngine:
                                       self.backbone.norm.weight if last else None)
         return hid
 
+    def _refuse_modules(self) -> None:
+        """The module path multiplies by the modules' own weights, which ``weight_bits=4`` does not."""
+        if self._mx is not None:
+            raise RuntimeError("weight_bits=4: a module was replaced or hooked, or gives rows in a layout the kernels do not read")
+
     def _dense_loop(self, hidden: torch.Tensor, cos, sin):
         """``dense_prefill_loop`` (flashloop/prefill.py:275-304): every row, causal attention."""
         weights = self._prefill_weights(hidden, cos, sin)
         if weights is None:
+            self._refuse_modules()
             return self._dense_loop_modules(hidden, cos, sin)
         _, t, d = hidden.shape
         a = self.layers[0].self_attn
@@ -376,6 +477,7 @@ class FlashLoopEngine:
         recomputed; their K/V replace the previous loop's rows of a composite cache."""
         weights = self._prefill_weights(hidden, cos, sin)
         if weights is None:
+            self._refuse_modules()
             return self._sparse_loop_modules(hidden, positions, prev_keys, prev_values, cos, sin)
         keys = [k.clone() for k in prev_keys]
         values = [v.clone() for v in prev_values]
@@ -463,7 +565,7 @@ class FlashLoopEngine:
         stage("loop4_sparse")
         receipts = (PrefillReceipt(1, t, t), PrefillReceipt(2, t, t), PrefillReceipt(3, t, pos3.numel()),
                     PrefillReceipt(4, t, pos4.numel()))
-        logits = self.model.lm_head(h4 if all_logits else h4[:, -1]).float()
+        logits = self._lm_head(h4 if all_logits else h4[:, -1])
         return _PrefillLoops([k1, k2, k3, k4], [v1, v2, v3, v4], mask3, mask4, receipts, logits)
 
     @torch.inference_mode()
@@ -508,7 +610,7 @@ class FlashLoopEngine:
         """One decode step (see ``_decode_core_fused``); the torch-module form runs when the
         fused kernels do not apply (``fused_decode`` off, non-bf16 weights, batch > 8).  The
         fused form writes the logits to ``out`` if given."""
-        if self.fused_decode and token_ids.shape[0] <= 8 and self._fused_weights() is not None:
+        if self._mx is not None or (self.fused_decode and token_ids.shape[0] <= 8 and self._fused_weights() is not None):
             return self._decode_core_fused(cache, *self._decode_inputs(token_ids, pos_t), logits_out=out)
         return self._decode_core_modules(cache, self.backbone.embed_tokens(token_ids), pos_t)
 
@@ -527,7 +629,9 @@ class FlashLoopEngine:
 
     def _fused_weights(self):
         """Per-layer weight tensors of the fused decode path, or None when a weight is not a
-        contiguous bf16 device tensor."""
+        contiguous bf16 device tensor; with ``weight_bits=4`` the 4-bit copies."""
+        if self._mx is not None:
+            return self._mx
         if self._wcache is None:
             def ok(t):
                 return t.dtype == torch.bfloat16 and t.is_cuda and t.is_contiguous()
@@ -565,6 +669,13 @@ class FlashLoopEngine:
         rope = (cos.reshape(bsz, hd), sin.reshape(bsz, hd))
         hid = h.reshape(bsz, -1)
         chained = self.fused_chain
+        gemv, gemv_chain = kernels.gemv, kernels.gemv_chain
+        if self._mx is not None:
+            gemv, gemv_chain = kernels.mx_gemv, kernels.mx_gemv_chain
+            if bsz > 8:
+                gemv, gemv_chain, chained = _mx_rows_gemv, _mx_rows_gemv_chain, True
+            elif hid.shape[1] > 4096:  # (the longest row that the chained GEMV takes)
+                chained = False
         # the chain whose output feeds the next GEMV: kwargs of norm_chain (h = hid + n_a(x),
         # optional final norm, z = n_b(h)); it runs inside that GEMV when chained
         pending = dict(w_b=layers_w[0]["ln1"])
@@ -573,10 +684,10 @@ class FlashLoopEngine:
         def chain_gemv(weights, **gk):
             nonlocal hid, first
             if chained:
-                h_new, y = kernels.gemv_chain(hid, weights, eps=eps, want_h=not first, **pending, **gk)
+                h_new, y = gemv_chain(hid, weights, eps=eps, want_h=not first, **pending, **gk)
             else:
                 h_new, z = kernels.norm_chain(hid, eps=eps, want_h=not first, **pending)
-                y = kernels.gemv(h_new if pending.get("w_b") is None else z, weights, **gk)
+                y = gemv(h_new if pending.get("w_b") is None else z, weights, **gk)
             if not first:
                 hid = h_new
             first = False
@@ -601,7 +712,7 @@ class FlashLoopEngine:
                     else:
                         out, _ = lc.dense_source_attention(loop, query=q, current_key=k, current_value=v,
                                                            scaling=a.scaling, return_logits=False)
-                    projected = kernels.gemv(out.reshape(bsz, -1), [w["o"]])
+                    projected = gemv(out.reshape(bsz, -1), [w["o"]])
                     if loop == 1 and sparse:
                         sources[li] = _LayerSource(projected, idx, valid, mass, sw, v, counts=cnt)
                 else:
@@ -617,11 +728,11 @@ class FlashLoopEngine:
                             loop, query=q, current_key=k, current_value=v, indices=src.indices, valid=src.valid,
                             source_selected_output=src.selected_output, global_mass=src.global_mass,
                             scaling=a.scaling, counts=src.counts)
-                    projected = kernels.gemv(delta.reshape(bsz, -1), [w["o"]], epilogue=kernels.EPI_ADD,
+                    projected = gemv(delta.reshape(bsz, -1), [w["o"]], epilogue=kernels.EPI_ADD,
                                              addend=src.projected_output)
                 pending = dict(x=projected, w_a=w["ln2"], w_b=w["ln3"])
                 act = chain_gemv([w["gate"], w["up"]], epilogue=kernels.EPI_SWIGLU)
-                mo = kernels.gemv(act, [w["down"]])
+                mo = gemv(act, [w["down"]])
                 last = li == nl - 1
                 nxt = None if (last and loop == 3) else layers_w[(li + 1) % nl]["ln1"]
                 pending = dict(x=mo, w_a=w["ln4"], w_f=extra["norm"] if last else None, w_b=nxt)

@@ -17,6 +17,8 @@ context both entry points of the model are routed through ``FlashLoopEngine``:
   with one token decodes one step on it (logits ``[1, 1, vocab]``);
 * ``model.generate(input_ids, max_new_tokens=...)`` is greedy generation on the engine.
 
+``flashloop(model, weight_bits=4)`` runs the Linear layers on microscaled 4-bit copies of their weights.
+
 Arguments the engine cannot honour raise (``TypeError`` for unknown ones, ``ValueError``
 for unsupported values) instead of being dropped.  The audit counters count what the
 engine actually ran (its prefill receipts, decode receipts and cache updates), and the
@@ -180,9 +182,10 @@ def _all_ones(mask) -> bool:
 
 
 @contextmanager
-def flashloop(model, *, attention_fraction: float = 0.10, fraction_loop3: float = 0.25, fraction_loop4: float = 0.10):
+def flashloop(model, *, attention_fraction: float = 0.10, fraction_loop3: float = 0.25, fraction_loop4: float = 0.10,
+              weight_bits: int = 16):
     config = FlashLoopConfig(prefill_fraction_loop3=fraction_loop3, prefill_fraction_loop4=fraction_loop4,
-                             decode_key_fraction=attention_fraction)
+                             decode_key_fraction=attention_fraction, weight_bits=weight_bits)
     engine = FlashLoopEngine(model, config=config)
     joint = TokenSparsePrefillCachedMassIntervention(engine, attention_fraction, fraction_loop3, fraction_loop4)
     kv = CrossLoopKVQuantizationIntervention(engine)

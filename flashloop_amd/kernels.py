@@ -738,14 +738,10 @@ def _launch(device: torch.device, what: str, call, *args) -> None:
         check(rc, what)
 
 
-def _pointers(tensors) -> C.Array:
-    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-
-
-def _same_device(device: torch.device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors lie on different devices ({t.device}, {device})")
+def _contiguous_rows(x: torch.Tensor) -> torch.Tensor:
+    if x.ndim != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def mx_quantize(x: torch.Tensor, bits: int = 8) -> MXTensor:
@@ -781,39 +777,37 @@ def mx_dequantize(t: MXTensor) -> torch.Tensor:
 
 def _chain_operands(r, x, w_a, w_f, w_b):
     """The chain's rows as contiguous bf16 [M, D], its gains checked."""
-    r2 = _rows2d(r, "r")
+    r2, x2 = _contiguous_rows(r), None
     device, d = r2.device, r2.shape[1]
-    if r2.dtype != torch.bfloat16:
+    if r2.dtype is not torch.bfloat16:
         raise ValueError("r must be bf16")
-    x2 = None
     if x is not None:
-        x2 = _rows2d(x, "x")
-        if x2.shape != r2.shape or x2.dtype != torch.bfloat16:
-            raise ValueError("x must be bf16 of the shape of r")
+        x2 = _contiguous_rows(x)
+        if x2.shape != r2.shape or x2.dtype is not torch.bfloat16 or x2.device != device:
+            raise ValueError("x must be bf16 of the shape of r, on its device")
         if w_a is None:
             raise ValueError("x needs its norm weight w_a")
-        if x2.device != device:
-            raise ValueError("x and r lie on different devices")
     for w in (w_a, w_f, w_b):
-        if w is not None and (w.dtype != torch.bfloat16 or w.numel() != d or w.device != device or not w.is_contiguous()):
+        if w is not None and (w.dtype is not torch.bfloat16 or w.numel() != d or w.device != device or not w.is_contiguous()):
             raise ValueError(f"norm weights must be {d} contiguous bf16 values on the rows' device")
     return r2, x2
 
 
 def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.Tensor | None = None,
-                  w_f: torch.Tensor | None = None, w_b: torch.Tensor, eps: float, want_h: bool = True):
+                  w_f: torch.Tensor | None = None, w_b: torch.Tensor | None = None, eps: float, want_h: bool = True):
     """``norm_chain`` with its ``z`` as the 8-bit rows that ``mx_matmul`` takes (``fl_norm_chain_mx``):
     ``h = r + RMSNorm_a(x)`` (or ``r``), through ``RMSNorm_f`` where given, and ``z = RMSNorm_b(h)``.
-    Returns (h bf16 [M, D] or None, z)."""
-    if w_b is None:
-        raise ValueError("w_b is required")
+    Returns (h bf16 [M, D] or None, z or None)."""
+    if w_b is None and not want_h:
+        raise ValueError("nothing to return: neither h nor w_b")
     r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
     m, d = r2.shape
     h = torch.empty_like(r2) if want_h else None
-    z = MXTensor._empty(m, d, 8, r2.device)
+    z = None if w_b is None else MXTensor._empty(m, d, 8, r2.device)
     if m:
-        _launch(z.device, "fl_norm_chain_mx", load().fl_norm_chain_mx, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f),
-                w_b.data_ptr(), _p(h), z.codes.data_ptr(), z.scales.data_ptr(), d)
+        codes, scales = (None, None) if z is None else (z.codes.data_ptr(), z.scales.data_ptr())
+        _launch(r2.device, "fl_norm_chain_mx", load().fl_norm_chain_mx, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f),
+                _p(w_b), _p(h), codes, scales, d)
     return h, z
 
 
@@ -840,18 +834,25 @@ def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, o
     if epilogue == EPI_ADD:
         if addend is None:
             raise ValueError("the epilogue takes an addend")
-        add = addend.reshape(m, n)
-        _require(add, torch.bfloat16, "addend")
-        _same_device(device, add)
+        add = _operand(addend, m, n, "addend", device)
     elif need == 3:
         if rope is None:
             raise ValueError("the epilogue takes rope tables")
-        cos, sin = (t.reshape(m, head_dim).contiguous() for t in rope)
-        _require(cos, torch.bfloat16, "rope cos")
-        _require(sin, torch.bfloat16, "rope sin")
-        _same_device(device, cos, sin)
-    return outs, (add, cos, sin), (_pointers([w.codes for w in weights]), _pointers([w.scales for w in weights]), n, epilogue,
-                                   _pointers(outs), n, _p(add), n, _p(cos), _p(sin), head_dim)
+        cos, sin = (_operand(t, m, head_dim, "rope table", device) for t in rope)
+    # one array of pointers: codes, scales, outputs
+    table = (C.c_void_p * (2 * need + len(outs)))(*[w.codes.data_ptr() for w in weights], *[w.scales.data_ptr() for w in weights],
+                                                  *[o.data_ptr() for o in outs])
+    at = C.addressof(table)
+    return outs, (add, cos, sin, table), (at, at + 8 * need, n, epilogue, at + 16 * need, n, _p(add), n, _p(cos), _p(sin), head_dim)
+
+
+def _operand(t: torch.Tensor, m: int, n: int, name: str, device) -> torch.Tensor:
+    """An epilogue's bf16 [m, n] (or of as many values)."""
+    if t.shape != (m, n):
+        t = t.reshape(m, n)
+    if t.dtype is not torch.bfloat16 or t.device != device:
+        raise ValueError(f"{name} must be bfloat16 on {device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torch.Tensor | None = None,
@@ -860,13 +861,15 @@ def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torc
     """``gemv`` with 4-bit weights (``fl_mx_gemv``): ``x`` [.., K] of 1 to 8 bf16 rows (f32 is rounded
     to bf16 first), ``weights`` a list of 4-bit ``MXTensor`` [N, K].  Sums and epilogues are fp32 and
     rounded once; EPI_F32 returns the sums.  Returns [M, N], or (q, k, v) for EPI_ROPE."""
-    x2 = _rows2d(x, "x")
+    x2 = _contiguous_rows(x)
     m, k = x2.shape
     if not 1 <= m <= 8:
         raise ValueError(f"mx_gemv takes 1 to 8 rows, got {m}")
-    device = x2.device
+    device, f32 = x2.device, x2.dtype is torch.float32
+    if not f32 and x2.dtype is not torch.bfloat16:
+        raise ValueError("x must be bf16 or f32")
     outs, held, args = _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out)
-    _launch(device, "fl_mx_gemv", load().fl_mx_gemv, x2.data_ptr(), x2.dtype == torch.float32, k, m, k, *args)
+    _launch(device, "fl_mx_gemv", load().fl_mx_gemv, x2.data_ptr(), f32, k, m, k, *args)
     return outs if epilogue == EPI_ROPE else outs[0]
 
 

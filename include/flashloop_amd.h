@@ -558,7 +558,8 @@ int32_t fl_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64
  * w_f: h = RMSNorm_f(h); h_out (optional) = bf16(h); z = RMSNorm_b(bf16(h)), quantised as above from
  * its unrounded value.  Sums and products are in 64 bits and only h and z are rounded (fl_norm_chain
  * rounds every norm and the sum to bf16, as the modules do).  bf16
- * tensors with row stride `stride`, d % 8 == 0, d <= 8192, 16-byte aligned; w_b is required.
+ * tensors with row stride `stride`, d % 8 == 0, d <= 8192, 16-byte aligned; without
+ * w_b there is no z.
  */
 int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_stride, int64_t rows, int32_t k,
                        int32_t bits, uint8_t* codes, uint8_t* scales, void* stream);

@@ -175,6 +175,9 @@ def test_norm_chain_mx(rows, d, add, final):
     _same_bytes(z, *mx.quantize(want_z, 8))
     none, z2 = kernels.norm_chain_mx(**s, eps=EPS, want_h=False)
     assert none is None and torch.equal(z2.codes, z.codes) and torch.equal(z2.scales, z.scales)
+    s.pop("w_b")
+    h2, none = kernels.norm_chain_mx(**s, eps=EPS)
+    assert none is None and torch.equal(h2, h)
 
 
 def test_norm_chain_mx_odd_rows():
@@ -471,7 +474,7 @@ def test_front_end_refusals_on_the_device():
                 lambda: kernels.mx_gemv(x, [w], epilogue=kernels.EPI_ADD), lambda: kernels.mx_gemv(x, [w, w, w], epilogue=kernels.EPI_ROPE),
                 lambda: kernels.mx_gemv(x, [kernels.mx_quantize(x, 8)]), lambda: kernels.mx_gemv(x.cpu().to(DEV), [w], out=gain),
                 lambda: kernels.norm_chain_mx(x, x=x, w_b=gain, eps=EPS), lambda: kernels.norm_chain_mx(x, w_b=gain[:56], eps=EPS),
-                lambda: kernels.norm_chain_mx(x, w_b=gain.float(), eps=EPS), lambda: kernels.norm_chain_mx(x, w_b=None, eps=EPS),
+                lambda: kernels.norm_chain_mx(x, w_b=gain.float(), eps=EPS), lambda: kernels.norm_chain_mx(x, eps=EPS, want_h=False),
                 lambda: kernels.mx_gemv_chain(x, [w], x=x[:1], w_a=gain, eps=EPS)):
         with pytest.raises(ValueError):
             bad()

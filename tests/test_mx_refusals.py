@@ -103,10 +103,10 @@ def test_c_abi_refusals():
     says(n(d=8200, stride=8200), b"up to 8192")
     says(n(stride=56), b"stride")
     says(n(m=-1), b"multiple of 8")
-    says(n(r=None), b"required")
-    says(n(wb=None), b"required")
-    says(n(codes=None), b"required")
-    says(n(scales=None), b"required")
+    says(n(r=None), b"null")
+    says(n(wb=None), b"nothing to write")
+    says(n(codes=None), b"outputs")
+    says(n(scales=None), b"outputs")
     says(n(x=0x500), b"norm weight")
     says(n(r=0x108), b"16-byte")
     says(n(h=0x508), b"16-byte")
@@ -176,3 +176,11 @@ def test_c_abi_gemv_refusals():
     says(chain(r=0x108), b"16-byte")
     says(chain(h=0x208), b"16-byte")
     says(chain(m=9), b"1..8")
+
+
+def test_weight_bits_is_16_or_4():
+    from flashloop_amd import FlashLoopConfig
+
+    assert FlashLoopConfig().weight_bits == 16 and FlashLoopConfig(weight_bits=4).weight_bits == 4
+    with pytest.raises(ValueError, match="weight_bits"):
+        FlashLoopConfig(weight_bits=8)
