@@ -255,15 +255,16 @@ struct MxWeights {
 };
 
 template <int MT, int NT, int CS>
-__device__ __forceinline__ void mx_load_weights(const MxRows<NT>& r, uint32_t blocks, uint32_t b0, MxWeights<NT, CS>& w) {
+__device__ __forceinline__ void mx_load_weights(const MxRows<NT>& r, uint32_t row_blocks, uint32_t blocks, uint32_t b0,
+                                                MxWeights<NT, CS>& w) {
 #pragma unroll
   for (int s = 0; s < CS; ++s) {
     const uint32_t b = b0 + s * (kMxStep / kMxBlock);
     const bool in = b < blocks;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      w.w[t][s] = buf_load16(r.codes[t], in ? (r.row[t] * blocks + b) * 16u : kOutside);
-      w.s[t][s] = __builtin_amdgcn_raw_buffer_load_b8(r.scales[t], static_cast<int>(in ? r.row[t] * blocks + b : kOutside), 0, 0);
+      w.w[t][s] = buf_load16(r.codes[t], in ? (r.row[t] * row_blocks + b) * 16u : kOutside);
+      w.s[t][s] = __builtin_amdgcn_raw_buffer_load_b8(r.scales[t], static_cast<int>(in ? r.row[t] * row_blocks + b : kOutside), 0, 0);
     }
   }
 }
@@ -330,22 +331,36 @@ __device__ __forceinline__ void mx_store(const MxGemvArgs& a, int u, int g, int 
 }
 
 // CS: steps of 2048 k whose weights are in registers together; K past CS of them goes round again
-// (LOOP).  MT: rows of x (1, or up to 8).  NT: tiles of a workgroup.
-template <int EPI, int MT, int CS, int NT, bool CHAIN, bool LOOP>
-__global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemvArgs a, NormArgs c) {
+// (LOOP).  MT: rows of x (1, or up to 8).  NT: tiles of a unit.  DEPTH: units whose weights are in flight (1: a
+// workgroup a unit; 2: a workgroup takes several, and the next one's weights are requested before the
+// products of the one in hand).
+template <int EPI, int MT, int CS, int NT, bool CHAIN, bool LOOP, int DEPTH>
+__global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemvArgs a, NormArgs c, int units) {
   using G = MxGeom<MT>;
+  static_assert(!LOOP || DEPTH == 1);
   constexpr int kCap = CS * kMxStep;
   constexpr int kRow = kCap + 8;  // x row in LDS, elements
   __shared__ uint16_t xs[CHAIN ? MT * kRow : 8];
-  __shared__ float red[G::kParts][NT][MT][G::kTile];
+  __shared__ float red[DEPTH][G::kParts][NT][MT][G::kTile];
   __shared__ float nred[2][kNormWaves];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int u = blockIdx.x;
   const uint32_t b0 = mx_lane_block<MT>();
   MxRows<NT> rows;
-  mx_unit_rows<EPI, MT, NT>(a, u, rows);
-  MxWeights<NT, CS> w;
+  MxWeights<NT, CS> w[DEPTH];
+  int u = blockIdx.x;
+  const int step = gridDim.x;
+  const auto load = [&](int unit, int d) __attribute__((always_inline)) {
+    // (past the last unit nothing is read)
+    const uint32_t blocks = DEPTH == 1 || unit < units ? a.blocks : 0u;
+    mx_unit_rows<EPI, MT, NT>(a, DEPTH == 1 ? unit : min(unit, units - 1), rows);
+    mx_load_weights<MT, NT, CS>(rows, a.blocks, blocks, b0, w[d]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const auto load_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(u + d * step, d);
+  };
   uint4 x[CHAIN ? 1 : CS][4];
   BufRes xr;
   if constexpr (CHAIN && MT == 1) {
@@ -356,8 +371,7 @@ __global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemv
     BlockSum bs{nred, 0};
     chain_load<NC>(c, 0, in);
     __builtin_amdgcn_sched_barrier(0);  // the chain's inputs return before the weights
-    mx_load_weights<MT, NT, CS>(rows, a.blocks, b0, w);
-    __builtin_amdgcn_sched_barrier(0);
+    load_first();
     mx_chain<NC>(c, blockIdx.x == 0, in, z, bs);
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -369,8 +383,7 @@ __global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemv
     const int64_t base = static_cast<int64_t>(min(wave, a.M - 1)) * c.stride;
     wave_chain_load<CH>(c, base, in);
     __builtin_amdgcn_sched_barrier(0);
-    mx_load_weights<MT, NT, CS>(rows, a.blocks, b0, w);
-    __builtin_amdgcn_sched_barrier(0);
+    load_first();
     if (wave < a.M) {
       mx_wave_chain<CH>(c, base, blockIdx.x == 0, in);
 #pragma unroll
@@ -383,14 +396,11 @@ __global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemv
   } else {
     xr = buf_res(a.x, (static_cast<uint32_t>(a.M - 1) * static_cast<uint32_t>(a.x_stride) + a.K) * (a.x_f32 ? 4u : 2u));
     mx_load_x<MT, CS>(a, xr, b0, x);
-    mx_load_weights<MT, NT, CS>(rows, a.blocks, b0, w);
+    load_first();
   }
 
-  f32x4_t acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const uint16_t* xl = &xs[CHAIN ? (MT == 1 ? 0 : (lane & 7)) * kRow + b0 * kMxBlock : 0];
-  for (uint32_t at = b0;;) {
+  const auto multiply = [&](int d, f32x4_t(&acc)[NT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < CS; ++s) {
 #pragma unroll
@@ -402,69 +412,122 @@ __global__ __launch_bounds__(MxGeom<MT>::kThreads, 2) void mx_gemv_kernel(MxGemv
           xv = __builtin_bit_cast(bf16x8_t, x[s][j]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const uint4 q = w.w[t][s];
+          const uint4 q = w[d].w[t][s];
           const uint32_t code = j == 0 ? q.x : (j == 1 ? q.y : (j == 2 ? q.z : q.w));
-          const uint4 wv = mx_decode4(code, mx_scale(w.s[t][s]));
+          const uint4 wv = mx_decode4(code, mx_scale(w[d].s[t][s]));
           acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, wv), xv, acc[t], 0, 0, 0);
         }
       }
     }
-    if constexpr (!LOOP) {
-      break;
-    } else {
-      at += CS * (kMxStep / kMxBlock);
-      if (at - b0 >= a.blocks) break;  // (uniform)
-      mx_load_x<MT, CS>(a, xr, at, x);
-      mx_load_weights<MT, NT, CS>(rows, a.blocks, at, w);
+  };
+  const auto compute = [&](int d, int unit) __attribute__((always_inline)) {
+    f32x4_t acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    multiply(d, acc);
+    if constexpr (LOOP) {
+      for (uint32_t at = b0 + CS * (kMxStep / kMxBlock); at - b0 < a.blocks; at += CS * (kMxStep / kMxBlock)) {  // (uniform)
+        mx_load_x<MT, CS>(a, xr, at, x);
+        mx_load_weights<MT, NT, CS>(rows, a.blocks, a.blocks, at, w[0]);
+        multiply(0, acc);
+      }
     }
-  }
-  // lane l holds rows 4 (l / 16) ..+3 of column l % 16: the diagonal blocks are kept
-  const int row = 4 * (lane >> 4), col = lane & 15;
-  if (row / G::kTile == col / G::kTile && col % G::kTile < MT)
+    // lane l holds rows 4 (l / 16) ..+3 of column l % 16: the diagonal blocks are kept
+    const int row = 4 * (lane >> 4), col = lane & 15;
+    if (row / G::kTile == col / G::kTile && col % G::kTile < MT)
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      *reinterpret_cast<f32x4_t*>(&red[wave * G::kSlices + row / G::kTile][t][col % G::kTile][row % G::kTile]) = acc[t];
-  lds_barrier();
-  constexpr int kOuts = kGroups<EPI, NT> * MT * G::kTile;
-  static_assert(kOuts <= G::kThreads, "one thread an output");
-  if (tid >= kOuts) return;
-  const int i = tid % G::kTile, m = tid / G::kTile % MT, g = tid / (G::kTile * MT);
-  if (m >= a.M) return;
-  const int t0 = kPairs<EPI> ? 2 * g : g, t1 = kPairs<EPI> ? t0 + 1 : t0;
-  float v = 0.0f, v2 = 0.0f;
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<f32x4_t*>(&red[d][wave * G::kSlices + row / G::kTile][t][col % G::kTile][row % G::kTile]) = acc[t];
+    lds_barrier();
+    constexpr int kOuts = kGroups<EPI, NT> * MT * G::kTile;
+    static_assert(kOuts <= G::kThreads, "one thread an output");
+    const int i = tid % G::kTile, m = tid / G::kTile % MT, g = tid / (G::kTile * MT);
+    if (tid < kOuts && m < a.M) {
+      const int t0 = kPairs<EPI> ? 2 * g : g, t1 = kPairs<EPI> ? t0 + 1 : t0;
+      float v = 0.0f, v2 = 0.0f;
 #pragma unroll
-  for (int p = 0; p < G::kParts; ++p) v += red[p][t0][m][i];
-  if constexpr (kPairs<EPI>)
+      for (int p = 0; p < G::kParts; ++p) v += red[d][p][t0][m][i];
+      if constexpr (kPairs<EPI>)
 #pragma unroll
-    for (int p = 0; p < G::kParts; ++p) v2 += red[p][t1][m][i];
-  mx_store<EPI, MT, NT>(a, u, g, m, i, v, v2);
+        for (int p = 0; p < G::kParts; ++p) v2 += red[d][p][t1][m][i];
+      mx_store<EPI, MT, NT>(a, unit, g, m, i, v, v2);
+    }
+  };
+  // (a buffer of partial sums is written again after the next unit's barrier)
+  for (;; u += DEPTH * step)
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      compute(d, u + d * step);
+      if (DEPTH == 1 || u + (d + 1) * step >= units) return;
+      load(u + (d + DEPTH) * step, d);
+    }
 }
 
-template <int EPI, int MT, int CS, int NT, bool CHAIN, bool LOOP>
-void mx_launch_form(const MxGemvArgs& a, const NormArgs& c, hipStream_t st) {
+template <int EPI, int MT, int CS, int NT, bool CHAIN, bool LOOP, int DEPTH>
+void mx_launch_form(const MxGemvArgs& a, const NormArgs& c, hipStream_t st, int workgroups) {
   const int units = mx_units<EPI, MT, NT>(a.N) * (EPI == kEpiRope ? 3 : 1);
-  hipLaunchKernelGGL((mx_gemv_kernel<EPI, MT, CS, NT, CHAIN, LOOP>), dim3(units), dim3(MxGeom<MT>::kThreads), 0, st, a, c);
+  int grid = units;
+  if (DEPTH > 1) {  // at most `workgroups`, each with the same number of units
+    const int rounds = (units + workgroups - 1) / workgroups;
+    grid = (units + rounds - 1) / rounds;
+  }
+  hipLaunchKernelGGL((mx_gemv_kernel<EPI, MT, CS, NT, CHAIN, LOOP, DEPTH>), dim3(grid), dim3(MxGeom<MT>::kThreads), 0, st, a, c,
+                     units);
 }
 
 template <int EPI, int MT, int NT, bool CHAIN>
 void mx_launch_k(const MxGemvArgs& a, const NormArgs& c, hipStream_t st) {
-  if (a.K <= kMxStep) return mx_launch_form<EPI, MT, 1, NT, CHAIN, false>(a, c, st);
-  if (CHAIN || a.K <= 2 * kMxStep) return mx_launch_form<EPI, MT, 2, NT, CHAIN, false>(a, c, st);
+  if (a.K <= kMxStep) return mx_launch_form<EPI, MT, 1, NT, CHAIN, false, 1>(a, c, st, 0);
+  if (CHAIN || a.K <= 2 * kMxStep) return mx_launch_form<EPI, MT, 2, NT, CHAIN, false, 1>(a, c, st, 0);
   if constexpr (!CHAIN) {
-    if (a.K <= 4 * kMxStep) return mx_launch_form<EPI, MT, 4, NT, false, false>(a, c, st);
-    mx_launch_form<EPI, MT, 4, NT, false, true>(a, c, st);
+    if (a.K <= 3 * kMxStep) return mx_launch_form<EPI, MT, 3, NT, false, false, 1>(a, c, st, 0);
+    if (a.K <= 4 * kMxStep) return mx_launch_form<EPI, MT, 4, NT, false, false, 1>(a, c, st, 0);
+    mx_launch_form<EPI, MT, 4, NT, false, true, 1>(a, c, st, 0);
   }
 }
 
+// Every workgroup reads x, as many bytes as 4 (bf16, one row) or 32 (8 rows) of its W rows, so a unit has as
+// many tiles as leave the CUs enough of them: 512 units, of 2 to 8 rows and one matrix 256.  Measured, us, one
+// tile (pair) a unit, two, four: one row, K x N 2048 x 8192 5.2, 4.6, 4.6; 8192 x 8192 12.9, 10.7, 11.3; 2048 x
+// 4096 3.7, 3.7, 3.8; SwiGLU 2048 x 5632 6.3, 5.4; q/k/v with RoPE 5.0, 5.2.  Eight rows, 2048 x 8192 7.9, 6.0,
+// 5.4; 8192 x 8192 22.5, 16.1, 13.0; 5632 x 2048 6.2, 6.8, 8.4; SwiGLU 11264 wide 12.3, 9.8.
+//
+// A workgroup takes several units where its prologue would cost more than their weights -- eight chained
+// rows, ~600 instructions each, run once a CU: SwiGLU 13.2 -> 8.0, q/k/v 9.8 -> 7.4, lm_head 49152 26.7
+// -> 15.5 -- and in a head-sized matrix (lm_head 49152: one row 12.1 -> 11.6, eight 16.7 -> 13.7; 16384
+// x 2048 loses, 6.1 -> 6.9 and 7.5 -> 7.8).
 template <int EPI, bool CHAIN>
 void mx_launch(const MxGemvArgs& a, const NormArgs& c, hipStream_t st) {
-  constexpr int kSmall = kPairs<EPI> ? 2 : 1;
+  constexpr int kMats = EPI == kEpiRope ? 3 : 1;
+  constexpr int kOne = kPairs<EPI> ? 2 : 1;  // tiles of the smallest unit
+  const bool head = !kPairs<EPI> && a.N >= 32768;
   if (a.M == 1) {
-    if (a.N >= 16384) return mx_launch_k<EPI, 1, 4, CHAIN>(a, c, st);
-    return mx_launch_k<EPI, 1, kSmall, CHAIN>(a, c, st);
+    if constexpr (!kPairs<EPI>) {
+      if (head && a.K <= kMxStep) return mx_launch_form<EPI, 1, 1, 2, CHAIN, false, 2>(a, c, st, 1024);
+      if (head && a.K <= 2 * kMxStep) return mx_launch_form<EPI, 1, 2, 2, CHAIN, false, 2>(a, c, st, 1024);
+    }
+    if (kMats * mx_units<EPI, 1, 4>(a.N) >= 512) return mx_launch_k<EPI, 1, 4, CHAIN>(a, c, st);
+    if (kMats * mx_units<EPI, 1, 2>(a.N) >= 512) return mx_launch_k<EPI, 1, 2, CHAIN>(a, c, st);
+    return mx_launch_k<EPI, 1, kOne, CHAIN>(a, c, st);
   }
-  if (a.N >= 16384) return mx_launch_k<EPI, 8, 4, CHAIN>(a, c, st);
-  mx_launch_k<EPI, 8, kSmall, CHAIN>(a, c, st);
+  if constexpr (CHAIN) {
+    if constexpr (!kPairs<EPI>) {
+      if (a.K <= kMxStep && head) return mx_launch_form<EPI, 8, 1, 4, true, false, 2>(a, c, st, 256);
+      if (a.K <= kMxStep && a.N >= 8192) return mx_launch_form<EPI, 8, 1, 2, true, false, 2>(a, c, st, 256);
+      if (head) return mx_launch_form<EPI, 8, 2, 2, true, false, 2>(a, c, st, 256);
+    }
+    if (a.K <= kMxStep) return mx_launch_form<EPI, 8, 1, kOne, true, false, 2>(a, c, st, 256);
+    mx_launch_form<EPI, 8, 2, kOne, true, false, 2>(a, c, st, 256);
+  } else {
+    if constexpr (!kPairs<EPI>) {
+      if (head && a.K <= kMxStep) return mx_launch_form<EPI, 8, 1, 2, false, false, 2>(a, c, st, 512);
+      if (head && a.K <= 2 * kMxStep) return mx_launch_form<EPI, 8, 2, 2, false, false, 2>(a, c, st, 512);
+    }
+    const int least = kPairs<EPI> ? 512 : 256;
+    if (kMats * mx_units<EPI, 8, 4>(a.N) >= least) return mx_launch_k<EPI, 8, 4, false>(a, c, st);
+    if (kMats * mx_units<EPI, 8, 2>(a.N) >= least) return mx_launch_k<EPI, 8, 2, false>(a, c, st);
+    mx_launch_k<EPI, 8, kOne, false>(a, c, st);
+  }
 }
 
 template <bool CHAIN>
