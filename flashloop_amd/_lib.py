@@ -113,6 +113,7 @@ SIGNATURES = {
     "fl_rope_store": (_I32, [_P, _P, _P, _I64, _P, _P, _P, _I64, _P, _P, _P, _I32, _I32, _I32, _P]),
     "fl_swiglu": (_I32, [_P, _P, _P, _I64, _P]),
     "fl_mx_quantize": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _P, _P, _P]),
+    "fl_mx_swiglu": (_I32, [_P, _P, _I64, _I64, _I32, _P, _P, _P]),
     "fl_mx_dequantize": (_I32, [_P, _P, _I64, _I32, _I32, _P, _I64, _P]),
     "fl_norm_chain_mx": (_I32, [_I32, _I32, _F64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
     # (the pointer arrays of these two as addresses: one array holds all three)

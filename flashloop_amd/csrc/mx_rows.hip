@@ -22,7 +22,6 @@ struct QuantArgs {
   int64_t x_stride;  // elements between rows
   int64_t pieces;    // rows * (padded K / 8)
   int k, per_row;    // pieces of a row
-  int rows_are_vectors;  // rows 16-byte aligned
   uint8_t* codes;
   uint8_t* scales;
 };
@@ -36,18 +35,41 @@ __device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
   }
 }
 
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2_t v = {f[2 * i], f[2 * i + 1]};
+    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_bf16x2_t));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16 bytes at an element's alignment (one load or store, as global memory takes any alignment)
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Bytes16 {
+  u32x4_t v;
+};
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* p) {
+  return __builtin_bit_cast(uint4, reinterpret_cast<const Bytes16*>(p)->v);
+}
+
 // values [8 c, 8 c + 8) of a row, zero from k on
 template <bool F32>
 __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, float* f) {
   const int64_t at = row * a.x_stride + 8 * static_cast<int64_t>(c);
   const int left = a.k - 8 * c;
-  if (a.rows_are_vectors && left >= 8) {
+  if (left >= 8) {
     if constexpr (F32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(a.x) + at);
-      const float4 u = p[0], v = p[1];
-      f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+      const float* p = static_cast<const float*>(a.x) + at;
+      const uint4 u = load16(p), v = load16(p + 4);
+      const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
     } else {
-      unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + at), f);
+      unpack_bf16x8(load16(static_cast<const uint16_t*>(a.x) + at), f);
     }
     return;
   }
@@ -59,17 +81,23 @@ __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int c, fl
   }
 }
 
-template <int BITS, bool F32>
-__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(QuantArgs a) {
-  // rows are whole quads of pieces, so a block's lanes are all inside or all past the end
+// This thread's piece: its row and its place in it.  Rows are whole quads of pieces, so the lanes of a block
+// are all inside or all past the end.
+struct Piece {
+  int64_t at, row;
+  int c;
+};
+__device__ __forceinline__ Piece piece_of(int per_row) {
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
-  const int64_t row0 = first / a.per_row;  // (uniform)
-  const uint32_t in = static_cast<uint32_t>(first - row0 * a.per_row) + threadIdx.x;
-  const uint32_t over = in / static_cast<uint32_t>(a.per_row);
-  const int64_t piece = first + threadIdx.x;
-  if (piece >= a.pieces) return;
-  float f[8];
-  load8<F32>(a, row0 + over, static_cast<int>(in - over * static_cast<uint32_t>(a.per_row)), f);
+  const int64_t row0 = first / per_row;  // (uniform)
+  const uint32_t in = static_cast<uint32_t>(first - row0 * per_row) + threadIdx.x;
+  const uint32_t over = in / static_cast<uint32_t>(per_row);
+  return Piece{first + threadIdx.x, row0 + over, static_cast<int>(in - over * static_cast<uint32_t>(per_row))};
+}
+
+// Eight values of a block, whose four lanes call this together, to their codes and the block's scale.
+template <int BITS>
+__device__ __forceinline__ void store_codes(const float* f, int64_t piece, uint8_t* codes, uint8_t* scales) {
   uint32_t peak = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(f[e]) & 0x7FFFFFFFu);
@@ -78,12 +106,45 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(QuantArgs a) {
   const float s = mx_scale(code);
   if constexpr (BITS == 4) {
     const uint32_t q = mx_encode4(f, s);
-    reinterpret_cast<uint32_t*>(a.codes)[piece] = code == 255u ? 0u : q;
+    reinterpret_cast<uint32_t*>(codes)[piece] = code == 255u ? 0u : q;
   } else {
     const uint2 q = mx_encode8(f, s);
-    reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
+    reinterpret_cast<uint2*>(codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
   }
-  if ((threadIdx.x & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+  if ((piece & 3) == 0) scales[piece >> 2] = static_cast<uint8_t>(code);
+}
+
+template <int BITS, bool F32>
+__global__ __launch_bounds__(kThreads) void mx_quantize_kernel(QuantArgs a) {
+  const Piece p = piece_of(a.per_row);
+  if (p.at >= a.pieces) return;
+  float f[8];
+  load8<F32>(a, p.row, p.c, f);
+  store_codes<BITS>(f, p.at, a.codes, a.scales);
+}
+
+// SwiGLU rows in 8 bits: bf16(bf16(silu(gate)) * up), as swiglu_kernel rounds, quantised without a trip
+// through memory (8192 x 5632: 55 us where the two calls take 44 + 25).
+struct SwigluMxArgs {
+  QuantArgs gate;
+  const uint16_t* up;
+};
+
+__global__ __launch_bounds__(kThreads) void mx_swiglu_kernel(SwigluMxArgs a) {
+  const Piece p = piece_of(a.gate.per_row);
+  if (p.at >= a.gate.pieces) return;
+  QuantArgs up = a.gate;
+  up.x = a.up;
+  float g[8], u[8];
+  load8<false>(a.gate, p.row, p.c, g);
+  load8<false>(up, p.row, p.c, u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] = g[e] / (1.0f + expf(-g[e]));
+  unpack_bf16x8(pack_bf16x8(g), g);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] *= u[e];
+  unpack_bf16x8(pack_bf16x8(g), g);
+  store_codes<8>(g, p.at, a.gate.codes, a.gate.scales);
 }
 
 struct DequantArgs {
@@ -92,29 +153,23 @@ struct DequantArgs {
   uint16_t* out;
   int64_t out_stride, pieces;
   int k, per_row;
-  int rows_are_vectors;
 };
 
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(DequantArgs a) {
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads;
-  const int64_t row0 = first / a.per_row;
-  const uint32_t in = static_cast<uint32_t>(first - row0 * a.per_row) + threadIdx.x;
-  const uint32_t over = in / static_cast<uint32_t>(a.per_row);
-  const int64_t piece = first + threadIdx.x;
-  if (piece >= a.pieces) return;
-  const int c = static_cast<int>(in - over * static_cast<uint32_t>(a.per_row));
-  const int left = a.k - 8 * c;
-  if (left <= 0) return;
+  const Piece p = piece_of(a.per_row);
+  const int64_t piece = p.at;
+  const int left = a.k - 8 * p.c;
+  if (piece >= a.pieces || left <= 0) return;
   const float s = mx_scale(a.scales[piece >> 2]);
   uint4 v;
   if constexpr (BITS == 4)
     v = mx_decode4(reinterpret_cast<const uint32_t*>(a.codes)[piece], s);
   else
     v = mx_decode8(reinterpret_cast<const uint2*>(a.codes)[piece], s);
-  uint16_t* out = a.out + (row0 + over) * a.out_stride + 8 * static_cast<int64_t>(c);
-  if (a.rows_are_vectors && left >= 8) {
-    *reinterpret_cast<uint4*>(out) = v;
+  uint16_t* out = a.out + p.row * a.out_stride + 8 * static_cast<int64_t>(p.c);
+  if (left >= 8) {
+    reinterpret_cast<Bytes16*>(out)->v = __builtin_bit_cast(u32x4_t, v);
     return;
   }
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -131,6 +186,10 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(DequantArgs a) 
 // came before (a step of e4m3 is 1/16 of the value), so the sums and the products are in 64 bits: h
 // becomes bf16 as torch converts a 64-bit value (by way of f32), and z, from that h, e4m3 in one
 // rounding.  (A 64-bit FMA costs here what a 32-bit one does.)  The order of the sums shows in no output.
+//
+// Bound by the VALU, ~260 instructions for 8 values and ~80 for each sum of a wave, which two pieces a lane
+// halve (8192 rows of 4096: 53 -> 42 us, of 8192 with 8 waves a row 152 -> 117, of 1000 18 -> 15): 8192 x 2048 takes 26
+// us (4.5 TB/s; norm_chain_kernel with bf16 z 31), a few rows 5 (one trip to memory and two sums).
 struct NormMxArgs {
   int64_t rows, stride;
   int d, per_row;  // values; 8-value pieces of a padded row
@@ -186,17 +245,6 @@ struct RowSum64 {
   }
 };
 
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2_t v = {f[2 * i], f[2 * i + 1]};
-    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_bf16x2_t));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // Eight 64-bit values as f32 that round on to e4m3 as the 64-bit ones do.  The nearest f32 does unless it
 // has reached a border (between two codes, or two scales: its last 19 bits are zero there), where the
 // value rounded to odd takes its place.
@@ -214,114 +262,136 @@ __device__ __forceinline__ f32x8_t round8_for_codes(const double (&v)[8]) {
   return f;
 }
 
-// W waves share a row, a lane holds one piece of it.  A workgroup takes one row, or as many as 4 waves
-// hold, and goes on to further ones, whose r and x are requested before the sums of the ones in hand.
+// W waves share a row, a lane holds its pieces t, t + 64 W, ... (NC of them).  A workgroup takes one row, or as
+// many as 4 waves hold, and goes on to further ones, whose r and x are requested before the sums of the
+// ones in hand.
 template <int W>
 constexpr int kNormThreads = W < 4 ? 256 : 64 * W;
 
-template <int W, bool ADD, bool FINAL>
+template <int NC, int W, bool ADD, bool FINAL>
 __global__ __launch_bounds__(kNormThreads<W>) void norm_chain_mx_kernel(NormMxArgs a) {
   __shared__ double red[2][W < 4 ? 4 : W];
   constexpr int kLanes = 64 * W, kRows = kNormThreads<W> / kLanes;
   const int t = threadIdx.x % kLanes, nq = a.d / 8;
   RowSum64<W> sum{red, 0};
-  uint4 r, x;
-  const bool in = t < nq;
-  const uint4 wa = ADD && in ? reinterpret_cast<const uint4*>(a.wa)[t] : make_uint4(0, 0, 0, 0);
-  const uint4 wf = FINAL && in ? reinterpret_cast<const uint4*>(a.wf)[t] : make_uint4(0, 0, 0, 0);
-  const uint4 wb = in && a.wb ? reinterpret_cast<const uint4*>(a.wb)[t] : make_uint4(0, 0, 0, 0);
+  uint4 r[NC], x[NC], wa[NC], wf[NC], wb[NC];
+  const auto piece = [&](const uint16_t* p, int i) {
+    const int c = t + i * kLanes;
+    return p != nullptr && c < nq ? reinterpret_cast<const uint4*>(p)[c] : make_uint4(0, 0, 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if constexpr (ADD) wa[i] = piece(a.wa, i);
+    if constexpr (FINAL) wf[i] = piece(a.wf, i);
+    wb[i] = piece(a.wb, i);
+  }
   const double inv_d = 1.0 / static_cast<double>(a.d);
   const auto inv_rms = [&](double ss) { return rsqrt(fma(sum(ss), inv_d, a.eps)); };
-  const auto request = [&](int64_t row, uint4& rr, uint4& xx) {
-    const int64_t base = row * a.stride;
-    rr = in ? reinterpret_cast<const uint4*>(a.r + base)[t] : make_uint4(0, 0, 0, 0);
-    if constexpr (ADD) xx = in ? reinterpret_cast<const uint4*>(a.x + base)[t] : make_uint4(0, 0, 0, 0);
-  };
-  const auto squares = [&](const uint4& v) {
-    double ss = 0.0;
-    float f[8];
-    unpack_bf16x8(v, f);
+  const auto request = [&](int64_t row, uint4(&rr)[NC], uint4(&xx)[NC]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ss);
-    return ss;
+    for (int i = 0; i < NC; ++i) {
+      rr[i] = piece(a.r + row * a.stride, i);
+      if constexpr (ADD) xx[i] = piece(a.x + row * a.stride, i);
+    }
+  };
+  const auto squares = [&](const uint4(&v)[NC]) {
+    double ss[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      float f[8];
+      unpack_bf16x8(v[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss[e & 1] = fma(static_cast<double>(f[e]), static_cast<double>(f[e]), ss[e & 1]);
+    }
+    return ss[0] + ss[1];
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kLanes;
   request(min(row, a.rows - 1), r, x);
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kRows; first < a.rows; first += step, row += step) {
     const bool live = row < a.rows;  // (a row past the last is the last again, not stored)
-    uint4 nr, nx;
+    uint4 nr[NC], nx[NC];
     if (first + step < a.rows) request(min(row + step, a.rows - 1), nr, nx);
     if constexpr (ADD || FINAL) {
       const double ia = ADD ? inv_rms(squares(x)) : 0.0;
-      double h[8];  // r + norm_a(x)
-      float f[8], w[8], o[8];
-      unpack_bf16x8(r, f);
+      double h[NC][8];  // r + norm_a(x)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = static_cast<double>(f[e]);
-      if constexpr (ADD) {
-        unpack_bf16x8(x, f);
-        unpack_bf16x8(wa, w);
+      for (int i = 0; i < NC; ++i) {
+        float f[8], w[8];
+        unpack_bf16x8(r[i], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = fma(static_cast<double>(w[e]) * static_cast<double>(f[e]), ia, h[e]);
+        for (int e = 0; e < 8; ++e) h[i][e] = static_cast<double>(f[e]);
+        if constexpr (ADD) {
+          unpack_bf16x8(x[i], f);
+          unpack_bf16x8(wa[i], w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[i][e] = fma(static_cast<double>(w[e]) * static_cast<double>(f[e]), ia, h[i][e]);
+        }
       }
+      double fi = 1.0;
       if constexpr (FINAL) {
         double ss = 0.0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fma(h[e], h[e], ss);
-        const double fi = inv_rms(ss);
-        unpack_bf16x8(wf, w);
+        for (int i = 0; i < NC; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] *= static_cast<double>(w[e]) * fi;
+          for (int e = 0; e < 8; ++e) ss = fma(h[i][e], h[i][e], ss);
+        fi = inv_rms(ss);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(h[e]);
-      r = pack_bf16x8(o);
+      for (int i = 0; i < NC; ++i) {
+        float o[8], w[8];
+        if constexpr (FINAL) unpack_bf16x8(wf[i], w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = static_cast<float>(FINAL ? h[i][e] * (static_cast<double>(w[e]) * fi) : h[i][e]);
+        r[i] = pack_bf16x8(o);
+      }
     }
-    if (a.h_out != nullptr && live && in) reinterpret_cast<uint4*>(a.h_out + row * a.stride)[t] = r;
+    if (a.h_out != nullptr && live) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (t + i * kLanes < nq) reinterpret_cast<uint4*>(a.h_out + row * a.stride)[t + i * kLanes] = r[i];
+    }
     if (a.wb != nullptr) {
-      // (0 past the row, also where the row's statistics are not finite)
-      const double ib = inv_rms(squares(r)), scale = in ? ib : 0.0;
-      float fh[8], fw[8], z[8];
-      double v[8];
-      unpack_bf16x8(r, fh);
-      unpack_bf16x8(wb, fw);
+      const double ib = inv_rms(squares(r));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * scale;
-      const f32x8_t rounded = round8_for_codes(v);
+      for (int i = 0; i < NC; ++i) {
+        const int c = t + i * kLanes;
+        // (0 past the row, also where the row's statistics are not finite)
+        const double scale = c < nq ? ib : 0.0;
+        float fh[8], fw[8], z[8];
+        double v[8];
+        unpack_bf16x8(r[i], fh);
+        unpack_bf16x8(wb[i], fw);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = rounded[e];
-      uint32_t peak = 0;
+        for (int e = 0; e < 8; ++e) v[e] = static_cast<double>(fw[e]) * static_cast<double>(fh[e]) * scale;
+        const f32x8_t rounded = round8_for_codes(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) peak = max(peak, __float_as_uint(z[e]) & 0x7FFFFFFFu);
-      peak = quad_max_u(peak);
-      if (t < a.per_row && live) {  // (whole quads)
-        const uint32_t code = mx_scale_code<8>(peak);
-        const uint2 q = mx_encode8(z, mx_scale(code));
-        const int64_t piece = row * a.per_row + t;
-        reinterpret_cast<uint2*>(a.codes)[piece] = code == 255u ? make_uint2(0u, 0u) : q;
-        if ((t & 3) == 0) a.scales[piece >> 2] = static_cast<uint8_t>(code);
+        for (int e = 0; e < 8; ++e) z[e] = rounded[e];
+        if (c < a.per_row && live) store_codes<8>(z, row * a.per_row + c, a.codes, a.scales);  // (whole quads)
       }
     }
-    r = nr;
-    if constexpr (ADD) x = nx;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      r[i] = nr[i];
+      if constexpr (ADD) x[i] = nx[i];
+    }
   }
 }
 
-template <int W>
+template <int NC, int W>
 void launch_norm(const NormMxArgs& a, hipStream_t st) {
   constexpr int kRows = kNormThreads<W> / (64 * W);
   const int64_t groups = (a.rows + kRows - 1) / kRows, most = kNormGrid * 256 / kNormThreads<W>;
   const dim3 g(static_cast<unsigned>(groups < most ? groups : most)), t(kNormThreads<W>);
   if (a.x != nullptr) {
     if (a.wf != nullptr)
-      hipLaunchKernelGGL((norm_chain_mx_kernel<W, true, true>), g, t, 0, st, a);
+      hipLaunchKernelGGL((norm_chain_mx_kernel<NC, W, true, true>), g, t, 0, st, a);
     else
-      hipLaunchKernelGGL((norm_chain_mx_kernel<W, true, false>), g, t, 0, st, a);
+      hipLaunchKernelGGL((norm_chain_mx_kernel<NC, W, true, false>), g, t, 0, st, a);
   } else if (a.wf != nullptr) {
-    hipLaunchKernelGGL((norm_chain_mx_kernel<W, false, true>), g, t, 0, st, a);
+    hipLaunchKernelGGL((norm_chain_mx_kernel<NC, W, false, true>), g, t, 0, st, a);
   } else {
-    hipLaunchKernelGGL((norm_chain_mx_kernel<W, false, false>), g, t, 0, st, a);
+    hipLaunchKernelGGL((norm_chain_mx_kernel<NC, W, false, false>), g, t, 0, st, a);
   }
 }
 
@@ -347,7 +417,6 @@ extern "C" int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_str
   a.per_row = static_cast<int>(mx_padded(k) / 8);
   FL_REQUIRE(rows <= INT64_MAX / 2 / a.per_row, "fl_mx_quantize: too many rows");
   a.pieces = rows * a.per_row;
-  a.rows_are_vectors = aligned(x, 16) && (x_stride * (x_is_f32 ? 4 : 2)) % 16 == 0;
   a.codes = codes;
   a.scales = scales;
   const int64_t blocks = (a.pieces + kThreads - 1) / kThreads;
@@ -366,6 +435,32 @@ extern "C" int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_str
       hipLaunchKernelGGL((mx_quantize_kernel<8, false>), g, t, 0, st, a);
   }
   FL_LAUNCH_CHECK("fl_mx_quantize");
+  return FL_OK;
+}
+
+extern "C" int32_t fl_mx_swiglu(const uint16_t* gate, const uint16_t* up, int64_t row_stride, int64_t rows, int32_t k,
+                                uint8_t* codes, uint8_t* scales, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(gate && up && codes && scales, "fl_mx_swiglu: null pointer");
+  FL_REQUIRE(rows >= 0 && k > 0 && k <= FL_MX_MAX_K && row_stride >= k, "fl_mx_swiglu: bad sizes");
+  FL_REQUIRE(aligned(gate, 2) && aligned(up, 2), "fl_mx_swiglu: gate or up is not aligned to its elements");
+  FL_REQUIRE(aligned(codes, 16), "fl_mx_swiglu: codes must be 16-byte aligned");
+  if (rows == 0) return FL_OK;
+  SwigluMxArgs a{};
+  a.gate.x = gate;
+  a.gate.x_stride = row_stride;
+  a.gate.k = k;
+  a.gate.per_row = static_cast<int>(mx_padded(k) / 8);
+  FL_REQUIRE(rows <= INT64_MAX / 2 / a.gate.per_row, "fl_mx_swiglu: too many rows");
+  a.gate.pieces = rows * a.gate.per_row;
+  a.gate.codes = codes;
+  a.gate.scales = scales;
+  a.up = up;
+  const int64_t blocks = (a.gate.pieces + kThreads - 1) / kThreads;
+  FL_REQUIRE(blocks <= 0xFFFFFFFFll / kThreads, "fl_mx_swiglu: grid too large");
+  hipLaunchKernelGGL(mx_swiglu_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+  FL_LAUNCH_CHECK("fl_mx_swiglu");
   return FL_OK;
 }
 
@@ -388,7 +483,6 @@ extern "C" int32_t fl_mx_dequantize(const uint8_t* codes, const uint8_t* scales,
   a.per_row = static_cast<int>(mx_padded(k) / 8);
   FL_REQUIRE(rows <= INT64_MAX / 2 / a.per_row, "fl_mx_dequantize: too many rows");
   a.pieces = rows * a.per_row;
-  a.rows_are_vectors = aligned(out, 16) && out_stride % 8 == 0;
   const int64_t blocks = (a.pieces + kThreads - 1) / kThreads;
   FL_REQUIRE(blocks <= 0xFFFFFFFFll / kThreads, "fl_mx_dequantize: grid too large");
   const dim3 g(static_cast<unsigned>(blocks)), t(kThreads);
@@ -421,15 +515,15 @@ extern "C" int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint
   const NormMxArgs a{m, stride, d, per_row, eps, x, r, w_a, w_f, w_b, h_out, z_codes, z_scales};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (per_row <= 64)
-    launch_norm<1>(a, st);
+    launch_norm<1, 1>(a, st);
   else if (per_row <= 128)
-    launch_norm<2>(a, st);
+    launch_norm<2, 1>(a, st);
   else if (per_row <= 256)
-    launch_norm<4>(a, st);
+    launch_norm<2, 2>(a, st);
   else if (per_row <= 512)
-    launch_norm<8>(a, st);
+    launch_norm<2, 4>(a, st);
   else
-    launch_norm<16>(a, st);
+    launch_norm<2, 8>(a, st);
   FL_LAUNCH_CHECK("fl_norm_chain_mx");
   return FL_OK;
 }

@@ -73,7 +73,7 @@ def _mx_rows_gemv(x, weights, *, epilogue=kernels.EPI_PLAIN, addend=None, rope=N
     if epilogue == kernels.EPI_ADD:
         return ys[0] + addend.reshape(ys[0].shape)
     if epilogue == kernels.EPI_SWIGLU:
-        return kernels.swiglu(*ys) if ys[0].numel() % 8 == 0 else F.silu(ys[0]) * ys[1]
+        return kernels.mx_swiglu(*ys)  # (8-bit rows, as the next product takes them)
     if epilogue == kernels.EPI_ROPE:
         q, k, v = (y.view(y.shape[0], -1, 1, head_dim) for y in ys)
         return (*(t.reshape(ys[0].shape) for t in apply_rope(q, k, *(t[:, None] for t in rope))), ys[2])
@@ -297,7 +297,7 @@ class FlashLoopEngine:
 
         hidden = self.backbone.norm.weight.numel()
         if hidden % 8 or hidden > 8192 or any(l.mlp.up_proj.weight.shape[0] % 8 for l in self.layers):
-            raise ValueError("weight_bits=4 needs a hidden width up to 8192 and an MLP width, multiples of 8")
+            raise ValueError("weight_bits=4 needs a hidden width (up to 8192) and an MLP width that are multiples of 8")
         layers = []
         for layer in self.layers:
             a, m = layer.self_attn, layer.mlp
@@ -415,8 +415,8 @@ class FlashLoopEngine:
                                       kv[0].shape[-1] ** -0.5, positions)
         x = kernels.mx_matmul(kernels.mx_quantize(o, 8), w["o"])
         hid, z = kernels.norm_chain_mx(hid, x=x, w_a=w["ln2"], w_b=w["ln3"], eps=eps)
-        act = kernels.swiglu(kernels.mx_matmul(z, w["gate"]), kernels.mx_matmul(z, w["up"]))
-        y = kernels.mx_matmul(kernels.mx_quantize(act, 8), w["down"])
+        act = kernels.mx_swiglu(kernels.mx_matmul(z, w["gate"]), kernels.mx_matmul(z, w["up"]))
+        y = kernels.mx_matmul(act, w["down"])
         return kernels.norm_chain_mx(hid, x=y, w_a=w["ln4"], w_f=w_final, w_b=w_next, eps=eps)
 
     def _layer_rows(self, weights, hid, z, rope, kv, positions, eps, w_next, w_final):

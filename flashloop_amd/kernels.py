@@ -775,6 +775,21 @@ def mx_dequantize(t: MXTensor) -> torch.Tensor:
     return out
 
 
+def mx_swiglu(gate: torch.Tensor, up: torch.Tensor) -> MXTensor:
+    """``mx_quantize(swiglu(gate, up), 8)`` of bf16 rows [.., K] in one pass (``fl_mx_swiglu``)."""
+    if gate.ndim == 0 or not 0 < gate.shape[-1] <= MX_MAX_K:
+        raise ValueError(f"gate needs at least one value a row, and at most {MX_MAX_K}")
+    if gate.shape != up.shape or gate.dtype is not torch.bfloat16 or up.dtype is not torch.bfloat16 or gate.device != up.device:
+        raise ValueError("gate and up must be bf16 of one shape on one device")
+    g2, u2 = _contiguous_rows(gate), _contiguous_rows(up)
+    rows, k = g2.shape
+    t = MXTensor._empty(rows, k, 8, g2.device)
+    if rows:
+        _launch(t.device, "fl_mx_swiglu", load().fl_mx_swiglu, g2.data_ptr(), u2.data_ptr(), k, rows, k, t.codes.data_ptr(),
+                t.scales.data_ptr())
+    return t
+
+
 def _chain_operands(r, x, w_a, w_f, w_b):
     """The chain's rows as contiguous bf16 [M, D], its gains checked."""
     r2, x2 = _contiguous_rows(r), None

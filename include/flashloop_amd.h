@@ -554,6 +554,8 @@ int32_t fl_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64
  * nothing saturates; values are rounded to the nearest, ties to the even code.  A block with a NaN
  * or an infinity gets scale 255 and codes of zero.
  * fl_mx_dequantize: the values as bf16 (exact, but for results under 2^-126 or past the range).
+ * fl_mx_swiglu: fl_swiglu of bf16 rows [rows, k] (`row_stride` elements apart, the same for gate and
+ * up) as 8-bit rows: the codes and scales that fl_mx_quantize makes of its result.
  * fl_norm_chain_mx: the chain of fl_norm_chain with z in 8 bits: h = x ? r + RMSNorm_a(x) : r; if
  * w_f: h = RMSNorm_f(h); h_out (optional) = bf16(h); z = RMSNorm_b(bf16(h)), quantised as above from
  * its unrounded value.  Sums and products are in 64 bits and only h and z are rounded (fl_norm_chain
@@ -565,6 +567,8 @@ int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_stride, int64_
                        int32_t bits, uint8_t* codes, uint8_t* scales, void* stream);
 int32_t fl_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int32_t k, int32_t bits,
                          uint16_t* out, int64_t out_stride, void* stream);
+int32_t fl_mx_swiglu(const uint16_t* gate, const uint16_t* up, int64_t row_stride, int64_t rows, int32_t k,
+                     uint8_t* codes, uint8_t* scales, void* stream);
 int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, const uint16_t* r,
                          const uint16_t* w_a, const uint16_t* w_f, const uint16_t* w_b, uint16_t* h_out,
                          uint8_t* z_codes, uint8_t* z_scales, int64_t stride, void* stream);

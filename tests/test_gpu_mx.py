@@ -142,6 +142,28 @@ def test_quantize_more_than_2_to_31_values():
     assert np.array_equal(_np(values[-2:]), mx.dequantize(codes, scales, k, 8)) and not values[:-2].any()
 
 
+@pytest.mark.parametrize("rows,k", [(1, 8), (3, 31), (2, 520), (300, 128), (17, 5632)])
+def test_mx_swiglu_is_swiglu_quantized(rows, k):
+    """bf16(bf16(silu(gate)) * up), quantised: as torch's modules round, and as the two calls give it."""
+    _say("mx_swiglu", rows, k)
+    rng = _rng(21, rows, k)
+    gate, up = _bf16(3 * rng.standard_normal((rows, k))), _bf16(_rows(rng, rows, k))
+    gate.view(-1)[0], up.view(-1)[-1] = float("-inf"), float("nan")
+    got = kernels.mx_swiglu(gate, up)
+    if rows * k % 8 == 0:
+        want = kernels.mx_quantize(kernels.swiglu(gate, up), 8)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    v, w = kernels.mx_dequantize(got), _np(gate)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = w / (1 + np.exp(-w)) * _np(up)
+    nan = torch.isnan(v).cpu().numpy()
+    assert nan[-1, -1] and nan[0, 0] and nan[:, :].sum() <= 64
+    s = np.repeat(np.exp2(got.scales.cpu().numpy().astype(float) - 127), 32, axis=1)[:, :k]
+    # silu and product 2^-8 each, e4m3 2^-4 of a normal value (2^-10 of the scale under that)
+    bound = (2.0**-4 + 3 * 2.0**-8) * abs(want) + 2.0**-10 * s
+    assert (abs(_np(v) - want) <= bound)[~nan].all()
+
+
 # ---------------------------------------------------------------------------- norm with 8-bit rows
 def _chain_case(rng, rows, d, add, final):
     s = dict(r=_bf16(_rows(rng, rows, d)), w_b=_bf16(1 + 0.2 * rng.standard_normal(d)))
@@ -404,8 +426,7 @@ def test_mx_matmul_no_rows_and_far_rows():
 def _together(r, w_b, gate, up, down):
     """norm -> gate and up -> SwiGLU -> 8-bit rows -> down, on the operators."""
     _, z = kernels.norm_chain_mx(r, w_b=w_b, eps=EPS)
-    act = kernels.swiglu(kernels.mx_matmul(z, gate), kernels.mx_matmul(z, up))
-    return kernels.mx_matmul(kernels.mx_quantize(act, 8), down)
+    return kernels.mx_matmul(kernels.mx_swiglu(kernels.mx_matmul(z, gate), kernels.mx_matmul(z, up)), down)
 
 
 def test_operators_together_on_another_stream_and_in_a_graph():

@@ -50,6 +50,10 @@ def test_front_end_refusals():
         kernels.mx_gemv(x, [w])
     with pytest.raises(RuntimeError, match="device"):
         kernels.norm_chain_mx(x, w_b=gain, eps=1e-6)
+    with pytest.raises(RuntimeError, match="device"):
+        kernels.mx_swiglu(x, x)
+    with pytest.raises(ValueError, match="one shape"):
+        kernels.mx_swiglu(x, x[:1])
     with pytest.raises(ValueError, match="bits"):
         kernels.mx_quantize(x, 6)
     with pytest.raises(ValueError, match="bfloat16 or float32"):
@@ -97,6 +101,16 @@ def test_c_abi_refusals():
     says(d(out=0x301), b"aligned")
     says(d(codes=0x108), b"16-byte")
     assert d(rows=0) == _lib.FL_OK
+    sw = lambda g=0x100, u=0x200, stride=64, rows=1, k=64, codes=0x300, scales=0x400: lib.fl_mx_swiglu(  # noqa: E731
+        g, u, stride, rows, k, codes, scales, None)
+    for name in ("g", "u", "codes", "scales"):
+        says(sw(**{name: None}), b"null")
+    says(sw(stride=63), b"bad sizes")
+    says(sw(k=0), b"bad sizes")
+    says(sw(u=0x201), b"aligned to its elements")
+    says(sw(codes=0x308), b"16-byte")
+    says(sw(rows=1 << 40), b"grid")
+    assert sw(rows=0) == _lib.FL_OK
     n = lambda m=1, d=64, x=None, r=0x100, wa=None, wb=0x200, codes=0x300, scales=0x400, stride=64, h=None: lib.fl_norm_chain_mx(  # noqa: E731
         m, d, 1e-6, x, r, wa, None, wb, h, codes, scales, stride, None)
     says(n(d=60), b"multiple of 8")
