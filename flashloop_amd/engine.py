@@ -63,7 +63,8 @@ def _is_plain(m: torch.nn.Module, kind: type) -> bool:
 
 def _mx_rows_gemv(x, weights, *, epilogue=kernels.EPI_PLAIN, addend=None, rope=None, head_dim=kernels.HEAD_DIM, out=None):
     """``kernels.mx_gemv`` for any number of rows (``x``: rows, or an 8-bit ``MXTensor``): 8-bit rows and
-    ``mx_matmul``."""
+    ``mx_matmul``.  ``rope`` holds a table row for every (row, head); SwiGLU gives 8-bit rows, as the
+    next product takes them."""
     if not isinstance(x, kernels.MXTensor):
         x = kernels.mx_quantize(x, 8)
     if epilogue == kernels.EPI_F32:
@@ -73,10 +74,12 @@ def _mx_rows_gemv(x, weights, *, epilogue=kernels.EPI_PLAIN, addend=None, rope=N
     if epilogue == kernels.EPI_ADD:
         return ys[0] + addend.reshape(ys[0].shape)
     if epilogue == kernels.EPI_SWIGLU:
-        return kernels.mx_swiglu(*ys)  # (8-bit rows, as the next product takes them)
-    if epilogue == kernels.EPI_ROPE:
-        q, k, v = (y.view(y.shape[0], -1, 1, head_dim) for y in ys)
-        return (*(t.reshape(ys[0].shape) for t in apply_rope(q, k, *(t[:, None] for t in rope))), ys[2])
+        return kernels.mx_swiglu(*ys)
+    if epilogue == kernels.EPI_ROPE:  # (each (row, head) as a row of one head: k and v leave in q's layout)
+        q, k, v = (y.view(-1, head_dim) for y in ys)
+        k_dst, v_dst = torch.empty((2, 1, *k.shape), dtype=k.dtype, device=k.device).unbind(0)
+        kernels.rope_store(q, k, v, rope, k_dst, v_dst)
+        return (ys[0], *(t.view(ys[0].shape) for t in (k_dst, v_dst)))
     return ys[0]
 
 
@@ -674,6 +677,7 @@ class FlashLoopEngine:
             gemv, gemv_chain = kernels.mx_gemv, kernels.mx_gemv_chain
             if bsz > 8:
                 gemv, gemv_chain, chained = _mx_rows_gemv, _mx_rows_gemv_chain, True
+                rope = tuple(t.repeat_interleave(heads, dim=0) for t in rope)
             elif hid.shape[1] > 4096:  # (the longest row that the chained GEMV takes)
                 chained = False
         # the chain whose output feeds the next GEMV: kwargs of norm_chain (h = hid + n_a(x),
