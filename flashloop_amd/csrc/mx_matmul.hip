@@ -44,7 +44,7 @@ struct MmArgs {
   int tiles_n, tiles_m;
 };
 
-// A lane's 16 + 32 bytes of one step and their scales into the sums.
+// A lane's 16 + 32 bytes of one step and their scales (low bytes) into the sums.
 template <bool EXACT>
 __device__ __forceinline__ mx_f32x4_t mx_step(const uint4& w, uint32_t ws, const uint4& x0, const uint4& x1, uint32_t xs,
                                               mx_f32x4_t c) {
@@ -53,8 +53,8 @@ __device__ __forceinline__ mx_f32x4_t mx_step(const uint4& w, uint32_t ws, const
     const uint2 p[4] = {make_uint2(x0.x, x0.y), make_uint2(x0.z, x0.w), make_uint2(x1.x, x1.y), make_uint2(x1.z, x1.w)};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8_t, mx_decode4(q[j], mx_scale(ws))),
-                                                  __builtin_bit_cast(mx_bf16x8_t, mx_decode8(p[j], mx_scale(xs))), c, 0, 0, 0);
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8_t, mx_decode4(q[j], mx_scale(ws & 255u))),
+                                                  __builtin_bit_cast(mx_bf16x8_t, mx_decode8(p[j], mx_scale(xs & 255u))), c, 0, 0, 0);
     return c;
   } else {
     const mx_i32x8_t a = {static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w), 0, 0, 0, 0};
@@ -131,6 +131,11 @@ __device__ __forceinline__ mx_i32x4_t raw_buffer(const void* p, int64_t bytes) {
 }
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+// Byte g of each of four dwords (pick: g, 4 + g), the first lowest.
+__device__ __forceinline__ uint32_t lane_scales(const uint4& q, uint32_t pick) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(q.w, q.z, pick), __builtin_amdgcn_perm(q.y, q.x, pick), 0x05040100u);
+}
 
 // Memory to LDS: lane l's 16 (or 4) bytes of buffer r at voff + soff go to lds + 16 (4) l.  The compiler counts
 // no LDS write for these, so the kernel waits for them itself (vmcnt, ahead of the step's barrier).
@@ -263,26 +268,35 @@ __global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArg
   const uint8_t* wl = lds + wrow * 64 + 16 * (g ^ ((i >> 2) & 3));
   const uint8_t* xl0 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 0) ^ ((i >> 1) & 7));
   const uint8_t* xl1 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 1) ^ ((i >> 1) & 7));
-  const uint8_t* sl = lds + 3 * G::kBuffer + g;
+  const uint32_t pick = static_cast<uint32_t>(g) | static_cast<uint32_t>(4 + g) << 8;
 
   uint4 w[G::kFN], x0[G::kFM], x1[G::kFM];
   uint32_t ws[G::kFN], xs[G::kFM];
   // the step in hand: tile, step in it, buffer, buffer of its scales
   int ctile = blockIdx.x, cs = 0, cbuf = 0, cscale = 1;
   const auto read_step = [&]() __attribute__((always_inline)) {
-    if ((cs & 3) == 0) cscale ^= 1;
-    const uint32_t at = cbuf * G::kBuffer, sat = cscale * G::kScales + 4 * (cs & 3);
+    const uint32_t at = cbuf * G::kBuffer;
     cbuf = cbuf == 2 ? 0 : cbuf + 1;
 #pragma unroll
-    for (int n = 0; n < G::kFN; ++n) {
-      w[n] = *reinterpret_cast<const uint4*>(wl + at + n * 1024);
-      ws[n] = sl[sat + (wrow + 16 * n) * 16];
-    }
+    for (int n = 0; n < G::kFN; ++n) w[n] = *reinterpret_cast<const uint4*>(wl + at + n * 1024);
 #pragma unroll
     for (int m = 0; m < G::kFM; ++m) {
       x0[m] = *reinterpret_cast<const uint4*>(xl0 + at + m * 2048);
       x1[m] = *reinterpret_cast<const uint4*>(xl1 + at + m * 2048);
-      xs[m] = sl[sat + (BN + xrow + 16 * m) * 16];
+    }
+    // scales: this lane's bytes of four steps at once, the step's own in the low byte
+    if ((cs & 3) == 0) {
+      cscale ^= 1;
+      const uint8_t* sl = lds + 3 * G::kBuffer + cscale * G::kScales;
+#pragma unroll
+      for (int n = 0; n < G::kFN; ++n) ws[n] = lane_scales(*reinterpret_cast<const uint4*>(sl + (wrow + 16 * n) * 16), pick);
+#pragma unroll
+      for (int m = 0; m < G::kFM; ++m) xs[m] = lane_scales(*reinterpret_cast<const uint4*>(sl + (BN + xrow + 16 * m) * 16), pick);
+    } else {
+#pragma unroll
+      for (int n = 0; n < G::kFN; ++n) ws[n] >>= 8;
+#pragma unroll
+      for (int m = 0; m < G::kFM; ++m) xs[m] >>= 8;
     }
   };
   const auto multiply = [&]() __attribute__((always_inline)) {
