@@ -88,6 +88,11 @@ class FlashLoopBatchEngine:
         self._state = None
         self._runner.reset()
 
+    def quantize_weights(self) -> None:
+        """``FlashLoopEngine.quantize_weights``: the 4-bit copies anew after the model's weights have changed."""
+        self._one.quantize_weights()
+        self._runner.reset()
+
     # ------------------------------------------------------------------ prefill
     @staticmethod
     def _lengths(input_ids: torch.Tensor, attention_mask: torch.Tensor | None) -> list[int]:

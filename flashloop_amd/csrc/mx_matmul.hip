@@ -3,12 +3,14 @@
 // bf16 results: v_mfma_scale_f32_16x16x128_f8f6f4 takes the codes as they are.  W is its first operand
 // (lane l: row l % 16, block g = l / 16 of 32 codes), X its second (row l % 16, bytes 16 g .. +15 and
 // 64 + 16 g .. +15 of the row's 128), and lane group g gives the scales of block g of both.  Results: a
-// lane holds four neighbouring n of row m = l % 16.  Inside one instruction the products are aligned
-// to the largest of them and cut: its sums are off by up to about 2^-14 of the sum of the products'
-// magnitudes (measured: 4e-6 of the result for equal channels, 2e-5 for channels e^N(0,1) apart), an
-// eighth of bf16's rounding and less.  Between instructions the sums are fp32.
-// f32 results: every code is exact in bf16, so the operands are widened in registers and
-// v_mfma_f32_16x16x32_bf16 sums exact products in fp32 (a quarter of the rate).
+// lane holds four neighbouring n of row m = l % 16.  Of every eight neighbouring products the instruction
+// drops what lies under 2^-13 of the largest of them (so it came out of values that were set against each
+// other; groups of eight and steps add up in fp32): less than 7 * 2^-13 of the sum of the products'
+// magnitudes, half of what the rounding to bf16 may cost, and 2^-18 to 2^-16 of the result for channels
+// e^N(0,1) apart.
+// f32 results: every value is exact in bf16 (but for rows' values under 2^-126, which become multiples of
+// 2^-133), so the operands are widened in registers and v_mfma_f32_16x16x32_bf16 sums exact products in
+// fp32 (a quarter of the rate).
 //
 // A workgroup's tile is BN rows of W by BM rows of X, K in steps of 128 through LDS.  The operands go from
 // memory to LDS without passing registers, two steps ahead, in three buffers (one barrier a step);
@@ -17,9 +19,12 @@
 // as zeros.  The largest tile takes the LDS of a CU: its eight waves alternate between reading and
 // multiplying, and it goes on to further tiles, whose first steps are on their way while it stores.
 //
-// Bound by the matrix cores' power: with operands in registers the instruction reaches 3500-3750 TFLOP/s on
-// random codes (4700 on zeros), 8192^3 here 2990, 8192 x 2048 -> 5632 2350 (80 us; 704 tiles in
-// three rounds of 256), 8192 x 5632 -> 2048 2660.  The bf16 library product of the same sizes: 1390, 1050, 1410.
+// What bounds it: with operands in registers the instruction reaches 3500-3750 TFLOP/s on random codes (4700
+// on zeros, by its power).  8192^3 takes 359 us (3060 TFLOP/s), 306 without the transfers, 311 without the LDS
+// reads, 273 without the products, and 278 with nothing but the products and barriers: the reading and
+// the multiplying turns are about equally long.  8192 x 2048 -> 5632 79-90 us (2100-2390; 704 tiles in three
+// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 68-73.  The bf16 library product
+// of the three: 777-816, 174-185, 132-137 us.
 #include <algorithm>
 
 #include "mx_common.h"

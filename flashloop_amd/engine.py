@@ -611,8 +611,11 @@ class FlashLoopEngine:
     def _decode_core(self, cache: CrossLoopKVCache, token_ids: torch.Tensor, pos_t: torch.Tensor,
                      out: torch.Tensor | None = None) -> torch.Tensor:
         """One decode step (see ``_decode_core_fused``); the torch-module form runs when the
-        fused kernels do not apply (``fused_decode`` off, non-bf16 weights, batch > 8).  The
-        fused form writes the logits to ``out`` if given."""
+        fused kernels do not apply (``fused_decode`` off, non-bf16 weights, batch > 8; 4-bit
+        weights have no module form and take any batch).  The fused form writes the logits to
+        ``out`` if given."""
+        if self._mx is not None and not self.fused_decode:
+            raise RuntimeError("weight_bits=4: the module path (fused_decode off) multiplies by the modules' own weights")
         if self._mx is not None or (self.fused_decode and token_ids.shape[0] <= 8 and self._fused_weights() is not None):
             return self._decode_core_fused(cache, *self._decode_inputs(token_ids, pos_t), logits_out=out)
         return self._decode_core_modules(cache, self.backbone.embed_tokens(token_ids), pos_t)

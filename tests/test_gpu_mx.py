@@ -3,8 +3,10 @@
 Quantisation, its inverse and the norm with 8-bit output are compared byte for byte (the norm's sums
 are in 64 bits on both sides).  Products are compared with derived bounds: the operands' values are
 exact, a sum of K exact products in fp32 is off by at most K * 2^-24 of the sum of their magnitudes,
-a rounding to bf16 by 2^-8 of the value, and the scaled matrix instruction by 2^-12 of the sum of the
-products' magnitudes (eight of its 24 bits and more are lost to the alignment of its 128 products)."""
+a rounding to bf16 by 2^-8 of the value.  The scaled matrix instruction drops of every eight neighbouring
+products what lies under 2^-13 of the largest of them: 7 * 2^-13 < 2^-10 of the sum of the products'
+magnitudes at worst (``test_mx_matmul_of_far_neighbours``); where neighbours are random, 2^-12 is
+allowed for."""
 
 import numpy as np
 import pytest
@@ -402,6 +404,68 @@ def test_mx_matmul_nonfinite_stays_in_its_row_and_column(m, dtype):
     bad = torch.zeros(m, n, dtype=torch.bool, device=DEV)
     bad[m - 1], bad[0], bad[:, 7], bad[:, n - 1] = True, True, True, True
     assert torch.equal(torch.isnan(y), bad)
+
+
+@pytest.mark.parametrize("m,n", [(3, 20), (300, 300), (4096, 4096)])
+def test_mx_matmul_of_far_neighbours(m, n):
+    """One value of eight far over the others, which add up: 7 products just under 2^-13 of it are dropped for a
+    bf16 result, and what is left of two that cancel is exact.  f32 results keep all of them."""
+    _say("far neighbours", m, n)
+    k = 256
+    xv, wv = np.zeros((m, k)), np.ones((n, k))
+    xv[:, 0::8] = 1
+    for j in range(1, 8):
+        xv[:, j::8] = 1.875 * 2.0**-14
+    xv[:, 128::16] *= -1  # in the second half every other far value cancels
+    (x, xv), (w, wv) = _mx(xv, 8), _mx(wv, 4)
+    want, mag = xv @ wv.T, abs(xv) @ abs(wv).T
+    y = kernels.mx_matmul(x, w)
+    _check([y], [want], [2.0**-10 * mag + 2.0**-8 * abs(want)], "bf16")
+    _check([kernels.mx_matmul(x, w, out_dtype=torch.float32)], [want], [k * 2.0**-24 * mag], "f32")
+
+
+@pytest.mark.parametrize("m", [5, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ex,ew", [(-100, 100), (100, -100), (-60, -50), (60, 50), (-126, 120)])
+def test_products_of_far_scales(m, dtype, ex, ew):
+    """Scales far from one, whose product lies in range.  f32 results are sums over the rows' values in bf16:
+    one under 2^-126 is rounded to a multiple of 2^-133 there (bf16's subnormal step: 7 bits under
+    2^-126), by 2^-134 at most, which moves a sum by at most 2^-134 of the sum of the weights' magnitudes."""
+    _say("far scales", m, dtype, ex, ew)
+    rng, n, k = _rng(m, ex + 200, ew + 200), 40, 300
+    (x, xv), (w, wv) = _mx(rng.standard_normal((m, k)) * 2.0**ex, 8), _mx(rng.standard_normal((n, k)) * 2.0**ew, 4)
+    want, mag = xv @ wv.T, abs(xv) @ abs(wv).T
+    y = kernels.mx_matmul(x, w, out_dtype=dtype)
+    f32 = k * 2.0**-24 * mag + 2.0**-134 * abs(wv).sum(axis=1)
+    _check([y], [want], [f32 if dtype == torch.float32 else 2.0**-12 * mag + 2.0**-8 * abs(want)], "matmul")
+
+
+@pytest.mark.parametrize("ex,ew", [(-100, 100), (100, -100), (-60, -50), (60, 50), (-126, 120)])
+def test_gemv_of_far_scales(ex, ew):
+    _say("gemv of far scales", ex, ew)
+    rng, m, n, k = _rng(5, ex + 200, ew + 200), 5, 40, 304  # (rows are multiples of 8 values)
+    x, (w, wv) = _bf16(rng.standard_normal((m, k)) * 2.0**ex), _mx(rng.standard_normal((n, k)) * 2.0**ew, 4)
+    want, mag = _np(x) @ wv.T, abs(_np(x)) @ abs(wv).T
+    _check([kernels.mx_gemv(x, [w], epilogue=kernels.EPI_F32)], [want], [k * 2.0**-24 * mag], "gemv")
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        kernels.mx_gemv(x[:, :300].contiguous(), [kernels.mx_quantize(x[:, :300], 4)])
+
+
+def test_mx_gemv_far_rows():
+    """Weights past 2^31 bytes."""
+    _say("mx_gemv far rows")
+    rng, n, k = _rng(18), 1_100_000, 4096
+    codes = torch.zeros(n, k // 2, dtype=torch.uint8, device=DEV)
+    scales = torch.full((n, k // 32), 127, dtype=torch.uint8, device=DEV)
+    w, wv = _mx(0.05 * rng.standard_normal((40, k)), 4)
+    codes[-40:], scales[-40:] = w.codes, w.scales
+    big = kernels.MXTensor(codes, scales, k, 4)
+    for m in (1, 3):
+        x = _bf16(_rows(rng, m, k))
+        y = kernels.mx_gemv(x, [big], epilogue=kernels.EPI_F32)
+        want, mag = _np(x) @ wv.T, abs(_np(x)) @ abs(wv).T
+        _check([y[:, -40:]], [want], [k * 2.0**-24 * mag], "far rows")
+        assert not y[:, :-40].any()
 
 
 def test_mx_matmul_no_rows_and_far_rows():

@@ -137,6 +137,16 @@ def test_changed_weights_are_quantized_again(models):
     eng.reset()
     eng.quantize_weights()
     assert torch.equal(eng.prefill(ids).logits, 2 * first)
+    batch = FlashLoopBatchEngine(model, config=FlashLoopConfig(weight_bits=4))
+    assert torch.equal(batch.prefill(ids).logits, 2 * first)
+    tok = _ids(1)
+    before = batch.decode(tok).logits.clone()
+    with torch.no_grad():
+        model.lm_head.weight.mul_(2)
+    batch.quantize_weights()
+    batch.reset()
+    batch.prefill(ids)
+    assert torch.equal(batch.decode(tok).logits, 2 * before)  # (a new graph, not the old copies')
 
 
 def test_replaced_modules_are_refused(models):
@@ -151,6 +161,10 @@ def test_replaced_modules_are_refused(models):
     with pytest.raises(ValueError, match="plain Linear"):
         FlashLoopEngine(model, config=FlashLoopConfig(weight_bits=4))
     handle.remove()
+    eng.prefill(_ids(10))
+    eng.fused_decode, eng.use_graphs = False, False
+    with pytest.raises(RuntimeError, match="weight_bits=4"):
+        eng.decode(_ids(1))
     model.lm_head.bias = torch.nn.Parameter(torch.zeros(MODEL.vocab_size, device=DEV))
     with pytest.raises(ValueError, match="plain Linear"):
         FlashLoopEngine(model, config=FlashLoopConfig(weight_bits=4))
