@@ -74,37 +74,27 @@ __device__ __forceinline__ int x_piece(int g, int half) {
   return EXACT ? 2 * g + half : g + 4 * half;
 }
 
-// four neighbouring outputs of row m from n on
-template <bool F32>
+// Outputs of row m from n on, 16 bytes a lane at an element's alignment (rows of any length: global memory
+// takes it).  f32: four neighbours.
+typedef uint32_t mx_u32x4_t __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Bytes16 {
+  mx_u32x4_t v;
+};
+
 __device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const mx_f32x4_t& v) {
   if (m >= a.m || n >= a.n) return;
-  const int64_t o = m * a.y_stride + n;
-  if constexpr (F32) {
-    float* y = static_cast<float*>(a.y) + o;
-    if (n + 4 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
-      *reinterpret_cast<float4*>(y) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.n) y[i] = v[i];
-    }
+  float* y = static_cast<float*>(a.y) + m * a.y_stride + n;
+  if (n + 4 <= a.n) {
+    reinterpret_cast<Bytes16*>(y)->v = __builtin_bit_cast(mx_u32x4_t, v);
   } else {
-    uint16_t* y = static_cast<uint16_t*>(a.y) + o;
-    uint16_t h[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = f32_to_bf16_rne(v[i]);
-    if (n + 4 <= a.n && reinterpret_cast<uintptr_t>(y) % 8 == 0) {
-      *reinterpret_cast<uint2*>(y) = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + i < a.n) y[i] = h[i];
-    }
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.n) y[i] = v[i];
   }
 }
 
-// The same of two groups of 16 n side by side (v, u): the odd rows of 16 lanes change their v for the u of
-// the even ones, so that a lane holds eight neighbours of one group and the four lanes of an m 32.
+// bf16, of two groups of 16 n side by side (v, u): the odd rows of 16 lanes change their v for the u of the even
+// ones, so that a lane holds eight neighbours of one group and the four lanes of an m 32.
 __device__ __forceinline__ void store8(const MmArgs& a, int64_t m, int n, int g, const mx_f32x4_t& v, const mx_f32x4_t& u) {
   const auto pair = [](float lo, float hi) {
     typedef float f32x2_t __attribute__((ext_vector_type(2)));
@@ -113,12 +103,12 @@ __device__ __forceinline__ void store8(const MmArgs& a, int64_t m, int n, int g,
   };
   const auto p = __builtin_amdgcn_permlane16_swap(pair(v[0], v[1]), pair(u[0], u[1]), false, false);
   const auto q = __builtin_amdgcn_permlane16_swap(pair(v[2], v[3]), pair(u[2], u[3]), false, false);
-  const uint32_t w[4] = {p[0], q[0], p[1], q[1]};
+  const mx_u32x4_t w = {p[0], q[0], p[1], q[1]};
   n += 16 * (g & 1) + 8 * (g >> 1);
   if (m >= a.m || n >= a.n) return;
   uint16_t* y = static_cast<uint16_t*>(a.y) + m * a.y_stride + n;
-  if (n + 8 <= a.n && reinterpret_cast<uintptr_t>(y) % 16 == 0) {
-    *reinterpret_cast<uint4*>(y) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (n + 8 <= a.n) {
+    reinterpret_cast<Bytes16*>(y)->v = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -339,8 +329,8 @@ __global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArg
         const int64_t row = tm * BM + xrow + 16 * m;
         const int col = tn * BN + wn * (BN / WN) + 16 * n;
         if constexpr (F32) {
-          store4<F32>(a, row, col + 4 * g, acc[n][m]);
-          store4<F32>(a, row, col + 16 + 4 * g, acc[n + 1][m]);
+          store4(a, row, col + 4 * g, acc[n][m]);
+          store4(a, row, col + 16 + 4 * g, acc[n + 1][m]);
         } else {
           store8(a, row, col, g, acc[n][m], acc[n + 1][m]);
         }
