@@ -14,16 +14,16 @@
 //
 // A workgroup's tile is BN rows of W by BM rows of X, K in steps of 128 through LDS.  The operands go from
 // memory to LDS without passing registers, two steps ahead, in three buffers (one barrier a step);
-// 16-byte pieces of a row are stored at a place that depends on the row, so that the 16 lanes of a read
-// phase meet all banks.  Scales come four steps at a time (a row's 16 bytes).  Rows past the matrix read
+// 16-byte pieces of a row are stored at a place that depends on the row, so that the lanes of a read
+// meet all banks.  Scales come four steps at a time (a row's 16 bytes).  Rows past the matrix read
 // as zeros.  The largest tile takes the LDS of a CU: its eight waves alternate between reading and
 // multiplying, and it goes on to further tiles, whose first steps are on their way while it stores.
 //
 // What bounds it: with operands in registers the instruction reaches 3500-3750 TFLOP/s on random codes (4700
-// on zeros, by its power).  8192^3 takes 359 us (3060 TFLOP/s), 306 without the transfers, 311 without the LDS
-// reads, 273 without the products, and 278 with nothing but the products and barriers: the reading and
-// the multiplying turns are about equally long.  8192 x 2048 -> 5632 79-90 us (2100-2390; 704 tiles in three
-// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 68-73.  The bf16 library product
+// on zeros, by its power).  8192^3 takes 355 us (3100 TFLOP/s; in parts, on a build at 359: 306 without the transfers, 311 without the LDS
+// reads, 273 without the products, and 278 with nothing but the products and barriers): the reading and
+// the multiplying turns are about equally long.  8192 x 2048 -> 5632 79-86 us (2200-2390; 704 tiles in three
+// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 67-73.  The bf16 library product
 // of the three: 777-816, 174-185, 132-137 us.
 #include <algorithm>
 
@@ -144,6 +144,11 @@ __device__ __forceinline__ void to_lds(mx_i32x4_t r, uint32_t voff, uint32_t sof
                  : "memory");
 }
 
+// A piece of a W row (four of 16 bytes) lies at its number xor this, one of an X row (eight) at its number xor
+// (row / 2) % 8.  A 16-byte LDS read serves 16 lanes at a time, of rows 0-3 and 12-15 of one k group and 4-11
+// of the next: their pieces then cover all 64 banks (with (row / 4) % 4 here, two of a bank).
+__device__ __forceinline__ int w_turn(int row) { return (4 - (row >> 2)) & 3; }
+
 template <int BN, int BM, int WN, int WM, int KS>
 struct TileGeom {
   static constexpr int kWaves = WN * WM;  // of one of the KS groups that divide K
@@ -199,7 +204,7 @@ __global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArg
   uint32_t wv[G::kWLoads], xv[G::kXLoads], sv[G::kSLoads];
 #pragma unroll
   for (int j = 0; j < G::kWLoads; ++j) {
-    const int p = (wave * G::kWLoads + j) * 64 + lane, row = p / 4, c = (p & 3) ^ ((row >> 2) & 3);
+    const int p = (wave * G::kWLoads + j) * 64 + lane, row = p / 4, c = (p & 3) ^ w_turn(row);
     wv[j] = static_cast<uint32_t>(row) * static_cast<uint32_t>(blocks) * 16u + 16u * c;
   }
 #pragma unroll
@@ -260,7 +265,7 @@ __global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArg
       for (int m = 0; m < G::kFM; ++m) acc[n][m] = mx_f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   };
   const int wrow = wn * (BN / WN) + i, xrow = wm * (BM / WM) + i;
-  const uint8_t* wl = lds + wrow * 64 + 16 * (g ^ ((i >> 2) & 3));
+  const uint8_t* wl = lds + wrow * 64 + 16 * (g ^ w_turn(i));
   const uint8_t* xl0 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 0) ^ ((i >> 1) & 7));
   const uint8_t* xl1 = lds + G::kWBytes + xrow * 128 + 16 * (x_piece<F32>(g, 1) ^ ((i >> 1) & 7));
   const uint32_t pick = static_cast<uint32_t>(g) | static_cast<uint32_t>(4 + g) << 8;
