@@ -65,13 +65,13 @@ __device__ __forceinline__ uint4 mx_decode8(uint2 u, float scale) {
 
 // A 64-bit value as f32, rounded to odd: the last bit is set where anything was cut off.  A later
 // rounding to fewer bits (bf16, e4m3), and any comparison with a value of fewer bits, then gives
-// what it would give for the 64-bit value itself.
+// what it would give for the 64-bit value itself.  Past f32's range it is an infinity, as of a conversion.
 __device__ __forceinline__ float round_odd(double v) {
   const float f = static_cast<float>(v);
   const double d = static_cast<double>(f);
   const uint32_t u = __float_as_uint(f);
   const uint32_t cut = (u - (fabs(d) > fabs(v) ? 1u : 0u)) | 1u;
-  return __uint_as_float(d == v ? u : cut);
+  return __uint_as_float(d == v || __builtin_isinf(f) ? u : cut);
 }
 
 }  // namespace fl

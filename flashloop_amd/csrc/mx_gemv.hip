@@ -548,8 +548,9 @@ int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_s
   const std::string w(who);
   FL_REQUIRE(x && codes && scales && outputs, w + ": null x/codes/scales/outputs");
   FL_REQUIRE(m >= 1 && m <= kMaxM, w + ": rows of x must be 1..8");
-  FL_REQUIRE(k > 0 && k % 8 == 0 && k <= FL_MX_MAX_K && n > 0 && n <= 0x7FFFFFFF - 64,
-             w + ": K must be a multiple of 8 (up to 2^20) and N positive");
+  // (a grid has at most 2^32 threads, 48 for each of N)
+  FL_REQUIRE(k > 0 && k % 8 == 0 && k <= FL_MX_MAX_K && n > 0 && n <= (1 << 26),
+             w + ": K must be a multiple of 8 (up to 2^20) and N positive (up to 2^26)");
   FL_REQUIRE(x_stride >= k && x_stride <= 0x7FFFFFFF / (4 * kMaxM) && out_stride >= n, w + ": bad row strides");
   FL_REQUIRE(reinterpret_cast<uintptr_t>(x) % 16 == 0 && (x_stride * (x_is_f32 ? 4 : 2)) % 16 == 0,
              w + ": x rows must be 16-byte aligned");
@@ -618,6 +619,7 @@ extern "C" int32_t fl_mx_gemv_chain(int32_t m, int32_t k, float eps, const uint1
   FL_REQUIRE(k <= kMxChainMaxK && stride >= k && stride % 8 == 0,
              "fl_mx_gemv_chain: K must be at most 4096 and the chain row stride a multiple of 8 >= K");
   FL_REQUIRE(x == nullptr || w_a != nullptr, "fl_mx_gemv_chain: x needs its norm weight");
+  FL_REQUIRE(h_out == nullptr || (h_out != r && h_out != x), "fl_mx_gemv_chain: h_out must be neither r nor x, which every workgroup reads");
   for (const void* p : {static_cast<const void*>(x), static_cast<const void*>(r), static_cast<const void*>(w_a),
                         static_cast<const void*>(w_f), static_cast<const void*>(w_b), static_cast<const void*>(h_out)})
     FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_mx_gemv_chain: every chain tensor must be 16-byte aligned");

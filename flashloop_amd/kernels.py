@@ -817,6 +817,8 @@ def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.
         raise ValueError("nothing to return: neither h nor w_b")
     r2, x2 = _chain_operands(r, x, w_a, w_f, w_b)
     m, d = r2.shape
+    if m > 0x7FFFFFFF:
+        raise ValueError(f"norm_chain_mx takes up to 2^31 - 1 rows, got {m}")
     h = torch.empty_like(r2) if want_h else None
     z = None if w_b is None else MXTensor._empty(m, d, 8, r2.device)
     if m:

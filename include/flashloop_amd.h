@@ -558,10 +558,9 @@ int32_t fl_swiglu(const uint16_t* gate, const uint16_t* up, uint16_t* out, int64
  * up) as 8-bit rows: the codes and scales that fl_mx_quantize makes of its result.
  * fl_norm_chain_mx: the chain of fl_norm_chain with z in 8 bits: h = x ? r + RMSNorm_a(x) : r; if
  * w_f: h = RMSNorm_f(h); h_out (optional) = bf16(h); z = RMSNorm_b(bf16(h)), quantised as above from
- * its unrounded value.  Sums and products are in 64 bits and only h and z are rounded (fl_norm_chain
- * rounds every norm and the sum to bf16, as the modules do).  bf16
- * tensors with row stride `stride`, d % 8 == 0, d <= 8192, 16-byte aligned; without
- * w_b there is no z.
+ * its unrounded value (an infinity past f32's range).  Sums and products are in 64 bits and only h and z
+ * are rounded (fl_norm_chain rounds every norm and the sum to bf16, as the modules do).  bf16 tensors with
+ * row stride `stride`, d % 8 == 0, d <= 8192, 16-byte aligned; without w_b there is no z.
  */
 int32_t fl_mx_quantize(const void* x, int32_t x_is_f32, int64_t x_stride, int64_t rows, int32_t k,
                        int32_t bits, uint8_t* codes, uint8_t* scales, void* stream);
@@ -576,10 +575,11 @@ int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, co
  * fl_mx_gemv: y[m, n] = sum_k bf16(x[m, k]) * W[n, k] for the 1..8 rows of a decode step and 4-bit
  * weights, with the arguments and epilogues of fl_gemv_bf16 (codes / scales in place of weights).
  * Sums and epilogues are fp32 and each output is rounded once (the bf16 Linear's rounding in
- * between has no counterpart here); epilogue 1 gives the fp32 sums.  K % 8 == 0, any N (RoPE: a
+ * between has no counterpart here); epilogue 1 gives the fp32 sums.  K % 8 == 0, any N up to 2^26 (RoPE: a
  * multiple of head_dim, itself a multiple of 8).  x rows 16-byte aligned.
  * fl_mx_gemv_chain: the chain of fl_norm_chain_mx, in fp32 and with z rounded to bf16, then
- * fl_mx_gemv of z (h when w_b is NULL), in one launch; K <= 4096.
+ * fl_mx_gemv of z (h when w_b is NULL), in one launch; K <= 4096.  Every workgroup reads r and x, so h_out
+ * must be neither of them.
  * fl_mx_matmul: y[m, n] = sum_k X[m, k] * W[n, k] for 8-bit rows X and 4-bit weights W, any m, n
  * and k, fp32 sums, y bf16 or f32 [m, n] with row stride y_stride.  f32 results sum exact products
  * (values of X under 2^-126 as bf16's subnormals); for bf16 results the matrix instruction

@@ -204,6 +204,21 @@ def test_norm_chain_mx(rows, d, add, final):
     assert none is None and torch.equal(h2, h)
 
 
+def test_norm_chain_mx_past_f32():
+    """A value of z past f32's range marks its block, as an infinity does (here 8 * 2^127 and -8 * 2^127
+    next to the row's zeros; the second row stays at 1 * 2^127, which f32 holds)."""
+    _say("norm_chain_mx past f32")
+    r = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
+    r[0, 40], r[1] = 1, 1
+    w_b = torch.full((64,), 2.0**127, dtype=torch.bfloat16, device=DEV)
+    for sign in (1, -1):
+        _, z = kernels.norm_chain_mx(sign * r, w_b=w_b, eps=0.0)
+        assert z.scales.tolist() == [[1, 255, 1, 1], [246, 246, 1, 1]]
+        # (a zero keeps its sign: sign * 0 is code 0 or 0x80; the marked block's codes are 0)
+        assert not z.codes[0, 32:].any() and not (z.codes[0, :32] & 127).any()
+        assert (z.codes[1, :64] == (0x78 if sign > 0 else 0xF8)).all()
+
+
 def test_norm_chain_mx_odd_rows():
     """Rows of zeros, and a row with a NaN or an infinity, which stays one row's matter."""
     _say("norm_chain_mx odd rows")

@@ -50,6 +50,8 @@ def test_front_end_refusals():
         kernels.mx_gemv(x, [w])
     with pytest.raises(RuntimeError, match="device"):
         kernels.norm_chain_mx(x, w_b=gain, eps=1e-6)
+    with pytest.raises(ValueError, match="rows"):
+        kernels.norm_chain_mx(torch.empty(1 << 32, 8, dtype=torch.bfloat16, device="meta"), w_f=gain[:8].to("meta"), eps=1e-6)
     with pytest.raises(RuntimeError, match="device"):
         kernels.mx_swiglu(x, x)
     with pytest.raises(ValueError, match="one shape"):
@@ -163,6 +165,7 @@ def test_c_abi_gemv_refusals():
     says(gemv(k=60), b"multiple of 8")
     says(gemv(k=(1 << 20) + 8, stride=1 << 21), b"2^20")
     says(gemv(n=0), b"positive")
+    says(gemv(n=(1 << 26) + 1, ostride=1 << 27), b"2^26")
     says(gemv(stride=56), b"strides")
     says(gemv(ostride=7), b"strides")
     says(gemv(stride=1 << 27), b"strides")
@@ -189,6 +192,8 @@ def test_c_abi_gemv_refusals():
     says(chain(x=0x200), b"norm weight")
     says(chain(r=0x108), b"16-byte")
     says(chain(h=0x208), b"16-byte")
+    says(chain(h=0x100), b"neither r nor x")
+    says(chain(x=0x200, wa=0x300, h=0x200), b"neither r nor x")
     says(chain(m=9), b"1..8")
 
 
