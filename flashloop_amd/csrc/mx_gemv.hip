@@ -541,6 +541,13 @@ void mx_launch_epi(int epilogue, const MxGemvArgs& a, const NormArgs& c, hipStre
   }
 }
 
+// Rows of `cols` elements, `stride` apart, at p and at q share no memory.
+bool apart(const void* p, int64_t p_stride, int64_t p_cols, int p_size, const void* q, int64_t q_stride, int64_t q_cols, int q_size,
+           int rows) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a == 0 || b == 0 || a + ((rows - 1) * p_stride + p_cols) * p_size <= b || b + ((rows - 1) * q_stride + q_cols) * q_size <= a;
+}
+
 int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_stride, int32_t m, int32_t k,
                      const uint8_t* const* codes, const uint8_t* const* scales, int32_t n, int32_t epilogue,
                      void* const* outputs, int64_t out_stride, const uint16_t* addend, int64_t addend_stride,
@@ -574,6 +581,9 @@ int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_s
     // (a unit's rows lie within one buffer of 2^31 bytes)
     FL_REQUIRE((static_cast<int64_t>(head_dim) + 64) * a.blocks * 16 < 0x7FFFFFFF, w + ": head too wide for this K");
   }
+  for (int i = 0; i < (epilogue == kEpiRope ? 3 : 1); ++i)
+    FL_REQUIRE(apart(outputs[i], out_stride, n, epilogue == kEpiF32 ? 4 : 2, x, x_stride, k, x_is_f32 ? 4 : 2, m),
+               w + ": an output lies on x, which every workgroup reads");
   a.x = x;
   a.x_f32 = x_is_f32 ? 1 : 0;
   a.x_stride = x_stride;
@@ -619,7 +629,6 @@ extern "C" int32_t fl_mx_gemv_chain(int32_t m, int32_t k, float eps, const uint1
   FL_REQUIRE(k <= kMxChainMaxK && stride >= k && stride % 8 == 0,
              "fl_mx_gemv_chain: K must be at most 4096 and the chain row stride a multiple of 8 >= K");
   FL_REQUIRE(x == nullptr || w_a != nullptr, "fl_mx_gemv_chain: x needs its norm weight");
-  FL_REQUIRE(h_out == nullptr || (h_out != r && h_out != x), "fl_mx_gemv_chain: h_out must be neither r nor x, which every workgroup reads");
   for (const void* p : {static_cast<const void*>(x), static_cast<const void*>(r), static_cast<const void*>(w_a),
                         static_cast<const void*>(w_f), static_cast<const void*>(w_b), static_cast<const void*>(h_out)})
     FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_mx_gemv_chain: every chain tensor must be 16-byte aligned");
@@ -628,6 +637,11 @@ extern "C" int32_t fl_mx_gemv_chain(int32_t m, int32_t k, float eps, const uint1
   const int32_t rc = make_mx_args(a, r, 0, stride, m, k, codes, scales, n, epilogue, outputs, out_stride, addend,
                                   addend_stride, rope_cos, rope_sin, head_dim, "fl_mx_gemv_chain");
   if (rc != FL_OK) return rc;
+  FL_REQUIRE(apart(h_out, stride, k, 2, r, stride, k, 2, m) && apart(h_out, stride, k, 2, x, stride, k, 2, m),
+             "fl_mx_gemv_chain: h_out lies on r or x, which every workgroup reads");
+  for (int i = 0; i < (epilogue == kEpiRope ? 3 : 1); ++i)
+    FL_REQUIRE(apart(outputs[i], out_stride, n, epilogue == kEpiF32 ? 4 : 2, x, stride, k, 2, m),
+               "fl_mx_gemv_chain: an output lies on x, which every workgroup reads");
   const NormArgs c{k, eps, x, r, w_a, w_f, w_b, h_out, nullptr, stride};
   mx_launch_epi<true>(epilogue, a, c, static_cast<hipStream_t>(stream));
   FL_LAUNCH_CHECK("fl_mx_gemv_chain");

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 
 import torch
 
@@ -694,22 +695,23 @@ class MXTensor:
         if not 0 < cols <= MX_MAX_K:
             raise ValueError(f"cols must be 1..{MX_MAX_K}, got {cols}")
         kp = -(-cols // MX_PAD) * MX_PAD
-        rows = codes.shape[0] if codes.ndim == 2 else -1
-        for t, width, name in ((codes, kp * bits // 8, "codes"), (scales, kp // MX_BLOCK, "scales")):
-            if t.dtype != torch.uint8 or t.ndim != 2 or t.shape[1] != width or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous uint8 [rows, {width}], got {t.dtype} {tuple(t.shape)}")
-        if scales.shape[0] != rows or codes.device != scales.device:
+        cs, ss = codes.shape, scales.shape
+        for t, shape, width, name in ((codes, cs, kp * bits // 8, "codes"), (scales, ss, kp // MX_BLOCK, "scales")):
+            if t.dtype is not torch.uint8 or len(shape) != 2 or shape[1] != width or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous uint8 [rows, {width}], got {t.dtype} {tuple(shape)}")
+        device = codes.device
+        if ss[0] != cs[0] or scales.device != device:
             raise ValueError("codes and scales must have the same rows and device")
-        self.codes, self.scales, self.cols, self.bits = codes, scales, cols, bits
-        self.rows, self.device = rows, codes.device
+        self.codes, self.scales, self.cols, self.bits, self.rows, self.device = codes, scales, cols, bits, cs[0], device
 
     @classmethod
-    def _empty(cls, rows: int, cols: int, bits: int, device) -> "MXTensor":
+    def _empty(cls, rows: int, cols: int, bits: int, like: torch.Tensor) -> "MXTensor":
+        """One without values, on the device of ``like``."""
         t = cls.__new__(cls)
         kp = -(-cols // MX_PAD) * MX_PAD
-        t.codes = torch.empty((rows, kp * bits // 8), dtype=torch.uint8, device=device)
-        t.scales = torch.empty((rows, kp // MX_BLOCK), dtype=torch.uint8, device=device)
-        t.cols, t.bits, t.rows, t.device = cols, bits, rows, device
+        t.codes = like.new_empty((rows, kp * bits // 8), dtype=torch.uint8)
+        t.scales = like.new_empty((rows, kp // MX_BLOCK), dtype=torch.uint8)
+        t.cols, t.bits, t.rows, t.device = cols, bits, rows, like.device
         return t
 
     @property
@@ -759,7 +761,7 @@ def mx_quantize(x: torch.Tensor, bits: int = 8) -> MXTensor:
     if x2.stride(1) != 1:  # (rows may lie at any distance, their values next to each other)
         x2 = x2.contiguous()
     rows, k = x2.shape
-    t = MXTensor._empty(rows, k, bits, x2.device)
+    t = MXTensor._empty(rows, k, bits, x2)
     if rows:
         _launch(t.device, "fl_mx_quantize", load().fl_mx_quantize, x2.data_ptr(), f32, x2.stride(0), rows, k, bits,
                 t.codes.data_ptr(), t.scales.data_ptr())
@@ -768,7 +770,7 @@ def mx_quantize(x: torch.Tensor, bits: int = 8) -> MXTensor:
 
 def mx_dequantize(t: MXTensor) -> torch.Tensor:
     """The values of ``t`` as bf16 ``[rows, cols]`` (``fl_mx_dequantize``)."""
-    out = torch.empty((t.rows, t.cols), dtype=torch.bfloat16, device=t.device)
+    out = t.codes.new_empty((t.rows, t.cols), dtype=torch.bfloat16)
     if t.rows:
         _launch(t.device, "fl_mx_dequantize", load().fl_mx_dequantize, t.codes.data_ptr(), t.scales.data_ptr(), t.rows, t.cols,
                 t.bits, out.data_ptr(), t.cols)
@@ -783,7 +785,7 @@ def mx_swiglu(gate: torch.Tensor, up: torch.Tensor) -> MXTensor:
         raise ValueError("gate and up must be bf16 of one shape on one device")
     g2, u2 = _contiguous_rows(gate), _contiguous_rows(up)
     rows, k = g2.shape
-    t = MXTensor._empty(rows, k, 8, g2.device)
+    t = MXTensor._empty(rows, k, 8, g2)
     if rows:
         _launch(t.device, "fl_mx_swiglu", load().fl_mx_swiglu, g2.data_ptr(), u2.data_ptr(), k, rows, k, t.codes.data_ptr(),
                 t.scales.data_ptr())
@@ -820,7 +822,7 @@ def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.
     if m > 0x7FFFFFFF:
         raise ValueError(f"norm_chain_mx takes up to 2^31 - 1 rows, got {m}")
     h = torch.empty_like(r2) if want_h else None
-    z = None if w_b is None else MXTensor._empty(m, d, 8, r2.device)
+    z = None if w_b is None else MXTensor._empty(m, d, 8, r2)
     if m:
         codes, scales = (None, None) if z is None else (z.codes.data_ptr(), z.scales.data_ptr())
         _launch(r2.device, "fl_norm_chain_mx", load().fl_norm_chain_mx, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f),
@@ -828,8 +830,10 @@ def norm_chain_mx(r: torch.Tensor, *, x: torch.Tensor | None = None, w_a: torch.
     return h, z
 
 
-def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out):
-    """(outputs, what the caller holds until the launch, arguments) of the 4-bit GEMVs, checked."""
+def _mx_gemv_operands(rows, weights, epilogue, addend, rope, head_dim, out):
+    """(outputs, what the caller holds until the launch, arguments) of the 4-bit GEMVs of ``rows`` [M, K],
+    checked."""
+    (m, k), device = rows.shape, rows.device
     need = 3 if epilogue == EPI_ROPE else (2 if epilogue == EPI_SWIGLU else 1)
     if not EPI_PLAIN <= epilogue <= EPI_ROPE or len(weights) != need:
         raise ValueError(f"epilogue {epilogue} with {len(weights)} weight(s)")
@@ -844,9 +848,9 @@ def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, o
             raise ValueError(f"out must be one [{m}, {n}] tensor on {device}")
         outs = (out,)
     elif need == 3:
-        outs = torch.empty((3, m, n), dtype=dt, device=device).unbind(0)
+        outs = rows.new_empty((3, m, n), dtype=dt).unbind(0)
     else:
-        outs = (torch.empty((m, n), dtype=dt, device=device),)
+        outs = (rows.new_empty((m, n), dtype=dt),)
     add = cos = sin = None
     if epilogue == EPI_ADD:
         if addend is None:
@@ -857,9 +861,9 @@ def _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, o
             raise ValueError("the epilogue takes rope tables")
         cos, sin = (_operand(t, m, head_dim, "rope table", device) for t in rope)
     # one array of pointers: codes, scales, outputs
-    table = (C.c_void_p * (2 * need + len(outs)))(*[w.codes.data_ptr() for w in weights], *[w.scales.data_ptr() for w in weights],
-                                                  *[o.data_ptr() for o in outs])
-    at = C.addressof(table)
+    table = array("Q", [w.codes.data_ptr() for w in weights] + [w.scales.data_ptr() for w in weights] +
+                  [o.data_ptr() for o in outs])
+    at = table.buffer_info()[0]
     return outs, (add, cos, sin, table), (at, at + 8 * need, n, epilogue, at + 16 * need, n, _p(add), n, _p(cos), _p(sin), head_dim)
 
 
@@ -885,7 +889,7 @@ def mx_gemv(x: torch.Tensor, weights, *, epilogue: int = EPI_PLAIN, addend: torc
     device, f32 = x2.device, x2.dtype is torch.float32
     if not f32 and x2.dtype is not torch.bfloat16:
         raise ValueError("x must be bf16 or f32")
-    outs, held, args = _mx_gemv_operands(device, m, k, weights, epilogue, addend, rope, head_dim, out)
+    outs, held, args = _mx_gemv_operands(x2, weights, epilogue, addend, rope, head_dim, out)
     _launch(device, "fl_mx_gemv", load().fl_mx_gemv, x2.data_ptr(), f32, k, m, k, *args)
     return outs if epilogue == EPI_ROPE else outs[0]
 
@@ -903,7 +907,7 @@ def mx_gemv_chain(r: torch.Tensor, weights, *, x: torch.Tensor | None = None, w_
     if not 1 <= m <= 8:
         raise ValueError(f"mx_gemv_chain takes 1 to 8 rows, got {m}")
     device = r2.device
-    outs, held, args = _mx_gemv_operands(device, m, d, weights, epilogue, addend, rope, head_dim, out)
+    outs, held, args = _mx_gemv_operands(r2, weights, epilogue, addend, rope, head_dim, out)
     h = torch.empty_like(r2) if want_h else None
     _launch(device, "fl_mx_gemv_chain", load().fl_mx_gemv_chain, m, d, eps, _p(x2), r2.data_ptr(), _p(w_a), _p(w_f), _p(w_b),
             _p(h), d, *args)
@@ -922,7 +926,7 @@ def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.b
     device, m, n = x.device, x.rows, weight.rows
     if weight.device != device:
         raise ValueError(f"x and weight lie on different devices ({device}, {weight.device})")
-    y = torch.empty((m, n), dtype=out_dtype, device=device)
+    y = x.codes.new_empty((m, n), dtype=out_dtype)
     if m and n:
         _launch(device, "fl_mx_matmul", load().fl_mx_matmul, x.codes.data_ptr(), x.scales.data_ptr(), m, x.cols,
                 weight.codes.data_ptr(), weight.scales.data_ptr(), n, y.data_ptr(), f32, n)

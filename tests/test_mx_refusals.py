@@ -176,6 +176,10 @@ def test_c_abi_gemv_refusals():
     says(gemv(scales=arr(0, 0, 0)), b"non-null")
     says(gemv(epi=3, codes=arr(0x1000, 0, 0)), b"non-null")
     says(gemv(epi=4, outs=arr(0x7000, 0x8000, 0)), b"null output")
+    says(gemv(x=0x7000), b"output lies on x")
+    says(gemv(x=0x7010, epi=1), b"output lies on x")
+    says(gemv(x=0x6F00, m=3), b"output lies on x")
+    says(gemv(x=0x8F90, epi=4, cos=0x10, sin=0x20, outs=arr(0x7000, 0x8000, 0x9000)), b"output lies on x")
     says(gemv(epi=2), b"addend")
     says(gemv(epi=4), b"rope")
     says(gemv(epi=4, cos=0x10, sin=0x20, hd=12), b"rope")
@@ -192,8 +196,10 @@ def test_c_abi_gemv_refusals():
     says(chain(x=0x200), b"norm weight")
     says(chain(r=0x108), b"16-byte")
     says(chain(h=0x208), b"16-byte")
-    says(chain(h=0x100), b"neither r nor x")
-    says(chain(x=0x200, wa=0x300, h=0x200), b"neither r nor x")
+    says(chain(h=0x100), b"lies on r or x")
+    says(chain(x=0x200, wa=0x300, h=0x270), b"lies on r or x")
+    says(chain(r=0x7000), b"output lies on x")
+    says(chain(x=0x7000, wa=0x300), b"output lies on x")
     says(chain(m=9), b"1..8")
 
 
