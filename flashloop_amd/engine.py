@@ -25,6 +25,7 @@ decode steps in bf16 through ``fl_mx_gemv[_chain]``.
 from __future__ import annotations
 
 import gc
+import itertools
 import math
 import weakref
 from dataclasses import dataclass, field
@@ -63,24 +64,25 @@ def _is_plain(m: torch.nn.Module, kind: type) -> bool:
 
 def _mx_rows_gemv(x, weights, *, epilogue=kernels.EPI_PLAIN, addend=None, rope=None, head_dim=kernels.HEAD_DIM, out=None):
     """``kernels.mx_gemv`` for any number of rows (``x``: rows, or an 8-bit ``MXTensor``): 8-bit rows and
-    ``mx_matmul``.  ``rope`` holds a table row for every (row, head); SwiGLU gives 8-bit rows, as the
-    next product takes them."""
+    one ``mx_matmul`` with ``weights[0]`` (q, k and v, or gate and up, one under the other).  ``rope`` holds a
+    table row for every (row, head); SwiGLU gives 8-bit rows, as the next product takes them."""
     if not isinstance(x, kernels.MXTensor):
         x = kernels.mx_quantize(x, 8)
     if epilogue == kernels.EPI_F32:
         y = kernels.mx_matmul(x, weights[0], out_dtype=torch.float32)
         return y if out is None else out.copy_(y)
-    ys = [kernels.mx_matmul(x, w) for w in weights]
+    y = kernels.mx_matmul(x, weights[0])
     if epilogue == kernels.EPI_ADD:
-        return ys[0] + addend.reshape(ys[0].shape)
+        return y + addend.reshape(y.shape)
     if epilogue == kernels.EPI_SWIGLU:
-        return kernels.mx_swiglu(*ys)
+        return kernels.mx_swiglu(*y.chunk(2, dim=1))
     if epilogue == kernels.EPI_ROPE:  # (each (row, head) as a row of one head: k and v leave in q's layout)
-        q, k, v = (y.view(-1, head_dim) for y in ys)
+        rows = y.shape[0]
+        q, k, v = y.view(rows, 3, -1).transpose(0, 1).reshape(3, -1, head_dim).unbind(0)
         k_dst, v_dst = torch.empty((2, 1, *k.shape), dtype=k.dtype, device=k.device).unbind(0)
         kernels.rope_store(q, k, v, rope, k_dst, v_dst)
-        return (ys[0], *(t.view(ys[0].shape) for t in (k_dst, v_dst)))
-    return ys[0]
+        return tuple(t.view(rows, -1) for t in (q, k_dst, v_dst))
+    return y
 
 
 def _mx_rows_gemv_chain(r, weights, *, x=None, w_a=None, w_f=None, w_b=None, eps, want_h=True, **gemv):
@@ -291,6 +293,15 @@ class FlashLoopEngine:
                 raise ValueError("weight_bits=4 needs plain Linear layers without a bias")
             return kernels.mx_quantize(m.weight.detach(), 4)
 
+        def joint(**parts):
+            """The parts by name, and all of them one under the other as one matrix under their joint name."""
+            ws = list(parts.values())
+            codes, scales = (torch.cat([getattr(w, n) for w in ws]) for n in ("codes", "scales"))
+            starts = itertools.accumulate((w.rows for w in ws), initial=0)
+            views = {n: kernels.MXTensor(codes[a:a + w.rows], scales[a:a + w.rows], w.cols, 4)
+                     for (n, w), a in zip(parts.items(), starts)}
+            return {**views, "_".join(parts): kernels.MXTensor(codes, scales, ws[0].cols, 4)}
+
         def norm(m):
             w = m.weight.detach() if _is_plain(m, RMSNorm) else None
             if (w is None or w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16
@@ -306,8 +317,8 @@ class FlashLoopEngine:
             a, m = layer.self_attn, layer.mlp
             if not _is_bare(m, MLP):
                 raise ValueError("weight_bits=4 needs plain MLP modules")
-            layers.append(dict(q=linear(a.q_proj), k=linear(a.k_proj), v=linear(a.v_proj), o=linear(a.o_proj),
-                               gate=linear(m.gate_proj), up=linear(m.up_proj), down=linear(m.down_proj),
+            layers.append(dict(**joint(q=linear(a.q_proj), k=linear(a.k_proj), v=linear(a.v_proj)), o=linear(a.o_proj),
+                               **joint(gate=linear(m.gate_proj), up=linear(m.up_proj)), down=linear(m.down_proj),
                                ln1=norm(layer.input_layernorm), ln2=norm(layer.input_layernorm_2),
                                ln3=norm(layer.post_attention_layernorm), ln4=norm(layer.post_attention_layernorm_2)))
         self._mx = (layers, dict(norm=norm(self.backbone.norm), lm_head=linear(self.model.lm_head)))
@@ -411,14 +422,14 @@ class FlashLoopEngine:
 
     def _mx_layer_rows(self, w, hid, z, rope, kv, positions, eps, w_next, w_final):
         """``_layer_rows`` on 4-bit weights; ``z`` and the input norm that it returns are 8-bit rows."""
-        q, k, v = (kernels.mx_matmul(z, w[n]) for n in ("q", "k", "v"))
+        q, k, v = kernels.mx_matmul(z, w["q_k_v"]).chunk(3, dim=1)
         kernels.rope_store(q, k, v, rope, kv[0], kv[1], positions)
         heads = kv[0].shape[0]
         o = kernels.prefill_attention(q.view(q.shape[0], heads, -1).transpose(0, 1), kv[0], kv[1],
                                       kv[0].shape[-1] ** -0.5, positions)
         x = kernels.mx_matmul(kernels.mx_quantize(o, 8), w["o"])
         hid, z = kernels.norm_chain_mx(hid, x=x, w_a=w["ln2"], w_b=w["ln3"], eps=eps)
-        act = kernels.mx_swiglu(kernels.mx_matmul(z, w["gate"]), kernels.mx_matmul(z, w["up"]))
+        act = kernels.mx_swiglu(*kernels.mx_matmul(z, w["gate_up"]).chunk(2, dim=1))
         y = kernels.mx_matmul(act, w["down"])
         return kernels.norm_chain_mx(hid, x=y, w_a=w["ln4"], w_f=w_final, w_b=w_next, eps=eps)
 
@@ -676,10 +687,12 @@ class FlashLoopEngine:
         hid = h.reshape(bsz, -1)
         chained = self.fused_chain
         gemv, gemv_chain = kernels.gemv, kernels.gemv_chain
+        qkv, gate_up = ("q", "k", "v"), ("gate", "up")
         if self._mx is not None:
             gemv, gemv_chain = kernels.mx_gemv, kernels.mx_gemv_chain
             if bsz > 8:
                 gemv, gemv_chain, chained = _mx_rows_gemv, _mx_rows_gemv_chain, True
+                qkv, gate_up = ("q_k_v",), ("gate_up",)
                 rope = tuple(t.repeat_interleave(heads, dim=0) for t in rope)
             elif hid.shape[1] > 4096:  # (the longest row that the chained GEMV takes)
                 chained = False
@@ -707,7 +720,7 @@ class FlashLoopEngine:
             for li, layer in enumerate(self.layers):
                 w = layers_w[li]
                 a = layer.self_attn
-                q, k, v = chain_gemv([w["q"], w["k"], w["v"]], epilogue=kernels.EPI_ROPE, rope=rope, head_dim=hd)
+                q, k, v = chain_gemv([w[n] for n in qkv], epilogue=kernels.EPI_ROPE, rope=rope, head_dim=hd)
                 q, k, v = (t.view(bsz, heads, 1, hd) for t in (q, k, v))
                 cur_k[li][loop] = k
                 cur_v[li][loop] = v
@@ -738,7 +751,7 @@ class FlashLoopEngine:
                     projected = gemv(delta.reshape(bsz, -1), [w["o"]], epilogue=kernels.EPI_ADD,
                                              addend=src.projected_output)
                 pending = dict(x=projected, w_a=w["ln2"], w_b=w["ln3"])
-                act = chain_gemv([w["gate"], w["up"]], epilogue=kernels.EPI_SWIGLU)
+                act = chain_gemv([w[n] for n in gate_up], epilogue=kernels.EPI_SWIGLU)
                 mo = gemv(act, [w["down"]])
                 last = li == nl - 1
                 nxt = None if (last and loop == 3) else layers_w[(li + 1) % nl]["ln1"]

@@ -648,12 +648,15 @@ def rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: tuple[to
                k_dst: torch.Tensor, v_dst: torch.Tensor, positions: torch.Tensor | None = None) -> None:
     """Rotary embedding of the projected rows ``q``, ``k`` [n, H*128] (``fl_rope_store``): q in
     place, k and the plain v into rows ``positions`` (or 0..n-1) of ``k_dst`` / ``v_dst``
-    [H, T, 128].  ``rope``: cos and sin [T, 128] bf16 by position."""
+    [H, T, 128].  ``rope``: cos and sin [T, 128] bf16 by position.  q, k and v may be columns of one
+    wider matrix."""
     h, t, c = k_dst.shape
     n = q.shape[0]
+    columns = n > 0 and q.ndim == k.ndim == v.ndim == 2 and q.stride() == k.stride() == v.stride() and q.stride(1) == 1
+    stride = q.stride(0) if columns and n > 1 and q.stride(0) >= h * c else h * c
     for x, name in ((q, "q"), (k, "k"), (v, "v"), (k_dst, "k_dst"), (v_dst, "v_dst"), (rope[0], "rope cos"),
                     (rope[1], "rope sin")):
-        _require(x, torch.bfloat16, name)
+        _require(x[:1] if stride > h * c and name in "qkv" else x, torch.bfloat16, name)
     if c != HEAD_DIM or k_dst.shape != v_dst.shape or any(tuple(x.shape) != (n, h * c) for x in (q, k, v)):
         raise ValueError("q, k and v must be [n, H*128] and the destinations [H, T, 128]")
     if any(tuple(x.shape) != (t, c) for x in rope):
@@ -662,7 +665,7 @@ def rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: tuple[to
         _require(positions, torch.int32, "positions")
         if positions.numel() != n:
             raise ValueError("positions needs one entry per row")
-    rc = load().fl_rope_store(q.data_ptr(), k.data_ptr(), v.data_ptr(), h * c, q.data_ptr(), k_dst.data_ptr(),
+    rc = load().fl_rope_store(q.data_ptr(), k.data_ptr(), v.data_ptr(), stride, q.data_ptr(), k_dst.data_ptr(),
                               v_dst.data_ptr(), t * c, rope[0].data_ptr(), rope[1].data_ptr(), _p(positions), n, h, t,
                               _stream())
     check(rc, "fl_rope_store")
@@ -778,16 +781,22 @@ def mx_dequantize(t: MXTensor) -> torch.Tensor:
 
 
 def mx_swiglu(gate: torch.Tensor, up: torch.Tensor) -> MXTensor:
-    """``mx_quantize(swiglu(gate, up), 8)`` of bf16 rows [.., K] in one pass (``fl_mx_swiglu``)."""
+    """``mx_quantize(swiglu(gate, up), 8)`` of bf16 rows [.., K] in one pass (``fl_mx_swiglu``).  Columns of
+    one wider matrix are taken where they are."""
     if gate.ndim == 0 or not 0 < gate.shape[-1] <= MX_MAX_K:
         raise ValueError(f"gate needs at least one value a row, and at most {MX_MAX_K}")
     if gate.shape != up.shape or gate.dtype is not torch.bfloat16 or up.dtype is not torch.bfloat16 or gate.device != up.device:
         raise ValueError("gate and up must be bf16 of one shape on one device")
-    g2, u2 = _contiguous_rows(gate), _contiguous_rows(up)
+    stride = gate.stride(0) if gate.ndim == 2 and gate.stride() == up.stride() and gate.stride(1) == 1 else 0
+    if stride >= gate.shape[-1]:
+        g2, u2 = gate, up
+    else:
+        g2, u2 = _contiguous_rows(gate), _contiguous_rows(up)
+        stride = g2.shape[1]
     rows, k = g2.shape
     t = MXTensor._empty(rows, k, 8, g2)
     if rows:
-        _launch(t.device, "fl_mx_swiglu", load().fl_mx_swiglu, g2.data_ptr(), u2.data_ptr(), k, rows, k, t.codes.data_ptr(),
+        _launch(t.device, "fl_mx_swiglu", load().fl_mx_swiglu, g2.data_ptr(), u2.data_ptr(), stride, rows, k, t.codes.data_ptr(),
                 t.scales.data_ptr())
     return t
 

@@ -166,6 +166,40 @@ def test_mx_swiglu_is_swiglu_quantized(rows, k):
     assert (abs(_np(v) - want) <= bound)[~nan].all()
 
 
+@pytest.mark.parametrize("rows,k", [(1, 40), (3, 31), (70, 5632)])
+def test_mx_swiglu_of_columns(rows, k):
+    """gate and up as the two halves of one matrix's columns, and as rows that no kernel reads in place."""
+    _say("mx_swiglu columns", rows, k)
+    y = _bf16(_rows(_rng(rows, k, 1), rows, 2 * k))
+    want = kernels.mx_swiglu(y[:, :k].contiguous(), y[:, k:].contiguous())
+    wide = torch.empty(rows, 3 * k, dtype=torch.bfloat16, device=DEV)
+    wide[:, :2 * k] = y
+    for gate, up in (y.chunk(2, dim=1), (wide[:, :k], wide[:, k:2 * k]), (y[:, :k].contiguous(), y[:, k:]),
+                     tuple(t.t().contiguous().t() for t in y.chunk(2, dim=1))):
+        got = kernels.mx_swiglu(gate, up)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+    got = kernels.mx_swiglu(y[:1, :k].expand(rows, k), y[:1, k:].expand(rows, k))
+    assert torch.equal(got.codes, want.codes[:1].expand_as(got.codes))
+
+
+@pytest.mark.parametrize("n,h", [(1, 2), (5, 3), (300, 1)])
+def test_rope_store_of_columns(n, h):
+    """q, k and v as columns of one product equal separate ones; what lies between and beside them stays."""
+    _say("rope store columns", n, h)
+    rng, d, t = _rng(n, h, 2), h * 128, n + 7
+    y = _bf16(rng.standard_normal((n, 3 * d + 8)))
+    rope = tuple(_bf16(rng.standard_normal((t, 128))) for _ in range(2))
+    pos = torch.arange(t - n, t, dtype=torch.int32, device=DEV)
+    parts = [p.contiguous() for p in y[:, :3 * d].chunk(3, dim=1)]
+    want, got = (torch.zeros(2, h, t, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    kernels.rope_store(*parts, rope, want[0], want[1], pos)
+    before = y.clone()
+    kernels.rope_store(*y[:, :3 * d].chunk(3, dim=1), rope, got[0], got[1], pos)
+    assert torch.equal(got, want) and torch.equal(y[:, :d], parts[0]) and torch.equal(y[:, d:], before[:, d:])
+    with pytest.raises(ValueError, match="contiguous"):
+        kernels.rope_store(y[:, :2 * d:2], parts[1], parts[2], rope, got[0], got[1], pos)
+
+
 # ---------------------------------------------------------------------------- norm with 8-bit rows
 def _chain_case(rng, rows, d, add, final):
     s = dict(r=_bf16(_rows(rng, rows, d)), w_b=_bf16(1 + 0.2 * rng.standard_normal(d)))
