@@ -20,10 +20,10 @@
 // multiplying, and it goes on to further tiles, whose first steps are on their way while it stores.
 //
 // What bounds it: with operands in registers the instruction reaches 3500-3750 TFLOP/s on random codes (4700
-// on zeros, by its power).  8192^3 takes 355 us (3100 TFLOP/s; in parts, on a build at 359: 306 without the transfers, 311 without the LDS
+// on zeros, by its power).  8192^3 takes 355-396 us (2780-3100 TFLOP/s; in parts, on a build at 359: 306 without the transfers, 311 without the LDS
 // reads, 273 without the products, and 278 with nothing but the products and barriers): the reading and
-// the multiplying turns are about equally long.  8192 x 2048 -> 5632 79-86 us (2200-2390; 704 tiles in three
-// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 67-73.  The bf16 library product
+// the multiplying turns are about equally long.  8192 x 2048 -> 5632 80-90 us (2100-2360; 704 tiles in three
+// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 67-75.  The bf16 library product
 // of the three: 777-816, 174-185, 132-137 us.
 #include <algorithm>
 
