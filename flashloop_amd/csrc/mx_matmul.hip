@@ -235,13 +235,14 @@ __global__ __launch_bounds__(KS* WN* WM* kWave) void mx_matmul_tile_kernel(MmArg
     if ((rs & 3) == 0) {
       rscale ^= 1;
       const uint32_t at = lds0 + 3 * G::kBuffer + rscale * G::kScales;
+      const uint32_t off = 4u * (first_step + rs);  // (in the lane's offset: past the last row's end it is past the buffer's)
 #pragma unroll
       for (int j = 0; j < G::kSLoads; ++j) {
         const int first = (wave * G::kSLoads + j) * 16;  // (16 rows a transfer: all of W or all of X)
         if (first < BN)
-          to_lds<4>(wsr, sv[j], 4u * (first_step + rs), at + 256u * (wave * G::kSLoads + j));
+          to_lds<4>(wsr, sv[j] + off, 0, at + 256u * (wave * G::kSLoads + j));
         else
-          to_lds<4>(xsr, sv[j], 4u * (first_step + rs), at + 256u * (wave * G::kSLoads + j));
+          to_lds<4>(xsr, sv[j] + off, 0, at + 256u * (wave * G::kSLoads + j));
       }
     }
     const uint32_t at = lds0 + rbuf * G::kBuffer;
