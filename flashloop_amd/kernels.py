@@ -926,7 +926,8 @@ def mx_gemv_chain(r: torch.Tensor, weights, *, x: torch.Tensor | None = None, w_
 def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``x @ weight.T`` of 8-bit rows [M, K] and 4-bit weights [N, K] (``fl_mx_matmul``): fp32 sums,
     returned as bf16 or f32 [M, N].  Any number of rows.  An f32 result takes about twice the time and sums
-    exact products (the header says what the bf16 one may drop)."""
+    exact products; a bf16 one may drop a part that a far neighbour hides (the header says how large),
+    all that is left where far products cancel."""
     if x.bits != 8 or weight.bits != 4 or x.cols != weight.cols:
         raise ValueError(f"takes 8-bit rows and 4-bit weights of one K, got {x} and {weight}")
     f32 = out_dtype == torch.float32
