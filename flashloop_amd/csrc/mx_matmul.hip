@@ -417,9 +417,12 @@ template <int BN, int BM, int WN, int WM, int KS, bool F32, bool TURNS>
 void launch_tiles(MmArgs a, hipStream_t st) {
   a.tiles_n = (a.n + BN - 1) / BN;
   a.tiles_m = static_cast<int>((a.m + BM - 1) / BM);
-  // A workgroup takes further tiles where all CUs are in use (one workgroup each).  The two buffers of scales
-  // then want no stretch of four steps that ends after one.
-  const int tiles = a.tiles_n * a.tiles_m, grid = TURNS && a.steps % 4 != 1 ? std::min(tiles, 256) : tiles;
+  // A workgroup takes further tiles where all CUs are in use (one workgroup each), but for tiles of a single
+  // step: a buffer of scales is filled again for the stretch after the next, whose first step is requested two
+  // steps ahead, so the stretch that it held has to start three steps before that one (the later waves read
+  // a step a turn after the earlier ones).  Stretches of 1, 1, ... steps break that; 4, 1, 4, 1 do not.  us with
+  // one tile a workgroup and with further ones, 8192 x 5632 by k 640: 45, 38; 1152: 57, 49; 2176: 85, 78.
+  const int tiles = a.tiles_n * a.tiles_m, grid = TURNS && a.steps > 1 ? std::min(tiles, 256) : tiles;
   hipLaunchKernelGGL((mx_matmul_tile_kernel<BN, BM, WN, WM, KS, F32, TURNS>), dim3(grid), dim3(KS * WN * WM * kWave), 0, st, a);
 }
 

@@ -44,3 +44,25 @@ def test_mx_matmul_in_relative_norm(m, n, k, spread):
     want = xv @ wv.T
     apart = np.linalg.norm(_np(kernels.mx_matmul(x, w)) - want) / np.linalg.norm(want)
     assert apart <= np.hypot(2.0**-8 / 3**0.5, 2.0**-10), apart
+
+
+# ---------------------------------------------------------------------------- long products of many tiles
+@pytest.mark.parametrize("k", [100, 128, 640, 1100, 1152, 2048, 2100])
+def test_mx_matmul_of_several_tiles_a_workgroup(k):
+    """289 tiles of 256 x 256 (bf16), with a last tile that is partly outside, rows of one step to 17, and every
+    block's scale its own."""
+    _say("several tiles a workgroup", k)
+    rng, m, n = _rng(k, 31), 4200, 4100
+    blocks = -(-k // 32)
+
+    def operand(rows, bits):
+        scale = np.exp2(rng.integers(-6, 7, (rows, blocks)).astype(float))
+        return _mx(rng.standard_normal((rows, k)) * np.repeat(scale, 32, axis=1)[:, :k], bits)
+
+    (x, xv), (w, wv) = operand(m, 8), operand(n, 4)
+    y = kernels.mx_matmul(x, w)
+    want, mag = xv @ wv.T, abs(xv) @ abs(wv).T
+    _check([y], [want], [2.0**-10 * mag + 2.0**-8 * abs(want)], "bf16")
+    # (a wrong block anywhere shows: next to its rounding a result is off by little)
+    assert np.linalg.norm(_np(y) - want) <= np.hypot(2.0**-8 / 3**0.5, 2.0**-10) * np.linalg.norm(want)
+    assert all(torch.equal(kernels.mx_matmul(x, w), y) for _ in range(3))
