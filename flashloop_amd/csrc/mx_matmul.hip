@@ -137,16 +137,20 @@ __device__ __forceinline__ uint32_t lane_scales(const uint4& q, uint32_t pick) {
 }
 
 // Memory to LDS: lane l's 16 (or 4) bytes of buffer r at voff + soff go to lds + 16 (4) l.  The compiler counts
-// no LDS write for these, so the kernel waits for them itself (vmcnt, ahead of the step's barrier).
+// no LDS write for these, so the kernel waits for them itself (vmcnt, ahead of the step's barrier).  m0 is
+// on the clobber list for what else a compiler sets it for; its warning says that no one saves it here.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int BYTES>
 __device__ __forceinline__ void to_lds(mx_i32x4_t r, uint32_t voff, uint32_t soff, uint32_t lds) {
   if constexpr (BYTES == 16)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "memory");
+                 : "m0", "memory");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "memory");
+                 : "m0", "memory");
 }
+#pragma clang diagnostic pop
 
 // A piece of a W row (four of 16 bytes) lies at its number xor this, one of an X row (eight) at its number xor
 // (row / 2) % 8.  A 16-byte LDS read serves 16 lanes at a time, of rows 0-3 and 12-15 of one k group and 4-11
