@@ -279,6 +279,7 @@ class FlashLoopEngine:
         self.fused_chain = True
         self._wcache = None
         self._mx = None  # weight_bits=4: (per layer, norm and lm_head) as _fused_weights gives them
+        self._mx_seen = []  # the modules that they were made of
         if self.config.weight_bits == 4:
             self.quantize_weights()
 
@@ -288,7 +289,15 @@ class FlashLoopEngine:
         if self.config.weight_bits != 4:
             raise ValueError("quantize_weights needs FlashLoopConfig(weight_bits=4)")
 
-        def linear(m):
+        seen = []  # (the table that a module is in, its name there, the module, its class and weight)
+
+        def child(owner, name, kind=None):
+            m = getattr(owner, name)
+            seen.append((owner._modules, name, m, kind, None if kind in (None, MLP) else m._parameters.get("weight")))
+            return m
+
+        def linear(owner, name):
+            m = child(owner, name, torch.nn.Linear)
             if not _is_plain(m, torch.nn.Linear) or m.bias is not None:
                 raise ValueError("weight_bits=4 needs plain Linear layers without a bias")
             return kernels.mx_quantize(m.weight.detach(), 4)
@@ -302,7 +311,8 @@ class FlashLoopEngine:
                      for (n, w), a in zip(parts.items(), starts)}
             return {**views, "_".join(parts): kernels.MXTensor(codes, scales, ws[0].cols, 4)}
 
-        def norm(m):
+        def norm(owner, name):
+            m = child(owner, name, RMSNorm)
             w = m.weight.detach() if _is_plain(m, RMSNorm) else None
             if (w is None or w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16
                     or m.eps != self.backbone.norm.eps):
@@ -313,21 +323,33 @@ class FlashLoopEngine:
         if hidden % 8 or hidden > 8192 or any(l.mlp.up_proj.weight.shape[0] % 8 for l in self.layers):
             raise ValueError("weight_bits=4 needs a hidden width (up to 8192) and an MLP width that are multiples of 8")
         layers = []
-        for layer in self.layers:
-            a, m = layer.self_attn, layer.mlp
+        for i in range(len(self.layers)):
+            layer = child(self.layers, str(i))
+            a, m = child(layer, "self_attn"), child(layer, "mlp", MLP)
             if not _is_bare(m, MLP):
                 raise ValueError("weight_bits=4 needs plain MLP modules")
-            layers.append(dict(**joint(q=linear(a.q_proj), k=linear(a.k_proj), v=linear(a.v_proj)), o=linear(a.o_proj),
-                               **joint(gate=linear(m.gate_proj), up=linear(m.up_proj)), down=linear(m.down_proj),
-                               ln1=norm(layer.input_layernorm), ln2=norm(layer.input_layernorm_2),
-                               ln3=norm(layer.post_attention_layernorm), ln4=norm(layer.post_attention_layernorm_2)))
-        self._mx = (layers, dict(norm=norm(self.backbone.norm), lm_head=linear(self.model.lm_head)))
+            layers.append(dict(**joint(q=linear(a, "q_proj"), k=linear(a, "k_proj"), v=linear(a, "v_proj")), o=linear(a, "o_proj"),
+                               **joint(gate=linear(m, "gate_proj"), up=linear(m, "up_proj")), down=linear(m, "down_proj"),
+                               ln1=norm(layer, "input_layernorm"), ln2=norm(layer, "input_layernorm_2"),
+                               ln3=norm(layer, "post_attention_layernorm"), ln4=norm(layer, "post_attention_layernorm_2")))
+        self._mx = (layers, dict(norm=norm(self.backbone, "norm"), lm_head=linear(self.model, "lm_head")))
+        self._mx_seen = seen
         self._runner.reset()  # (captured steps hold the old copies)
+
+    def _check_modules(self) -> None:
+        """Refuse modules that are not those, plain and with the weights, that the 4-bit copies were made of.
+        (A replayed decode step runs what was captured, as bf16 steps do.)"""
+        if not (_calls_are_plain() and len(self.layers) == len(self._mx[0]) and all(
+                table.get(name) is m and (kind is None or _is_bare(m, kind) and m._parameters.get("weight") is w
+                                          and m._parameters.get("bias") is None and "bias" not in m.__dict__)
+                for table, name, m, kind, w in self._mx_seen)):
+            self._refuse_modules()
 
     def _lm_head(self, h: torch.Tensor) -> torch.Tensor:
         """Logits f32 of hidden rows [.., hidden]."""
         if self._mx is None:
             return self.model.lm_head(h).float()
+        self._check_modules()  # (while the GPU is at the last loop)
         rows = h.reshape(-1, h.shape[-1])
         product = kernels.mx_gemv if rows.shape[0] <= 8 else _mx_rows_gemv
         return product(rows, [self._mx[1]["lm_head"]], epilogue=kernels.EPI_F32).view(*h.shape[:-1], -1)
@@ -470,7 +492,8 @@ class FlashLoopEngine:
     def _refuse_modules(self) -> None:
         """The module path multiplies by the modules' own weights, which ``weight_bits=4`` does not."""
         if self._mx is not None:
-            raise RuntimeError("weight_bits=4: a module was replaced or hooked, or gives rows in a layout the kernels do not read")
+            raise RuntimeError("weight_bits=4: a module was replaced or hooked, or has another weight (quantize_weights takes new "
+                               "modules and weights), or gives rows in a layout the kernels do not read")
 
     def _dense_loop(self, hidden: torch.Tensor, cos, sin):
         """``dense_prefill_loop`` (flashloop/prefill.py:275-304): every row, causal attention."""
@@ -625,8 +648,10 @@ class FlashLoopEngine:
         fused kernels do not apply (``fused_decode`` off, non-bf16 weights, batch > 8; 4-bit
         weights have no module form and take any batch).  The fused form writes the logits to
         ``out`` if given."""
-        if self._mx is not None and not self.fused_decode:
-            raise RuntimeError("weight_bits=4: the module path (fused_decode off) multiplies by the modules' own weights")
+        if self._mx is not None:
+            if not self.fused_decode:
+                raise RuntimeError("weight_bits=4: the module path (fused_decode off) multiplies by the modules' own weights")
+            self._check_modules()
         if self._mx is not None or (self.fused_decode and token_ids.shape[0] <= 8 and self._fused_weights() is not None):
             return self._decode_core_fused(cache, *self._decode_inputs(token_ids, pos_t), logits_out=out)
         return self._decode_core_modules(cache, self.backbone.embed_tokens(token_ids), pos_t)
