@@ -9,7 +9,8 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from flashloop_amd import kernels  # noqa: E402
-from test_gpu_mx import DEV, _bf16, _check, _mx, _np, _rng, _rows, _say  # noqa: E402
+from test_gpu_mx import (DEV, EPI, _bf16, _chain_case, _chain_oracle, _check, _gemv_extra, _gemv_oracle, _mx, _np,  # noqa: E402
+                         _rng, _rows, _say)
 
 
 # ---------------------------------------------------------------------------- what a bf16 product drops
@@ -66,3 +67,73 @@ def test_mx_matmul_of_several_tiles_a_workgroup(k):
     # (a wrong block anywhere shows: next to its rounding a result is off by little)
     assert np.linalg.norm(_np(y) - want) <= np.hypot(2.0**-8 / 3**0.5, 2.0**-10) * np.linalg.norm(want)
     assert all(torch.equal(kernels.mx_matmul(x, w), y) for _ in range(3))
+
+
+# ---------------------------------------------------------------------------- GEMVs of ordinary widths
+def _weights(n, k, count, seed):
+    """4-bit matrices and their values in 64 bits, on the device."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    ws = [kernels.mx_quantize(0.05 * torch.randn(n, k, generator=gen, device=DEV), 4) for _ in range(count)]
+    return ws, [kernels.mx_dequantize(w).double() for w in ws]
+
+
+def _gemv_wanted(x, values, kind, s, n, hd=128):
+    ys, mags = ([_np(p @ q.t().contiguous()) for q in vs] for p, vs in ((x, values), (x.abs(), [v.abs() for v in values])))
+    return _gemv_oracle(ys, mags, x.shape[1], kind, s, x.shape[0], n, hd)
+
+
+def _gemv_checked(call, x, n, kind, seed):
+    count = {"swiglu": 2, "rope": 3}.get(kind, 1)
+    ws, values = _weights(n, x.shape[1], count, seed)
+    s = _gemv_extra(_rng(seed), kind, x.shape[0], n, 128)
+    y = call(x, ws, epilogue=EPI[kind], **s)
+    want, bound = _gemv_wanted(x.double(), values, kind, s, n)
+    _check(y if kind == "rope" else [y], want, bound, kind)
+
+
+# (8 rows, one tile or pair a unit: 256 workgroups hold N 2048, rope 1365 of each matrix)
+@pytest.mark.parametrize("kind", ["plain", "f32", "add", "swiglu", "rope"])
+@pytest.mark.parametrize("m,n,k", [(2, 2048, 2048), (8, 2176, 2048), (8, 5632, 2048), (3, 6272, 1000), (5, 4224, 4096), (8, 8192, 136),
+                                   (7, 16512, 2048), (2, 33024, 2048), (8, 49152, 200), (3, 33024, 4096), (1, 5632, 2048),
+                                   (1, 8320, 2048), (1, 16512, 4096), (1, 49152, 2048), (1, 33024, 4096)])
+def test_mx_gemv_chain_of_many_units(m, n, k, kind):
+    """Workgroups that take several units, chained: without a norm of its own the chain passes its rows on, so
+    the products' rows are known.  (A head-sized N with every epilogue: the choice of units goes by N.)"""
+    _say("mx_gemv_chain of many units", m, n, k, kind)
+    x = _bf16(_rows(_rng(m, n, k, 7), m, k))
+
+    def call(rows, ws, **kw):
+        h, y = kernels.mx_gemv_chain(rows, ws, eps=1e-6, **kw)
+        assert torch.equal(h, rows)
+        none, again = kernels.mx_gemv_chain(rows, ws, eps=1e-6, want_h=False, **kw)
+        assert none is None and all(torch.equal(a, b) for a, b in zip(*((t if isinstance(t, tuple) else [t]) for t in (y, again))))
+        return y
+
+    _gemv_checked(call, x, n, kind, n + k)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 5632, 2048), (3, 16512, 1000), (2, 33024, 2048), (8, 6272, 4096), (1, 5632, 2048), (1, 33024, 2048)])
+@pytest.mark.parametrize("add,final", [(True, False), (True, True), (False, False)])
+def test_mx_gemv_chain_with_norms_of_many_units(m, n, k, add, final):
+    """With its norms, against the product of the same rows in 64 bits: each of z's roundings moves it by 2^-8 of
+    the value, and h, where it takes the other neighbour, by 2^-7 more."""
+    _say("mx_gemv_chain with norms", m, n, k, add, final)
+    s = _chain_case(_rng(m, n, k, add, final), m, k, add, final)
+    want_h, want_z = _chain_oracle(s)
+    (w,), (v,) = _weights(n, k, 1, n)
+    h, y = kernels.mx_gemv_chain(**s, weights=[w], eps=1e-6, epilogue=kernels.EPI_F32)
+    err_h = 2.0**-7 * abs(want_h) + 2.0**-20 * (abs(_np(s["r"])) + 16)
+    assert (abs(_np(h) - want_h) <= err_h).all()
+    off = torch.from_numpy(2.0**-7 * abs(want_z) + err_h * abs(want_z) / np.maximum(abs(want_h), 1e-30)).to(DEV)
+    z, mag = torch.from_numpy(want_z).to(DEV), v.abs().t().contiguous()
+    bound = off @ mag + k * 2.0**-24 * (z.abs() @ mag) + 1e-6
+    assert ((y.double() - z @ v.t().contiguous()).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("kind", ["plain", "f32", "add", "swiglu", "rope"])
+@pytest.mark.parametrize("m,n,k", [(1, 33024, 2048), (1, 49152, 136), (1, 33024, 4096), (2, 33024, 2048), (8, 49152, 2048), (5, 33024, 4096),
+                                   (8, 32768, 1000), (8, 32640, 1000), (4, 5632, 2048), (8, 2176, 8192)])
+def test_mx_gemv_of_heads(m, n, k, kind):
+    """Head-sized matrices, and sizes on both sides of where they begin."""
+    _say("mx_gemv of heads", m, n, k, kind)
+    _gemv_checked(kernels.mx_gemv, _bf16(_rows(_rng(m, n, k, 8), m, k)), n, kind, n + k)
