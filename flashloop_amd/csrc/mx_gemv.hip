@@ -541,11 +541,17 @@ void mx_launch_epi(int epilogue, const MxGemvArgs& a, const NormArgs& c, hipStre
   }
 }
 
-// Rows of `cols` elements, `stride` apart, at p and at q share no memory.
+// Rows of `cols` elements, `stride` apart, at p and at q share no memory: one lies behind the other, or both are
+// columns of one wider matrix.
 bool apart(const void* p, int64_t p_stride, int64_t p_cols, int p_size, const void* q, int64_t q_stride, int64_t q_cols, int q_size,
            int rows) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return a == 0 || b == 0 || a + ((rows - 1) * p_stride + p_cols) * p_size <= b || b + ((rows - 1) * q_stride + q_cols) * q_size <= a;
+  const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
+  if (a == 0 || b == 0 || a + ((rows - 1) * p_stride + p_cols) * p_size <= b || b + ((rows - 1) * q_stride + q_cols) * q_size <= a)
+    return true;
+  const int64_t step = p_stride * p_size;
+  if (step == 0 || step != q_stride * q_size) return false;
+  const int64_t at = ((b - a) % step + step) % step;  // q's columns from p's first
+  return p_cols * p_size <= at && at + q_cols * q_size <= step;
 }
 
 int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_stride, int32_t m, int32_t k,
@@ -584,6 +590,15 @@ int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_s
   for (int i = 0; i < (epilogue == kEpiRope ? 3 : 1); ++i)
     FL_REQUIRE(apart(outputs[i], out_stride, n, epilogue == kEpiF32 ? 4 : 2, x, x_stride, k, x_is_f32 ? 4 : 2, m),
                w + ": an output lies on x, which every workgroup reads");
+  // (the addend's own place is fine: the thread that writes a value has read it)
+  if (epilogue == kEpiAdd)
+    FL_REQUIRE((outputs[0] == addend && out_stride == addend_stride) || apart(outputs[0], out_stride, n, 2, addend, addend_stride, n, 2, m),
+               w + ": the output lies on other values of the addend");
+  if (epilogue == kEpiRope)
+    for (int i = 0; i < 3; ++i)
+      FL_REQUIRE(apart(outputs[i], out_stride, n, 2, rope_cos, head_dim, head_dim, 2, m) &&
+                     apart(outputs[i], out_stride, n, 2, rope_sin, head_dim, head_dim, 2, m),
+                 w + ": an output lies on a rope table, which every head reads");
   a.x = x;
   a.x_f32 = x_is_f32 ? 1 : 0;
   a.x_stride = x_stride;

@@ -579,7 +579,9 @@ int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, co
  * multiple of head_dim, itself a multiple of 8).  x rows 16-byte aligned.
  * fl_mx_gemv_chain: the chain of fl_norm_chain_mx, in fp32 and with z rounded to bf16, then
  * fl_mx_gemv of z (h when w_b is NULL), in one launch; K <= 4096.
- * Every workgroup of these two reads all input rows: no output (h_out among them) may lie on them.
+ * Every workgroup of these two reads all input rows, and every head the rope tables: no output (h_out
+ * among them) may lie on them, nor on an addend but exactly in its place.  Columns of one wider matrix
+ * (rows of one stride) do not lie on each other.
  * fl_mx_matmul: y[m, n] = sum_k X[m, k] * W[n, k] for 8-bit rows X and 4-bit weights W, any m, n
  * and k, fp32 sums, y bf16 or f32 [m, n] with row stride y_stride.  f32 results sum exact products
  * (values of X under 2^-126 as bf16's subnormals).  For bf16 results the matrix instruction drops, of

@@ -137,3 +137,30 @@ def test_mx_gemv_of_heads(m, n, k, kind):
     """Head-sized matrices, and sizes on both sides of where they begin."""
     _say("mx_gemv of heads", m, n, k, kind)
     _gemv_checked(kernels.mx_gemv, _bf16(_rows(_rng(m, n, k, 8), m, k)), n, kind, n + k)
+
+
+@pytest.mark.parametrize("m", [1, 3, 8])
+def test_mx_gemv_in_a_wider_matrix_and_in_place(m):
+    """x, addend and output as columns of one matrix; the output in the addend's place; what lies beside stays."""
+    _say("mx_gemv in a wider matrix", m)
+    from flashloop_amd import _lib
+
+    rng, n, k = _rng(m, 51), 72, 136
+    w = kernels.mx_quantize(_bf16(0.05 * rng.standard_normal((n, k))), 4)
+    wide = _bf16(rng.standard_normal((m, k + 2 * n + 8)))
+    before, stride = wide.clone(), wide.shape[1]
+    x, add, out = wide[:, :k], wide[:, k:k + n], wide[:, k + n:k + 2 * n]
+    want = kernels.mx_gemv(x.contiguous(), [w], epilogue=kernels.EPI_ADD, addend=add.contiguous())
+
+    def call(y):
+        rc = _lib.load().fl_mx_gemv(x.data_ptr(), 0, stride, m, k, _lib.ptr_array((w.codes.data_ptr(),)),
+                                    _lib.ptr_array((w.scales.data_ptr(),)), n, kernels.EPI_ADD, _lib.ptr_array((y.data_ptr(),)),
+                                    stride, add.data_ptr(), stride, None, None, 128, torch.cuda.current_stream().cuda_stream)
+        _lib.check(rc, "fl_mx_gemv")
+
+    call(out)
+    before[:, k + n:k + 2 * n] = want
+    assert torch.equal(wide, before)
+    call(add)
+    before[:, k:k + n] = want
+    assert torch.equal(wide, before)

@@ -209,3 +209,27 @@ def test_weight_bits_is_16_or_4():
     assert FlashLoopConfig().weight_bits == 16 and FlashLoopConfig(weight_bits=4).weight_bits == 4
     with pytest.raises(ValueError, match="weight_bits"):
         FlashLoopConfig(weight_bits=8)
+
+
+@needs_library
+def test_c_abi_gemv_refuses_outputs_on_the_epilogue_operands():
+    lib = _lib.load()
+    arr = lambda *p: C.cast(_lib.ptr_array(p), _lib._PP)  # noqa: E731
+    codes, scales = arr(0x1000, 0x2000, 0x3000), arr(0x4000, 0x5000, 0x6000)
+
+    def gemv(x=0x100, stride=64, m=3, epi=2, outs=(0x7000, 0x8000, 0x9000), ostride=8, add=None, astride=8, cos=0x20000, sin=0x30000):
+        return lib.fl_mx_gemv(x, 0, stride, m, 64, codes, scales, 8, epi, arr(*outs), ostride, add, astride, cos, sin, 8, None)
+
+    def says(rc, text):
+        assert rc == _lib.FL_E_INVALID and text in lib.fl_last_error(), (rc, lib.fl_last_error())
+
+    says(gemv(add=0x7002), b"addend")  # one value on
+    says(gemv(add=0x6FF0), b"addend")  # a row before
+    says(gemv(add=0x7000, astride=16), b"addend")  # the same place in other rows
+    says(gemv(ostride=24, add=0x700E, astride=24), b"addend")  # columns of one matrix that share one
+    for table in ("cos", "sin"):
+        says(gemv(epi=4, **{table: 0x8010}), b"rope table")
+    # columns of one matrix that share some with x, on either side (rows of 256 bytes, x 128 of them)
+    says(gemv(epi=0, x=0x7000, stride=128, outs=(0x7070, 0, 0), ostride=128), b"output lies on x")
+    says(gemv(epi=0, x=0x7000, stride=128, outs=(0x6FF2, 0, 0), ostride=128), b"output lies on x")
+    says(gemv(epi=1, x=0x7000, stride=128, outs=(0x70F0, 0, 0), ostride=64), b"output lies on x")
