@@ -13,7 +13,7 @@
 // instruction is taken for its rate all the same, four times that of exact products: an f32 result has
 // those, for a caller to round.
 // f32 results: every value is exact in bf16 (but for rows' values under 2^-126, which become multiples of
-// 2^-133), so the operands are widened in registers and v_mfma_f32_16x16x32_bf16 sums exact products in
+// 2^-133, and 2^128, to which finite values next to f32's largest are rounded: an infinity), so the operands are widened in registers and v_mfma_f32_16x16x32_bf16 sums exact products in
 // fp32 (a quarter of the rate).
 //
 // A workgroup's tile is BN rows of W by BM rows of X, K in steps of 128 through LDS.  The operands go from

@@ -575,7 +575,8 @@ int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, co
  * fl_mx_gemv: y[m, n] = sum_k bf16(x[m, k]) * W[n, k] for the 1..8 rows of a decode step and 4-bit
  * weights, with the arguments and epilogues of fl_gemv_bf16 (codes / scales in place of weights).
  * Sums and epilogues are fp32 and each output is rounded once (the bf16 Linear's rounding in
- * between has no counterpart here); epilogue 1 gives the fp32 sums.  K % 8 == 0, any N up to 2^26 (RoPE: a
+ * between has no counterpart here); epilogue 1 gives the fp32 sums.  A weight that its 4 bits round to
+ * 2^128 (from 1.75 * 2^127 on) is an infinity, as in bf16.  K % 8 == 0, any N up to 2^26 (RoPE: a
  * multiple of head_dim, itself a multiple of 8).  x rows 16-byte aligned.
  * fl_mx_gemv_chain: the chain of fl_norm_chain_mx, in fp32 and with z rounded to bf16, then
  * fl_mx_gemv of z (h when w_b is NULL), in one launch; K <= 4096.
@@ -584,7 +585,7 @@ int32_t fl_norm_chain_mx(int32_t m, int32_t d, double eps, const uint16_t* x, co
  * (rows of one stride) do not lie on each other.
  * fl_mx_matmul: y[m, n] = sum_k X[m, k] * W[n, k] for 8-bit rows X and 4-bit weights W, any m, n
  * and k, fp32 sums, y bf16 or f32 [m, n] with row stride y_stride.  f32 results sum exact products
- * (values of X under 2^-126 as bf16's subnormals).  For bf16 results the matrix instruction drops, of
+ * (values of X under 2^-126 as bf16's subnormals, one of 2^128 as an infinity).  For bf16 results the matrix instruction drops, of
  * every eight neighbouring products, what lies under 2^-13 of the largest of them: less than 2^-10 of the
  * sum of the products' magnitudes, but any part of a result whose far products cancel (normal rows with
  * channels e^N(0, s^2) apart: 2^-18, 2^-16, 2^-14 of the results in norm at s = 0, 1, 2, under the 2^-9.2 of

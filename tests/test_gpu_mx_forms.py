@@ -164,3 +164,27 @@ def test_mx_gemv_in_a_wider_matrix_and_in_place(m):
     call(add)
     before[:, k:k + n] = want
     assert torch.equal(wide, before)
+
+
+def test_products_of_values_next_to_the_largest():
+    """Values that their rounding takes to 2^128 -- in 8 bits from 1.9375 * 2^127 on (halfway from 240 to 256), in 4
+    bits from 1.75 * 2^127 (halfway from 3 to 4) -- are infinities in bf16, and so in dequantised rows, in
+    GEMVs and in f32 products; the bf16 product takes them as they are."""
+    _say("values next to the largest")
+    far = {8: (1.9375, 1.875), 4: (1.75, 1.5)}
+    for bits, (up, down) in far.items():
+        rows = torch.zeros(2, 64, device=DEV)
+        rows[0, 3], rows[1, 40] = up * 2.0**127, -down * 2.0**127
+        t = kernels.mx_quantize(rows, bits)
+        v = kernels.mx_dequantize(t)
+        assert v[0, 3] == float("inf") and v[1, 40] == -down * 2.0**127
+        if bits == 8:
+            other = kernels.mx_quantize(torch.full((3, 64), 2.0**-100, device=DEV), 4)
+            exact, short = (kernels.mx_matmul(t, other, out_dtype=d) for d in (torch.float32, torch.bfloat16))
+        else:
+            ones = torch.full((3, 64), 2.0**-100, device=DEV)
+            exact, short = (kernels.mx_matmul(kernels.mx_quantize(ones, 8), t, out_dtype=d).t() for d in (torch.float32, torch.bfloat16))
+            y = kernels.mx_gemv(ones, [t], epilogue=kernels.EPI_F32)
+            assert (y[:, 0] == float("inf")).all() and (y[:, 1] == -down * 2.0**27).all()
+        assert (exact[0] == float("inf")).all() and (exact[1] == -down * 2.0**27).all()
+        assert (short[0] == 2.0**28).all() and (short[1] == -down * 2.0**27).all()
