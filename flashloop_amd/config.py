@@ -17,7 +17,8 @@ class FlashLoopConfig:
     enable_sparse_decode: bool = True
     quantize_cross_loop_kv: bool = True
     decode_capacity: int = 4096  # packed-prefix room reserved for decode tokens
-    weight_bits: int = 16  # Linear weights: bf16, or a microscaled copy of 4 bits
+    weight_bits: int = 16  # Linear weights: bf16, or a microscaled copy of 4 bits (then rows of prompts, and of
+    # decode steps of more than 8 sequences, are rounded to 8 bits where they meet them)
 
     def __post_init__(self) -> None:
         if not 0.0 < self.prefill_fraction_loop4 <= self.prefill_fraction_loop3 <= 1.0:

@@ -19,7 +19,12 @@ residuals (``fl_norm_chain``) and SwiGLU (``fl_swiglu``) are HIP kernels.
 With ``FlashLoopConfig(weight_bits=4)`` every Linear layer runs on a microscaled 4-bit copy of its
 weights (a looped model reads each weight once per loop): prompt rows, and decode steps of more than
 8 sequences, in 8 bits through ``fl_norm_chain_mx``, ``fl_mx_quantize`` and ``fl_mx_matmul``, smaller
-decode steps in bf16 through ``fl_mx_gemv[_chain]``.
+decode steps in bf16 through ``fl_mx_gemv[_chain]``.  So the rows that a prompt, or a step of more than 8
+sequences, multiplies by the weights are rounded to 8 bits (e4m3) too: the norms' outputs, the attention's,
+SwiGLU's, and the last hidden rows where more than 8 of them give logits.  The norms round as their
+kernels do: in 64 bits with 8-bit rows, in fp32 within the GEMVs, and as the modules where rows of more than
+4096 values take a launch of their own.  The model's own weights stay on the device, and its copies take
+17/64 of the Linear layers' bytes besides.
 """
 
 from __future__ import annotations
@@ -275,7 +280,10 @@ class FlashLoopEngine:
         # decode-step model ops on the fused HIP kernels (False: torch modules)
         self.fused_decode = True
         # with fused_decode: each residual/norm chain runs in the prologue of the GEMV that
-        # consumes it (False: separate fl_norm_chain launches; same results bit for bit)
+        # consumes it (False: separate fl_norm_chain launches).  On bf16 weights both give the same
+        # results bit for bit; on 4-bit ones the chained GEMV keeps the chain in fp32 and rounds h and z,
+        # the separate launch rounds every norm and the sum as the modules do, and more than 8
+        # sequences always take separate launches (fl_norm_chain_mx)
         self.fused_chain = True
         self._wcache = None
         self._mx = None  # weight_bits=4: (per layer, norm and lm_head) as _fused_weights gives them

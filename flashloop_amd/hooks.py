@@ -17,7 +17,8 @@ context both entry points of the model are routed through ``FlashLoopEngine``:
   with one token decodes one step on it (logits ``[1, 1, vocab]``);
 * ``model.generate(input_ids, max_new_tokens=...)`` is greedy generation on the engine.
 
-``flashloop(model, weight_bits=4)`` runs the Linear layers on microscaled 4-bit copies of their weights.
+``flashloop(model, weight_bits=4)`` runs the Linear layers on microscaled 4-bit copies of their weights, with
+a prompt's rows rounded to 8 bits where they meet them.
 
 Arguments the engine cannot honour raise (``TypeError`` for unknown ones, ``ValueError``
 for unsupported values) instead of being dropped.  The audit counters count what the
