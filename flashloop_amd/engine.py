@@ -715,7 +715,8 @@ class FlashLoopEngine:
         loop one q/k/v GEMV with RoPE, the cache readers, one o_proj GEMV (+ the loop-2
         projection for loops 3/4), one residual/norm chain, one SwiGLU GEMV, one down GEMV
         and one chain that also applies the next layer's input norm (and the final norm at
-        the end of a loop).  Each op rounds to bf16 where the torch modules do."""
+        the end of a loop).  On bf16 weights each op rounds to bf16 where the torch modules do; a
+        product with 4-bit ones rounds its output once."""
         cfg = self.config
         sparse = cfg.enable_sparse_decode
         fraction = cfg.effective_decode_key_fraction
