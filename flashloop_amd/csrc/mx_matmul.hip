@@ -434,7 +434,10 @@ void launch_tiles(MmArgs a, hipStream_t st) {
 // a CU has few of them KS groups of waves divide K, so that its steps do not follow one another.  Measured, us,
 // bf16 results, m x n x k (tile of n by m, groups):
 //   8192 x 5632 x 2048: 256 x 256 80.5, 128 x 128 129; 8192^3: 367, 656
-//   820 x 5632 x 2048: 128 x 128 18.6, 64 x 64 18.9; 64 x 49152 x 2048: 64 x 64 14.4, two groups 16.0
+//   820 x 5632 x 2048: 128 x 128 18.6, 64 x 64 18.9
+//   up to 64 rows, of which larger tiles would be half empty (64 x 64, 128 x 128, two groups of 64 x 64): 40 x 49152
+//   x 2048 12.0, 17.1, 14.1; 64 13.3, 17.8, 15.0; 100 19.5, 19.2, 23.7; f32 results of 64 20.1, 32.0, 21.4, of 100
+//   32.5, 33.3, 39.1; 64 x 131072 42.6, 41.9 (256 x 256: 50.6)
 //   820 x 2048 x 2048: 64 x 64 in two groups 9.7, one 9.8; 512 x 2048 x 2048: 7.4, 8.5; 32 x 32 in four 10.2
 //   128 x 2048 x 2048: 32 x 32 in four groups 5.0, 64 x 64 in one, two, four 8.1, 7.0, 7.1
 //   256 x 2048 x 2048: 6.4, 64 x 64 in two 7.1; 128 x 5632 x 2048: 8.7, 7.2
@@ -445,6 +448,7 @@ void launch_matmul(const MmArgs& a, hipStream_t st) {
   if (tiles(32, 32) <= 512) return launch_tiles<32, 32, 1, 2, 4, F32, false>(a, st);
   if (a.m <= 32) return launch_tiles<64, 32, 2, 2, 1, F32, false>(a, st);
   if (tiles(64, 64) <= 512) return launch_tiles<64, 64, 2, 2, 2, F32, false>(a, st);
+  if (a.m <= 64) return launch_tiles<64, 64, 2, 2, 1, F32, false>(a, st);
   if constexpr (!F32)
     if (tiles(256, 256) >= 256) return launch_tiles<256, 256, 2, 4, 1, F32, true>(a, st);
   if (tiles(128, 128) >= 256) return launch_tiles<128, 128, 2, 2, 1, F32, false>(a, st);

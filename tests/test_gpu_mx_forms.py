@@ -188,3 +188,15 @@ def test_products_of_values_next_to_the_largest():
             assert (y[:, 0] == float("inf")).all() and (y[:, 1] == -down * 2.0**27).all()
         assert (exact[0] == float("inf")).all() and (exact[1] == -down * 2.0**27).all()
         assert (short[0] == 2.0**28).all() and (short[1] == -down * 2.0**27).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(33, 33000, 264), (64, 49152, 200), (65, 33000, 264), (64, 65600, 130), (130, 65600, 130)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_mx_matmul_of_heads(m, n, k, dtype):
+    """Few rows, many outputs: sizes on both sides of each choice of tiles there."""
+    _say("mx_matmul of heads", m, n, k, dtype)
+    rng = _rng(m, n, k)
+    (x, xv), (w, wv) = _mx(_rows(rng, m, k), 8), _mx(0.05 * rng.standard_normal((n, k)), 4)
+    want, mag = xv @ wv.T, abs(xv) @ abs(wv).T
+    bound = k * 2.0**-24 * mag if dtype == torch.float32 else 2.0**-10 * mag + 2.0**-8 * abs(want)
+    _check([kernels.mx_matmul(x, w, out_dtype=dtype)], [want], [bound], str(dtype))
