@@ -495,7 +495,10 @@ void mx_launch_k(const MxGemvArgs& a, const NormArgs& c, hipStream_t st) {
 // A workgroup takes several units where its prologue would cost more than their weights -- eight chained
 // rows, ~600 instructions each, run once a CU: SwiGLU 13.2 -> 8.0, q/k/v 9.8 -> 7.4, lm_head 49152 26.7
 // -> 15.5 -- and in a head-sized matrix (lm_head 49152: one row 12.1 -> 11.6, eight 16.7 -> 13.7; 16384
-// x 2048 loses, 6.1 -> 6.9 and 7.5 -> 7.8).
+// x 2048 loses, 6.1 -> 6.9 and 7.5 -> 7.8).  Around N 32768, where heads begin, a unit a workgroup and several, on
+// weights that no cache holds, K 2048: one row 28672 8.5, 9.3; 32768 9.5, 9.6; 36864 10.9, 10.5; two rows
+// 28672 9.9, 10.3; 36864 12.0, 11.9; 49152 15.5, 13.7; eight 28672 12.8, 11.0; 36864 15.3, 13.1.  K 4096, one row:
+// 28672 15.3, 16.2; 32768 17.5, 16.5; 36864 19.9, 19.3.
 template <int EPI, bool CHAIN>
 void mx_launch(const MxGemvArgs& a, const NormArgs& c, hipStream_t st) {
   constexpr int kMats = EPI == kEpiRope ? 3 : 1;

@@ -26,8 +26,8 @@
 // What bounds it: with operands in registers the instruction reaches 3500-3750 TFLOP/s on random codes (4700
 // on zeros, by its power).  8192^3 takes 355-396 us (2780-3100 TFLOP/s; in parts, on a build at 359: 306 without the transfers, 311 without the LDS
 // reads, 273 without the products, and 278 with nothing but the products and barriers): the reading and
-// the multiplying turns are about equally long.  8192 x 2048 -> 5632 80-90 us (2100-2360; 704 tiles in three
-// rounds of 256, matrix cores busy 45% of the time), 8192 x 5632 -> 2048 67-75.  The bf16 library product
+// the multiplying turns are about equally long.  8192 x 2048 -> 5632 80-90 us (2100-2380; 704 tiles in three
+// rounds of 256, matrix cores busy 47-49% of the time), 8192 x 5632 -> 2048 67-75.  The bf16 library product
 // of the three: 777-816, 174-185, 132-137 us.
 #include <algorithm>
 
@@ -178,7 +178,9 @@ struct TileGeom {
 };
 
 // XCD-aware order: workgroups go to the 8 XCDs in turn, so XCD d takes the d-th stretch of the tiles; a
-// stretch walks groups of 8 tile rows of X, whose operands an XCD's L2 then holds.
+// stretch walks groups of 8 tile rows of X.  One tile of 256 x 256 for each of an XCD's 32 CUs then takes 8
+// panels of X and 4 of W: they stay in its 4 MB L2 up to K of about 1500, and past that X is read again for
+// every such round (8192 x 2048 -> 5632: 4.3 + 1.1 MB, three rounds, 129 MB read for operands of 23).
 __device__ __forceinline__ void tile_of(const MmArgs& a, int id, int* tn, int64_t* tm) {
   const int total = a.tiles_n * a.tiles_m;
   const int d = id & 7, per = total >> 3, more = total & 7;
@@ -442,6 +444,11 @@ void launch_tiles(MmArgs a, hipStream_t st) {
 //   128 x 2048 x 2048: 32 x 32 in four groups 5.0, 64 x 64 in one, two, four 8.1, 7.0, 7.1
 //   256 x 2048 x 2048: 6.4, 64 x 64 in two 7.1; 128 x 5632 x 2048: 8.7, 7.2
 //   32 x 49152 x 2048: 64 x 32 11.2, 64 x 64 12.6, 32 x 32 in four groups 15.2
+//   around 256 tiles of 256 x 256 (these, then 128 x 128), k 2048: 96 of them 27.5, 19.0; 176 28.1, 29.0; 192 28.3,
+//   29.2; 240 29.6, 34.0; 256 30.1, 34.7; 288 48.2, 43.1; 352 49.3, 48.6.  k 5632: 128 56.7, 45.0; 192 58.8,
+//   69.1; 256 64.8, 86.2
+// f32 results by m, n 49152, k 2048 (bf16 ones of the same rows): 16 14.8 (10.2), 64 20.1 (13.3), 512 94.6 (50.1),
+// 2048 372 (165), 8192 1460 (644; 1130 TFLOP/s of the 1400 that a bf16 library product reaches).
 template <bool F32>
 void launch_matmul(const MmArgs& a, hipStream_t st) {
   const auto tiles = [&](int64_t bn, int64_t bm) { return ((a.n + bn - 1) / bn) * ((a.m + bm - 1) / bm); };

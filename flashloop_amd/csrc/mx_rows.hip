@@ -187,9 +187,11 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(DequantArgs a) 
 // becomes bf16 as torch converts a 64-bit value (by way of f32), and z, from that h, e4m3 in one
 // rounding.  (A 64-bit FMA costs here what a 32-bit one does.)  The order of the sums shows in no output.
 //
-// Bound by the VALU, ~260 instructions for 8 values and ~80 for each sum of a wave, which two pieces a lane
-// halve (8192 rows of 4096: 53 -> 42 us, of 8192 with 8 waves a row 152 -> 117, of 1000 18 -> 15): 8192 x 2048 takes 26
-// us (4.5 TB/s; norm_chain_kernel with bf16 z 31), a few rows 5 (one trip to memory and two sums).
+// ~260 instructions for 8 values and ~80 for each sum of a wave, which two pieces a lane halve (8192 rows of
+// 4096: 53 -> 42 us, of 8192 with 8 waves a row 152 -> 117, of 1000 18 -> 15).  8192 x 2048 takes 26 us, 118 MB at
+// 4.6 TB/s, where a large copy reaches 5.0 and the VALU is busy 59% of the time (norm_chain_kernel with bf16 z
+// 31); 2051 x 1000 with the final norm 7.0, of which 2.8 are instructions, in waves that wait 45% of their time for
+// r and x; a few rows 4-5 (one trip to memory and two sums).
 struct NormMxArgs {
   int64_t rows, stride;
   int d, per_row;  // values; 8-value pieces of a padded row
