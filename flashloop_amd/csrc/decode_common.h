@@ -13,17 +13,6 @@ enum GemvEpi : int { kEpiPlain = 0, kEpiF32 = 1, kEpiAdd = 2, kEpiSwiGlu = 3, kE
 
 __device__ __forceinline__ float bf16_round(float v) { return round_bf16(v); }
 
-__device__ __forceinline__ void unpack8(const uint4& u, float* f) {
-  f[0] = bf16lo_to_f32(u.x);
-  f[1] = bf16hi_to_f32(u.x);
-  f[2] = bf16lo_to_f32(u.y);
-  f[3] = bf16hi_to_f32(u.y);
-  f[4] = bf16lo_to_f32(u.z);
-  f[5] = bf16hi_to_f32(u.z);
-  f[6] = bf16lo_to_f32(u.w);
-  f[7] = bf16hi_to_f32(u.w);
-}
-
 // A raw buffer resource over `bytes` bytes at p (wave-uniform): loads past the end (or
 // from a resource of size 0) return zero.  Word 3 is the gfx9 raw-buffer format.
 using BufRes = __amdgpu_buffer_rsrc_t;
@@ -36,17 +25,6 @@ __device__ __forceinline__ uint4 buf_load16(BufRes r, uint32_t off) {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-
-// Two values rounded to bf16 and packed (v_cvt_pk_bf16_f32, nearest even, NaN kept NaN).
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-  const f32x2_t f = {lo, hi};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
-}
-__device__ __forceinline__ uint4 bf16_pack8(const float* f) {
-  return make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
-}
 
 // ---------------------------------------------------------------------------------
 // Residual / RMSNorm chain of one row (one workgroup per row).  Thread t owns the
@@ -105,7 +83,7 @@ __device__ __forceinline__ void rms_apply(float (*v)[8], const uint4* w, int nc,
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     float wf[8];
-    unpack8(w[i], wf);
+    unpack_bf16x8(w[i], wf);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[i][e] = bf16_round(wf[e] * (v[i][e] * inv));
   }
@@ -159,11 +137,11 @@ __device__ __forceinline__ void chain_finish(const NormArgs& a, int64_t base, bo
                                              float (*h)[8], BlockSum& bs) {
   const int nc = (a.D / 8 - static_cast<int>(threadIdx.x) + kNormThreads - 1) / kNormThreads;
 #pragma unroll
-  for (int i = 0; i < NC; ++i) unpack8(in.rr[i], h[i]);
+  for (int i = 0; i < NC; ++i) unpack_bf16x8(in.rr[i], h[i]);
   if (a.x != nullptr) {
     float xv[NC][8];
 #pragma unroll
-    for (int i = 0; i < NC; ++i) unpack8(in.xr[i], xv[i]);
+    for (int i = 0; i < NC; ++i) unpack_bf16x8(in.xr[i], xv[i]);
     rms_apply<NC>(xv, in.wa, nc, a.D, a.eps, bs);
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -217,7 +195,7 @@ __device__ __forceinline__ void wave_rms(uint4 (&v)[CH], const uint4 (&w)[CH], i
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     float f[8];
-    unpack8(v[j], f);
+    unpack_bf16x8(v[j], f);
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss[j & 3] = fmaf(f[e], f[e], ss[j & 3]);
   }
@@ -227,11 +205,11 @@ __device__ __forceinline__ void wave_rms(uint4 (&v)[CH], const uint4 (&w)[CH], i
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     float f[8], g[8];
-    unpack8(v[j], f);
-    unpack8(w[j], g);
+    unpack_bf16x8(v[j], f);
+    unpack_bf16x8(w[j], g);
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = g[e] * (f[e] * inv);
-    v[j] = bf16_pack8(f);
+    v[j] = pack_bf16x8(f);
   }
 }
 
@@ -243,11 +221,11 @@ __device__ __forceinline__ void wave_chain(const NormArgs& c, int64_t base, bool
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       float f[8], g[8];
-      unpack8(in.r[j], f);
-      unpack8(in.x[j], g);
+      unpack_bf16x8(in.r[j], f);
+      unpack_bf16x8(in.x[j], g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] += g[e];
-      in.r[j] = bf16_pack8(f);
+      in.r[j] = pack_bf16x8(f);
     }
   }
   if (c.wf != nullptr) {  // the last chain of a loop only: loaded here, so that the others keep the registers

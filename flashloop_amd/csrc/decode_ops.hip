@@ -54,7 +54,7 @@ __device__ __forceinline__ void load_x8(const GemvArgs& a, int m, int q, float* 
     f[6] = bf16_round(v.z);
     f[7] = bf16_round(v.w);
   } else {
-    unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + m * a.x_stride + 8 * q), f);
+    unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.x) + m * a.x_stride + 8 * q), f);
   }
 }
 
@@ -195,10 +195,10 @@ __global__ __launch_bounds__(kGemvThreads) void gemv_kernel(GemvArgs a) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           float f[8];
-          unpack8(w0[r], f);
+          unpack_bf16x8(w0[r], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[m][r] = fmaf(x0[e], f[e], acc[m][r]);
-          unpack8(w1[r], f);
+          unpack_bf16x8(w1[r], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[m][r] = fmaf(x1[e], f[e], acc[m][r]);
         }
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(kGemvThreads) void gemv_kernel(GemvArgs a) {
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           float f[8];
-          unpack8(w0[r], f);
+          unpack_bf16x8(w0[r], f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[m][r] = fmaf(x0[e], f[e], acc[m][r]);
         }
@@ -276,12 +276,12 @@ __global__ __launch_bounds__(kGemvThreads) void gemv_flat_kernel(GemvArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = bf16_round(__uint_as_float(w8[e]));
       } else {
-        unpack8(xv[m][s][0], x);
+        unpack_bf16x8(xv[m][s][0], x);
       }
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         float f[8];
-        unpack8(wv[s][r], f);
+        unpack_bf16x8(wv[s][r], f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[m][r] = fmaf(x[e], f[e], acc[m][r]);
       }
@@ -513,7 +513,7 @@ __device__ __forceinline__ void load_x(const GemvArgs& a, bf16x8_t (&x)[CS]) {
       const float f[8] = {__uint_as_float(lo[s].x), __uint_as_float(lo[s].y), __uint_as_float(lo[s].z),
                           __uint_as_float(lo[s].w), __uint_as_float(hi[s].x), __uint_as_float(hi[s].y),
                           __uint_as_float(hi[s].z), __uint_as_float(hi[s].w)};
-      x[s] = __builtin_bit_cast(bf16x8_t, bf16_pack8(f));
+      x[s] = __builtin_bit_cast(bf16x8_t, pack_bf16x8(f));
     }
   } else {
 #pragma unroll
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(MmGeom<MT>::kThreads, 2) void gemv_mfma_kernel(Gemv
     chain_finish<NC>(c, 0, blockIdx.x == 0, in, z, bs);
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      *reinterpret_cast<uint4*>(&xs[8 * (tid + i * kNormThreads)]) = bf16_pack8(z[i]);  // (zero past K)
+      *reinterpret_cast<uint4*>(&xs[8 * (tid + i * kNormThreads)]) = pack_bf16x8(z[i]);  // (zero past K)
   } else if constexpr (CHAIN) {
     constexpr int CH = KCAP / 512;
     WaveChainIn<CH> in;  // wave w: row w (rows past M repeat the last: columns no output reads)

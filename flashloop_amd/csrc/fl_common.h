@@ -56,6 +56,26 @@ __device__ __forceinline__ uint16_t f32_to_bf16_rne(float f) {
 }
 __device__ __forceinline__ float round_bf16(float f) { return bf16_to_f32(f32_to_bf16_rne(f)); }
 
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+// Two values rounded to bf16 and packed (v_cvt_pk_bf16_f32, nearest even, NaN kept NaN); eight of them, and back.
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  const f32x2_t f = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+}
+__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
+  return make_uint4(bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7]));
+}
+__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = bf16lo_to_f32(w[i]);
+    f[2 * i + 1] = bf16hi_to_f32(w[i]);
+  }
+}
+
 // fp16 bits: narrowing rounds to nearest even, with fp16 subnormals, and finite values
 // beyond the fp16 range become +-inf (torch's .to(torch.float16)); widening is exact.
 __device__ __forceinline__ uint16_t f32_to_f16(float f) {

@@ -14,8 +14,13 @@ constexpr int kMxPad = FL_MX_PAD;
 
 __host__ __device__ __forceinline__ int64_t mx_padded(int64_t k) { return (k + kMxPad - 1) / kMxPad * kMxPad; }
 
-typedef __bf16 mx_bf16x2_t __attribute__((ext_vector_type(2)));
 typedef short mx_i16x2_t __attribute__((ext_vector_type(2)));
+
+// 16 bytes at an element's alignment (one load or store, as global memory takes any alignment)
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) Bytes16 {
+  u32x4_t v;
+};
 
 // Stored scale of a block from the largest magnitude of its values, as f32 bits without the sign
 // (compared as integers, so that a NaN counts as the largest).  1.m > 1.5 (6 = 1.5 * 2^2) or > 1.75

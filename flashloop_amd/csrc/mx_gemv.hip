@@ -113,7 +113,7 @@ __device__ __forceinline__ void mx_chain(const NormArgs& c, bool write_h, const 
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       float f[8];
-      unpack8(in.xr[i], f);
+      unpack_bf16x8(in.xr[i], f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) add(f[e]);
     }
@@ -122,9 +122,9 @@ __device__ __forceinline__ void mx_chain(const NormArgs& c, bool write_h, const 
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     float f[8], w[8];
-    unpack8(in.rr[i], h[i]);
-    unpack8(in.xr[i], f);
-    unpack8(in.wa[i], w);
+    unpack_bf16x8(in.rr[i], h[i]);
+    unpack_bf16x8(in.xr[i], f);
+    unpack_bf16x8(in.wa[i], w);
     if (c.x != nullptr)
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[i][e] = fmaf(w[e], f[e] * ia, h[i][e]);
@@ -136,7 +136,7 @@ __device__ __forceinline__ void mx_chain(const NormArgs& c, bool write_h, const 
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       float w[8];
-      unpack8(in.wf[i], w);
+      unpack_bf16x8(in.wf[i], w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[i][e] = w[e] * (h[i][e] * fi);
     }
@@ -144,8 +144,8 @@ __device__ __forceinline__ void mx_chain(const NormArgs& c, bool write_h, const 
   ss = 0.0f;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    z[i] = bf16_pack8(h[i]);
-    unpack8(z[i], h[i]);
+    z[i] = pack_bf16x8(h[i]);
+    unpack_bf16x8(z[i], h[i]);
     const int q = static_cast<int>(threadIdx.x) + i * kNormThreads;
     if (write_h && c.h_out != nullptr && q < c.D / 8) reinterpret_cast<uint4*>(c.h_out)[q] = z[i];
 #pragma unroll
@@ -156,10 +156,10 @@ __device__ __forceinline__ void mx_chain(const NormArgs& c, bool write_h, const 
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     float w[8];
-    unpack8(in.wb[i], w);
+    unpack_bf16x8(in.wb[i], w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[i][e] = w[e] * (h[i][e] * ib);
-    z[i] = bf16_pack8(h[i]);
+    z[i] = pack_bf16x8(h[i]);
   }
 }
 
@@ -186,17 +186,17 @@ __device__ __forceinline__ void mx_wave_chain(const NormArgs& c, int64_t base, b
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       float f[8];
-      unpack8(in.x[j], f);
+      unpack_bf16x8(in.x[j], f);
       add(j, f);
     }
     ia = mx_wave_inv(ss, c.D, c.eps);
   }
   const auto sum_of = [&](int j, float* h) __attribute__((always_inline)) {
-    unpack8(in.r[j], h);
+    unpack_bf16x8(in.r[j], h);
     if (c.x == nullptr) return;
     float f[8], w[8];
-    unpack8(in.x[j], f);
-    unpack8(in.wa[j], w);
+    unpack_bf16x8(in.x[j], f);
+    unpack_bf16x8(in.wa[j], w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = fmaf(w[e], f[e] * ia, h[e]);
   };
@@ -217,14 +217,14 @@ __device__ __forceinline__ void mx_wave_chain(const NormArgs& c, int64_t base, b
     sum_of(j, h);
     if (c.wf != nullptr) {  // the last chain of a loop only: loaded here, so that the others keep the registers
       float w[8];
-      unpack8(buf_load16(wf, 16u * (threadIdx.x & 63u) + 1024u * j), w);
+      unpack_bf16x8(buf_load16(wf, 16u * (threadIdx.x & 63u) + 1024u * j), w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[e] = w[e] * (h[e] * fi);
     }
-    in.r[j] = bf16_pack8(h);
+    in.r[j] = pack_bf16x8(h);
     const int q = static_cast<int>(threadIdx.x & 63u) + 64 * j;
     if (write_h && c.h_out != nullptr && q < c.D / 8) reinterpret_cast<uint4*>(c.h_out + base)[q] = in.r[j];
-    unpack8(in.r[j], h);
+    unpack_bf16x8(in.r[j], h);
     add(j, h);
   }
   if (c.wb == nullptr) return;
@@ -232,11 +232,11 @@ __device__ __forceinline__ void mx_wave_chain(const NormArgs& c, int64_t base, b
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     float h[8], w[8];
-    unpack8(in.r[j], h);
-    unpack8(in.wb[j], w);
+    unpack_bf16x8(in.r[j], h);
+    unpack_bf16x8(in.wb[j], w);
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] = w[e] * (h[e] * ib);
-    in.r[j] = bf16_pack8(h);
+    in.r[j] = pack_bf16x8(h);
   }
 }
 
@@ -287,7 +287,7 @@ __device__ __forceinline__ void mx_load_x(const MxGemvArgs& a, BufRes xr, uint32
         const uint4 lo = buf_load16(xr, o), hi = buf_load16(xr, o + 16u);
         const float f[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
                             __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
-        x[s][j] = bf16_pack8(f);
+        x[s][j] = pack_bf16x8(f);
       } else {
         x[s][j] = buf_load16(xr, o);
       }

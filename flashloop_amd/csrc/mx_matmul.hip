@@ -80,16 +80,11 @@ __device__ __forceinline__ int x_piece(int g, int half) {
 
 // Outputs of row m from n on, 16 bytes a lane at an element's alignment (rows of any length: global memory
 // takes it).  f32: four neighbours.
-typedef uint32_t mx_u32x4_t __attribute__((ext_vector_type(4)));
-struct __attribute__((packed, aligned(2))) Bytes16 {
-  mx_u32x4_t v;
-};
-
 __device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const mx_f32x4_t& v) {
   if (m >= a.m || n >= a.n) return;
   float* y = static_cast<float*>(a.y) + m * a.y_stride + n;
   if (n + 4 <= a.n) {
-    reinterpret_cast<Bytes16*>(y)->v = __builtin_bit_cast(mx_u32x4_t, v);
+    reinterpret_cast<Bytes16*>(y)->v = __builtin_bit_cast(u32x4_t, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -100,14 +95,9 @@ __device__ __forceinline__ void store4(const MmArgs& a, int64_t m, int n, const 
 // bf16, of two groups of 16 n side by side (v, u): the odd rows of 16 lanes change their v for the u of the even
 // ones, so that a lane holds eight neighbours of one group and the four lanes of an m 32.
 __device__ __forceinline__ void store8(const MmArgs& a, int64_t m, int n, int g, const mx_f32x4_t& v, const mx_f32x4_t& u) {
-  const auto pair = [](float lo, float hi) {
-    typedef float f32x2_t __attribute__((ext_vector_type(2)));
-    const f32x2_t f = {lo, hi};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, mx_bf16x2_t));
-  };
-  const auto p = __builtin_amdgcn_permlane16_swap(pair(v[0], v[1]), pair(u[0], u[1]), false, false);
-  const auto q = __builtin_amdgcn_permlane16_swap(pair(v[2], v[3]), pair(u[2], u[3]), false, false);
-  const mx_u32x4_t w = {p[0], q[0], p[1], q[1]};
+  const auto p = __builtin_amdgcn_permlane16_swap(bf16_pair(v[0], v[1]), bf16_pair(u[0], u[1]), false, false);
+  const auto q = __builtin_amdgcn_permlane16_swap(bf16_pair(v[2], v[3]), bf16_pair(u[2], u[3]), false, false);
+  const u32x4_t w = {p[0], q[0], p[1], q[1]};
   n += 16 * (g & 1) + 8 * (g >> 1);
   if (m >= a.m || n >= a.n) return;
   uint16_t* y = static_cast<uint16_t*>(a.y) + m * a.y_stride + n;

@@ -26,31 +26,6 @@ struct QuantArgs {
   uint8_t* scales;
 };
 
-__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16lo_to_f32(w[i]);
-    f[2 * i + 1] = bf16hi_to_f32(w[i]);
-  }
-}
-
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2_t v = {f[2 * i], f[2 * i + 1]};
-    w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, mx_bf16x2_t));
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// 16 bytes at an element's alignment (one load or store, as global memory takes any alignment)
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-struct __attribute__((packed, aligned(2))) Bytes16 {
-  u32x4_t v;
-};
 template <typename T>
 __device__ __forceinline__ uint4 load16(const T* p) {
   return __builtin_bit_cast(uint4, reinterpret_cast<const Bytes16*>(p)->v);

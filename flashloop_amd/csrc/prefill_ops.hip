@@ -28,25 +28,6 @@ struct RopeStoreArgs {
   int n, heads, rows;
 };
 
-__device__ __forceinline__ void unpack_bf16x8(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = bf16lo_to_f32(w[i]);
-    f[2 * i + 1] = bf16hi_to_f32(w[i]);
-  }
-}
-
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16_pair(float lo, float hi) {
-  const f32x2_t f = {lo, hi};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
-}
-__device__ __forceinline__ uint4 pack_bf16x8(const float* f) {
-  return make_uint4(pack_bf16_pair(f[0], f[1]), pack_bf16_pair(f[2], f[3]), pack_bf16_pair(f[4], f[5]),
-                    pack_bf16_pair(f[6], f[7]));
-}
 // eight values rounded to bf16 and widened again
 __device__ __forceinline__ void round8(float* f) {
   const uint4 u = pack_bf16x8(f);
