@@ -189,3 +189,19 @@ def test_new_modules_are_taken_anew():
     eng.quantize_weights()
     assert torch.equal(eng.prefill(_ids(20)).logits, 2 * first)
     eng.decode(_ids(1))
+
+
+@pytest.mark.parametrize("name", ["small", "layer"])
+@pytest.mark.parametrize("batch", [1, 8])
+def test_separate_norms_follow_the_chained_ones(name, batch):
+    """Separate launches round the norms and the sum on their own: roundings apart, no more."""
+    _say("separate norms", name, batch)
+    model, _ = _models(name)
+    cfg = FlashLoopConfig(weight_bits=4, **KEPT)
+    ids, mask, _ = _prompts(batch)
+    chained, apart = (FlashLoopBatchEngine(model, config=cfg, use_graphs=False) for _ in range(2))
+    apart._one.fused_chain = False
+    assert torch.equal(chained.prefill(ids, mask).logits, apart.prefill(ids, mask).logits)
+    for step in range(3):
+        tok = torch.cat([_ids(1, seed=100 * step + b) for b in range(batch)])
+        _near(apart.decode(tok).logits, chained.decode(tok).logits, ROUNDINGS)

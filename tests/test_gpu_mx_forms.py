@@ -200,3 +200,61 @@ def test_mx_matmul_of_heads(m, n, k, dtype):
     want, mag = xv @ wv.T, abs(xv) @ abs(wv).T
     bound = k * 2.0**-24 * mag if dtype == torch.float32 else 2.0**-10 * mag + 2.0**-8 * abs(want)
     _check([kernels.mx_matmul(x, w, out_dtype=dtype)], [want], [bound], str(dtype))
+
+
+# ---------------------------------------------------------------------------- rows and streams by themselves
+@pytest.mark.parametrize("n,k", [(24, 1000), (5632, 2048), (2176, 4096)])
+@pytest.mark.parametrize("final", [False, True])
+def test_mx_gemv_chain_rows_by_themselves(n, k, final):
+    """Rows with a NaN, an infinity or nothing but zeros stay their own matter, and a row does not depend on how
+    many come with it."""
+    _say("mx_gemv_chain rows", n, k, final)
+    s = _chain_case(_rng(n, k, 61), 8, k, True, final)
+    (w,), _ = _weights(n, k, 1, 3)
+
+    def run(rows):
+        part = dict(s, r=s["r"][rows].clone(), x=s["x"][rows].clone())
+        return kernels.mx_gemv_chain(**part, weights=[w], eps=1e-6, epilogue=kernels.EPI_F32)
+
+    h, y = run(slice(0, 8))
+    for rows in (slice(0, 2), slice(3, 8)):
+        h2, y2 = run(rows)
+        assert torch.equal(h2, h[rows]) and torch.equal(y2, y[rows])
+    s["r"][1, k - 1], s["x"][4, 3] = float("inf"), float("nan")
+    s["r"][6], s["x"][6] = 0, 0
+    h3, y3 = run(slice(0, 8))
+    same = [0, 2, 3, 5, 7]
+    assert torch.equal(h3[same], h[same]) and torch.equal(y3[same], y[same])
+    assert torch.isnan(y3[4]).all() and not torch.isfinite(y3[1]).any() and not y3[6].any() and not h3[6].any()
+    for row in (1, 4, 6):  # one row at a time: the same rows are bad, to the same values where they are numbers
+        h1, y1 = run(slice(row, row + 1))
+        assert torch.equal(torch.isfinite(y1), torch.isfinite(y3[row:row + 1]))
+
+
+def test_operators_on_two_streams_at_once():
+    """None of them keeps anything between calls: work of two streams in turn gives what each alone gives."""
+    _say("two streams")
+    rng, d, f = _rng(71), 1024, 2048
+    gain = _bf16(1 + 0.1 * rng.standard_normal(d))
+    (wide,), _ = _weights(f, d, 1, 1)
+    (back,), _ = _weights(d, f, 1, 2)
+
+    def work(rows):
+        h, z = kernels.norm_chain_mx(rows, w_b=gain, eps=1e-6)
+        y = kernels.mx_matmul(kernels.mx_quantize(kernels.mx_matmul(z, wide), 8), back, out_dtype=torch.float32)
+        _, g = kernels.mx_gemv_chain(rows[:8], [wide], w_b=gain, eps=1e-6)
+        return h, y, kernels.mx_gemv(g, [back], epilogue=kernels.EPI_ADD, addend=rows[:8])
+
+    rows = [_bf16(_rows(rng, m, d)) for m in (300, 40)]
+    want = [work(r) for r in rows]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in rows]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(work(rows[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
