@@ -652,11 +652,13 @@ def rope_store(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: tuple[to
     wider matrix."""
     h, t, c = k_dst.shape
     n = q.shape[0]
-    columns = n > 0 and q.ndim == k.ndim == v.ndim == 2 and q.stride() == k.stride() == v.stride() and q.stride(1) == 1
-    stride = q.stride(0) if columns and n > 1 and q.stride(0) >= h * c else h * c
-    for x, name in ((q, "q"), (k, "k"), (v, "v"), (k_dst, "k_dst"), (v_dst, "v_dst"), (rope[0], "rope cos"),
+    stride, rows = h * c, (q, k, v)
+    if not q.is_contiguous() and n > 1 and q.ndim == 2 and q.stride() == k.stride() == v.stride() and q.stride(1) == 1:
+        if q.stride(0) > stride:  # columns: a row of each has to be whole
+            stride, rows = q.stride(0), (q[:1], k[:1], v[:1])
+    for x, name in (*zip(rows, "qkv"), (k_dst, "k_dst"), (v_dst, "v_dst"), (rope[0], "rope cos"),
                     (rope[1], "rope sin")):
-        _require(x[:1] if stride > h * c and name in "qkv" else x, torch.bfloat16, name)
+        _require(x, torch.bfloat16, name)
     if c != HEAD_DIM or k_dst.shape != v_dst.shape or any(tuple(x.shape) != (n, h * c) for x in (q, k, v)):
         raise ValueError("q, k and v must be [n, H*128] and the destinations [H, T, 128]")
     if any(tuple(x.shape) != (t, c) for x in rope):
