@@ -24,6 +24,7 @@ GROUP = 64
 MX_BLOCK = 32
 MX_PAD = 128
 MX_MAX_K = 1 << 20
+MAX_BEAMS = 64
 
 
 class FlCacheView(C.Structure):
@@ -121,6 +122,14 @@ SIGNATURES = {
     "fl_mx_gemv_chain": (_I32, [_I32, _I32, _F32, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _P, _I64, _P, _I64,
                                 _P, _P, _I32, _P]),
     "fl_mx_matmul": (_I32, [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I64, _P]),
+    "fl_paged_append": (_I32, [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _I32, _I32,
+                               _I32, _I32, _I32, _I32, _I32, _P]),
+    "fl_paged_attention_workspace": (_SZ, [_I32, _I32, _I32, _I32, _I32, _I32]),
+    "fl_paged_attention": (_I32, [_P, _I64, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32,
+                                  _F32, _P, _SZ, _P]),
+    "fl_beam_select_workspace": (_SZ, [_I32, _I32, _I64, _I32]),
+    "fl_beam_select": (_I32, [_P, _I32, _I64, _P, _I32, _I32, _I64, _I32, _P, _P, _P, _P, _SZ, _P]),
+    "fl_paged_reorder": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P]),
 }
 
 _lib: C.CDLL | None = None

@@ -1,0 +1,361 @@
+// Beam search's selection: of every sequence's beams k and tokens t the `count` largest
+//   total[k, t] = score[k] + x[k, t] - log(sum_t' exp(x[k, t'])),
+// ties to the lower beam, then the lower token.
+//
+// One pass over the logits: a workgroup takes a part of a beam's row and keeps, per wave, the largest values
+// so far as one sorted entry a lane, and the sum of exponentials.  The part's largest that a wave has not
+// seen yet are few: with 16 values a lane, a value enters only if it reaches the count-th largest of the
+// lanes' maxima (first step) or passes the list's last entry, so insertions (a vote and a shift of the
+// list) stay near `count` a step.  A second launch joins the parts of a sequence's beams, one list a lane.
+//
+// The sums and totals are in 64 bits: totals of different beams decide the order among nearly equal
+// candidates, and 32 bits would leave it to the order of the sum.  Within a beam the logits decide.
+#include <algorithm>
+
+#include "fl_common.h"
+
+namespace fl {
+namespace {
+
+constexpr int kBeamThreads = 256;
+constexpr int kBeamWaves = kBeamThreads / kWave;
+constexpr int kPer = 16;                         // values of a lane in a step
+constexpr int kBeamStep = kBeamThreads * kPer;   // values of a workgroup's step
+constexpr int kMaxCount = kWave;                 // one list entry a lane
+constexpr int kLists = kWave;                    // lists of a sequence (beams * parts), one a lane
+
+struct Entry {
+  float value;
+  int index;
+};
+
+struct PartHead {
+  double sum;  // of exp(x - top); NaN where the part holds a NaN or +inf
+  float top;
+  int unused;
+};
+
+struct BeamArgs {
+  const void* logits;  // [seqs * beams, vocab], row_stride apart
+  int64_t row_stride;
+  const float* scores;  // [seqs, beams]
+  int seqs, beams, vocab, count, parts, part_len;
+  PartHead* heads;  // [rows, parts]
+  Entry* lists;     // [rows, parts, count]
+  float* out_scores;
+  int32_t* out_beams;
+  int64_t* out_tokens;
+};
+
+// exp(t), t <= 0, to 1e-11: t = k ln 2 + r, |r| <= ln 2 / 2, and the series of exp(r) up to r^9.
+__device__ __forceinline__ double exp64(double t) {
+  t = fmax(t, -800.0);
+  const double k = rint(t * 1.4426950408889634);
+  double r = fma(k, -0.69314718055994529, t);
+  r = fma(k, -2.3190468138462996e-17, r);
+  double p = 1.0 / 362880;
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, static_cast<int>(k));
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+// a comes before b
+__device__ __forceinline__ bool before(float av, int ai, float bv, int bi) { return av > bv || (av == bv && ai < bi); }
+
+// x[kPer] <- values at index .. of the row; past `end`: -inf.  Four neighbouring values a lane and load.
+template <bool F32, bool ALIGNED>
+__device__ __forceinline__ void load_values(const BeamArgs& a, int64_t row, int from, int end, float* x) {
+#pragma unroll
+  for (int j = 0; j < kPer / 4; ++j) {
+    const int at = from + j * 4 * kWave;
+    const int64_t p = row * a.row_stride + at;
+    if (ALIGNED && at + 3 < end) {
+      if (F32) {
+        const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + p);
+        x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + p);
+        x[4 * j] = bf16lo_to_f32(v.x), x[4 * j + 1] = bf16hi_to_f32(v.x);
+        x[4 * j + 2] = bf16lo_to_f32(v.y), x[4 * j + 3] = bf16hi_to_f32(v.y);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        x[4 * j + i] = at + i >= end ? -INFINITY
+                       : F32         ? static_cast<const float*>(a.logits)[p + i]
+                                     : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[p + i]);
+    }
+  }
+}
+
+template <bool F32, bool ALIGNED>
+__global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
+  __shared__ Entry lists[kBeamWaves][kMaxCount];
+  __shared__ PartHead heads[kBeamWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = static_cast<int>(blockIdx.x - row * a.parts);
+  const int begin = part * a.part_len, end = min(begin + a.part_len, a.vocab);
+
+  float lv = -INFINITY;  // the wave's list: entry `lane`, largest first
+  int li = 0x7FFFFFFF;
+  float last_v = -INFINITY, top = -INFINITY;
+  int last_i = 0x7FFFFFFF;  // entry count - 1
+  double sum = 0.0;         // of this lane's exp(x - top)
+  bool bad = false;
+  float x[kPer], next[kPer];
+  // a wave's values of a step are neighbours: 1024 of them
+  const int mine = begin + wave * (kWave * kPer) + 4 * lane;
+  load_values<F32, ALIGNED>(a, row, mine, end, x);
+  for (int base = begin; base < end; base += kBeamStep) {
+    const int from = mine + (base - begin);
+    if (base + kBeamStep < end) load_values<F32, ALIGNED>(a, row, from + kBeamStep, end, next);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      bad = bad || !(x[e] < INFINITY);
+      x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
+      mx = fmaxf(mx, x[e]);
+    }
+    const float wave_top = wave_max(mx);
+    if (wave_top > top) {
+      sum *= top == -INFINITY ? 0.0 : exp64(static_cast<double>(top) - wave_top);
+      top = wave_top;
+    }
+    if (top > -INFINITY) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const double w = exp64(static_cast<double>(x[e]) - top);
+        sum += x[e] == -INFINITY ? 0.0 : w;
+      }
+    }
+    // what a value has to reach to be among the `count` largest of this step
+    float reach = last_v;
+    if (base == begin) {
+      int rank = 0;
+#pragma unroll
+      for (int j = 0; j < kWave; ++j) {
+        const float other = row_lane(mx, j);
+        rank += other > mx || (other == mx && j < lane) ? 1 : 0;
+      }
+      const unsigned long long at = __builtin_amdgcn_ballot_w64(rank == a.count - 1);
+      reach = row_lane(mx, __builtin_ctzll(at));
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int index = from + (e >> 2) * 4 * kWave + (e & 3);
+      unsigned long long in = __builtin_amdgcn_ballot_w64(x[e] >= reach && index < end && before(x[e], index, last_v, last_i));
+      while (in != 0ull) {
+        const int l = __builtin_ctzll(in);
+        in &= in - 1;
+        const float v = row_lane(x[e], l);
+        const int i = __builtin_amdgcn_readlane(index, l);
+        if (!before(v, i, last_v, last_i)) continue;
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(lv, li, v, i)));
+        const float uv = __shfl_up(lv, 1, kWave);
+        const int ui = __shfl_up(li, 1, kWave);
+        lv = lane < at ? lv : (lane == at ? v : uv);
+        li = lane < at ? li : (lane == at ? i : ui);
+        last_v = row_lane(lv, a.count - 1);
+        last_i = __builtin_amdgcn_readlane(li, a.count - 1);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = next[e];
+  }
+
+  if (lane < a.count) lists[wave][lane] = Entry{lv, li};
+  sum = wave_sum64(sum);
+  if (__builtin_amdgcn_ballot_w64(bad) != 0ull) sum = NAN;
+  if (lane == 0) heads[wave] = PartHead{sum, top, 0};
+  __syncthreads();
+  // the waves' lists into one: an entry's place is the number of entries before it
+  const int64_t out = row * a.parts + part;
+  if (lane < a.count) {
+    int place = lane;
+    for (int w = 0; w < kBeamWaves; ++w) {
+      if (w == wave) continue;
+      for (int j = 0; j < a.count; ++j) {
+        const Entry other = lists[w][j];
+        place += before(other.value, other.index, lv, li) || (other.value == lv && other.index == li && w < wave) ? 1 : 0;
+      }
+    }
+    if (place < a.count) a.lists[out * a.count + place] = Entry{lv, li};
+  }
+  if (tid == 0) {
+    float t = heads[0].top;
+    for (int w = 1; w < kBeamWaves; ++w) t = fmaxf(t, heads[w].top);
+    double s = 0.0;
+    for (int w = 0; w < kBeamWaves; ++w) {
+      const double f = heads[w].top == t ? 1.0 : (heads[w].top == -INFINITY ? 0.0 : exp64(static_cast<double>(heads[w].top) - t));
+      s += heads[w].sum * f;
+    }
+    a.heads[out] = PartHead{s, t, 0};
+  }
+}
+
+// log(s) in 64 bits of a sum 1 <= s <= vocab, or of parts of one
+__device__ __forceinline__ double log64(double s) { return log(s); }
+
+// order-preserving image of a double
+__device__ __forceinline__ unsigned long long image(double v) {
+  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(v));
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned long long dpp_max(unsigned long long v) {
+  const unsigned lo = static_cast<unsigned>(dpp_i<CTRL>(static_cast<int>(v)));
+  const unsigned hi = static_cast<unsigned>(dpp_i<CTRL>(static_cast<int>(v >> 32)));
+  const unsigned long long u = (static_cast<unsigned long long>(hi) << 32) | lo;
+  return u > v ? u : v;
+}
+__device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int l) {
+  return (static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32) |
+         static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
+}
+__device__ __forceinline__ unsigned long long wave_max64(unsigned long long v) {
+  v = dpp_max<kDppXor1>(v);
+  v = dpp_max<kDppXor2>(v);
+  v = dpp_max<kDppHalfMirror>(v);
+  v = dpp_max<kDppMirror>(v);
+  const unsigned long long a = lane_of(v, 0), b = lane_of(v, 16), c = lane_of(v, 32), d = lane_of(v, 48);
+  const unsigned long long e = a > b ? a : b, f = c > d ? c : d;
+  return e > f ? e : f;
+}
+
+// One sequence: list `lane` is part lane % parts of beam lane / parts, so equal candidates go to the lower lane.
+__global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
+  __shared__ Entry lists[kLists * kMaxCount];
+  const int tid = threadIdx.x, lane = tid & 63, seq = blockIdx.x;
+  const int used = a.beams * a.parts;
+  const int64_t first = static_cast<int64_t>(seq) * used;
+  for (int i = tid; i < used * a.count; i += kBeamThreads) lists[i] = a.lists[first * a.count + i];
+  __syncthreads();
+  if (tid >= kWave) return;
+  // the beam's shift: score - logsumexp; -inf where it has no distribution or no finite score
+  const int beam = lane / a.parts, part = lane - beam * a.parts;
+  double shift = -INFINITY;
+  if (beam < a.beams) {
+    const PartHead* h = a.heads + first + beam * a.parts;
+    float top = h[0].top;
+    for (int p = 1; p < a.parts; ++p) top = fmaxf(top, h[p].top);
+    double s = 0.0;
+    for (int p = 0; p < a.parts; ++p)
+      s += h[p].sum * (h[p].top == top ? 1.0 : (h[p].top == -INFINITY ? 0.0 : exp64(static_cast<double>(h[p].top) - top)));
+    const float score = a.scores[seq * a.beams + beam];
+    if (top > -INFINITY && s == s && fabsf(score) < INFINITY) shift = static_cast<double>(score) - (top + log64(s));
+  }
+  const bool dead = shift == -INFINITY;
+  const int left = min(a.part_len, a.vocab - part * a.part_len);  // values of the part
+  const int held = beam < a.beams ? (dead && part > 0 ? 0 : min(a.count, dead ? a.vocab : left)) : 0;
+  int at = 0, token = 0;
+  float value = 0.0f;
+  unsigned long long key = 0ull;  // of the list's next candidate; 0: none is left
+  double total = 0.0;
+  const auto look = [&]() __attribute__((always_inline)) {
+    key = 0ull;
+    if (at < held) {
+      const Entry e = lists[lane * a.count + at];
+      token = dead ? at : e.index;  // (equal totals: the tokens in order)
+      value = dead ? 0.0f : e.value;
+      total = dead ? -INFINITY : shift + static_cast<double>(e.value);
+      key = image(total);
+    }
+  };
+  look();
+  for (int n = 0; n < a.count; ++n) {
+    const unsigned long long best = wave_max64(key);
+    const unsigned long long who = __builtin_amdgcn_ballot_w64(key == best && key != 0ull);
+    if (who == 0ull) break;
+    int winner = __builtin_ctzll(who);
+    // totals of one beam may be equal in 64 bits where its logits are not: the logits decide
+    for (unsigned long long rest = who & (who - 1); rest != 0ull; rest &= rest - 1) {
+      const int l = __builtin_ctzll(rest);
+      if (__builtin_amdgcn_readlane(beam, l) != __builtin_amdgcn_readlane(beam, winner)) break;
+      if (row_lane(value, l) > row_lane(value, winner)) winner = l;
+    }
+    if (lane == winner) {
+      const int64_t out = static_cast<int64_t>(seq) * a.count + n;
+      a.out_scores[out] = static_cast<float>(total);
+      a.out_beams[out] = beam;
+      a.out_tokens[out] = token;
+      ++at;
+      look();
+    }
+  }
+}
+
+// Parts of a row: enough workgroups for the chip while a part keeps a step's worth of values, and no more lists
+// a sequence than lanes.
+int beam_parts(int64_t rows, int beams, int64_t vocab) {
+  const int64_t by_rows = (2048 + rows - 1) / rows;
+  const int64_t parts = std::min<int64_t>(std::min<int64_t>(by_rows, kLists / beams), (vocab + kBeamStep - 1) / kBeamStep);
+  return static_cast<int>(std::max<int64_t>(1, parts));
+}
+
+}  // namespace
+}  // namespace fl
+
+extern "C" size_t fl_beam_select_workspace(int32_t seqs, int32_t beams, int64_t vocab, int32_t count) {
+  using namespace fl;
+  if (seqs <= 0 || beams <= 0 || beams > kLists || vocab <= 0 || count <= 0 || count > kMaxCount) return 0;
+  const int64_t rows = static_cast<int64_t>(seqs) * beams;
+  return static_cast<size_t>(rows * beam_parts(rows, beams, vocab)) * (sizeof(PartHead) + count * sizeof(Entry));
+}
+
+extern "C" int32_t fl_beam_select(const void* logits, int32_t logits_is_f32, int64_t row_stride, const float* scores, int32_t seqs,
+                                  int32_t beams, int64_t vocab, int32_t count, float* out_scores, int32_t* out_beams,
+                                  int64_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(logits && scores && out_scores && out_beams && out_tokens, "fl_beam_select: null pointer");
+  FL_REQUIRE(seqs >= 0 && beams > 0 && beams <= kLists, "fl_beam_select: 1 to 64 beams");
+  FL_REQUIRE(vocab > 0 && vocab <= (1 << 30), "fl_beam_select: 1 to 2^30 tokens");
+  FL_REQUIRE(count > 0 && count <= kMaxCount && count <= beams * vocab, "fl_beam_select: 1 to 64 candidates, no more than there are");
+  FL_REQUIRE(row_stride >= vocab, "fl_beam_select: rows must not overlap");
+  FL_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (logits_is_f32 ? 4 : 2) == 0, "fl_beam_select: logits must be aligned");
+  if (seqs == 0) return FL_OK;
+  const int64_t rows = static_cast<int64_t>(seqs) * beams;
+  FL_REQUIRE(rows <= 0x7FFFFFFF / kLists / kBeamThreads, "fl_beam_select: too many rows");
+  FL_REQUIRE(workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                 workspace_bytes >= fl_beam_select_workspace(seqs, beams, vocab, count),
+             "fl_beam_select: workspace too small or not 16-byte aligned");
+  const int parts = beam_parts(rows, beams, vocab);
+  // whole steps of 4 values a part, so that aligned rows give aligned parts
+  const int part_len = static_cast<int>((vocab + 4 * parts - 1) / (4 * parts) * 4);
+  PartHead* heads = static_cast<PartHead*>(workspace);
+  const BeamArgs a{logits, row_stride, scores, seqs, beams, static_cast<int>(vocab), count, parts, part_len, heads,
+                   reinterpret_cast<Entry*>(heads + rows * parts), out_scores, out_beams, out_tokens};
+  const bool aligned = reinterpret_cast<uintptr_t>(logits) % (logits_is_f32 ? 16 : 8) == 0 && row_stride % 4 == 0;
+  const dim3 grid(static_cast<unsigned>(rows * parts)), block(kBeamThreads);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (logits_is_f32) {
+    if (aligned)
+      hipLaunchKernelGGL((beam_part_kernel<true, true>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((beam_part_kernel<true, false>), grid, block, 0, st, a);
+  } else {
+    if (aligned)
+      hipLaunchKernelGGL((beam_part_kernel<false, true>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((beam_part_kernel<false, false>), grid, block, 0, st, a);
+  }
+  FL_LAUNCH_CHECK("fl_beam_select");
+  hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(seqs)), block, 0, st, a);
+  FL_LAUNCH_CHECK("fl_beam_select(join)");
+  return FL_OK;
+}

@@ -1,0 +1,732 @@
+// Attention of new tokens over K/V pages: softmax(q K^T) V of a ragged batch whose keys and values lie in
+// pages [pages, KV heads, page, 128] named by a table.  The rows of a sequence are its last tokens, a row
+// sees the keys up to its own position; the query heads of a group share one KV head, so a group's rows
+// (token i, head g of the group: row i * group + g) are the queries of that head's keys.
+//
+//  * chunk_kernel: the tiles of attention.hip (128 queries a workgroup, 64 keys a step through LDS, S^T and
+//    O^T on v_mfma_f32_32x32x16_bf16), the rows' sequence found by a scan of the sequences' tile counts.
+//  * step_kernel: few queries a sequence (one decode step).  A wave owns steps of 32 keys and up to 16
+//    queries on v_mfma_f32_16x16x32_bf16: K goes from memory into the first product's operand, V through a
+//    part of LDS of the wave's own, the next step's loads in flight, no barrier until the waves' join.
+//  * merge_kernel joins the key ranges where a launch divides them.
+//
+// A key that a row does not see has no part in its result, whatever its K and V rows hold: scores are
+// replaced, V rows past a sequence's end are zeroed, and where some row of a tile does not see a key, the
+// key's infinite and NaN values are zeroed too and added for the rows that see it afterwards.
+#include <algorithm>
+
+#include "attn_common.h"
+
+namespace fl {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * kWave;
+constexpr int kChunkRows = 32 * kWaves;  // queries of a workgroup of chunk_kernel
+constexpr int kStepKeys = 32;            // keys of a wave's step in step_kernel
+constexpr int kStepRows = 16;            // its queries
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+struct PagedArgs {
+  const uint16_t* q;  // rows [n, heads * 128], q_row apart
+  int64_t q_row;
+  const uint16_t* k;  // pages [pages, kv, page, 128]
+  const uint16_t* v;
+  uint16_t* o;           // [n, heads * 128]
+  const int32_t* table;  // [seqs, width]
+  const int32_t* lens;   // [seqs]
+  const int32_t* starts; // [seqs + 1], or null: row s is sequence s's
+  int n, seqs, heads, kv, group, width, pages, page_log2;
+  float scale;  // scaling * log2(e)
+  int splits;   // key ranges
+  float* part_o;   // splits > 1: f32 [splits][n * heads][128], row i * heads + head
+  float* part_ml;  // f32 [splits][n * heads][2]: maximum of q.k (kUnseen: no key) and sum
+};
+
+// the maximum of a query that sees no key (kNone: its scores are all -inf)
+constexpr float kUnseen = -INFINITY;
+
+// The rows [first, first + rows) of sequence s, within the call's whatever `starts` holds.
+__device__ __forceinline__ int2 rows_of(const PagedArgs& a, int s) {
+  if (a.starts == nullptr) return make_int2(s, 1);
+  const int first = min(max(a.starts[s], 0), a.n);
+  return make_int2(first, min(max(a.starts[s + 1], first), a.n) - first);
+}
+
+// One sequence's pages of one KV head.
+struct Pages {
+  const int32_t* table;
+  int width, pages, log2, last;  // last: its last key that a table entry can name
+  int64_t page_elems, head_elems;
+  // Page of 16 keys from `key` (a multiple of 16) on, or -1 where the table names none.
+  __device__ __forceinline__ int page(int key) const {
+    const int i = key >> log2;
+    const int id = i < width ? table[i] : -1;
+    return static_cast<unsigned>(id) < static_cast<unsigned>(pages) ? id : -1;
+  }
+  // First element of these 16 keys; of page 0 where they have none.
+  __device__ __forceinline__ int64_t at(int id, int key) const {
+    return max(id, 0) * page_elems + head_elems + static_cast<int64_t>(key & ((1 << log2) - 1)) * kDim;
+  }
+};
+
+__device__ __forceinline__ Pages pages_of(const PagedArgs& a, int s, int head, int len) {
+  Pages p;
+  p.table = a.table + static_cast<int64_t>(s) * a.width;
+  p.width = a.width;
+  p.pages = a.pages;
+  p.log2 = a.page_log2;
+  p.last = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(a.width) << a.page_log2)) - 1;
+  p.page_elems = static_cast<int64_t>(a.kv) << (a.page_log2 + 7);
+  p.head_elems = static_cast<int64_t>(head) << (a.page_log2 + 7);
+  return p;
+}
+
+// Infinite and NaN values of a chunk of 8 bf16 become zeros; returns whether there were any.
+__device__ __forceinline__ bool drop_nonfinite(u32x4_t& w) {
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (w[i] & 0x7F80u) == 0x7F80u, hi = (w[i] & 0x7F800000u) == 0x7F800000u;
+    any = any || lo || hi;
+    w[i] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+  }
+  return any;
+}
+// w * v where v is infinite or NaN, else 0
+__device__ __forceinline__ float nonfinite_part(float w, uint16_t v) {
+  return (v & 0x7F80u) == 0x7F80u ? w * bf16_to_f32(v) : 0.0f;
+}
+
+__device__ __forceinline__ uint2 pair4(const float* o, float inv) {
+  return make_uint2(attn_bf16_pair(o[0] * inv, o[1] * inv), attn_bf16_pair(o[2] * inv, o[3] * inv));
+}
+
+template <bool SPLIT>
+__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
+  __shared__ AttnLds L;
+  __shared__ int wave_pos[2][kWaves];
+  __shared__ unsigned long long odd_keys[4];  // by tile % 4: keys of a tile with infinite or NaN values
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int head = static_cast<int>(blockIdx.x) % a.kv;
+  const int rest = static_cast<int>(blockIdx.x) / a.kv;
+  const int split = SPLIT ? rest % a.splits : 0;
+  const int index = SPLIT ? rest / a.splits : rest;
+
+  // The index-th tile from the end (a sequence's later rows see more keys): sequences in lanes.
+  int total = 0;
+  for (int base = 0; base < a.seqs; base += kWave) {
+    const int s = base + lane;
+    int t = s < a.seqs ? (rows_of(a, s).y * a.group + kChunkRows - 1) / kChunkRows : 0;
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) t += __shfl_xor(t, off, kWave);
+    total += t;
+  }
+  total = __builtin_amdgcn_readfirstlane(total);
+  if (index >= total) {  // rows that belong to no sequence: zeros
+    if (split != 0) return;
+    const int behind = min(max(a.starts[a.seqs], 0), a.n);
+    const int spare = static_cast<int>(gridDim.x) / a.kv / a.splits - total, width = a.group * kDim / 8;
+    for (int64_t row = behind + index - total; row < a.n; row += spare)
+      for (int c = tid; c < width; c += kThreads)
+        *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * c) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int want = total - 1 - index;
+  int seq = 0, tile_of_seq = 0, before = 0;
+  for (int base = 0; base < a.seqs; base += kWave) {
+    const int s = base + lane;
+    const int mine = s < a.seqs ? (rows_of(a, s).y * a.group + kChunkRows - 1) / kChunkRows : 0;
+    int t = mine;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int u = __shfl_up(t, off, kWave);
+      t += lane >= off ? u : 0;
+    }
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + t > want);
+    if (past != 0ull) {
+      const int l = __builtin_ctzll(past);
+      seq = base + l;
+      tile_of_seq = want - before - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(mine, l));
+      break;
+    }
+    before += __builtin_amdgcn_readlane(t, kWave - 1);
+  }
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  tile_of_seq = __builtin_amdgcn_readfirstlane(tile_of_seq);
+
+  const int2 rows = rows_of(a, seq);
+  const int len = max(a.lens[seq], 0);
+  const Pages pages = pages_of(a, seq, head, len);
+  const int r = tile_of_seq * kChunkRows + wave * 32 + (lane & 31);
+  const bool valid = r < rows.y * a.group;
+  const int rc = valid ? r : rows.y * a.group - 1;
+  const int token = rc / a.group, out_head = head * a.group + rc - token * a.group;
+  const int64_t row = rows.x + token;
+  const int pos = len - rows.y + token;
+  int wmin = pos, wmax = pos;
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) {
+    wmin = min(wmin, __shfl_xor(wmin, off, kWave));
+    wmax = max(wmax, __shfl_xor(wmax, off, kWave));
+  }
+  if (lane == 0) {
+    wave_pos[0][wave] = wmin;
+    wave_pos[1][wave] = wmax;
+  }
+  if (tid < 4) odd_keys[tid] = 0ull;
+
+  bf16x8_t q[8];
+  {
+    const uint16_t* qp = a.q + row * a.q_row + out_head * kDim + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
+  }
+  lds_barrier();
+  int low = wave_pos[0][0], end = wave_pos[1][0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) {
+    low = min(low, wave_pos[0][w]);
+    end = max(end, wave_pos[1][w]);
+  }
+  low = __builtin_amdgcn_readfirstlane(low);
+  // a sequence longer than its table row: its rows are NaN
+  float poison = len - 1 > pages.last ? NAN : 0.0f;
+  int tiles = __builtin_amdgcn_readfirstlane(min(end, pages.last)) / kKeys + 1;
+  if (min(end, pages.last) < 0) tiles = 0;
+  int first = 0;
+  if (SPLIT) {
+    first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+    tiles = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  }
+
+  // this thread's 16-byte chunks of a tile: rows tid / 16 of the tile's four blocks of 16 keys
+  const int lrow = tid >> 4, lcol = (tid & 15) * 8;
+  u32x4_t kr[4], vr[4];
+  int ids[4];
+  const auto look_up = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ids[i] = pages.page(min(tile * kKeys + 16 * i, pages.last & ~15));
+  };
+  const auto fetch = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = pages.at(ids[i], min(tile * kKeys + 16 * i, pages.last & ~15)) + lrow * kDim + lcol;
+      kr[i] = *reinterpret_cast<const u32x4_t*>(a.k + at);
+      vr[i] = *reinterpret_cast<const u32x4_t*>(a.v + at);
+    }
+  };
+  const auto stage = [&](int tile) __attribute__((always_inline)) {
+    const int buf = (tile - first) & 1;
+    if (tile * kKeys + kKeys - 1 > low) {  // some row does not see some key of the tile
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * i + lrow;
+        if (tile * kKeys + key > pages.last) {
+          vr[i] = u32x4_t{0, 0, 0, 0};
+        } else if (drop_nonfinite(vr[i])) {
+          atomicOr(&odd_keys[tile & 3], 1ull << key);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<u32x4_t*>(&L.k[buf][(lrow + 16 * i) * kKRow + lcol]) = kr[i];
+      *reinterpret_cast<u32x4_t*>(&L.v[buf][(lrow + 16 * i) * kVRow + lcol]) = vr[i];
+    }
+  };
+  f32x16_t o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  // running maximum (of q.k, and scaled to base 2) and this lane's part of the sum
+  float raw = kNone, m = scaled_max(kNone, a.scale), l = 0.0f;
+  bool far = false;  // (wave-uniform) some query's maximum lies past kFar
+
+  if (first < tiles) {
+    look_up(first);
+    // a block of keys without a page: NaN for the rows that see it
+    const auto check = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ids[i] < 0 && pos >= min(tile * kKeys + 16 * i, pages.last & ~15)) poison = NAN;
+    };
+    check(first);
+    fetch(first);
+    stage(first);
+    look_up(min(first + 1, tiles - 1));
+    lds_barrier();
+    for (int tile = first; tile < tiles; ++tile) {
+      const int buf = (tile - first) & 1, next = min(tile + 1, tiles - 1);
+      if (tid == 0) odd_keys[(tile + 2) & 3] = 0ull;
+      check(next);
+      fetch(next);
+      look_up(min(tile + 2, tiles - 1));
+      if (tile * kKeys <= wmax) {  // (wave-uniform) some query of the wave sees this tile
+        f32x16_t s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+          const uint16_t* kl = &L.k[buf][(32 * b + (lane & 31)) * kKRow + 8 * h];
+#pragma unroll
+          for (int st = 0; st < 8; ++st)
+            s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kl + 16 * st), q[st], s[b], 0, 0, 0);
+        }
+        if (tile * kKeys + kKeys - 1 > wmin) {  // keys past a query's position
+          const int lim = pos - tile * kKeys - 4 * h;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * b + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+        mx = fmaxf(mx, swap_half(mx));
+        if (__builtin_amdgcn_ballot_w64(mx > raw) != 0ull) {
+          const float top = fmaxf(raw, mx), mn = scaled_max(top, a.scale);
+          const float alpha = exp2_between(raw, top, m, mn, a.scale);
+          raw = top;
+          m = mn;
+          l *= alpha;
+          far = __builtin_amdgcn_ballot_w64(fabsf(m) > kFar && raw > kNone) != 0ull;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        }
+        float off = -m;
+        if (far) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] -= raw;
+          off = 0.0f;
+        }
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        bf16x8_t p[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          u32x4_t w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = 8 * (t & 1) + 2 * i;
+            const float p0 = fast_exp2(fmaf(s[t >> 1][e], a.scale, off));
+            const float p1 = fast_exp2(fmaf(s[t >> 1][e + 1], a.scale, off));
+            w[i] = attn_bf16_pair(p0, p1);
+            sum[i] = add_pair(w[i], sum[i]);
+          }
+          p[t] = __builtin_bit_cast(bf16x8_t, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const int i16 = lane & 15;
+        const uint16_t* vl = &L.v[buf][(4 * h + (i16 >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (i16 & 3)];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const bf16x4_t lo = read_v_tr(vl + (16 * t) * kVRow + 32 * d);
+            const bf16x4_t hi = read_v_tr(vl + (16 * t + 8) * kVRow + 32 * d);
+            const bf16x8_t va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[t], o[d], 0, 0, 0);
+          }
+        if (tile * kKeys + kKeys - 1 > low) {
+          for (unsigned long long odd = odd_keys[tile & 3]; odd != 0ull; odd &= odd - 1) {
+            // key j lies in result register 4 (j / 8) + j % 4 of lane half j / 4 % 2
+            const int j = __builtin_amdgcn_readfirstlane(__builtin_ctzll(odd)), e = 4 * (j >> 3) + (j & 3);
+            float w = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (8 * t + i == e) w = static_cast<float>(p[t][i]);
+            w = __shfl(w, (lane & 31) + 32 * ((j >> 2) & 1), kWave);
+            const int key = tile * kKeys + j;
+            if (key <= pos) {
+              const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * h;
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  o[d][i] += nonfinite_part(w, vp[32 * d + 8 * (i >> 2) + (i & 3)]);
+            }
+          }
+        }
+      }
+      if (tile + 1 < tiles) stage(next);  // (its buffer was read by every wave before the previous tile's barrier)
+      lds_barrier();
+    }
+  }
+
+  l += swap_half(l) + poison;
+  if (!valid) return;
+  if (SPLIT) {
+    const int64_t part = (static_cast<int64_t>(split) * a.n + row) * a.heads + out_head;
+    float* op = a.part_o + part * kDim + 4 * h;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(op + 32 * d + 8 * g) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    const bool seen = pos >= first * kKeys && first < tiles;
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(seen ? raw : kUnseen, l);
+    return;
+  }
+  const float inv = pos >= 0 ? 1.0f / l : 0.0f;
+  uint16_t* op = a.o + (row * a.heads + out_head) * kDim + 4 * h;
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float part[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      *reinterpret_cast<uint2*>(op + 32 * d + 8 * g) = pair4(part, inv);
+    }
+}
+
+// The key ranges that a sequence of `steps` steps is divided into: at least one step for each wave of a range.
+__device__ __forceinline__ int step_ranges(int splits, int steps) { return max(1, min(splits, steps / kWaves)); }
+
+template <bool SPLIT>
+__global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kWaves][kStepKeys * kVRow];
+  __shared__ float2 wave_ml[kWaves][kStepRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int head = static_cast<int>(blockIdx.x) % a.kv;
+  const int rest = static_cast<int>(blockIdx.x) / a.kv;
+  const int split = SPLIT ? rest % a.splits : 0;
+  const int seq = SPLIT ? rest / a.splits : rest;
+  if (seq == a.seqs) {  // rows that belong to no sequence: zeros
+    if (split != 0) return;
+    const int width = a.group * kDim / 8;
+    for (int64_t row = min(max(a.starts[a.seqs], 0), a.n); row < a.n; ++row)
+      for (int i = tid; i < width; i += kThreads)
+        *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * i) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const int2 rows = rows_of(a, seq);
+  const int len = max(a.lens[seq], 0);
+  const Pages pages = pages_of(a, seq, head, len);
+
+  for (int base = 0; base < rows.y * a.group; base += kStepRows) {
+    const int rc = min(base + c, rows.y * a.group - 1);
+    const int token = rc / a.group, out_head = head * a.group + rc - token * a.group;
+    const int64_t row = rows.x + token;
+    const int pos = len - rows.y + token;
+    const int low = len - rows.y + base / a.group;
+    const int end = min(len - rows.y + min(base + kStepRows - 1, rows.y * a.group - 1) / a.group, pages.last);
+    int steps = end >= 0 ? end / kStepKeys + 1 : 0, first = 0;
+    if (SPLIT) {
+      const int ranges = step_ranges(a.splits, steps);
+      first = split < ranges ? static_cast<int>(static_cast<int64_t>(steps) * split / ranges) : steps;
+      steps = split < ranges ? static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / ranges) : steps;
+    }
+    bf16x8_t q[4];
+    {
+      const uint16_t* qp = a.q + row * a.q_row + out_head * kDim + 8 * g;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) q[st] = *reinterpret_cast<const bf16x8_t*>(qp + 32 * st);
+    }
+    f32x4_t o[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float raw = kNone, m = scaled_max(kNone, a.scale), l = 0.0f;
+    float poison = len - 1 > pages.last ? NAN : 0.0f;
+    bool far = false;
+
+    bf16x8_t kr[2][4];
+    u32x4_t vr[8];
+    int ids[2];
+    const auto look_up = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) ids[b] = pages.page(min(step * kStepKeys + 16 * b, pages.last & ~15));
+    };
+    const auto fetch = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int key = min(step * kStepKeys + 16 * b, pages.last & ~15);
+        if (ids[b] < 0 && pos >= key) poison = NAN;
+        const int64_t at = pages.at(ids[b], key);
+        const uint16_t* kp = a.k + at + c * kDim + 8 * g;
+        const uint16_t* vp = a.v + at + g * kDim + 8 * c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          kr[b][i] = *reinterpret_cast<const bf16x8_t*>(kp + 32 * i);
+          vr[4 * b + i] = *reinterpret_cast<const u32x4_t*>(vp + 4 * i * kDim);
+        }
+      }
+    };
+    uint16_t* const vl = lds[wave];
+    const uint16_t* const vt = vl + (4 * g + (c >> 2)) * kVRow + 4 * (c & 3);
+    const int begin = __builtin_amdgcn_readfirstlane(first + wave);
+    if (begin < steps) {
+      look_up(begin);
+      fetch(begin);
+      look_up(min(begin + kWaves, steps - 1));
+    }
+    for (int step = begin; step < steps; step += kWaves) {
+      f32x4_t s[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        s[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < 4; ++st) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[b][st], q[st], s[b], 0, 0, 0);
+      }
+      uint32_t odd = 0;  // keys with infinite or NaN values that some row does not see
+      if (step * kStepKeys + kStepKeys - 1 > low) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = step * kStepKeys + 4 * i + g;
+          bool any = false;
+          if (key > pages.last) {
+            vr[i] = u32x4_t{0, 0, 0, 0};
+          } else if (key > low) {
+            any = drop_nonfinite(vr[i]);
+          }
+          const unsigned long long lanes = __builtin_amdgcn_ballot_w64(any);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((lanes >> (16 * j)) & 0xFFFFull) odd |= 1u << (4 * i + j);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (step * kStepKeys + 16 * b + 4 * g + i > pos) s[b][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4_t*>(&vl[(4 * i + g) * kVRow + 8 * c]) = vr[i];
+      if (step + kWaves < steps) {
+        fetch(step + kWaves);
+        look_up(min(step + 2 * kWaves, steps - 1));
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      if (__builtin_amdgcn_ballot_w64(mx > raw) != 0ull) {
+        const float top = fmaxf(raw, mx), mn = scaled_max(top, a.scale);
+        const float alpha = exp2_between(raw, top, m, mn, a.scale);
+        raw = top;
+        m = mn;
+        l *= alpha;
+        far = __builtin_amdgcn_ballot_w64(fabsf(m) > kFar && raw > kNone) != 0ull;
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][i] *= alpha;
+      }
+      float off = -m;
+      if (far) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[b][i] -= raw;
+        off = 0.0f;
+      }
+      // the second product's k index 8 g + 4 b + i is key 16 b + 4 g + i: the scores stay in their lanes
+      u32x4_t w;
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float p0 = fast_exp2(fmaf(s[b][2 * i], a.scale, off)), p1 = fast_exp2(fmaf(s[b][2 * i + 1], a.scale, off));
+          w[2 * b + i] = attn_bf16_pair(p0, p1);
+          sum[b] = add_pair(w[2 * b + i], sum[b]);
+        }
+      l += sum[0] + sum[1];
+      const bf16x8_t p = __builtin_bit_cast(bf16x8_t, w);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const bf16x4_t lo = read_v_tr(vt + 16 * d), hi = read_v_tr(vt + 16 * kVRow + 16 * d);
+        const bf16x8_t va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p, o[d], 0, 0, 0);
+      }
+      __builtin_amdgcn_wave_barrier();
+      for (odd = __builtin_amdgcn_readfirstlane(odd); odd != 0; odd &= odd - 1) {
+        const int j = __builtin_ctz(odd), e = 4 * (j >> 4) + (j & 3);  // register e of lane group j / 4 % 4
+        float pw = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i == e) pw = static_cast<float>(p[i]);
+        pw = __shfl(pw, c + 16 * ((j >> 2) & 3), kWave);
+        const int key = step * kStepKeys + j;
+        if (key <= pos) {
+          const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * g;
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[d][i] += nonfinite_part(pw, vp[16 * d + i]);
+        }
+      }
+    }
+
+    // the waves' join: their outputs through LDS (each wave over its own V rows)
+    l += __shfl_xor(l, 16, kWave);
+    l += __shfl_xor(l, 32, kWave);
+    l += poison;
+    const bool seen = begin < steps && pos >= begin * kStepKeys;
+    if (g == 0) wave_ml[wave][c] = make_float2(seen || l != l ? raw : kUnseen, l);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    float* const wo = reinterpret_cast<float*>(vl);
+    static_assert(kStepRows * kDim * sizeof(float) <= kStepKeys * kVRow * sizeof(uint16_t), "a wave's outputs fit its V rows");
+#pragma unroll
+    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&wo[c * kDim + 16 * d + 4 * g]) = o[d];
+    lds_barrier();
+    const int jr = tid >> 4, ch = 8 * (tid & 15);
+    if (base + jr < rows.y * a.group) {
+      float top = kUnseen;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, wave_ml[w][jr].x);
+      const float st = scaled_max(top, a.scale);
+      float sum = 0.0f, acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float2 ml = wave_ml[w][jr];
+        if (ml.x == kUnseen) continue;
+        const float f = exp2_between(ml.x, top, scaled_max(ml.x, a.scale), st, a.scale);
+        sum = fmaf(f, ml.y, sum);
+        const float* src = reinterpret_cast<const float*>(lds[w]) + jr * kDim + ch;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+      }
+      const int tok = (base + jr) / a.group, oh = head * a.group + base + jr - tok * a.group;
+      const int64_t orow = static_cast<int64_t>(rows.x + tok) * a.heads + oh;
+      if (SPLIT) {
+        const int64_t part = static_cast<int64_t>(split) * a.n * a.heads + orow;
+        float* op = a.part_o + part * kDim + ch;
+        if (top != kUnseen) {
+          *reinterpret_cast<float4*>(op) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+          *reinterpret_cast<float4*>(op + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+        }
+        if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(top, sum);
+      } else {
+        const float inv = top != kUnseen ? 1.0f / sum : 0.0f;
+        const uint2 x = pair4(acc, inv), y = pair4(acc + 4, inv);
+        *reinterpret_cast<uint4*>(a.o + orow * kDim + ch) = make_uint4(x.x, x.y, y.x, y.y);
+      }
+    }
+    lds_barrier();  // (the next rows' V goes where these outputs lie)
+  }
+}
+
+// Joins the key ranges: 32 lanes per (row, head), 4 channels each.
+__global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
+  const int64_t rows = (a.starts ? min(max(a.starts[a.seqs], 0), a.n) : a.n) * static_cast<int64_t>(a.heads);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int64_t all = static_cast<int64_t>(a.n) * a.heads;
+  const int c = (threadIdx.x & 31) * 4;
+  float top = kUnseen;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + row)]);
+  const float st = scaled_max(top, a.scale);
+  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * all + row));
+    if (ml.x == kUnseen) {
+      l += ml.y != ml.y ? ml.y : 0.0f;
+      continue;
+    }
+    const float4 p = *reinterpret_cast<const float4*>(a.part_o + (s * all + row) * kDim + c);
+    const float w = exp2_between(ml.x, top, scaled_max(ml.x, a.scale), st, a.scale);
+    l = fmaf(w, ml.y, l);
+    o[0] = fmaf(w, p.x, o[0]);
+    o[1] = fmaf(w, p.y, o[1]);
+    o[2] = fmaf(w, p.z, o[2]);
+    o[3] = fmaf(w, p.w, o[3]);
+  }
+  const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint2*>(a.o + row * kDim + c) = pair4(o, inv);
+}
+
+// Sequences of few rows take step_kernel: up to 16 queries of a KV head are one pass over its keys there.
+bool few_rows(int max_q, int group) { return static_cast<int64_t>(max_q) * group <= kStepRows; }
+
+// Key ranges: enough workgroups to fill the chip, of at least 128 (step) or 448 (chunk) keys each.
+int paged_splits(int seqs, int n, int kv, int group, int max_q, int max_kv) {
+  const bool step = few_rows(max_q, group);
+  const int64_t groups = step ? static_cast<int64_t>(seqs) * kv
+                              : ((static_cast<int64_t>(n) * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs / 2 : 0)) * kv;
+  const int64_t want = ((step ? 1024 : 640) + groups - 1) / std::max<int64_t>(groups, 1);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), max_kv / (step ? 128 : 448))));
+}
+
+size_t paged_split_bytes(int64_t n, int64_t heads) { return static_cast<size_t>(n) * heads * (kDim + 2) * sizeof(float); }
+
+}  // namespace
+}  // namespace fl
+
+extern "C" size_t fl_paged_attention_workspace(int32_t rows, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q,
+                                               int32_t max_kv) {
+  using namespace fl;
+  if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || heads % kv_heads || max_q <= 0 || max_kv <= 0) return 0;
+  const int s = paged_splits(seqs, rows, kv_heads, heads / kv_heads, max_q, max_kv);
+  return s > 1 ? s * paged_split_bytes(rows, heads) : 0;
+}
+
+extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, const uint16_t* k_pages, const uint16_t* v_pages,
+                                      uint16_t* out, const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_starts,
+                                      int32_t rows, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t table_width,
+                                      int32_t pages, int32_t page_size, int32_t max_q, int32_t max_kv, float scaling,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace fl;
+  clear_error();
+  FL_REQUIRE(q && k_pages && v_pages && out && page_table && kv_lens, "fl_paged_attention: null pointer");
+  FL_REQUIRE(rows >= 0 && seqs >= 0 && table_width > 0 && pages > 0, "fl_paged_attention: bad sizes");
+  FL_REQUIRE(kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "fl_paged_attention: heads must be a multiple of the KV heads");
+  FL_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+             "fl_paged_attention: the page size must be a power of two from 16 to 1024");
+  FL_REQUIRE(q_row_stride >= static_cast<int64_t>(heads) * kDim && q_row_stride % 8 == 0, "fl_paged_attention: bad row stride");
+  FL_REQUIRE(q_starts != nullptr || rows == seqs, "fl_paged_attention: one row a sequence without q_starts");
+  FL_REQUIRE(max_q > 0 && max_kv > 0, "fl_paged_attention: max_q and max_kv must be positive");
+  FL_REQUIRE(scaling > 0.0f && std::isfinite(scaling), "fl_paged_attention: scaling must be positive and finite");
+  FL_REQUIRE(static_cast<int64_t>(table_width) * page_size <= 0x7FFFFFFF - 4096, "fl_paged_attention: a sequence's pages hold too many tokens");
+  const int group = heads / kv_heads;
+  FL_REQUIRE(static_cast<int64_t>(rows) * group <= 0x7FFFFFFF - 4096, "fl_paged_attention: too many rows");
+  for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k_pages), static_cast<const void*>(v_pages),
+                        static_cast<const void*>(out)})
+    FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_paged_attention: every tensor must be 16-byte aligned");
+  if (rows == 0) return FL_OK;
+  FL_REQUIRE(seqs > 0, "fl_paged_attention: rows without a sequence");
+  if (q_starts == nullptr) max_q = 1;
+  PagedArgs a{q, q_row_stride, k_pages, v_pages, out, page_table, kv_lens, q_starts, rows, seqs, heads, kv_heads, group,
+              table_width, pages, __builtin_ctz(static_cast<unsigned>(page_size)), scaling * kLog2e,
+              paged_splits(seqs, rows, kv_heads, group, max_q, max_kv), nullptr, nullptr};
+  // as many ranges as the workspace holds (one without it)
+  const size_t one = paged_split_bytes(rows, heads);
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) workspace_bytes = 0;
+  a.splits = static_cast<int>(std::max<size_t>(1, std::min<size_t>(a.splits, workspace_bytes / one)));
+  const bool step = q_starts == nullptr || few_rows(max_q, group);
+  const int64_t tiles = step ? seqs + (q_starts ? 1 : 0) : (static_cast<int64_t>(rows) * group + kChunkRows - 1) / kChunkRows + seqs;
+  FL_REQUIRE(tiles * kv_heads * a.splits <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
+  const dim3 grid(static_cast<unsigned>(tiles * kv_heads * a.splits)), block(kThreads);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a.splits <= 1) {
+    if (step)
+      hipLaunchKernelGGL(step_kernel<false>, grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL(chunk_kernel<false>, grid, block, 0, st, a);
+    FL_LAUNCH_CHECK("fl_paged_attention");
+    return FL_OK;
+  }
+  const int64_t all = static_cast<int64_t>(rows) * heads;
+  FL_REQUIRE((all + 7) / 8 <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + a.splits * all * kDim;
+  if (step)
+    hipLaunchKernelGGL(step_kernel<true>, grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL(chunk_kernel<true>, grid, block, 0, st, a);
+  FL_LAUNCH_CHECK("fl_paged_attention");
+  hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((all + 7) / 8)), dim3(256), 0, st, a);
+  FL_LAUNCH_CHECK("fl_paged_attention(join)");
+  return FL_OK;
+}

@@ -14,7 +14,7 @@ from array import array
 import torch
 
 from . import _lib
-from ._lib import GROUP, HEAD_DIM, MX_BLOCK, MX_MAX_K, MX_PAD, check, load, ptr_array
+from ._lib import GROUP, HEAD_DIM, MAX_BEAMS, MX_BLOCK, MX_MAX_K, MX_PAD, check, load, ptr_array
 
 
 def _stream() -> int:
@@ -943,3 +943,187 @@ def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.b
         _launch(device, "fl_mx_matmul", load().fl_mx_matmul, x.codes.data_ptr(), x.scales.data_ptr(), m, x.cols,
                 weight.codes.data_ptr(), weight.scales.data_ptr(), n, y.data_ptr(), f32, n)
     return y
+
+
+# ---------------------------------------------------------------------------- K/V pages and beams
+def _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, rows):
+    """(pages, KV heads, page size, sequences, table width) of a call on K/V pages, checked."""
+    device, shape = k_pages.device, k_pages.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v_pages.shape != shape:
+        raise ValueError(f"k_pages and v_pages must be [pages, KV heads, page, {HEAD_DIM}] of one shape")
+    if k_pages.dtype is not torch.bfloat16 or v_pages.dtype is not torch.bfloat16 or v_pages.device != device:
+        raise ValueError("k_pages and v_pages must be bfloat16 on one device")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous")
+    if page_table.ndim != 2 or kv_lens.ndim != 1 or kv_lens.shape[0] != page_table.shape[0]:
+        raise ValueError("page_table must be [sequences, pages of a sequence] and kv_lens [sequences]")
+    seqs, width = page_table.shape
+    for t, name in ((page_table, "page_table"), (kv_lens, "kv_lens"), (q_starts, "q_starts")):
+        if t is not None and (t.dtype is not torch.int32 or t.device != device or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous int32 on {device}")
+    if q_starts is None:
+        if rows != seqs:
+            raise ValueError(f"one row a sequence without q_starts: got {rows} rows and {seqs} sequences")
+    elif q_starts.ndim != 1 or q_starts.shape[0] != seqs + 1:
+        raise ValueError("q_starts must be [sequences + 1]")
+    return shape[0], shape[1], shape[2], seqs, width
+
+
+def _head_rows(x: torch.Tensor, name: str, device) -> torch.Tensor:
+    """bf16 rows [n, heads * 128], at any distance that is a multiple of 8 values."""
+    if x.ndim != 2 or x.shape[1] == 0 or x.shape[1] % HEAD_DIM or x.dtype is not torch.bfloat16 or x.device != device:
+        raise ValueError(f"{name} must be bfloat16 [rows, heads * {HEAD_DIM}] on {device}")
+    if x.stride(1) != 1 or x.stride(0) % 8 or (x.stride(0) < x.shape[1] and x.shape[0] > 1) or x.data_ptr() % 16:
+        return x.contiguous()
+    return x
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    return max(x.stride(0), x.shape[1])
+
+
+def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rope: tuple[torch.Tensor, torch.Tensor] | None,
+                 k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                 q_starts: torch.Tensor | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Rows of several sequences into their K/V pages, rotated on the way (``fl_paged_append``).  ``q`` [n, H*128],
+    ``k`` and ``v`` [n, KV*128] bf16 (columns of one wider matrix are taken where they are); ``rope``: cos and
+    sin [positions, 128], bf16 or f32, or None (then ``k`` is stored as it is and ``q`` is returned untouched);
+    ``k_pages`` / ``v_pages`` bf16 [pages, KV, page, 128], written in place; ``page_table`` i32 [S, W]; ``kv_lens`` i32
+    [S], with the call's rows counted; ``q_starts`` i32 [S + 1]: rows q_starts[s] .. q_starts[s + 1] - 1 are
+    the last tokens of sequence s (None: one row a sequence).  Returns the rotated rows of ``q``, in ``out``
+    (``q`` itself, or rows that do not lie on it) if given; rows behind the last sequence as they are."""
+    device = k_pages.device
+    k, v = _head_rows(k, "k", device), _head_rows(v, "v", device)
+    n = k.shape[0]
+    pages, kv, page, seqs, width = _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, n)
+    if k.shape != v.shape or k.shape[1] != kv * HEAD_DIM:
+        raise ValueError(f"k and v must be [{n}, {kv * HEAD_DIM}], as the pages have {kv} heads")
+    heads, positions, f32, cos, sin, q_stride, out_stride = 1, 0, False, None, None, 0, 0
+    q2 = None
+    if rope is not None:
+        if q is None:
+            raise ValueError("rope tables without q")
+        cos, sin = rope
+        f32 = cos.dtype is torch.float32
+        if (cos.ndim != 2 or cos.shape[1] != HEAD_DIM or sin.shape != cos.shape or not (f32 or cos.dtype is torch.bfloat16)
+                or sin.dtype is not cos.dtype or cos.device != device or sin.device != device):
+            raise ValueError(f"rope tables must be bfloat16 or float32 [positions, {HEAD_DIM}] on {device}")
+        if not (cos.is_contiguous() and sin.is_contiguous()):
+            raise ValueError("rope tables must be contiguous")
+        q2 = _head_rows(q, "q", device)
+        if q2.shape[0] != n:
+            raise ValueError(f"q has {q2.shape[0]} rows, k {n}")
+        heads, positions, q_stride = q2.shape[1] // HEAD_DIM, cos.shape[0], _row_stride(q2)
+        if out is None:
+            out = q2.new_empty(q2.shape)
+        elif out.shape != q2.shape or out.dtype is not torch.bfloat16 or out.device != device or out.stride(1) != 1 or out.stride(0) % 8:
+            raise ValueError("out must be bfloat16 of the shape of q, on its device, with contiguous rows")
+        elif out.data_ptr() == q.data_ptr() and q2 is q and out.stride(0) != q.stride(0) and n > 1:
+            raise ValueError("out lies on q with another row stride")
+        out_stride = _row_stride(out)
+    elif out is not None:
+        raise ValueError("without rope tables q is returned as it is: there is no out")
+    if n:
+        _launch(device, "fl_paged_append", load().fl_paged_append, _p(q2), q_stride, k.data_ptr(), _row_stride(k), v.data_ptr(),
+                _row_stride(v), _p(out), out_stride, _p(cos), _p(sin), f32, positions, k_pages.data_ptr(), v_pages.data_ptr(),
+                page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, heads, kv, width, pages, page)
+    return q if rope is None else out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                    kv_lens: torch.Tensor, scaling: float, q_starts: torch.Tensor | None = None, *, max_q: int | None = None,
+                    max_kv: int | None = None) -> torch.Tensor:
+    """Causal attention of new tokens over K/V pages (``fl_paged_attention``): ``q`` [n, H*128] bf16, the last
+    tokens of their sequences (``paged_append`` has put their keys and values in the pages), each seeing the
+    keys up to its own position; H a multiple of the pages' KV heads.  The other arguments as in ``paged_append``.
+    ``max_q`` and ``max_kv``: the most rows and tokens of a sequence, if known (by default the call's rows and the
+    table's capacity): they divide the work and have no part in the result.  Returns bf16 [n, H*128]: zeros for
+    rows that see no key or belong to no sequence, NaN for rows that see a key without a page."""
+    device = k_pages.device
+    q = _head_rows(q, "q", device)
+    n, cols = q.shape
+    pages, kv, page, seqs, width = _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, n)
+    heads = cols // HEAD_DIM
+    if heads % kv:
+        raise ValueError(f"{heads} query heads do not share {kv} KV heads")
+    out = q.new_empty((n, cols))
+    if not n:
+        return out
+    max_q = 1 if q_starts is None else max(1, n if max_q is None else min(int(max_q), n))
+    max_kv = max(1, width * page if max_kv is None else min(int(max_kv), width * page))
+    lib = load()
+    size = lib.fl_paged_attention_workspace(n, seqs, heads, kv, max_q, max_kv)
+    ws = q.new_empty(size, dtype=torch.uint8) if size else None
+    _launch(device, "fl_paged_attention", lib.fl_paged_attention, q.data_ptr(), _row_stride(q), k_pages.data_ptr(),
+            v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, heads, kv, width,
+            pages, page, max_q, max_kv, scaling, _p(ws), size)
+    return out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = None):
+    """The ``count`` (2 K by default) best continuations of each sequence's beams (``fl_beam_select``): ``logits``
+    [S*K, vocab] f32 or bf16 (rows at any distance), ``scores`` f32 [S, K], the beams' log-probabilities.  Returns (scores f32,
+    beams i32, tokens i64), each [S, count], the best first: scores[s, k] + log_softmax(logits)[s*K + k, t], ties
+    to the lower beam, then the lower token."""
+    if scores.ndim != 2 or scores.dtype is not torch.float32:
+        raise ValueError("scores must be float32 [sequences, beams]")
+    seqs, beams = scores.shape
+    if logits.ndim != 2 or logits.shape[0] != seqs * beams:
+        raise ValueError(f"logits must be [{seqs * beams}, vocab]")
+    f32 = logits.dtype is torch.float32
+    if not f32 and logits.dtype is not torch.bfloat16:
+        raise ValueError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    device, vocab = logits.device, logits.shape[1]
+    if scores.device != device:
+        raise ValueError("logits and scores lie on different devices")
+    count = 2 * beams if count is None else int(count)
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"1 to {MAX_BEAMS} beams, got {beams}")
+    if not 1 <= count <= min(MAX_BEAMS, beams * vocab):
+        raise ValueError(f"count must be 1..{min(MAX_BEAMS, beams * vocab)}, got {count}")
+    if logits.stride(1) != 1 or (logits.stride(0) < vocab and seqs * beams > 1):
+        logits = logits.contiguous()
+    scores = scores if scores.is_contiguous() else scores.contiguous()
+    out = (scores.new_empty((seqs, count)), scores.new_empty((seqs, count), dtype=torch.int32),
+           scores.new_empty((seqs, count), dtype=torch.int64))
+    if seqs:
+        lib = load()
+        size = lib.fl_beam_select_workspace(seqs, beams, vocab, count)
+        ws = scores.new_empty(size, dtype=torch.uint8)
+        _launch(device, "fl_beam_select", lib.fl_beam_select, logits.data_ptr(), f32, _row_stride(logits), scores.data_ptr(), seqs,
+                beams, vocab, count, *(t.data_ptr() for t in out), ws.data_ptr(), size)
+    return out
+
+
+def paged_reorder(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                  parents: torch.Tensor) -> torch.Tensor:
+    """Beam k of sequence s takes over the state of beam ``parents[s, k]`` (``fl_paged_reorder``): ``k_pages`` /
+    ``v_pages`` bf16 [layers, pages, KV, page, 128] (or one layer's [pages, KV, page, 128]), ``page_table`` i32
+    [S*K, W], ``kv_lens`` i32 [S*K] (beams of a sequence have one length), ``parents`` i32 [S, K].  Returns the
+    new table: full pages are shared by a beam's children, and the rows of the page being filled are copied, in
+    place, for every child but the first into the page of a beam that has none."""
+    if k_pages.ndim == 4:
+        k_pages, v_pages = k_pages[None], v_pages[None]
+    device, shape = k_pages.device, k_pages.shape
+    if len(shape) != 5 or shape[4] != HEAD_DIM or v_pages.shape != shape or not shape[0]:
+        raise ValueError(f"k_pages and v_pages must be [layers, pages, KV heads, page, {HEAD_DIM}] of one shape")
+    if k_pages.dtype is not torch.bfloat16 or v_pages.dtype is not torch.bfloat16 or v_pages.device != device:
+        raise ValueError("k_pages and v_pages must be bfloat16 on one device")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous")
+    if parents.ndim != 2:
+        raise ValueError("parents must be [sequences, beams]")
+    seqs, beams = parents.shape
+    if not 1 <= beams <= MAX_BEAMS:
+        raise ValueError(f"1 to {MAX_BEAMS} beams, got {beams}")
+    if page_table.ndim != 2 or page_table.shape[0] != seqs * beams or kv_lens.shape != (seqs * beams,):
+        raise ValueError(f"page_table must be [{seqs * beams}, pages of a sequence] and kv_lens [{seqs * beams}]")
+    for t, name in ((page_table, "page_table"), (kv_lens, "kv_lens"), (parents, "parents")):
+        if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 on {device}")
+    table = torch.empty_like(page_table)
+    if seqs:
+        _launch(device, "fl_paged_reorder", load().fl_paged_reorder, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+                table.data_ptr(), kv_lens.data_ptr(), parents.data_ptr(), seqs, beams, shape[0], page_table.shape[1], shape[1],
+                shape[2], shape[3])
+    return table

@@ -604,6 +604,74 @@ int32_t fl_mx_gemv_chain(int32_t m, int32_t k, float eps, const uint16_t* x, con
 int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m, int32_t k, const uint8_t* w_codes,
                      const uint8_t* w_scales, int32_t n, void* y, int32_t y_is_f32, int64_t y_stride, void* stream);
 
+/*
+ * Decoding over K/V pages: the looped model with every loop dense and a bf16 cache (no reference
+ * counterpart: the reference's dense model keeps a Hugging Face cache, flashloop/engine.py:134-150, and its
+ * own cache is the packed one above), and beam search over it.
+ *
+ * Keys and values of one layer lie in pages: bf16 [pages, kv_heads, page_size, 128], page_size a power of two
+ * from 16 to 1024.  page_table i32 [seqs, table_width] names the pages of each sequence in order (entries
+ * past its last page are not read), kv_lens i32 [seqs] counts its tokens, those of the call among them.  A
+ * call's rows are tokens of several sequences one after another: q_starts i32 [seqs + 1] is non-decreasing
+ * from 0, rows q_starts[s] .. q_starts[s + 1] - 1 are the last tokens of sequence s (q_starts NULL: one row a
+ * sequence); rows from q_starts[seqs] on belong to none.  All of these lie in device memory.  A page that
+ * several sequences name (a common prompt) is read by all of them; only one may append to it.
+ *
+ * fl_paged_append: rotate-half rotary embedding of the rows of q (to q_out, which may be q) and k with row p
+ * of rope_cos / rope_sin ([rope_positions, 128], bf16 or f32, both halves of a row alike or not) at position
+ * p, in fp32 and rounded once; k and the plain v to their pages.  Without rope tables k is stored as it is and
+ * q is neither read nor written.  A row whose page or rope row does not exist is stored nowhere and its q_out
+ * is NaN; rows that belong to no sequence are copied to q_out as they are.  Row strides in elements, multiples
+ * of 8; tensors 16-byte aligned.
+ *
+ * fl_paged_attention: out[i, h, :] = sum_j softmax_j(scaling * q[i, h] . K[j]) V[j] over the keys j of the
+ * row's sequence up to its own position, query heads h * kv_heads / heads sharing a KV head; out bf16 [rows,
+ * heads * 128].  Scores, softmax and sums are fp32, probabilities are rounded to bf16 for the second product.
+ * Keys that a row does not see have no part in its result, whatever their rows hold.  A row with no key (its
+ * position is negative) and rows that belong to no sequence are zeros; a row that sees a key without a page
+ * is NaN.  max_q and max_kv, the most rows and tokens of a sequence, choose how the work is divided and change
+ * no result beyond rounding; larger ones than there are only cost time, and so do smaller ones.  With a
+ * workspace (16-byte aligned, of fl_paged_attention_workspace bytes; nullable) calls of few rows divide the
+ * keys over several workgroups and join them; a smaller one divides them less.
+ *
+ * fl_beam_select: the `count` (at most 64) best continuations of each sequence's beams (at most 64):
+ *   total[k, t] = scores[s, k] + x[k, t] - log(sum_t exp(x[k, t])),  x = logits[s * beams + k] (f32 or bf16)
+ * in descending order, ties to the lower beam, then the lower token.  Sums and totals are in 64 bits (out_scores:
+ * rounded to f32); where totals of one beam are equal in 64 bits and its logits are not, the logits decide.  A
+ * beam whose score is not finite, or whose row holds a NaN or +inf or nothing but -inf, has totals of -inf: its
+ * tokens come after all others, in order.  out_scores f32, out_beams i32, out_tokens i64: [seqs, count].
+ *
+ * fl_paged_reorder: beam k of each sequence takes over the state of beam parents[s, k] (i32, 0 .. beams - 1;
+ * at most 64 beams) before its next token.  k_pages / v_pages are those of `layers` layers, [layers, pages,
+ * kv_heads, page_size, 128]; tables and lengths as above with seqs * beams rows, beams of a sequence next to
+ * each other and of one length (that of its first beam is read).  table_out (another buffer) gets the parent's
+ * full pages, which the children share from then on, and the beam's own entries past the page being filled.
+ * That page stays with the parent's first child; every further child takes the page of a beam without
+ * children, in order, and the filled rows are copied there.  The beams' pages being filled have to differ. A
+ * parent outside its range gives a table row of -1.
+ */
+int32_t fl_paged_append(const uint16_t* q, int64_t q_row_stride, const uint16_t* k, int64_t k_row_stride,
+                        const uint16_t* v, int64_t v_row_stride, uint16_t* q_out, int64_t q_out_row_stride,
+                        const void* rope_cos, const void* rope_sin, int32_t rope_is_f32, int32_t rope_positions,
+                        uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                        const int32_t* q_starts, int32_t rows, int32_t seqs, int32_t heads, int32_t kv_heads,
+                        int32_t table_width, int32_t pages, int32_t page_size, void* stream);
+size_t fl_paged_attention_workspace(int32_t rows, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t max_q,
+                                    int32_t max_kv);
+int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, const uint16_t* k_pages, const uint16_t* v_pages,
+                           uint16_t* out, const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_starts,
+                           int32_t rows, int32_t seqs, int32_t heads, int32_t kv_heads, int32_t table_width,
+                           int32_t pages, int32_t page_size, int32_t max_q, int32_t max_kv, float scaling,
+                           void* workspace, size_t workspace_bytes, void* stream);
+size_t fl_beam_select_workspace(int32_t seqs, int32_t beams, int64_t vocab, int32_t count);
+int32_t fl_beam_select(const void* logits, int32_t logits_is_f32, int64_t row_stride, const float* scores,
+                       int32_t seqs, int32_t beams, int64_t vocab, int32_t count, float* out_scores,
+                       int32_t* out_beams, int64_t* out_tokens, void* workspace, size_t workspace_bytes,
+                       void* stream);
+int32_t fl_paged_reorder(uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table, int32_t* table_out,
+                         const int32_t* kv_lens, const int32_t* parents, int32_t seqs, int32_t beams, int32_t layers,
+                         int32_t table_width, int32_t pages, int32_t kv_heads, int32_t page_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
