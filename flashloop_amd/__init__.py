@@ -16,6 +16,7 @@ from .cache import (  # noqa: F401
 from .config import FlashLoopConfig  # noqa: F401
 from .batch_engine import FlashLoopBatchEngine
 from .batch_engine import FlashLoopBatchEngine  # noqa: F401
+from .dense_engine import DenseEngine, PagedKVCache  # noqa: F401
 from .engine import FlashLoopEngine  # noqa: F401
 from .hooks import flashloop  # noqa: F401
 
@@ -27,6 +28,8 @@ __all__ = [
     "decode_attention_step",
     "packed_prefix_tokens",
     "FlashLoopConfig",
+    "DenseEngine",
+    "PagedKVCache",
     "FlashLoopBatchEngine",
     "FlashLoopEngine",
     "flashloop",
