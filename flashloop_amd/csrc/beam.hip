@@ -2,11 +2,12 @@
 //   total[k, t] = score[k] + x[k, t] - log(sum_t' exp(x[k, t'])),
 // ties to the lower beam, then the lower token.
 //
-// One pass over the logits: a workgroup takes a part of a beam's row and keeps, per wave, the largest values
-// so far as one sorted entry a lane, and the sum of exponentials.  The part's largest that a wave has not
-// seen yet are few: with 16 values a lane, a value enters only if it reaches the count-th largest of the
-// lanes' maxima (first step) or passes the list's last entry, so insertions (a vote and a shift of the
-// list) stay near `count` a step.  A second launch joins the parts of a sequence's beams, one list a lane.
+// One pass over the logits: a workgroup takes a part of a beam's row, 48 values a thread in registers, and
+// gives the part's largest values in order and its sum of exponentials.  Of the 64 columns of threads (a lane of
+// every wave) `count` have a maximum of at least the count-th largest of the columns' maxima, so only values that
+// reach it can be among the largest: 18 of 12288 normal values for 16.  They are gathered in LDS and placed by
+// counting.  Rows in which more values reach it than LDS holds (equal ones, masked ones) are inserted one by one
+// into sorted lists, an entry a lane.  A second launch joins the parts of a sequence's beams, one list a lane.
 //
 // The sums and totals are in 64 bits: totals of different beams decide the order among nearly equal
 // candidates, and 32 bits would leave it to the order of the sum.  Within a beam the logits decide.
@@ -19,10 +20,13 @@ namespace {
 
 constexpr int kBeamThreads = 256;
 constexpr int kBeamWaves = kBeamThreads / kWave;
-constexpr int kPer = 16;                         // values of a lane in a step
-constexpr int kBeamStep = kBeamThreads * kPer;   // values of a workgroup's step
-constexpr int kMaxCount = kWave;                 // one list entry a lane
-constexpr int kLists = kWave;                    // lists of a sequence (beams * parts), one a lane
+constexpr int kPer = 16;                              // values of a thread in a chunk
+constexpr int kChunks = 3;                            // chunks of a step
+constexpr int kBeamChunk = kBeamThreads * kPer;       // values of a workgroup's chunk
+constexpr int kBeamStep = kBeamChunk * kChunks;       // and step
+constexpr int kMaxCount = kWave;                      // one list entry a lane
+constexpr int kGathered = 512;                        // values that are placed by counting
+constexpr int kLists = kWave;                         // lists of a sequence (beams * parts), one a lane
 
 struct Entry {
   float value;
@@ -30,8 +34,8 @@ struct Entry {
 };
 
 struct PartHead {
-  double sum;  // of exp(x - top); NaN where the part holds a NaN or +inf
-  float top;
+  double sum;   // of exp(x - shift); NaN where the part holds a NaN or +inf
+  float shift;  // a value of the part, at most 600 under its largest; -inf: the part holds nothing else
   int unused;
 };
 
@@ -47,7 +51,7 @@ struct BeamArgs {
   int64_t* out_tokens;
 };
 
-// exp(t), t <= 0, to 1e-11: t = k ln 2 + r, |r| <= ln 2 / 2, and the series of exp(r) up to r^9.
+// exp(t), t <= 600, to 1e-11 of it: t = k ln 2 + r, |r| <= ln 2 / 2, and the series of exp(r) up to r^9.
 __device__ __forceinline__ double exp64(double t) {
   t = fmax(t, -800.0);
   const double k = rint(t * 1.4426950408889634);
@@ -70,6 +74,11 @@ __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, kWave);
   return v;
+}
+
+// exp(shift - top): what sums with one shift are worth with another
+__device__ __forceinline__ double scale_to(float shift, float top) {
+  return shift == top ? 1.0 : (shift == -INFINITY ? 0.0 : exp64(static_cast<double>(shift) - top));
 }
 
 // a comes before b
@@ -103,112 +112,144 @@ __device__ __forceinline__ void load_values(const BeamArgs& a, int64_t row, int 
 
 template <bool F32, bool ALIGNED>
 __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
-  __shared__ Entry lists[kBeamWaves][kMaxCount];
+  __shared__ Entry gathered[kMaxCount + kGathered];  // the largest of earlier steps, then this one's
+  __shared__ Entry best[kMaxCount];
+  __shared__ float column[kBeamWaves][kWave];
   __shared__ PartHead heads[kBeamWaves];
+  __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x - row * a.parts);
   const int begin = part * a.part_len, end = min(begin + a.part_len, a.vocab);
 
-  float lv = -INFINITY;  // the wave's list: entry `lane`, largest first
-  int li = 0x7FFFFFFF;
-  float last_v = -INFINITY, top = -INFINITY;
-  int last_i = 0x7FFFFFFF;  // entry count - 1
-  double sum = 0.0;         // of this lane's exp(x - top)
+  float shift = -INFINITY;  // (wave-uniform)
+  double sum = 0.0;         // of this lane's exp(x - shift)
   bool bad = false;
-  float x[kPer], next[kPer];
-  // a wave's values of a step are neighbours: 1024 of them
+  int held = 0;  // entries of `best`
+  // a wave's values of a chunk are neighbours: 1024 of them
   const int mine = begin + wave * (kWave * kPer) + 4 * lane;
-  load_values<F32, ALIGNED>(a, row, mine, end, x);
   for (int base = begin; base < end; base += kBeamStep) {
     const int from = mine + (base - begin);
-    if (base + kBeamStep < end) load_values<F32, ALIGNED>(a, row, from + kBeamStep, end, next);
-    float mx = -INFINITY;
+    float x[kChunks][kPer], mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      bad = bad || !(x[e] < INFINITY);
-      x[e] = x[e] < INFINITY ? x[e] : -INFINITY;
-      mx = fmaxf(mx, x[e]);
+    for (int c = 0; c < kChunks; ++c) {
+      if (base + c * kBeamChunk < end) {
+        load_values<F32, ALIGNED>(a, row, from + c * kBeamChunk, end, x[c]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[c][e] = -INFINITY;
+      }
     }
-    const float wave_top = wave_max(mx);
-    if (wave_top > top) {
-      sum *= top == -INFINITY ? 0.0 : exp64(static_cast<double>(top) - wave_top);
-      top = wave_top;
-    }
-    if (top > -INFINITY) {
+    if (tid == 0) found = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (base + c * kBeamChunk >= end) continue;
+      float top = x[c][0];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        const double w = exp64(static_cast<double>(x[e]) - top);
-        sum += x[e] == -INFINITY ? 0.0 : w;
+        bad = bad || !(x[c][e] < INFINITY);
+        top = fmaxf(top, x[c][e]);
+      }
+      mx = fmaxf(mx, top);
+      top = wave_max(top);
+      if (top > shift && (shift == -INFINITY || top - shift > 600.0f)) {
+        sum *= shift == -INFINITY ? 0.0 : exp64(static_cast<double>(shift) - top);
+        shift = top;
+      }
+      if (shift > -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) sum += exp64(static_cast<double>(x[c][e]) - shift);
       }
     }
-    // what a value has to reach to be among the `count` largest of this step
-    float reach = last_v;
-    if (base == begin) {
-      int rank = 0;
+    column[wave][lane] = mx;
+    __syncthreads();
+    // what a value has to reach: the count-th largest of the columns' maxima
 #pragma unroll
-      for (int j = 0; j < kWave; ++j) {
-        const float other = row_lane(mx, j);
-        rank += other > mx || (other == mx && j < lane) ? 1 : 0;
-      }
-      const unsigned long long at = __builtin_amdgcn_ballot_w64(rank == a.count - 1);
-      reach = row_lane(mx, __builtin_ctzll(at));
-    }
+    for (int w = 0; w < kBeamWaves; ++w) mx = fmaxf(mx, column[w][lane]);
+    int above = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int index = from + (e >> 2) * 4 * kWave + (e & 3);
-      unsigned long long in = __builtin_amdgcn_ballot_w64(x[e] >= reach && index < end && before(x[e], index, last_v, last_i));
-      while (in != 0ull) {
-        const int l = __builtin_ctzll(in);
-        in &= in - 1;
-        const float v = row_lane(x[e], l);
-        const int i = __builtin_amdgcn_readlane(index, l);
-        if (!before(v, i, last_v, last_i)) continue;
-        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(lv, li, v, i)));
-        const float uv = __shfl_up(lv, 1, kWave);
-        const int ui = __shfl_up(li, 1, kWave);
-        lv = lane < at ? lv : (lane == at ? v : uv);
-        li = lane < at ? li : (lane == at ? i : ui);
-        last_v = row_lane(lv, a.count - 1);
-        last_i = __builtin_amdgcn_readlane(li, a.count - 1);
+    for (int j = 0; j < kWave; ++j) above += row_lane(mx, j) > mx ? 1 : 0;
+    float reach = -wave_max(above < a.count ? -mx : -INFINITY);
+    if (held == a.count) reach = fmaxf(reach, best[a.count - 1].value);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (base + c * kBeamChunk >= end) continue;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int index = from + c * kBeamChunk + (e >> 2) * 4 * kWave + (e & 3);
+        const bool in = x[c][e] >= reach && index < end;
+        const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+        if (who != 0ull) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&found, __builtin_popcountll(who));
+          at = __builtin_amdgcn_readfirstlane(at) + __builtin_popcountll(who & ((1ull << lane) - 1));
+          if (in && at < kGathered) gathered[kMaxCount + at] = Entry{x[c][e], index};
+        }
       }
     }
+    if (tid < held) gathered[tid] = best[tid];
+    __syncthreads();
+    int fresh = found;
+    if (fresh > kGathered) {  // a sorted list a wave, entry `lane`, largest first
+      __syncthreads();        // (every wave has read `found`, and none writes to the list before)
+      float lv = -INFINITY, last_v = -INFINITY;
+      int li = 0x7FFFFFFF, last_i = 0x7FFFFFFF;  // last: entry count - 1
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = next[e];
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const int index = from + c * kBeamChunk + (e >> 2) * 4 * kWave + (e & 3);
+          const float v = x[c][e];
+          unsigned long long in = __builtin_amdgcn_ballot_w64(v >= reach && index < end && before(v, index, last_v, last_i));
+          while (in != 0ull) {
+            const int l = __builtin_ctzll(in);
+            in &= in - 1;
+            const float cv = row_lane(v, l);
+            const int ci = __builtin_amdgcn_readlane(index, l);
+            if (!before(cv, ci, last_v, last_i)) continue;
+            const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(lv, li, cv, ci)));
+            const float uv = __shfl_up(lv, 1, kWave);
+            const int ui = __shfl_up(li, 1, kWave);
+            lv = lane < at ? lv : (lane == at ? cv : uv);
+            li = lane < at ? li : (lane == at ? ci : ui);
+            last_v = row_lane(lv, a.count - 1);
+            last_i = __builtin_amdgcn_readlane(li, a.count - 1);
+          }
+        }
+      }
+      // (entries that no value took come last: their index is no value's)
+      gathered[kMaxCount + tid] = Entry{lv, li < 0x7FFFFFFF ? li : 0x7FFFFF00 + tid};
+      fresh = kBeamThreads;
+      __syncthreads();
+    }
+    // an entry's place is the number of entries before it
+    const int total = held + fresh;
+    for (int i = tid; i < total; i += kBeamThreads) {
+      const Entry one = gathered[i < held ? i : kMaxCount + i - held];
+      int place = 0;
+      for (int j = 0; j < held; ++j) place += before(gathered[j].value, gathered[j].index, one.value, one.index) ? 1 : 0;
+      for (int j = 0; j < fresh; ++j)
+        place += before(gathered[kMaxCount + j].value, gathered[kMaxCount + j].index, one.value, one.index) ? 1 : 0;
+      if (place < a.count) best[place] = one;
+    }
+    held = min(a.count, total);
+    __syncthreads();
   }
 
-  if (lane < a.count) lists[wave][lane] = Entry{lv, li};
+  const int64_t out = row * a.parts + part;
+  if (tid < held) a.lists[out * a.count + tid] = best[tid];
   sum = wave_sum64(sum);
   if (__builtin_amdgcn_ballot_w64(bad) != 0ull) sum = NAN;
-  if (lane == 0) heads[wave] = PartHead{sum, top, 0};
+  if (lane == 0) heads[wave] = PartHead{sum, shift, 0};
   __syncthreads();
-  // the waves' lists into one: an entry's place is the number of entries before it
-  const int64_t out = row * a.parts + part;
-  if (lane < a.count) {
-    int place = lane;
-    for (int w = 0; w < kBeamWaves; ++w) {
-      if (w == wave) continue;
-      for (int j = 0; j < a.count; ++j) {
-        const Entry other = lists[w][j];
-        place += before(other.value, other.index, lv, li) || (other.value == lv && other.index == li && w < wave) ? 1 : 0;
-      }
-    }
-    if (place < a.count) a.lists[out * a.count + place] = Entry{lv, li};
-  }
   if (tid == 0) {
-    float t = heads[0].top;
-    for (int w = 1; w < kBeamWaves; ++w) t = fmaxf(t, heads[w].top);
+    float t = heads[0].shift;
+    for (int w = 1; w < kBeamWaves; ++w) t = fmaxf(t, heads[w].shift);
     double s = 0.0;
-    for (int w = 0; w < kBeamWaves; ++w) {
-      const double f = heads[w].top == t ? 1.0 : (heads[w].top == -INFINITY ? 0.0 : exp64(static_cast<double>(heads[w].top) - t));
-      s += heads[w].sum * f;
-    }
+    for (int w = 0; w < kBeamWaves; ++w) s += heads[w].sum * scale_to(heads[w].shift, t);
     a.heads[out] = PartHead{s, t, 0};
   }
 }
-
-// log(s) in 64 bits of a sum 1 <= s <= vocab, or of parts of one
-__device__ __forceinline__ double log64(double s) { return log(s); }
 
 // order-preserving image of a double
 __device__ __forceinline__ unsigned long long image(double v) {
@@ -249,16 +290,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   // the beam's shift: score - logsumexp; -inf where it has no distribution or no finite score
   const int beam = lane / a.parts, part = lane - beam * a.parts;
   double shift = -INFINITY;
-  if (beam < a.beams) {
-    const PartHead* h = a.heads + first + beam * a.parts;
-    float top = h[0].top;
-    for (int p = 1; p < a.parts; ++p) top = fmaxf(top, h[p].top);
-    double s = 0.0;
-    for (int p = 0; p < a.parts; ++p)
-      s += h[p].sum * (h[p].top == top ? 1.0 : (h[p].top == -INFINITY ? 0.0 : exp64(static_cast<double>(h[p].top) - top)));
-    const float score = a.scores[seq * a.beams + beam];
-    if (top > -INFINITY && s == s && fabsf(score) < INFINITY) shift = static_cast<double>(score) - (top + log64(s));
-  }
+  const bool any = beam < a.beams;
+  const PartHead head = any ? a.heads[first + lane] : PartHead{0.0, -INFINITY, 0};
+  const float score = any ? a.scores[seq * a.beams + beam] : 0.0f;
+  float top = head.shift;
+  for (int p = 0; p < a.parts; ++p) top = fmaxf(top, __shfl(head.shift, beam * a.parts + p, kWave));
+  const double mine = head.sum * scale_to(head.shift, top);
+  double s = 0.0;
+  for (int p = 0; p < a.parts; ++p) s += __shfl(mine, beam * a.parts + p, kWave);
+  if (any && top > -INFINITY && s == s && fabsf(score) < INFINITY) shift = static_cast<double>(score) - (top + log(s));
   const bool dead = shift == -INFINITY;
   const int left = min(a.part_len, a.vocab - part * a.part_len);  // values of the part
   const int held = beam < a.beams ? (dead && part > 0 ? 0 : min(a.count, dead ? a.vocab : left)) : 0;
@@ -299,11 +339,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   }
 }
 
-// Parts of a row: enough workgroups for the chip while a part keeps a step's worth of values, and no more lists
-// a sequence than lanes.
+// Parts of a row: one step each, more where the rows are too few for the chip, and no more lists a sequence than
+// lanes (then a part takes several steps).
 int beam_parts(int64_t rows, int beams, int64_t vocab) {
-  const int64_t by_rows = (2048 + rows - 1) / rows;
-  const int64_t parts = std::min<int64_t>(std::min<int64_t>(by_rows, kLists / beams), (vocab + kBeamStep - 1) / kBeamStep);
+  const int64_t least = (vocab + kBeamStep - 1) / kBeamStep, fill = (1024 + rows - 1) / rows;
+  const int64_t parts = std::min<int64_t>(std::max(least, std::min<int64_t>(fill, (vocab + 1023) / 1024)), kLists / beams);
   return static_cast<int>(std::max<int64_t>(1, parts));
 }
 

@@ -28,6 +28,13 @@ constexpr int kStepRows = 16;            // its queries
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+// Arrays that a launch only reads, at wave-uniform indexes: as constant memory their loads are scalar ones, which
+// leave the vector loads in flight alone (read as ordinary memory, each page number waited for all of them).
+typedef const __attribute__((address_space(4))) int32_t* uniform_ints;
+__device__ __forceinline__ uniform_ints uniform(const int32_t* p) {
+  return reinterpret_cast<uniform_ints>(reinterpret_cast<uintptr_t>(p));
+}
+
 struct PagedArgs {
   const uint16_t* q;  // rows [n, heads * 128], q_row apart
   int64_t q_row;
@@ -54,26 +61,31 @@ __device__ __forceinline__ int2 rows_of(const PagedArgs& a, int s) {
   return make_int2(first, min(max(a.starts[s + 1], first), a.n) - first);
 }
 
+// The same of one sequence of the whole wave.
+__device__ __forceinline__ int2 rows_of_one(const PagedArgs& a, int s) {
+  if (a.starts == nullptr) return make_int2(s, 1);
+  const uniform_ints starts = uniform(a.starts);
+  const int first = min(max(starts[s], 0), a.n);
+  return make_int2(first, min(max(starts[s + 1], first), a.n) - first);
+}
+
 // One sequence's pages of one KV head.
 struct Pages {
-  const int32_t* table;
+  uniform_ints table;
   int width, pages, log2, last;  // last: its last key that a table entry can name
   int64_t page_elems, head_elems;
-  // Page of 16 keys from `key` (a multiple of 16) on, or -1 where the table names none.
-  __device__ __forceinline__ int page(int key) const {
-    const int i = key >> log2;
-    const int id = i < width ? table[i] : -1;
-    return static_cast<unsigned>(id) < static_cast<unsigned>(pages) ? id : -1;
-  }
-  // First element of these 16 keys; of page 0 where they have none.
+  // Page of the 16 keys from `key` (a multiple of 16, at most `last`) on, as the table has it.
+  __device__ __forceinline__ int page(int key) const { return table[key >> log2]; }
+  __device__ __forceinline__ bool exists(int id) const { return static_cast<unsigned>(id) < static_cast<unsigned>(pages); }
+  // First element of these 16 keys; of page 0 where they have no page.
   __device__ __forceinline__ int64_t at(int id, int key) const {
-    return max(id, 0) * page_elems + head_elems + static_cast<int64_t>(key & ((1 << log2) - 1)) * kDim;
+    return (exists(id) ? id : 0) * page_elems + head_elems + static_cast<int64_t>(key & ((1 << log2) - 1)) * kDim;
   }
 };
 
 __device__ __forceinline__ Pages pages_of(const PagedArgs& a, int s, int head, int len) {
   Pages p;
-  p.table = a.table + static_cast<int64_t>(s) * a.width;
+  p.table = uniform(a.table + static_cast<int64_t>(s) * a.width);
   p.width = a.width;
   p.pages = a.pages;
   p.log2 = a.page_log2;
@@ -95,8 +107,12 @@ __device__ __forceinline__ bool drop_nonfinite(u32x4_t& w) {
   return any;
 }
 // w * v where v is infinite or NaN, else 0
-__device__ __forceinline__ float nonfinite_part(float w, uint16_t v) {
-  return (v & 0x7F80u) == 0x7F80u ? w * bf16_to_f32(v) : 0.0f;
+__device__ __forceinline__ float nonfinite_part(float w, float v) { return fabsf(v) < INFINITY ? 0.0f : w * v; }
+__device__ __forceinline__ void add_nonfinite(float w, uint2 v, float& a, float& b, float& c, float& d) {
+  a += nonfinite_part(w, bf16lo_to_f32(v.x));
+  b += nonfinite_part(w, bf16hi_to_f32(v.x));
+  c += nonfinite_part(w, bf16lo_to_f32(v.y));
+  d += nonfinite_part(w, bf16hi_to_f32(v.y));
 }
 
 __device__ __forceinline__ uint2 pair4(const float* o, float inv) {
@@ -156,8 +172,8 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
   seq = __builtin_amdgcn_readfirstlane(seq);
   tile_of_seq = __builtin_amdgcn_readfirstlane(tile_of_seq);
 
-  const int2 rows = rows_of(a, seq);
-  const int len = max(a.lens[seq], 0);
+  const int2 rows = rows_of_one(a, seq);
+  const int len = max(uniform(a.lens)[seq], 0);
   const Pages pages = pages_of(a, seq, head, len);
   const int r = tile_of_seq * kChunkRows + wave * 32 + (lane & 31);
   const bool valid = r < rows.y * a.group;
@@ -251,7 +267,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
     const auto check = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (ids[i] < 0 && pos >= min(tile * kKeys + 16 * i, pages.last & ~15)) poison = NAN;
+        if (!pages.exists(ids[i]) && pos >= min(tile * kKeys + 16 * i, pages.last & ~15)) poison = NAN;
     };
     check(first);
     fetch(first);
@@ -353,8 +369,14 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
 #pragma unroll
               for (int d = 0; d < 4; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  o[d][i] += nonfinite_part(w, vp[32 * d + 8 * (i >> 2) + (i & 3)]);
+                for (int g = 0; g < 4; ++g) {
+                  const uint2 v = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * g);
+                  float e[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                  add_nonfinite(w, v, e[0], e[1], e[2], e[3]);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) o[d][4 * g + i] = e[i];
+                  __builtin_amdgcn_sched_barrier(0);  // (a piece at a time: this path must not set the kernel's registers)
+                }
             }
           }
         }
@@ -393,9 +415,21 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
 // The key ranges that a sequence of `steps` steps is divided into: at least one step for each wave of a range.
 __device__ __forceinline__ int step_ranges(int splits, int steps) { return max(1, min(splits, steps / kWaves)); }
 
+// read_v_tr (attn_common.h) of an address that is known to be one in LDS, so that fixed distances are offsets of the read
+typedef const __attribute__((address_space(3))) uint16_t* lds_rows;
+__device__ __forceinline__ lds_rows as_lds(const uint16_t* p) {
+  return reinterpret_cast<lds_rows>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+__device__ __forceinline__ bf16x4_t read_tr(lds_rows p) {
+  typedef __attribute__((address_space(3))) bf16x4_t lds_t;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_t*)p);
+}
+
 template <bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t lds[kWaves][kStepKeys * kVRow];
+  // a wave's V rows of 256 bytes; 32-byte piece d of row r lies at d ^ (r % 8), so that the 16 rows of a transposed
+  // read cover all banks without padding 
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kWaves][kStepKeys * kDim];
   __shared__ float2 wave_ml[kWaves][kStepRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
   const int head = static_cast<int>(blockIdx.x) % a.kv;
@@ -410,8 +444,8 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
         *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * i) = make_uint4(0, 0, 0, 0);
     return;
   }
-  const int2 rows = rows_of(a, seq);
-  const int len = max(a.lens[seq], 0);
+  const int2 rows = rows_of_one(a, seq);
+  const int len = max(uniform(a.lens)[seq], 0);
   const Pages pages = pages_of(a, seq, head, len);
 
   for (int base = 0; base < rows.y * a.group; base += kStepRows) {
@@ -451,7 +485,7 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const int key = min(step * kStepKeys + 16 * b, pages.last & ~15);
-        if (ids[b] < 0 && pos >= key) poison = NAN;
+        if (!pages.exists(ids[b]) && pos >= key) poison = NAN;
         const int64_t at = pages.at(ids[b], key);
         const uint16_t* kp = a.k + at + c * kDim + 8 * g;
         const uint16_t* vp = a.v + at + g * kDim + 8 * c;
@@ -463,7 +497,8 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
       }
     };
     uint16_t* const vl = lds[wave];
-    const uint16_t* const vt = vl + (4 * g + (c >> 2)) * kVRow + 4 * (c & 3);
+    const int turn = (4 * g + (c >> 2)) & 7;  // of the rows that this lane reads, 4 g + c / 4 and 16 further
+    const lds_rows vt = as_lds(vl + (4 * g + (c >> 2)) * kDim + 4 * (c & 3));
     const int begin = __builtin_amdgcn_readfirstlane(first + wave);
     if (begin < steps) {
       look_up(begin);
@@ -478,17 +513,25 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
 #pragma unroll
         for (int st = 0; st < 4; ++st) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[b][st], q[st], s[b], 0, 0, 0);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + g;
+        *reinterpret_cast<u32x4_t*>(&vl[r * kDim + 8 * (c ^ (2 * (r & 7)))]) = vr[i];
+      }
       uint32_t odd = 0;  // keys with infinite or NaN values that some row does not see
       if (step * kStepKeys + kStepKeys - 1 > low) {
+        // (rows are mended where they lie: mended before they are written, they would all be copied first)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int key = step * kStepKeys + 4 * i + g;
+          const int r = 4 * i + g, key = step * kStepKeys + r;
+          u32x4_t v = vr[i];
           bool any = false;
           if (key > pages.last) {
-            vr[i] = u32x4_t{0, 0, 0, 0};
+            v = u32x4_t{0, 0, 0, 0};
           } else if (key > low) {
-            any = drop_nonfinite(vr[i]);
+            any = drop_nonfinite(v);
           }
+          if (any || key > pages.last) *reinterpret_cast<u32x4_t*>(&vl[r * kDim + 8 * (c ^ (2 * (r & 7)))]) = v;
           const unsigned long long lanes = __builtin_amdgcn_ballot_w64(any);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -500,12 +543,11 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
           for (int i = 0; i < 4; ++i)
             if (step * kStepKeys + 16 * b + 4 * g + i > pos) s[b][i] = -INFINITY;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4_t*>(&vl[(4 * i + g) * kVRow + 8 * c]) = vr[i];
       if (step + kWaves < steps) {
         fetch(step + kWaves);
         look_up(min(step + 2 * kWaves, steps - 1));
       }
+      __builtin_amdgcn_sched_barrier(0);  // the loads leave before the softmax, however many registers that takes
       float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
@@ -546,7 +588,8 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        const bf16x4_t lo = read_v_tr(vt + 16 * d), hi = read_v_tr(vt + 16 * kVRow + 16 * d);
+        const lds_rows piece = vt + 16 * (d ^ turn);
+        const bf16x4_t lo = read_tr(piece), hi = read_tr(piece + 16 * kDim);
         const bf16x8_t va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p, o[d], 0, 0, 0);
       }
@@ -562,9 +605,13 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
         if (key <= pos) {
           const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * g;
 #pragma unroll
-          for (int d = 0; d < 8; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[d][i] += nonfinite_part(pw, vp[16 * d + i]);
+          for (int d = 0; d < 8; ++d) {  // (a piece at a time: this path must not set the kernel's registers)
+            const uint2 v = *reinterpret_cast<const uint2*>(vp + 16 * d);
+            float e[4] = {o[d][0], o[d][1], o[d][2], o[d][3]};
+            add_nonfinite(pw, v, e[0], e[1], e[2], e[3]);
+            o[d] = f32x4_t{e[0], e[1], e[2], e[3]};
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
       }
     }
@@ -577,7 +624,7 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
     if (g == 0) wave_ml[wave][c] = make_float2(seen || l != l ? raw : kUnseen, l);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     float* const wo = reinterpret_cast<float*>(vl);
-    static_assert(kStepRows * kDim * sizeof(float) <= kStepKeys * kVRow * sizeof(uint16_t), "a wave's outputs fit its V rows");
+    static_assert(kStepRows * kDim * sizeof(float) <= kStepKeys * kDim * sizeof(uint16_t), "a wave's outputs fit its V rows");
 #pragma unroll
     for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&wo[c * kDim + 16 * d + 4 * g]) = o[d];
     lds_barrier();
@@ -618,33 +665,38 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
   }
 }
 
-// Joins the key ranges: 32 lanes per (row, head), 4 channels each.
-__global__ __launch_bounds__(256) void join_kernel(PagedArgs a) {
+// Joins the key ranges: a wave per (row, head), 2 channels a lane.  Range s's maximum and sum come to lane s in
+// one load, and the ranges' rows are loaded eight at a time, so that a join costs two or three memory latencies
+// (one load after another: 13 us for one row of 16 ranges).
+__global__ __launch_bounds__(kThreads) void join_kernel(PagedArgs a) {
   const int64_t rows = (a.starts ? min(max(a.starts[a.seqs], 0), a.n) : a.n) * static_cast<int64_t>(a.heads);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= rows) return;
   const int64_t all = static_cast<int64_t>(a.n) * a.heads;
-  const int c = (threadIdx.x & 31) * 4;
-  float top = kUnseen;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[2 * (s * all + row)]);
-  const float st = scaled_max(top, a.scale);
-  float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * all + row));
-    if (ml.x == kUnseen) {
-      l += ml.y != ml.y ? ml.y : 0.0f;
-      continue;
+  const int lane = threadIdx.x & 63;
+  const bool mine = lane < a.splits;
+  const float2 ml = mine ? *reinterpret_cast<const float2*>(a.part_ml + 2 * (lane * all + row)) : make_float2(kUnseen, 0.0f);
+  const float* const part = a.part_o + row * kDim + 2 * lane;
+  const float top = wave_max(ml.x);
+  const bool seen = ml.x != kUnseen;
+  const float w = seen ? exp2_between(ml.x, top, scaled_max(ml.x, a.scale), scaled_max(top, a.scale), a.scale) : 0.0f;
+  const float l = wave_sum(seen ? w * ml.y : (ml.y != ml.y ? ml.y : 0.0f));
+  const unsigned long long parts = __builtin_amdgcn_ballot_w64(seen);
+  float o0 = 0.0f, o1 = 0.0f;
+  for (int base = 0; base < a.splits; base += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = (parts >> (base + i)) & 1 ? *reinterpret_cast<const float2*>(part + (base + i) * all * kDim) : make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = row_lane(w, base + i);
+      o0 = fmaf(f, v[i].x, o0);
+      o1 = fmaf(f, v[i].y, o1);
     }
-    const float4 p = *reinterpret_cast<const float4*>(a.part_o + (s * all + row) * kDim + c);
-    const float w = exp2_between(ml.x, top, scaled_max(ml.x, a.scale), st, a.scale);
-    l = fmaf(w, ml.y, l);
-    o[0] = fmaf(w, p.x, o[0]);
-    o[1] = fmaf(w, p.y, o[1]);
-    o[2] = fmaf(w, p.z, o[2]);
-    o[3] = fmaf(w, p.w, o[3]);
   }
   const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
-  *reinterpret_cast<uint2*>(a.o + row * kDim + c) = pair4(o, inv);
+  *reinterpret_cast<uint32_t*>(a.o + row * kDim + 2 * lane) = attn_bf16_pair(o0 * inv, o1 * inv);
 }
 
 // Sequences of few rows take step_kernel: up to 16 queries of a KV head are one pass over its keys there.
@@ -655,7 +707,7 @@ int paged_splits(int seqs, int n, int kv, int group, int max_q, int max_kv) {
   const bool step = few_rows(max_q, group);
   const int64_t groups = step ? static_cast<int64_t>(seqs) * kv
                               : ((static_cast<int64_t>(n) * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs / 2 : 0)) * kv;
-  const int64_t want = ((step ? 1024 : 640) + groups - 1) / std::max<int64_t>(groups, 1);
+  const int64_t want = ((step ? 1536 : 640) + groups - 1) / std::max<int64_t>(groups, 1);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), max_kv / (step ? 128 : 448))));
 }
 
@@ -718,7 +770,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
     return FL_OK;
   }
   const int64_t all = static_cast<int64_t>(rows) * heads;
-  FL_REQUIRE((all + 7) / 8 <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
+  FL_REQUIRE((all + kWaves - 1) / kWaves <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + a.splits * all * kDim;
   if (step)
@@ -726,7 +778,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   else
     hipLaunchKernelGGL(chunk_kernel<true>, grid, block, 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention");
-  hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((all + 7) / 8)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((all + kWaves - 1) / kWaves)), block, 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention(join)");
   return FL_OK;
 }
