@@ -31,6 +31,7 @@
 // of the three: 777-816, 174-185, 132-137 us.
 #include <algorithm>
 
+#include "lds_load.h"
 #include "mx_common.h"
 
 namespace fl {
@@ -111,36 +112,10 @@ __device__ __forceinline__ void store8(const MmArgs& a, int64_t m, int n, int g,
 }
 
 // ---------------------------------------------------------------------------------
-// A raw buffer over `bytes` bytes at p (wave-uniform): what a load finds past the end is zero.  Word 3
-// is the gfx9 raw-buffer format.
-__device__ __forceinline__ mx_i32x4_t raw_buffer(const void* p, int64_t bytes) {
-  const uint64_t u = reinterpret_cast<uintptr_t>(p);
-  return mx_i32x4_t{__builtin_amdgcn_readfirstlane(static_cast<int>(u)), __builtin_amdgcn_readfirstlane(static_cast<int>(u >> 32)),
-                    __builtin_amdgcn_readfirstlane(static_cast<int>(min(bytes, static_cast<int64_t>(0x7FFFFFFF)))), 0x00020000};
-}
-
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
-
 // Byte g of each of four dwords (pick: g, 4 + g), the first lowest.
 __device__ __forceinline__ uint32_t lane_scales(const uint4& q, uint32_t pick) {
   return __builtin_amdgcn_perm(__builtin_amdgcn_perm(q.w, q.z, pick), __builtin_amdgcn_perm(q.y, q.x, pick), 0x05040100u);
 }
-
-// Memory to LDS: lane l's 16 (or 4) bytes of buffer r at voff + soff go to lds + 16 (4) l.  The compiler counts
-// no LDS write for these, so the kernel waits for them itself (vmcnt, ahead of the step's barrier).  m0 is
-// on the clobber list for what else a compiler sets it for; its warning says that no one saves it here.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-template <int BYTES>
-__device__ __forceinline__ void to_lds(mx_i32x4_t r, uint32_t voff, uint32_t soff, uint32_t lds) {
-  if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "m0", "memory");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds), "v"(voff), "s"(r), "s"(soff)
-                 : "m0", "memory");
-}
-#pragma clang diagnostic pop
 
 // A piece of a W row (four of 16 bytes) lies at its number xor this, one of an X row (eight) at its number xor
 // (row / 2) % 8.  A 16-byte LDS read serves 16 lanes at a time, of rows 0-3 and 12-15 of one k group and 4-11

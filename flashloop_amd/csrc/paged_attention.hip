@@ -14,15 +14,20 @@
 // replaced, V rows past a sequence's end are zeroed, and where some row of a tile does not see a key, the
 // key's infinite and NaN values are zeroed too and added for the rows that see it afterwards.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "attn_common.h"
+#include "lds_load.h"
 
 namespace fl {
 namespace {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kChunkRows = 32 * kWaves;  // queries of a workgroup of chunk_kernel
+constexpr int kChunkWaves = 8;           // waves of a workgroup of chunk_kernel
+constexpr int kChunkThreads = kChunkWaves * kWave;
+constexpr int kChunkRows = 32 * kChunkWaves;  // its queries
 constexpr int kStepKeys = 32;            // keys of a wave's step in step_kernel
 constexpr int kStepRows = 16;            // its queries
 
@@ -119,12 +124,35 @@ __device__ __forceinline__ uint2 pair4(const float* o, float inv) {
   return make_uint2(attn_bf16_pair(o[0] * inv, o[1] * inv), attn_bf16_pair(o[2] * inv, o[3] * inv));
 }
 
+// read_v_tr (attn_common.h) of an address that is known to be one in LDS, so that fixed distances are offsets of the read
+typedef const __attribute__((address_space(3))) uint16_t* lds_rows;
+__device__ __forceinline__ lds_rows as_lds(const uint16_t* p) {
+  return reinterpret_cast<lds_rows>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+__device__ __forceinline__ bf16x4_t read_tr(lds_rows p) {
+  typedef __attribute__((address_space(3))) bf16x4_t lds_t;
+  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_t*)p);
+}
+
+// The chunk kernel's LDS: four tiles each of K and V, rows of 256 bytes as 16 pieces of 16.  Piece p of K row r lies at
+// p ^ (r % 16): the 32 rows of an operand read meet all banks.  Piece p of V row r at p ^ 4 (r % 4): so do the four rows of a
+// transposed read's 16 lanes.
+constexpr int kRing = 4;
+constexpr int kTileBytes = kKeys * kDim * 2;
+
+// f(0), f(1), .. with constant arguments
+template <int... I, class F>
+__device__ __forceinline__ void slots(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 template <bool SPLIT>
-__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
-  __shared__ AttnLds L;
-  __shared__ int wave_pos[2][kWaves];
+__global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds_all[2 * kRing * kTileBytes];
+  __shared__ int wave_pos[2][kChunkWaves];
   __shared__ unsigned long long odd_keys[4];  // by tile % 4: keys of a tile with infinite or NaN values
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  __shared__ int no_page;                     // the first key without a page
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int head = static_cast<int>(blockIdx.x) % a.kv;
   const int rest = static_cast<int>(blockIdx.x) / a.kv;
   const int split = SPLIT ? rest % a.splits : 0;
@@ -145,7 +173,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
     const int behind = min(max(a.starts[a.seqs], 0), a.n);
     const int spare = static_cast<int>(gridDim.x) / a.kv / a.splits - total, width = a.group * kDim / 8;
     for (int64_t row = behind + index - total; row < a.n; row += spare)
-      for (int c = tid; c < width; c += kThreads)
+      for (int c = tid; c < width; c += kChunkThreads)
         *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * c) = make_uint4(0, 0, 0, 0);
     return;
   }
@@ -175,222 +203,358 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
   const int2 rows = rows_of_one(a, seq);
   const int len = max(uniform(a.lens)[seq], 0);
   const Pages pages = pages_of(a, seq, head, len);
+  // this lane's query: column lane % 32 of the wave's
   const int r = tile_of_seq * kChunkRows + wave * 32 + (lane & 31);
   const bool valid = r < rows.y * a.group;
   const int rc = valid ? r : rows.y * a.group - 1;
   const int token = rc / a.group, out_head = head * a.group + rc - token * a.group;
-  const int64_t row = rows.x + token;
   const int pos = len - rows.y + token;
+  const int64_t out_at = (static_cast<int64_t>(rows.x + token) * a.heads + out_head) * kDim;  // elements of o
+  bf16x8_t q[8];
+  {
+    const uint16_t* qp = a.q + (rows.x + token) * a.q_row + out_head * kDim + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
+  }
   int wmin = pos, wmax = pos;
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) {
     wmin = min(wmin, __shfl_xor(wmin, off, kWave));
     wmax = max(wmax, __shfl_xor(wmax, off, kWave));
   }
+  wmin = __builtin_amdgcn_readfirstlane(wmin);
+  wmax = __builtin_amdgcn_readfirstlane(wmax);
   if (lane == 0) {
     wave_pos[0][wave] = wmin;
     wave_pos[1][wave] = wmax;
   }
   if (tid < 4) odd_keys[tid] = 0ull;
-
-  bf16x8_t q[8];
-  {
-    const uint16_t* qp = a.q + row * a.q_row + out_head * kDim + 8 * h;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
-  }
+  if (tid == 0) no_page = 0x7FFFFFFF;
   lds_barrier();
   int low = wave_pos[0][0], end = wave_pos[1][0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
+  for (int w = 1; w < kChunkWaves; ++w) {
     low = min(low, wave_pos[0][w]);
     end = max(end, wave_pos[1][w]);
   }
   low = __builtin_amdgcn_readfirstlane(low);
-  // a sequence longer than its table row: its rows are NaN
-  float poison = len - 1 > pages.last ? NAN : 0.0f;
-  int tiles = __builtin_amdgcn_readfirstlane(min(end, pages.last)) / kKeys + 1;
-  if (min(end, pages.last) < 0) tiles = 0;
-  int first = 0;
+  end = __builtin_amdgcn_readfirstlane(min(end, pages.last));
+  int tiles = end >= 0 ? end / kKeys + 1 : 0, first = 0;
   if (SPLIT) {
     first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
     tiles = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
   }
+  const int mine = min(tiles, (wmax >> 6) + 1);  // tiles that some query of the wave sees (none: at most `first`)
 
-  // this thread's 16-byte chunks of a tile: rows tid / 16 of the tile's four blocks of 16 keys
-  const int lrow = tid >> 4, lcol = (tid & 15) * 8;
-  u32x4_t kr[4], vr[4];
-  int ids[4];
-  const auto look_up = [&](int tile) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ids[i] = pages.page(min(tile * kKeys + 16 * i, pages.last & ~15));
-  };
-  const auto fetch = [&](int tile) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t at = pages.at(ids[i], min(tile * kKeys + 16 * i, pages.last & ~15)) + lrow * kDim + lcol;
-      kr[i] = *reinterpret_cast<const u32x4_t*>(a.k + at);
-      vr[i] = *reinterpret_cast<const u32x4_t*>(a.v + at);
-    }
-  };
-  const auto stage = [&](int tile) __attribute__((always_inline)) {
-    const int buf = (tile - first) & 1;
-    if (tile * kKeys + kKeys - 1 > low) {  // some row does not see some key of the tile
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 16 * i + lrow;
-        if (tile * kKeys + key > pages.last) {
-          vr[i] = u32x4_t{0, 0, 0, 0};
-        } else if (drop_nonfinite(vr[i])) {
-          atomicOr(&odd_keys[tile & 3], 1ull << key);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *reinterpret_cast<u32x4_t*>(&L.k[buf][(lrow + 16 * i) * kKRow + lcol]) = kr[i];
-      *reinterpret_cast<u32x4_t*>(&L.v[buf][(lrow + 16 * i) * kVRow + lcol]) = vr[i];
-    }
-  };
   f32x16_t o[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-  // running maximum (of q.k, and scaled to base 2) and this lane's part of the sum
-  float raw = kNone, m = scaled_max(kNone, a.scale), l = 0.0f;
-  bool far = false;  // (wave-uniform) some query's maximum lies past kFar
+  // the reference of the running softmax (a score, and it scaled to base 2), this lane's parts of the sum
+  float raw = kNone, off = -scaled_max(kNone, a.scale), sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  // Scores may pass the reference by 2^8 before it moves: the probabilities are as exact in bf16 as under 1, and most tiles
+  // then leave the outputs alone.
+  const float slack = 8.0f / a.scale;
+  bool far = false;  // (wave-uniform) some query's reference lies past kFar
 
   if (first < tiles) {
-    look_up(first);
-    // a block of keys without a page: NaN for the rows that see it
-    const auto check = [&](int tile) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): q has arrived (or every use of it would wait for the transfers, too)
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds_all));
+    constexpr uint32_t kV = kRing * kTileBytes;  // V's tiles lie behind K's
+
+    // Transfers: a wave brings the 8 keys 8 w .. of a tile, which share a page: twice four rows.  The page numbers of 64
+    // tiles lie in the lanes of one register (a scalar load among a tile's LDS reads would make their waits wait for all).
+    uint32_t kv[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!pages.exists(ids[i]) && pos >= min(tile * kKeys + 16 * i, pages.last & ~15)) poison = NAN;
+    for (int i = 0; i < 2; ++i) kv[i] = 1024 * i + 256 * (lane >> 4) + 16 * ((lane & 15) ^ (8 * (wave & 1) + 4 * i + (lane >> 4)));
+    const uint32_t vv = 256 * (lane >> 4) + 16 * ((lane & 15) ^ (4 * (lane >> 4)));
+    const auto block_key = [&](int tile) __attribute__((always_inline)) {
+      return min(min(tile, tiles - 1) * kKeys + 8 * (wave & ~1), pages.last & ~15);
     };
-    check(first);
-    fetch(first);
-    stage(first);
-    look_up(min(first + 1, tiles - 1));
-    lds_barrier();
-    for (int tile = first; tile < tiles; ++tile) {
-      const int buf = (tile - first) & 1, next = min(tile + 1, tiles - 1);
-      if (tid == 0) odd_keys[(tile + 2) & 3] = 0ull;
-      check(next);
-      fetch(next);
-      look_up(min(tile + 2, tiles - 1));
-      if (tile * kKeys <= wmax) {  // (wave-uniform) some query of the wave sees this tile
-        f32x16_t s[2];
+    int ids = 0, ids_from = 0, lost = 0x7FFFFFFF;  // lost: the first key of this wave's without a page
+    const auto look_up = [&](int tile) __attribute__((always_inline)) {
+      ids_from = tile;
+      ids = *(a.table + static_cast<int64_t>(seq) * a.width + (block_key(tile + lane) >> pages.log2));
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): here, and not at every use
+    };
+    const auto place = [&](int tile) __attribute__((always_inline)) {  // of the wave's keys of a tile, in elements of the pool
+      const int id = __builtin_amdgcn_readlane(ids, tile - ids_from), key = block_key(tile);
+      lost = pages.exists(id) ? lost : min(lost, key);
+      return pages.at(id, key) + 8 * (wave & 1) * kDim;
+    };
+    const auto ring = [&](int tile) __attribute__((always_inline)) { return static_cast<uint32_t>((tile - first) % kRing) * kTileBytes; };
+    const auto bring_k = [&](int tile, int64_t at) __attribute__((always_inline)) {
+      const lds_buffer_t r = raw_buffer(a.k + at, 8 * kDim * 2);
+      const uint32_t to = lds0 + ring(tile) + 2048u * wave;
+      to_lds<16>(r, kv[0], 0, to);
+      to_lds<16>(r, kv[1], 0, to + 1024u);
+    };
+    const auto bring_v = [&](int tile, int64_t at) __attribute__((always_inline)) {
+      const lds_buffer_t r = raw_buffer(a.v + at, 8 * kDim * 2);
+      const uint32_t to = lds0 + kV + ring(tile) + 2048u * wave;
+      to_lds<16>(r, vv, 0, to);
+      to_lds<16>(r, vv, 1024u, to + 1024u);
+    };
+    // This wave's V rows of a tile, arrived: zeros past the sequence's end, and in the place of infinite and NaN values that
+    // some row does not see
+    const auto mend = [&](int tile) __attribute__((always_inline)) {
+      if (tile >= tiles || tile * kKeys + kKeys - 1 <= low) return;
+      uint32_t bits = 0;
+      uint8_t* const at = lds_all + kV + ring(tile) + 2048 * wave + 16 * lane;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+      for (int i = 0; i < 2; ++i) {
+        const int key = tile * kKeys + 8 * wave + 4 * i + (lane >> 4);
+        u32x4_t v = *reinterpret_cast<u32x4_t*>(at + 1024 * i);
+        bool any = false;
+        if (key > pages.last)
+          v = u32x4_t{0, 0, 0, 0};
+        else if (key > low)
+          any = drop_nonfinite(v);
+        if (any || key > pages.last) *reinterpret_cast<u32x4_t*>(at + 1024 * i) = v;
+        const unsigned long long lanes = __builtin_amdgcn_ballot_w64(any);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-          const uint16_t* kl = &L.k[buf][(32 * b + (lane & 31)) * kKRow + 8 * h];
+        for (int j = 0; j < 4; ++j)
+          if ((lanes >> (16 * j)) & 0xFFFFull) bits |= 1u << (4 * i + j);
+      }
+      if (bits != 0 && lane == 0) atomicOr(&odd_keys[tile & 3], static_cast<unsigned long long>(bits) << (8 * wave));
+    };
+
+    // Operands: K fragment i is rows lane % 32 of half i % 2 of the tile, channels 16 (i / 2) + 8 h ..; V fragment j rows
+    // 16 (j / 4) + 4 h .. (+ 8), channels 32 (j % 4) + ..
+    typedef const __attribute__((address_space(3))) uint8_t* lds_at;
+    uint32_t kx[8], vx[4];
+    const int i16 = lane & 15;
 #pragma unroll
-          for (int st = 0; st < 8; ++st)
-            s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8_t*>(kl + 16 * st), q[st], s[b], 0, 0, 0);
-        }
-        if (tile * kKeys + kKeys - 1 > wmin) {  // keys past a query's position
-          const int lim = pos - tile * kKeys - 4 * h;
+    for (int st = 0; st < 8; ++st) kx[st] = lds0 + 256 * (lane & 31) + (16 * (h ^ i16) ^ 32 * st);
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+    for (int d = 0; d < 4; ++d) vx[d] = lds0 + kV + 256 * (4 * h + (i16 >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3) + (64 * (i16 >> 2) ^ 64 * d);
+    const auto k_part = [&](uint32_t of, int i) __attribute__((always_inline)) {
+      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>((lds_at)(kx[i >> 1] + of) + 8192 * (i & 1));
+    };
+    const auto v_part = [&](uint32_t of, int j) __attribute__((always_inline)) {
+      const lds_at at = (lds_at)(vx[j & 3] + of) + 4096 * (j >> 2);
+      const bf16x4_t lo = read_tr((lds_rows)at), hi = read_tr((lds_rows)(at + 2048));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    const auto scores_part = [&](int i, bf16x8_t k, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+      f32x16_t zero;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (32 * b + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
-        }
-        float mx = s[0][0];
+      for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+      s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
+    };
+    // probabilities 2 k and 2 k + 1 of the tile's 32 a lane: words of the second product's operand
+    u32x4_t p[4];
+    const auto pair = [&](int k, const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+      const int t = k >> 2, e = 8 * (t & 1) + 2 * (k & 3);
+      const float p0 = fast_exp2(fmaf(s[t >> 1][e], a.scale, off)), p1 = fast_exp2(fmaf(s[t >> 1][e + 1], a.scale, off));
+      p[t][k & 3] = attn_bf16_pair(p0, p1);
+      sum[k & 3] = add_pair(p[t][k & 3], sum[k & 3]);
+    };
+    const auto outputs_part = [&](int j, bf16x8_t v) __attribute__((always_inline)) {
+      o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8_t, p[j >> 2]), o[j & 3], 0, 0, 0);
+    };
+    const auto hide = [&](int tile, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+      if (tile * kKeys + kKeys - 1 > wmin) {  // keys past a query's position
+        const int lim = pos - tile * kKeys - 4 * h;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
-        mx = fmaxf(mx, swap_half(mx));
-        if (__builtin_amdgcn_ballot_w64(mx > raw) != 0ull) {
-          const float top = fmaxf(raw, mx), mn = scaled_max(top, a.scale);
-          const float alpha = exp2_between(raw, top, m, mn, a.scale);
-          raw = top;
-          m = mn;
-          l *= alpha;
-          far = __builtin_amdgcn_ballot_w64(fabsf(m) > kFar && raw > kNone) != 0ull;
+          for (int i = 0; i < 16; ++i)
+            if (32 * b + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
+      }
+    };
+    const auto largest = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+      float m = s[0][0];
 #pragma unroll
-          for (int d = 0; d < 4; ++d)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-        }
-        float off = -m;
-        if (far) {
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
+      return m;
+    };
+    // the reference moves where a score passes it too far
+    const auto move_to = [&](float m, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+      m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+      if (__builtin_amdgcn_ballot_w64(m > raw + slack) != 0ull) {
+        const float top = fmaxf(raw, m), mn = scaled_max(top, a.scale);
+        const float alpha = exp2_between(raw, top, scaled_max(raw, a.scale), mn, a.scale);
+        raw = top;
+        off = -mn;
+        far = __builtin_amdgcn_ballot_w64(fabsf(mn) > kFar && top > kNone) != 0ull;
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
+        for (int i = 0; i < 4; ++i) sum[i] *= alpha;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] -= raw;
-          off = 0.0f;
-        }
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        bf16x8_t p[4];
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          u32x4_t w;
+          for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+      }
+      if (far) {  // (differences before the scale)
+        off = 0.0f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = 8 * (t & 1) + 2 * i;
-            const float p0 = fast_exp2(fmaf(s[t >> 1][e], a.scale, off));
-            const float p1 = fast_exp2(fmaf(s[t >> 1][e + 1], a.scale, off));
-            w[i] = attn_bf16_pair(p0, p1);
-            sum[i] = add_pair(w[i], sum[i]);
-          }
-          p[t] = __builtin_bit_cast(bf16x8_t, w);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        const int i16 = lane & 15;
-        const uint16_t* vl = &L.v[buf][(4 * h + (i16 >> 2)) * kVRow + ((lane >> 4) & 1) * 16 + 4 * (i16 & 3)];
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] -= raw;
+      }
+    };
+    const auto add_odd = [&](int tile) __attribute__((always_inline)) {
+      if (tile * kKeys + kKeys - 1 <= low) return;
+      for (unsigned long long odd = odd_keys[tile & 3]; odd != 0ull; odd &= odd - 1) {
+        // key j lies in result register 4 (j / 8) + j % 4 of lane half j / 4 % 2
+        const int j = __builtin_amdgcn_readfirstlane(__builtin_ctzll(odd)), e = 4 * (j >> 3) + (j & 3);
+        const int key = tile * kKeys + j;
+        const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * h;
+        float w = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const bf16x4_t lo = read_v_tr(vl + (16 * t) * kVRow + 32 * d);
-            const bf16x4_t hi = read_v_tr(vl + (16 * t + 8) * kVRow + 32 * d);
-            const bf16x8_t va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, p[t], o[d], 0, 0, 0);
-          }
-        if (tile * kKeys + kKeys - 1 > low) {
-          for (unsigned long long odd = odd_keys[tile & 3]; odd != 0ull; odd &= odd - 1) {
-            // key j lies in result register 4 (j / 8) + j % 4 of lane half j / 4 % 2
-            const int j = __builtin_amdgcn_readfirstlane(__builtin_ctzll(odd)), e = 4 * (j >> 3) + (j & 3);
-            float w = 0.0f;
+          for (int i = 0; i < 8; ++i)
+            if (8 * t + i == e) w = static_cast<float>(__builtin_bit_cast(bf16x8_t, p[t])[i]);
+        w = __shfl(w, (lane & 31) + 32 * ((j >> 2) & 1), kWave);
+        if (key <= pos) {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+          for (int d = 0; d < 4; ++d)
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (8 * t + i == e) w = static_cast<float>(p[t][i]);
-            w = __shfl(w, (lane & 31) + 32 * ((j >> 2) & 1), kWave);
-            const int key = tile * kKeys + j;
-            if (key <= pos) {
-              const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * h;
+            for (int g = 0; g < 4; ++g) {
+              const uint2 v = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * g);
+              float x[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+              add_nonfinite(w, v, x[0], x[1], x[2], x[3]);
 #pragma unroll
-              for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  const uint2 v = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * g);
-                  float e[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-                  add_nonfinite(w, v, e[0], e[1], e[2], e[3]);
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) o[d][4 * g + i] = e[i];
-                  __builtin_amdgcn_sched_barrier(0);  // (a piece at a time: this path must not set the kernel's registers)
-                }
+              for (int i = 0; i < 4; ++i) o[d][4 * g + i] = x[i];
+              __builtin_amdgcn_sched_barrier(0);  // (a piece at a time: this path must not set the kernel's registers)
             }
-          }
         }
       }
-      if (tile + 1 < tiles) stage(next);  // (its buffer was read by every wave before the previous tile's barrier)
-      lds_barrier();
+    };
+
+    look_up(first);
+    int64_t at_v = 0;  // place of the tile whose V goes next
+    {
+      int64_t at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[i] = place(first + i);
+      bring_k(first, at[0]);
+      bring_v(first, at[0]);
+      bring_k(first + 1, at[1]);
+      bring_k(first + 2, at[2]);
+      bring_v(first + 1, at[1]);
+      bring_k(first + 3, at[3]);
+      bring_v(first + 2, at[2]);
+      at_v = at[3];
     }
+    // All but K of the fourth tile and V of the third have arrived.
+    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    lds_barrier();
+    f32x16_t sa[2], sb[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) scores_part(i, k_part(ring(first), i), sa);
+    hide(first, sa);
+    move_to(largest(sa), sa);
+
+    // One tile: the next one's scores (matrix slots 0-15) and this one's outputs (16-31), with this one's exponentials and
+    // then the next one's maximum spread over the slots, so that the vector unit works in the matrix core's shadow.
+    // Fragments are read four slots ahead, the first four of the tile after that before the barrier: K arrives two tiles
+    // before its scores, V one before its outputs.  EDGE: some row of the workgroup does not see some key of this tile or
+    // the next.  The order is kept by hand: left to it, the compiler computes all exponentials at once.
+    bf16x8_t ahead[4];
+    const auto flow = [&](int tile, uint32_t v_at, uint32_t k_at, uint32_t k_then, f32x16_t (&now)[2], f32x16_t (&next)[2],
+                          auto edge_tag) __attribute__((always_inline)) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      bf16x8_t kf[16], vf[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kf[i] = ahead[i];
+      float m = kNone;
+      int64_t at = 0;
+      slots(std::make_integer_sequence<int, 32>{}, [&](auto slot) __attribute__((always_inline)) {
+        constexpr int i = decltype(slot)::value;
+        if constexpr (i < 12)
+          kf[i + 4] = k_part(k_at, i + 4);
+        else if constexpr (i < 28)
+          vf[i - 12] = v_part(v_at, i - 12);
+        else
+          ahead[i - 28] = k_part(k_then, i - 28);
+        if constexpr (i < 16)
+          scores_part(i, kf[i], next);
+        else
+          outputs_part(i - 16, vf[i - 16]);
+        // 16 pairs over the slots 0-25 (operand t is complete well before slot 16 + 4 t)
+        constexpr int k = (3 * i + 2) / 5;
+        if constexpr (i < 26 && 5 * k / 3 == i) {
+          asm volatile("" : "+v"(off));  // (no pair is computed before its slot)
+          pair(k, now);
+        }
+        if constexpr (i == 2) bring_v(tile + 3, at_v);
+        if constexpr (i == 4) at = place(tile + 4);
+        if constexpr (i == 7) bring_k(tile + 4, at);
+        if constexpr (EDGE && (i == 17 || i == 18)) {  // keys past a query's position
+          const int lim = pos - (tile + 1) * kKeys - 4 * h;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (32 * (i - 17) + 8 * (e >> 2) + (e & 3) > lim) next[i - 17][e] = -INFINITY;
+        }
+        if constexpr (i >= 26 || i == 19 || i == 24) {  // 4 scores a time
+          constexpr int e = i >= 26 ? 2 + (i - 26) : (i == 19 ? 0 : 1);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) m = fmaxf(m, next[e >> 2][4 * (e & 3) + x]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      at_v = at;
+      if (EDGE) add_odd(tile);
+      move_to(m, next);
+    };
+    const auto arrive = [&](int tile) __attribute__((always_inline)) {
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      __builtin_amdgcn_s_barrier();  // (this wave's reads of what the next transfers replace are done: their results were used)
+      asm volatile("" ::: "memory");
+      if (tile + 8 >= ids_from + kWave) look_up(tile + 5);
+    };
+    int tile = first;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ahead[i] = k_part(ring(tile + 1), i);
+    // (four tiles at a time: their places in the ring are constants, and the scores change places)
+    for (; tile + 4 < tiles && (tile + 5) * kKeys - 1 <= low; tile += 4) {
+      constexpr uint32_t kT = kTileBytes;
+      flow(tile, 0 * kT, 1 * kT, 2 * kT, sa, sb, std::false_type{});
+      arrive(tile);
+      flow(tile + 1, 1 * kT, 2 * kT, 3 * kT, sb, sa, std::false_type{});
+      arrive(tile + 1);
+      flow(tile + 2, 2 * kT, 3 * kT, 0 * kT, sa, sb, std::false_type{});
+      arrive(tile + 2);
+      flow(tile + 3, 3 * kT, 0 * kT, 1 * kT, sb, sa, std::false_type{});
+      arrive(tile + 3);
+    }
+    // The last tiles, of which some row does not see some key
+    mend(tile);
+    lds_barrier();
+    for (; tile < tiles; ++tile) {
+      if (tid == 0) odd_keys[(tile + 2) & 3] = 0ull;
+      if (tile < mine) {
+        flow(tile, ring(tile), ring(tile + 1), ring(tile + 2), sa, sb, std::true_type{});
+#pragma unroll
+        for (int b = 0; b < 2; ++b) sa[b] = sb[b];
+      } else {
+        bring_v(tile + 3, at_v);
+        at_v = place(tile + 4);
+        bring_k(tile + 4, at_v);
+      }
+      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+      mend(tile + 1);
+      lds_barrier();
+      if (tile + 8 >= ids_from + kWave) look_up(tile + 5);
+    }
+    if (lost != 0x7FFFFFFF && lane == 0) atomicMin(&no_page, lost);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into LDS when the workgroup ends)
+    lds_barrier();
   }
 
-  l += swap_half(l) + poison;
+  float l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  // NaN: a sequence longer than its table row, a key without a page
+  l += swap_half(l) + (len - 1 > pages.last || pos >= no_page ? NAN : 0.0f);
   if (!valid) return;
   if (SPLIT) {
-    const int64_t part = (static_cast<int64_t>(split) * a.n + row) * a.heads + out_head;
-    float* op = a.part_o + part * kDim + 4 * h;
+    const int64_t part = static_cast<int64_t>(split) * a.n * a.heads * kDim + out_at;
+    float* op = a.part_o + part + 4 * h;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -398,32 +562,22 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(PagedArgs a) {
         *reinterpret_cast<float4*>(op + 32 * d + 8 * g) =
             make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
     const bool seen = pos >= first * kKeys && first < tiles;
-    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(seen ? raw : kUnseen, l);
+    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + part / (kDim / 2)) = make_float2(seen ? raw : kUnseen, l);
     return;
   }
   const float inv = pos >= 0 ? 1.0f / l : 0.0f;
-  uint16_t* op = a.o + (row * a.heads + out_head) * kDim + 4 * h;
+  uint16_t* op = a.o + out_at + 4 * h;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const float part[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-      *reinterpret_cast<uint2*>(op + 32 * d + 8 * g) = pair4(part, inv);
+      const float x[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      *reinterpret_cast<uint2*>(op + 32 * d + 8 * g) = pair4(x, inv);
     }
 }
 
 // The key ranges that a sequence of `steps` steps is divided into: at least one step for each wave of a range.
 __device__ __forceinline__ int step_ranges(int splits, int steps) { return max(1, min(splits, steps / kWaves)); }
-
-// read_v_tr (attn_common.h) of an address that is known to be one in LDS, so that fixed distances are offsets of the read
-typedef const __attribute__((address_space(3))) uint16_t* lds_rows;
-__device__ __forceinline__ lds_rows as_lds(const uint16_t* p) {
-  return reinterpret_cast<lds_rows>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
-}
-__device__ __forceinline__ bf16x4_t read_tr(lds_rows p) {
-  typedef __attribute__((address_space(3))) bf16x4_t lds_t;
-  return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_t*)p);
-}
 
 template <bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
@@ -707,7 +861,7 @@ int paged_splits(int seqs, int n, int kv, int group, int max_q, int max_kv) {
   const bool step = few_rows(max_q, group);
   const int64_t groups = step ? static_cast<int64_t>(seqs) * kv
                               : ((static_cast<int64_t>(n) * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs / 2 : 0)) * kv;
-  const int64_t want = ((step ? 1536 : 640) + groups - 1) / std::max<int64_t>(groups, 1);
+  const int64_t want = ((step ? 1536 : 256) + groups - 1) / std::max<int64_t>(groups, 1);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), max_kv / (step ? 128 : 448))));
 }
 
@@ -758,14 +912,14 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   a.splits = static_cast<int>(std::max<size_t>(1, std::min<size_t>(a.splits, workspace_bytes / one)));
   const bool step = q_starts == nullptr || few_rows(max_q, group);
   const int64_t tiles = step ? seqs + (q_starts ? 1 : 0) : (static_cast<int64_t>(rows) * group + kChunkRows - 1) / kChunkRows + seqs;
-  FL_REQUIRE(tiles * kv_heads * a.splits <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
+  FL_REQUIRE(tiles * kv_heads * a.splits <= 0x7FFFFFFF / kChunkThreads, "fl_paged_attention: grid too large");
   const dim3 grid(static_cast<unsigned>(tiles * kv_heads * a.splits)), block(kThreads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (a.splits <= 1) {
     if (step)
       hipLaunchKernelGGL(step_kernel<false>, grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL(chunk_kernel<false>, grid, block, 0, st, a);
+      hipLaunchKernelGGL(chunk_kernel<false>, grid, dim3(kChunkThreads), 0, st, a);
     FL_LAUNCH_CHECK("fl_paged_attention");
     return FL_OK;
   }
@@ -776,7 +930,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   if (step)
     hipLaunchKernelGGL(step_kernel<true>, grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL(chunk_kernel<true>, grid, block, 0, st, a);
+    hipLaunchKernelGGL(chunk_kernel<true>, grid, dim3(kChunkThreads), 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention");
   hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((all + kWaves - 1) / kWaves)), block, 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention(join)");
