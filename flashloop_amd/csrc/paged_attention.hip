@@ -30,6 +30,10 @@ constexpr int kChunkThreads = kChunkWaves * kWave;
 constexpr int kChunkRows = 32 * kChunkWaves;  // its queries
 constexpr int kStepKeys = 32;            // keys of a wave's step in step_kernel
 constexpr int kStepRows = 16;            // its queries
+constexpr int kMaxRanges = kWave;        // ranges of an item's keys: the join has one a lane
+// Workgroups that a call aims at, and the least steps of a range
+constexpr int kStepAim = 1024, kStepLeast = kWaves;
+constexpr int kChunkAim = 256, kChunkLeast = 7;  // (one a CU)
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -51,9 +55,17 @@ struct PagedArgs {
   const int32_t* starts; // [seqs + 1], or null: row s is sequence s's
   int n, seqs, heads, kv, group, width, pages, page_log2;
   float scale;  // scaling * log2(e)
-  int splits;   // key ranges
-  float* part_o;   // splits > 1: f32 [splits][n * heads][128], row i * heads + head
-  float* part_ml;  // f32 [splits][n * heads][2]: maximum of q.k (kUnseen: no key) and sum
+  // Key ranges (Work): workgroups aimed at, or 0: every item is one; and the workspace for their outputs
+  int aim, ranges, slots, items;  // ranges of an item at most; ranges' outputs a KV head and divided items that there is room for
+  int32_t* divided;       // number of divided items
+  struct Divided* list;   // [items]
+  float2* part_ml;        // [kv][slots][rows of an item]: maximum of q.k (kUnseen: no key) and sum
+  float* part_o;          // [kv][slots][rows of an item][128]
+};
+
+// An item whose keys are divided: queries [item * ROWS, ..) of the rows [first, first + rows), in `ranges` slots.
+struct Divided {
+  int32_t first, rows, item, ranges, slot;
 };
 
 // the maximum of a query that sees no key (kNone: its scores are all -inf)
@@ -98,6 +110,110 @@ __device__ __forceinline__ Pages pages_of(const PagedArgs& a, int s, int head, i
   p.page_elems = static_cast<int64_t>(a.kv) << (a.page_log2 + 7);
   p.head_elems = static_cast<int64_t>(head) << (a.page_log2 + 7);
   return p;
+}
+
+// A workgroup's work.  An item is up to ROWS queries of a sequence, against its keys in UNIT-key steps; where the
+// items are too few for the chip, or too unequal, a sequence's are divided into ranges of about T steps, T such that the
+// call makes about `aim` workgroups.  Every workgroup finds this out for itself, sequences in lanes: the lengths are on
+// the device alone.  Since a divided item has more than T steps, there are at most 2 aim / kv ranges of divided ones.
+struct Work {
+  int seq, item, range, ranges;
+  int slot;     // of its first range's output (ranges > 1)
+  int total;    // workgroups that have work, a KV head
+};
+
+template <int ROWS>
+__device__ __forceinline__ int items_of(const PagedArgs& a, int rows) { return (rows * a.group + ROWS - 1) / ROWS; }
+
+__device__ __forceinline__ int scan_lanes(int v, int lane) {  // sum over the lanes up to this one
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int u = __shfl_up(v, off, kWave);
+    v += lane >= off ? u : 0;
+  }
+  return v;
+}
+
+// index: this workgroup's number for its KV head.  ONE: items of more than ROWS queries are one, and never divided.
+template <int ROWS, int UNIT, int LEAST, bool ONE, bool FIT>
+__device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int index, Work& w) {
+  const int lane = threadIdx.x & 63;
+  const auto look = [&](int s, int& items, int& steps, bool& whole) __attribute__((always_inline)) {
+    const int2 rows = s < a.seqs ? rows_of(a, s) : make_int2(0, 0);
+    const int64_t keys = s < a.seqs ? min(static_cast<int64_t>(max(a.lens[s], 0)), static_cast<int64_t>(a.width) << a.page_log2) : 0;
+    items = items_of<ROWS>(a, rows.y);
+    whole = ONE && items > 1;
+    if (ONE) items = min(items, 1);
+    steps = static_cast<int>((keys + UNIT - 1) / UNIT);
+  };
+  int items, steps;
+  bool whole;
+  look(lane, items, steps, whole);
+  int most = 1 << 30;  // T
+  if (a.aim > 0) {
+    float sum = wave_sum(static_cast<float>(items) * static_cast<float>(steps)), count = wave_sum(static_cast<float>(items));
+    for (int base = kWave; base < a.seqs; base += kWave) {
+      int its, sts;
+      bool all;
+      look(base + lane, its, sts, all);
+      sum += wave_sum(static_cast<float>(its) * static_cast<float>(sts));
+      count += wave_sum(static_cast<float>(its));
+    }
+    most = max(LEAST, static_cast<int>(fminf(ceilf(sum * a.kv / a.aim), 1e9f)));
+    // one round of workgroups, if there can be: ranges a little longer rather than some in a second round
+    if (FIT && a.seqs <= kWave && count * a.kv <= a.aim)
+      for (int i = 0; i < 24; ++i) {
+        const int groups = items * (whole ? 1 : min(max(1, (steps + most - 1) / most), a.ranges));
+        if (wave_sum(static_cast<float>(groups)) * a.kv <= a.aim) break;
+        most += max(1, most / 16);
+      }
+  }
+  w.seq = -1;
+  w.total = 0;
+  int slots = 0, divided = 0;
+  for (int base = 0; base < a.seqs; base += kWave) {
+    if (base > 0) look(base + lane, items, steps, whole);
+    const int ranges = whole ? 1 : min(max(1, (steps + most - 1) / most), a.ranges);
+    const int groups = items * ranges, parts = ranges > 1 ? groups : 0, split = ranges > 1 ? items : 0;
+    const int to = w.total + scan_lanes(groups, lane), slots_to = slots + scan_lanes(parts, lane), split_to = divided + scan_lanes(split, lane);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(to > index);
+    if (w.seq < 0 && past != 0ull) {
+      const int l = __builtin_ctzll(past);
+      const int its = __builtin_amdgcn_readlane(items, l);
+      w.seq = base + l;
+      w.ranges = __builtin_amdgcn_readlane(ranges, l);
+      const int local = index - (__builtin_amdgcn_readlane(to, l) - its * w.ranges);
+      const int nth = local / w.ranges;  // (the last items first: they see more keys)
+      w.range = local - nth * w.ranges;
+      w.item = its - 1 - nth;
+      w.slot = __builtin_amdgcn_readlane(slots_to, l) - its * w.ranges + nth * w.ranges;
+      if (w.ranges > 1 && w.slot + w.ranges > a.slots) {  // (only where the rows of q_starts overlap)
+        w.seq = -1;
+        return false;
+      }
+      if (w.ranges > 1 && head == 0 && w.range == 0 && threadIdx.x == 0) {
+        const int at = __builtin_amdgcn_readlane(split_to, l) - its + nth;
+        const int2 rows = rows_of_one(a, w.seq);
+        if (at < a.items) a.list[at] = Divided{rows.x, rows.y, w.item, w.ranges, w.slot};
+      }
+      if (index != 0) return true;
+    }
+    w.total = __builtin_amdgcn_readlane(to, kWave - 1);
+    slots = __builtin_amdgcn_readlane(slots_to, kWave - 1);
+    divided = __builtin_amdgcn_readlane(split_to, kWave - 1);
+  }
+  if (a.aim > 0 && head == 0 && index == 0 && threadIdx.x == 0) *a.divided = min(divided, a.items);
+  return w.seq >= 0;
+}
+
+// Rows that belong to no sequence: zeros, by the workgroups without work.
+__device__ __forceinline__ void clear_behind(const PagedArgs& a, int head, int index, int total, int threads) {
+  if (a.starts == nullptr) return;
+  const int behind = min(max(a.starts[a.seqs], 0), a.n);
+  const int spare = static_cast<int>(gridDim.x) / a.kv - total, width = a.group * kDim / 8;
+  for (int64_t row = behind + index - total; row < a.n; row += spare)
+    for (int c = threadIdx.x; c < width; c += threads)
+      *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * c) = make_uint4(0, 0, 0, 0);
 }
 
 // Infinite and NaN values of a chunk of 8 bf16 become zeros; returns whether there were any.
@@ -146,65 +262,24 @@ __device__ __forceinline__ void slots(std::integer_sequence<int, I...>, F f) {
   (f(std::integral_constant<int, I>{}), ...);
 }
 
-template <bool SPLIT>
 __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds_all[2 * kRing * kTileBytes];
   __shared__ int wave_pos[2][kChunkWaves];
   __shared__ unsigned long long odd_keys[4];  // by tile % 4: keys of a tile with infinite or NaN values
   __shared__ int no_page;                     // the first key without a page
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = static_cast<int>(blockIdx.x) % a.kv;
-  const int rest = static_cast<int>(blockIdx.x) / a.kv;
-  const int split = SPLIT ? rest % a.splits : 0;
-  const int index = SPLIT ? rest / a.splits : rest;
-
-  // The index-th tile from the end (a sequence's later rows see more keys): sequences in lanes.
-  int total = 0;
-  for (int base = 0; base < a.seqs; base += kWave) {
-    const int s = base + lane;
-    int t = s < a.seqs ? (rows_of(a, s).y * a.group + kChunkRows - 1) / kChunkRows : 0;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) t += __shfl_xor(t, off, kWave);
-    total += t;
-  }
-  total = __builtin_amdgcn_readfirstlane(total);
-  if (index >= total) {  // rows that belong to no sequence: zeros
-    if (split != 0) return;
-    const int behind = min(max(a.starts[a.seqs], 0), a.n);
-    const int spare = static_cast<int>(gridDim.x) / a.kv / a.splits - total, width = a.group * kDim / 8;
-    for (int64_t row = behind + index - total; row < a.n; row += spare)
-      for (int c = tid; c < width; c += kChunkThreads)
-        *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * c) = make_uint4(0, 0, 0, 0);
+  const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
+  Work w;
+  if (!find_work<kChunkRows, kKeys, kChunkLeast, false, true>(a, head, index, w)) {
+    clear_behind(a, head, index, w.total, kChunkThreads);
     return;
   }
-  const int want = total - 1 - index;
-  int seq = 0, tile_of_seq = 0, before = 0;
-  for (int base = 0; base < a.seqs; base += kWave) {
-    const int s = base + lane;
-    const int mine = s < a.seqs ? (rows_of(a, s).y * a.group + kChunkRows - 1) / kChunkRows : 0;
-    int t = mine;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int u = __shfl_up(t, off, kWave);
-      t += lane >= off ? u : 0;
-    }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + t > want);
-    if (past != 0ull) {
-      const int l = __builtin_ctzll(past);
-      seq = base + l;
-      tile_of_seq = want - before - (__builtin_amdgcn_readlane(t, l) - __builtin_amdgcn_readlane(mine, l));
-      break;
-    }
-    before += __builtin_amdgcn_readlane(t, kWave - 1);
-  }
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  tile_of_seq = __builtin_amdgcn_readfirstlane(tile_of_seq);
-
+  const int seq = __builtin_amdgcn_readfirstlane(w.seq), ranges = __builtin_amdgcn_readfirstlane(w.ranges);
   const int2 rows = rows_of_one(a, seq);
   const int len = max(uniform(a.lens)[seq], 0);
   const Pages pages = pages_of(a, seq, head, len);
   // this lane's query: column lane % 32 of the wave's
-  const int r = tile_of_seq * kChunkRows + wave * 32 + (lane & 31);
+  const int r = __builtin_amdgcn_readfirstlane(w.item) * kChunkRows + wave * 32 + (lane & 31);
   const bool valid = r < rows.y * a.group;
   const int rc = valid ? r : rows.y * a.group - 1;
   const int token = rc / a.group, out_head = head * a.group + rc - token * a.group;
@@ -240,9 +315,10 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
   low = __builtin_amdgcn_readfirstlane(low);
   end = __builtin_amdgcn_readfirstlane(min(end, pages.last));
   int tiles = end >= 0 ? end / kKeys + 1 : 0, first = 0;
-  if (SPLIT) {
-    first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-    tiles = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  if (ranges > 1) {
+    const int range = __builtin_amdgcn_readfirstlane(w.range);
+    first = static_cast<int>(static_cast<int64_t>(tiles) * range / ranges);
+    tiles = static_cast<int>(static_cast<int64_t>(tiles) * (range + 1) / ranges);
   }
   const int mine = min(tiles, (wmax >> 6) + 1);  // tiles that some query of the wave sees (none: at most `first`)
 
@@ -259,12 +335,11 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
   bool far = false;  // (wave-uniform) some query's reference lies past kFar
 
   if (first < tiles) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): q has arrived (or every use of it would wait for the transfers, too)
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds_all));
     constexpr uint32_t kV = kRing * kTileBytes;  // V's tiles lie behind K's
 
-    // Transfers: a wave brings the 8 keys 8 w .. of a tile, which share a page: twice four rows.  The page numbers of 64
-    // tiles lie in the lanes of one register (a scalar load among a tile's LDS reads would make their waits wait for all).
+    // Transfers: a wave brings the 8 keys 8 w .. of a tile, which share a page: twice four rows.  Their places for 64
+    // tiles lie in the lanes of two registers (a scalar load among a tile's LDS reads would make their waits wait for all).
     uint32_t kv[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) kv[i] = 1024 * i + 256 * (lane >> 4) + 16 * ((lane & 15) ^ (8 * (wave & 1) + 4 * i + (lane >> 4)));
@@ -272,26 +347,36 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
     const auto block_key = [&](int tile) __attribute__((always_inline)) {
       return min(min(tile, tiles - 1) * kKeys + 8 * (wave & ~1), pages.last & ~15);
     };
-    int ids = 0, ids_from = 0, lost = 0x7FFFFFFF;  // lost: the first key of this wave's without a page
+    uint32_t at_lo = 0, at_hi = 0;  // bytes from the pool's start
+    int at_from = 0, lost = 0x7FFFFFFF;  // lost: the first key of this wave's without a page
     const auto look_up = [&](int tile) __attribute__((always_inline)) {
-      ids_from = tile;
-      ids = *(a.table + static_cast<int64_t>(seq) * a.width + (block_key(tile + lane) >> pages.log2));
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): here, and not at every use
+      at_from = tile;
+      const int key = block_key(tile + lane);
+      const int id = *(a.table + static_cast<int64_t>(seq) * a.width + (key >> pages.log2));
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it, and q before the first, have arrived here, and no use waits for them
+      const uint64_t at = 2 * static_cast<uint64_t>(pages.at(id, key) + 8 * (wave & 1) * kDim);
+      at_lo = static_cast<uint32_t>(at);
+      at_hi = static_cast<uint32_t>(at >> 32);
+      const unsigned long long none = __builtin_amdgcn_ballot_w64(!pages.exists(id));
+      if (none != 0ull) lost = min(lost, __builtin_amdgcn_readlane(key, __builtin_ctzll(none)));
     };
-    const auto place = [&](int tile) __attribute__((always_inline)) {  // of the wave's keys of a tile, in elements of the pool
-      const int id = __builtin_amdgcn_readlane(ids, tile - ids_from), key = block_key(tile);
-      lost = pages.exists(id) ? lost : min(lost, key);
-      return pages.at(id, key) + 8 * (wave & 1) * kDim;
+    const auto place = [&](int tile) __attribute__((always_inline)) {  // of the wave's keys of a tile
+      return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_hi), tile - at_from))) << 32) |
+             static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_lo), tile - at_from));
+    };
+    const auto part_of = [&](const uint16_t* pool, uint64_t at) __attribute__((always_inline)) {
+      const uint64_t u = reinterpret_cast<uintptr_t>(pool) + at;
+      return lds_buffer_t{static_cast<int>(u), static_cast<int>(u >> 32), 8 * kDim * 2, 0x00020000};
     };
     const auto ring = [&](int tile) __attribute__((always_inline)) { return static_cast<uint32_t>((tile - first) % kRing) * kTileBytes; };
-    const auto bring_k = [&](int tile, int64_t at) __attribute__((always_inline)) {
-      const lds_buffer_t r = raw_buffer(a.k + at, 8 * kDim * 2);
+    const auto bring_k = [&](int tile, uint64_t at) __attribute__((always_inline)) {
+      const lds_buffer_t r = part_of(a.k, at);
       const uint32_t to = lds0 + ring(tile) + 2048u * wave;
       to_lds<16>(r, kv[0], 0, to);
       to_lds<16>(r, kv[1], 0, to + 1024u);
     };
-    const auto bring_v = [&](int tile, int64_t at) __attribute__((always_inline)) {
-      const lds_buffer_t r = raw_buffer(a.v + at, 8 * kDim * 2);
+    const auto bring_v = [&](int tile, uint64_t at) __attribute__((always_inline)) {
+      const lds_buffer_t r = part_of(a.v, at);
       const uint32_t to = lds0 + kV + ring(tile) + 2048u * wave;
       to_lds<16>(r, vv, 0, to);
       to_lds<16>(r, vv, 1024u, to + 1024u);
@@ -330,10 +415,10 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) vx[d] = lds0 + kV + 256 * (4 * h + (i16 >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3) + (64 * (i16 >> 2) ^ 64 * d);
     const auto k_part = [&](uint32_t of, int i) __attribute__((always_inline)) {
-      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>((lds_at)(kx[i >> 1] + of) + 8192 * (i & 1));
+      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(reinterpret_cast<lds_at>(kx[i >> 1] + of) + 8192 * (i & 1));
     };
     const auto v_part = [&](uint32_t of, int j) __attribute__((always_inline)) {
-      const lds_at at = (lds_at)(vx[j & 3] + of) + 4096 * (j >> 2);
+      const lds_at at = reinterpret_cast<lds_at>(vx[j & 3] + of) + 4096 * (j >> 2);
       const bf16x4_t lo = read_tr((lds_rows)at), hi = read_tr((lds_rows)(at + 2048));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
@@ -428,9 +513,9 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
     };
 
     look_up(first);
-    int64_t at_v = 0;  // place of the tile whose V goes next
+    uint64_t at_v = 0;  // place of the tile whose V goes next
     {
-      int64_t at[4];
+      uint64_t at[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) at[i] = place(first + i);
       bring_k(first, at[0]);
@@ -464,7 +549,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) kf[i] = ahead[i];
       float m = kNone;
-      int64_t at = 0;
+      uint64_t at = 0;
       slots(std::make_integer_sequence<int, 32>{}, [&](auto slot) __attribute__((always_inline)) {
         constexpr int i = decltype(slot)::value;
         if constexpr (i < 12)
@@ -507,7 +592,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
       asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       __builtin_amdgcn_s_barrier();  // (this wave's reads of what the next transfers replace are done: their results were used)
       asm volatile("" ::: "memory");
-      if (tile + 8 >= ids_from + kWave) look_up(tile + 5);
+      if (tile + 8 >= at_from + kWave) look_up(tile + 5);
     };
     int tile = first;
 #pragma unroll
@@ -541,7 +626,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
       asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
       mend(tile + 1);
       lds_barrier();
-      if (tile + 8 >= ids_from + kWave) look_up(tile + 5);
+      if (tile + 8 >= at_from + kWave) look_up(tile + 5);
     }
     if (lost != 0x7FFFFFFF && lane == 0) atomicMin(&no_page, lost);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into LDS when the workgroup ends)
@@ -552,9 +637,9 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
   // NaN: a sequence longer than its table row, a key without a page
   l += swap_half(l) + (len - 1 > pages.last || pos >= no_page ? NAN : 0.0f);
   if (!valid) return;
-  if (SPLIT) {
-    const int64_t part = static_cast<int64_t>(split) * a.n * a.heads * kDim + out_at;
-    float* op = a.part_o + part + 4 * h;
+  if (ranges > 1) {
+    const int64_t part = (static_cast<int64_t>(head) * a.slots + w.slot + w.range) * kChunkRows + wave * 32 + (lane & 31);
+    float* op = a.part_o + part * kDim + 4 * h;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -562,7 +647,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
         *reinterpret_cast<float4*>(op + 32 * d + 8 * g) =
             make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
     const bool seen = pos >= first * kKeys && first < tiles;
-    if (h == 0) *reinterpret_cast<float2*>(a.part_ml + part / (kDim / 2)) = make_float2(seen ? raw : kUnseen, l);
+    if (h == 0) a.part_ml[part] = make_float2(seen ? raw : kUnseen, l);
     return;
   }
   const float inv = pos >= 0 ? 1.0f / l : 0.0f;
@@ -576,28 +661,19 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
     }
 }
 
-// The key ranges that a sequence of `steps` steps is divided into: at least one step for each wave of a range.
-__device__ __forceinline__ int step_ranges(int splits, int steps) { return max(1, min(splits, steps / kWaves)); }
-
-template <bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
   // a wave's V rows of 256 bytes; 32-byte piece d of row r lies at d ^ (r % 8), so that the 16 rows of a transposed
   // read cover all banks without padding 
   __shared__ __attribute__((aligned(16))) uint16_t lds[kWaves][kStepKeys * kDim];
   __shared__ float2 wave_ml[kWaves][kStepRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-  const int head = static_cast<int>(blockIdx.x) % a.kv;
-  const int rest = static_cast<int>(blockIdx.x) / a.kv;
-  const int split = SPLIT ? rest % a.splits : 0;
-  const int seq = SPLIT ? rest / a.splits : rest;
-  if (seq == a.seqs) {  // rows that belong to no sequence: zeros
-    if (split != 0) return;
-    const int width = a.group * kDim / 8;
-    for (int64_t row = min(max(a.starts[a.seqs], 0), a.n); row < a.n; ++row)
-      for (int i = tid; i < width; i += kThreads)
-        *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * i) = make_uint4(0, 0, 0, 0);
+  const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
+  Work w{index, 0, 0, 1, 0, a.seqs};
+  if (a.aim > 0 ? !find_work<kStepRows, kStepKeys, kStepLeast, true, false>(a, head, index, w) : index >= a.seqs) {
+    clear_behind(a, head, index, w.total, kThreads);
     return;
   }
+  const int seq = __builtin_amdgcn_readfirstlane(w.seq), ranges = __builtin_amdgcn_readfirstlane(w.ranges);
   const int2 rows = rows_of_one(a, seq);
   const int len = max(uniform(a.lens)[seq], 0);
   const Pages pages = pages_of(a, seq, head, len);
@@ -610,10 +686,10 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
     const int low = len - rows.y + base / a.group;
     const int end = min(len - rows.y + min(base + kStepRows - 1, rows.y * a.group - 1) / a.group, pages.last);
     int steps = end >= 0 ? end / kStepKeys + 1 : 0, first = 0;
-    if (SPLIT) {
-      const int ranges = step_ranges(a.splits, steps);
-      first = split < ranges ? static_cast<int>(static_cast<int64_t>(steps) * split / ranges) : steps;
-      steps = split < ranges ? static_cast<int>(static_cast<int64_t>(steps) * (split + 1) / ranges) : steps;
+    if (ranges > 1) {
+      const int range = __builtin_amdgcn_readfirstlane(w.range);
+      first = static_cast<int>(static_cast<int64_t>(steps) * range / ranges);
+      steps = static_cast<int>(static_cast<int64_t>(steps) * (range + 1) / ranges);
     }
     bf16x8_t q[4];
     {
@@ -801,14 +877,14 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
       }
       const int tok = (base + jr) / a.group, oh = head * a.group + base + jr - tok * a.group;
       const int64_t orow = static_cast<int64_t>(rows.x + tok) * a.heads + oh;
-      if (SPLIT) {
-        const int64_t part = static_cast<int64_t>(split) * a.n * a.heads + orow;
+      if (ranges > 1) {
+        const int64_t part = (static_cast<int64_t>(head) * a.slots + w.slot + w.range) * kStepRows + jr;
         float* op = a.part_o + part * kDim + ch;
         if (top != kUnseen) {
           *reinterpret_cast<float4*>(op) = make_float4(acc[0], acc[1], acc[2], acc[3]);
           *reinterpret_cast<float4*>(op + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
         }
-        if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(top, sum);
+        if (ch == 0) a.part_ml[part] = make_float2(top, sum);
       } else {
         const float inv = top != kUnseen ? 1.0f / sum : 0.0f;
         const uint2 x = pair4(acc, inv), y = pair4(acc + 4, inv);
@@ -819,53 +895,80 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
   }
 }
 
-// Joins the key ranges: a wave per (row, head), 2 channels a lane.  Range s's maximum and sum come to lane s in
-// one load, and the ranges' rows are loaded eight at a time, so that a join costs two or three memory latencies
-// (one load after another: 13 us for one row of 16 ranges).
+// Joins the key ranges of divided items of ROWS queries: a wave takes ROWS / gridDim.y / 4 rows of one KV head, 2 channels a
+// lane.  Range r's maximum and sum come to lane r in one load, and the ranges' rows are loaded eight at a time, so that a
+// join costs two or three memory latencies (one load after another: 13 us for one row of 16 ranges).
+template <int ROWS>
 __global__ __launch_bounds__(kThreads) void join_kernel(PagedArgs a) {
-  const int64_t rows = (a.starts ? min(max(a.starts[a.seqs], 0), a.n) : a.n) * static_cast<int64_t>(a.heads);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= rows) return;
-  const int64_t all = static_cast<int64_t>(a.n) * a.heads;
-  const int lane = threadIdx.x & 63;
-  const bool mine = lane < a.splits;
-  const float2 ml = mine ? *reinterpret_cast<const float2*>(a.part_ml + 2 * (lane * all + row)) : make_float2(kUnseen, 0.0f);
-  const float* const part = a.part_o + row * kDim + 2 * lane;
-  const float top = wave_max(ml.x);
-  const bool seen = ml.x != kUnseen;
-  const float w = seen ? exp2_between(ml.x, top, scaled_max(ml.x, a.scale), scaled_max(top, a.scale), a.scale) : 0.0f;
-  const float l = wave_sum(seen ? w * ml.y : (ml.y != ml.y ? ml.y : 0.0f));
-  const unsigned long long parts = __builtin_amdgcn_ballot_w64(seen);
-  float o0 = 0.0f, o1 = 0.0f;
-  for (int base = 0; base < a.splits; base += 8) {
-    float2 v[8];
+  const int head = static_cast<int>(blockIdx.x) % a.kv, nth = static_cast<int>(blockIdx.x) / a.kv;
+  if (nth >= *a.divided) return;
+  const Divided d = a.list[nth];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int each = ROWS / kWaves / static_cast<int>(gridDim.y);
+  const int64_t slot = static_cast<int64_t>(head) * a.slots + d.slot;
+  for (int i = 0; i < each; ++i) {
+    const int r = (static_cast<int>(blockIdx.y) * each + i) * kWaves + wave, q = d.item * ROWS + r;
+    if (q >= d.rows * a.group) return;
+    const int token = q / a.group;
+    const int64_t out = (static_cast<int64_t>(d.first + token) * a.heads + head * a.group + q - token * a.group) * kDim + 2 * lane;
+    const float2 ml = lane < d.ranges ? a.part_ml[(slot + lane) * ROWS + r] : make_float2(kUnseen, 0.0f);
+    const float* const part = a.part_o + (slot * ROWS + r) * kDim + 2 * lane;
+    const float top = wave_max(ml.x);
+    const bool seen = ml.x != kUnseen;
+    const float w = seen ? exp2_between(ml.x, top, scaled_max(ml.x, a.scale), scaled_max(top, a.scale), a.scale) : 0.0f;
+    const float l = wave_sum(seen ? w * ml.y : (ml.y != ml.y ? ml.y : 0.0f));
+    const unsigned long long parts = __builtin_amdgcn_ballot_w64(seen);
+    float o0 = 0.0f, o1 = 0.0f;
+    for (int base = 0; base < d.ranges; base += 8) {
+      float2 v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = (parts >> (base + i)) & 1 ? *reinterpret_cast<const float2*>(part + (base + i) * all * kDim) : make_float2(0.0f, 0.0f);
+      for (int k = 0; k < 8; ++k)
+        v[k] = (parts >> (base + k)) & 1 ? *reinterpret_cast<const float2*>(part + static_cast<int64_t>(base + k) * ROWS * kDim)
+                                         : make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float f = row_lane(w, base + i);
-      o0 = fmaf(f, v[i].x, o0);
-      o1 = fmaf(f, v[i].y, o1);
+      for (int k = 0; k < 8; ++k) {
+        const float f = row_lane(w, base + k);
+        o0 = fmaf(f, v[k].x, o0);
+        o1 = fmaf(f, v[k].y, o1);
+      }
     }
+    const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
+    *reinterpret_cast<uint32_t*>(a.o + out) = attn_bf16_pair(o0 * inv, o1 * inv);
   }
-  const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
-  *reinterpret_cast<uint32_t*>(a.o + row * kDim + 2 * lane) = attn_bf16_pair(o0 * inv, o1 * inv);
 }
 
-// Sequences of few rows take step_kernel: up to 16 queries of a KV head are one pass over its keys there.
-bool few_rows(int max_q, int group) { return static_cast<int64_t>(max_q) * group <= kStepRows; }
+// How a call is launched: which kernel, and the room for divided items.
+struct Launch {
+  bool step;
+  int aim, ranges, slots, items;
+  int64_t groups;  // workgroups a KV head, at most
+  size_t list_at, ml_at, o_at, bytes;
+};
 
-// Key ranges: enough workgroups to fill the chip, of at least 128 (step) or 448 (chunk) keys each.
-int paged_splits(int seqs, int n, int kv, int group, int max_q, int max_kv) {
-  const bool step = few_rows(max_q, group);
-  const int64_t groups = step ? static_cast<int64_t>(seqs) * kv
-                              : ((static_cast<int64_t>(n) * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs / 2 : 0)) * kv;
-  const int64_t want = ((step ? 1536 : 256) + groups - 1) / std::max<int64_t>(groups, 1);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 64), max_kv / (step ? 128 : 448))));
+Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t max_kv, bool starts) {
+  Launch p{};
+  // up to 16 queries of a KV head are one pass over its keys in step_kernel
+  p.step = !starts || max_q * group <= kStepRows;
+  const int rows = p.step ? kStepRows : kChunkRows, unit = p.step ? kStepKeys : kKeys, least = p.step ? kStepLeast : kChunkLeast;
+  const int64_t items = p.step ? seqs : (n * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs : 0);
+  p.aim = p.step ? kStepAim : kChunkAim;
+  // nothing is divided where the longest sequence is one range, or (one sequence, or single rows) items alone make as many
+  // workgroups as ranges would
+  const int64_t steps = (max_kv + unit - 1) / unit;
+  if (steps <= least || ((p.step || seqs == 1) && items * kv >= p.aim)) p.aim = 0;
+  p.groups = items + (starts ? 1 : 0);
+  p.ranges = 1;
+  if (p.aim == 0) return p;
+  p.ranges = static_cast<int>(std::min<int64_t>(kMaxRanges, (steps + least - 1) / least));
+  p.slots = static_cast<int>(std::min<int64_t>(2 * (p.aim / kv) + 8, items * p.ranges));
+  p.items = static_cast<int>(std::min<int64_t>(p.aim / kv + 8, items));
+  p.groups += p.slots;
+  p.list_at = 16;
+  p.ml_at = (p.list_at + p.items * sizeof(Divided) + 15) / 16 * 16;
+  p.o_at = p.ml_at + static_cast<size_t>(kv) * p.slots * rows * sizeof(float2);
+  p.bytes = p.o_at + static_cast<size_t>(kv) * p.slots * rows * kDim * sizeof(float);
+  return p;
 }
-
-size_t paged_split_bytes(int64_t n, int64_t heads) { return static_cast<size_t>(n) * heads * (kDim + 2) * sizeof(float); }
 
 }  // namespace
 }  // namespace fl
@@ -874,8 +977,9 @@ extern "C" size_t fl_paged_attention_workspace(int32_t rows, int32_t seqs, int32
                                                int32_t max_kv) {
   using namespace fl;
   if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || heads % kv_heads || max_q <= 0 || max_kv <= 0) return 0;
-  const int s = paged_splits(seqs, rows, kv_heads, heads / kv_heads, max_q, max_kv);
-  return s > 1 ? s * paged_split_bytes(rows, heads) : 0;
+  // (with or without q_starts: what both may take)
+  const size_t a = plan(rows, seqs, kv_heads, heads / kv_heads, max_q, max_kv, true).bytes;
+  return rows == seqs ? std::max(a, plan(rows, seqs, kv_heads, heads / kv_heads, 1, max_kv, false).bytes) : a;
 }
 
 extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, const uint16_t* k_pages, const uint16_t* v_pages,
@@ -902,37 +1006,31 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
     FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_paged_attention: every tensor must be 16-byte aligned");
   if (rows == 0) return FL_OK;
   FL_REQUIRE(seqs > 0, "fl_paged_attention: rows without a sequence");
-  if (q_starts == nullptr) max_q = 1;
-  PagedArgs a{q, q_row_stride, k_pages, v_pages, out, page_table, kv_lens, q_starts, rows, seqs, heads, kv_heads, group,
-              table_width, pages, __builtin_ctz(static_cast<unsigned>(page_size)), scaling * kLog2e,
-              paged_splits(seqs, rows, kv_heads, group, max_q, max_kv), nullptr, nullptr};
-  // as many ranges as the workspace holds (one without it)
-  const size_t one = paged_split_bytes(rows, heads);
-  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) workspace_bytes = 0;
-  a.splits = static_cast<int>(std::max<size_t>(1, std::min<size_t>(a.splits, workspace_bytes / one)));
-  const bool step = q_starts == nullptr || few_rows(max_q, group);
-  const int64_t tiles = step ? seqs + (q_starts ? 1 : 0) : (static_cast<int64_t>(rows) * group + kChunkRows - 1) / kChunkRows + seqs;
-  FL_REQUIRE(tiles * kv_heads * a.splits <= 0x7FFFFFFF / kChunkThreads, "fl_paged_attention: grid too large");
-  const dim3 grid(static_cast<unsigned>(tiles * kv_heads * a.splits)), block(kThreads);
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (a.splits <= 1) {
-    if (step)
-      hipLaunchKernelGGL(step_kernel<false>, grid, block, 0, st, a);
-    else
-      hipLaunchKernelGGL(chunk_kernel<false>, grid, dim3(kChunkThreads), 0, st, a);
-    FL_LAUNCH_CHECK("fl_paged_attention");
-    return FL_OK;
+  Launch p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, max_kv, q_starts != nullptr);
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < p.bytes) {
+    p.aim = 0;  // (no room for divided items: none is divided)
+    p.groups -= p.slots;
+    p.ranges = 1;
   }
-  const int64_t all = static_cast<int64_t>(rows) * heads;
-  FL_REQUIRE((all + kWaves - 1) / kWaves <= 0x7FFFFFFF / kThreads, "fl_paged_attention: grid too large");
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + a.splits * all * kDim;
-  if (step)
-    hipLaunchKernelGGL(step_kernel<true>, grid, block, 0, st, a);
+  FL_REQUIRE(p.groups * kv_heads <= 0x7FFFFFFF / kChunkThreads, "fl_paged_attention: grid too large");
+  uint8_t* const ws = static_cast<uint8_t*>(workspace);
+  const PagedArgs a{q, q_row_stride, k_pages, v_pages, out, page_table, kv_lens, q_starts, rows, seqs, heads, kv_heads, group,
+                    table_width, pages, __builtin_ctz(static_cast<unsigned>(page_size)), scaling * kLog2e,
+                    p.aim, p.ranges, p.slots, p.items, reinterpret_cast<int32_t*>(ws), reinterpret_cast<Divided*>(ws + p.list_at),
+                    reinterpret_cast<float2*>(ws + p.ml_at), reinterpret_cast<float*>(ws + p.o_at)};
+  const dim3 grid(static_cast<unsigned>(p.groups * kv_heads));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (p.step)
+    hipLaunchKernelGGL(step_kernel, grid, dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL(chunk_kernel<true>, grid, dim3(kChunkThreads), 0, st, a);
+    hipLaunchKernelGGL(chunk_kernel, grid, dim3(kChunkThreads), 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention");
-  hipLaunchKernelGGL(join_kernel, dim3(static_cast<unsigned>((all + kWaves - 1) / kWaves)), block, 0, st, a);
+  if (p.aim == 0) return FL_OK;
+  const unsigned items = static_cast<unsigned>(p.items * kv_heads);
+  if (p.step)
+    hipLaunchKernelGGL(join_kernel<kStepRows>, dim3(items, kStepRows / kWaves), dim3(kThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL(join_kernel<kChunkRows>, dim3(items, 16), dim3(kThreads), 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention(join)");
   return FL_OK;
 }
