@@ -284,20 +284,19 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, seq = blockIdx.x;
   const int used = a.beams * a.parts;
   const int64_t first = static_cast<int64_t>(seq) * used;
+  const int beam = lane / a.parts, part = lane - beam * a.parts;  // (parts: a power of two)
+  const bool any = beam < a.beams;
+  const PartHead head = any ? a.heads[first + lane] : PartHead{0.0, -INFINITY, 0};
+  const float score = any ? a.scores[seq * a.beams + beam] : 0.0f;
   for (int i = tid; i < used * a.count; i += kBeamThreads) lists[i] = a.lists[first * a.count + i];
   __syncthreads();
   if (tid >= kWave) return;
   // the beam's shift: score - logsumexp; -inf where it has no distribution or no finite score
-  const int beam = lane / a.parts, part = lane - beam * a.parts;
   double shift = -INFINITY;
-  const bool any = beam < a.beams;
-  const PartHead head = any ? a.heads[first + lane] : PartHead{0.0, -INFINITY, 0};
-  const float score = any ? a.scores[seq * a.beams + beam] : 0.0f;
   float top = head.shift;
-  for (int p = 0; p < a.parts; ++p) top = fmaxf(top, __shfl(head.shift, beam * a.parts + p, kWave));
-  const double mine = head.sum * scale_to(head.shift, top);
-  double s = 0.0;
-  for (int p = 0; p < a.parts; ++p) s += __shfl(mine, beam * a.parts + p, kWave);
+  for (int off = 1; off < a.parts; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+  double s = head.sum * scale_to(head.shift, top);
+  for (int off = 1; off < a.parts; off <<= 1) s += __shfl_xor(s, off, kWave);
   if (any && top > -INFINITY && s == s && fabsf(score) < INFINITY) shift = static_cast<double>(score) - (top + log(s));
   const bool dead = shift == -INFINITY;
   const int left = min(a.part_len, a.vocab - part * a.part_len);  // values of the part
@@ -344,7 +343,9 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
 int beam_parts(int64_t rows, int beams, int64_t vocab) {
   const int64_t least = (vocab + kBeamStep - 1) / kBeamStep, fill = (1024 + rows - 1) / rows;
   const int64_t parts = std::min<int64_t>(std::max(least, std::min<int64_t>(fill, (vocab + 1023) / 1024)), kLists / beams);
-  return static_cast<int>(std::max<int64_t>(1, parts));
+  int p = 1;  // (a power of two: a beam's parts are joined by exchanges)
+  while (2 * p <= parts) p *= 2;
+  return p;
 }
 
 }  // namespace

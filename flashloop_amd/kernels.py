@@ -8,6 +8,7 @@ flashloop/engine.py:346-498, flashloop/prefill.py:158-237).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from array import array
 
@@ -946,6 +947,7 @@ def mx_matmul(x: MXTensor, weight: MXTensor, *, out_dtype: torch.dtype = torch.b
 
 
 # ---------------------------------------------------------------------------- K/V pages and beams
+# (A decode step's calls take 3 to 12 us on the GPU, so their checks take each attribute once.)
 def _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, rows):
     """(pages, KV heads, page size, sequences, table width) of a call on K/V pages, checked."""
     device, shape = k_pages.device, k_pages.shape
@@ -955,31 +957,37 @@ def _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, rows):
         raise ValueError("k_pages and v_pages must be bfloat16 on one device")
     if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("k_pages and v_pages must be contiguous")
-    if page_table.ndim != 2 or kv_lens.ndim != 1 or kv_lens.shape[0] != page_table.shape[0]:
+    table_shape, lens_shape = page_table.shape, kv_lens.shape
+    if len(table_shape) != 2 or len(lens_shape) != 1 or lens_shape[0] != table_shape[0]:
         raise ValueError("page_table must be [sequences, pages of a sequence] and kv_lens [sequences]")
-    seqs, width = page_table.shape
-    for t, name in ((page_table, "page_table"), (kv_lens, "kv_lens"), (q_starts, "q_starts")):
-        if t is not None and (t.dtype is not torch.int32 or t.device != device or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous int32 on {device}")
+    seqs, width = table_shape
+    if not (page_table.dtype is torch.int32 and page_table.is_contiguous() and page_table.device == device):
+        raise ValueError(f"page_table must be contiguous int32 on {device}")
+    if not (kv_lens.dtype is torch.int32 and kv_lens.is_contiguous() and kv_lens.device == device):
+        raise ValueError(f"kv_lens must be contiguous int32 on {device}")
     if q_starts is None:
         if rows != seqs:
             raise ValueError(f"one row a sequence without q_starts: got {rows} rows and {seqs} sequences")
-    elif q_starts.ndim != 1 or q_starts.shape[0] != seqs + 1:
+    elif not (q_starts.dtype is torch.int32 and q_starts.is_contiguous() and q_starts.device == device):
+        raise ValueError(f"q_starts must be contiguous int32 on {device}")
+    elif q_starts.shape != (seqs + 1,):
         raise ValueError("q_starts must be [sequences + 1]")
     return shape[0], shape[1], shape[2], seqs, width
 
 
-def _head_rows(x: torch.Tensor, name: str, device) -> torch.Tensor:
-    """bf16 rows [n, heads * 128], at any distance that is a multiple of 8 values."""
-    if x.ndim != 2 or x.shape[1] == 0 or x.shape[1] % HEAD_DIM or x.dtype is not torch.bfloat16 or x.device != device:
+def _head_rows(x: torch.Tensor, name: str, device):
+    """(rows, their distance, their number, their width) of bf16 rows [n, heads * 128]: at any distance that is a multiple
+    of 8 values, else as contiguous ones."""
+    shape = x.shape
+    if len(shape) != 2 or x.dtype is not torch.bfloat16 or shape[1] == 0 or shape[1] % HEAD_DIM or x.device != device:
         raise ValueError(f"{name} must be bfloat16 [rows, heads * {HEAD_DIM}] on {device}")
-    if x.stride(1) != 1 or x.stride(0) % 8 or (x.stride(0) < x.shape[1] and x.shape[0] > 1) or x.data_ptr() % 16:
-        return x.contiguous()
-    return x
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    return max(x.stride(0), x.shape[1])
+    n, cols = shape
+    stride, step = x.stride()
+    if n == 1 and step == 1:
+        stride = cols  # (one row lies at no distance)
+    if step != 1 or stride % 8 or stride < cols or x.data_ptr() % 16:
+        return x.contiguous(), cols, n, cols
+    return x, stride, n, cols
 
 
 def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rope: tuple[torch.Tensor, torch.Tensor] | None,
@@ -993,41 +1001,57 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rope:
     the last tokens of sequence s (None: one row a sequence).  Returns the rotated rows of ``q``, in ``out``
     (``q`` itself, or rows that do not lie on it) if given; rows behind the last sequence as they are."""
     device = k_pages.device
-    k, v = _head_rows(k, "k", device), _head_rows(v, "v", device)
-    n = k.shape[0]
+    k, k_stride, n, cols = _head_rows(k, "k", device)
+    v, v_stride, n_v, cols_v = _head_rows(v, "v", device)
     pages, kv, page, seqs, width = _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, n)
-    if k.shape != v.shape or k.shape[1] != kv * HEAD_DIM:
+    if n_v != n or cols_v != cols or cols != kv * HEAD_DIM:
         raise ValueError(f"k and v must be [{n}, {kv * HEAD_DIM}], as the pages have {kv} heads")
-    heads, positions, f32, cos, sin, q_stride, out_stride = 1, 0, False, None, None, 0, 0
-    q2 = None
-    if rope is not None:
-        if q is None:
-            raise ValueError("rope tables without q")
-        cos, sin = rope
-        f32 = cos.dtype is torch.float32
-        if (cos.ndim != 2 or cos.shape[1] != HEAD_DIM or sin.shape != cos.shape or not (f32 or cos.dtype is torch.bfloat16)
-                or sin.dtype is not cos.dtype or cos.device != device or sin.device != device):
-            raise ValueError(f"rope tables must be bfloat16 or float32 [positions, {HEAD_DIM}] on {device}")
-        if not (cos.is_contiguous() and sin.is_contiguous()):
-            raise ValueError("rope tables must be contiguous")
-        q2 = _head_rows(q, "q", device)
-        if q2.shape[0] != n:
-            raise ValueError(f"q has {q2.shape[0]} rows, k {n}")
-        heads, positions, q_stride = q2.shape[1] // HEAD_DIM, cos.shape[0], _row_stride(q2)
-        if out is None:
-            out = q2.new_empty(q2.shape)
-        elif out.shape != q2.shape or out.dtype is not torch.bfloat16 or out.device != device or out.stride(1) != 1 or out.stride(0) % 8:
-            raise ValueError("out must be bfloat16 of the shape of q, on its device, with contiguous rows")
-        elif out.data_ptr() == q.data_ptr() and q2 is q and out.stride(0) != q.stride(0) and n > 1:
+    if rope is None:
+        if out is not None:
+            raise ValueError("without rope tables q is returned as it is: there is no out")
+        if n:
+            _launch(device, "fl_paged_append", load().fl_paged_append, None, 0, k.data_ptr(), k_stride, v.data_ptr(), v_stride, None, 0,
+                    None, None, False, 0, k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(),
+                    _p(q_starts), n, seqs, 1, kv, width, pages, page)
+        return q
+    if q is None:
+        raise ValueError("rope tables without q")
+    cos, sin = rope
+    table, dtype = cos.shape, cos.dtype
+    f32 = dtype is torch.float32
+    if (len(table) != 2 or table[1] != HEAD_DIM or sin.shape != table or not (f32 or dtype is torch.bfloat16)
+            or sin.dtype is not dtype or cos.device != device or sin.device != device):
+        raise ValueError(f"rope tables must be bfloat16 or float32 [positions, {HEAD_DIM}] on {device}")
+    if not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("rope tables must be contiguous")
+    q2, q_stride, n_q, q_cols = _head_rows(q, "q", device)
+    if n_q != n:
+        raise ValueError(f"q has {n_q} rows, k {n}")
+    if out is None:
+        out, out_stride = q2.new_empty((n, q_cols)), q_cols
+    else:
+        if out.shape != (n, q_cols) or out.dtype is not torch.bfloat16 or out.device != device or out.stride(1) != 1 or (
+                n > 1 and (out.stride(0) % 8 or out.stride(0) < q_cols)):
+            raise ValueError("out must be bfloat16 of the shape of q, on its device, with contiguous rows at a multiple of 8 values")
+        out_stride = out.stride(0) if n > 1 else q_cols
+        if out.data_ptr() == q.data_ptr() and q2 is q and out_stride != q_stride:
             raise ValueError("out lies on q with another row stride")
-        out_stride = _row_stride(out)
-    elif out is not None:
-        raise ValueError("without rope tables q is returned as it is: there is no out")
     if n:
-        _launch(device, "fl_paged_append", load().fl_paged_append, _p(q2), q_stride, k.data_ptr(), _row_stride(k), v.data_ptr(),
-                _row_stride(v), _p(out), out_stride, _p(cos), _p(sin), f32, positions, k_pages.data_ptr(), v_pages.data_ptr(),
-                page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, heads, kv, width, pages, page)
-    return q if rope is None else out
+        _launch(device, "fl_paged_append", load().fl_paged_append, q2.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(),
+                v_stride, out.data_ptr(), out_stride, cos.data_ptr(), sin.data_ptr(), f32, table[0], k_pages.data_ptr(),
+                v_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, q_cols // HEAD_DIM, kv, width,
+                pages, page)
+    return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(n: int, seqs: int, heads: int, kv: int, max_q: int, max_kv: int) -> int:
+    return load().fl_paged_attention_workspace(n, seqs, heads, kv, max_q, max_kv)
+
+
+@functools.lru_cache(maxsize=4096)
+def _select_workspace(seqs: int, beams: int, vocab: int, count: int) -> int:
+    return load().fl_beam_select_workspace(seqs, beams, vocab, count)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -1040,23 +1064,21 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table's capacity): they divide the work and have no part in the result.  Returns bf16 [n, H*128]: zeros for
     rows that see no key or belong to no sequence, NaN for rows that see a key without a page."""
     device = k_pages.device
-    q = _head_rows(q, "q", device)
-    n, cols = q.shape
+    q, q_stride, n, cols = _head_rows(q, "q", device)
     pages, kv, page, seqs, width = _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, n)
     heads = cols // HEAD_DIM
-    if heads % kv:
+    if not kv or heads % kv:
         raise ValueError(f"{heads} query heads do not share {kv} KV heads")
     out = q.new_empty((n, cols))
     if not n:
         return out
     max_q = 1 if q_starts is None else max(1, n if max_q is None else min(int(max_q), n))
     max_kv = max(1, width * page if max_kv is None else min(int(max_kv), width * page))
-    lib = load()
-    size = lib.fl_paged_attention_workspace(n, seqs, heads, kv, max_q, max_kv)
+    size = _attention_workspace(n, seqs, heads, kv, max_q, max_kv)
     ws = q.new_empty(size, dtype=torch.uint8) if size else None
-    _launch(device, "fl_paged_attention", lib.fl_paged_attention, q.data_ptr(), _row_stride(q), k_pages.data_ptr(),
-            v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, heads, kv, width,
-            pages, page, max_q, max_kv, scaling, _p(ws), size)
+    _launch(device, "fl_paged_attention", load().fl_paged_attention, q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(),
+            out.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(), _p(q_starts), n, seqs, heads, kv, width, pages, page, max_q,
+            max_kv, scaling, _p(ws), size)
     return out
 
 
@@ -1081,17 +1103,19 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int | None = 
         raise ValueError(f"1 to {MAX_BEAMS} beams, got {beams}")
     if not 1 <= count <= min(MAX_BEAMS, beams * vocab):
         raise ValueError(f"count must be 1..{min(MAX_BEAMS, beams * vocab)}, got {count}")
-    if logits.stride(1) != 1 or (logits.stride(0) < vocab and seqs * beams > 1):
-        logits = logits.contiguous()
+    row, step = logits.stride()
+    if seqs * beams <= 1:
+        row = vocab
+    if step != 1 or row < vocab:
+        logits, row = logits.contiguous(), vocab
     scores = scores if scores.is_contiguous() else scores.contiguous()
     out = (scores.new_empty((seqs, count)), scores.new_empty((seqs, count), dtype=torch.int32),
            scores.new_empty((seqs, count), dtype=torch.int64))
     if seqs:
-        lib = load()
-        size = lib.fl_beam_select_workspace(seqs, beams, vocab, count)
+        size = _select_workspace(seqs, beams, vocab, count)
         ws = scores.new_empty(size, dtype=torch.uint8)
-        _launch(device, "fl_beam_select", lib.fl_beam_select, logits.data_ptr(), f32, _row_stride(logits), scores.data_ptr(), seqs,
-                beams, vocab, count, *(t.data_ptr() for t in out), ws.data_ptr(), size)
+        _launch(device, "fl_beam_select", load().fl_beam_select, logits.data_ptr(), f32, row, scores.data_ptr(), seqs, beams, vocab,
+                count, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), size)
     return out
 
 
