@@ -25,7 +25,7 @@ constexpr int kChunks = 3;                            // chunks of a step
 constexpr int kBeamChunk = kBeamThreads * kPer;       // values of a workgroup's chunk
 constexpr int kBeamStep = kBeamChunk * kChunks;       // and step
 constexpr int kMaxCount = kWave;                      // one list entry a lane
-constexpr int kGathered = 512;                        // values that are placed by counting
+constexpr int kGathered = 128;                        // values of a wave that are placed by counting
 constexpr int kLists = kWave;                         // lists of a sequence (beams * parts), one a lane
 
 struct Entry {
@@ -112,11 +112,11 @@ __device__ __forceinline__ void load_values(const BeamArgs& a, int64_t row, int 
 
 template <bool F32, bool ALIGNED>
 __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
-  __shared__ Entry gathered[kMaxCount + kGathered];  // the largest of earlier steps, then this one's
+  __shared__ Entry gathered[kBeamWaves][kGathered], earlier[kMaxCount];  // this step's; the largest of those before
   __shared__ Entry best[kMaxCount];
   __shared__ float column[kBeamWaves][kWave];
   __shared__ PartHead heads[kBeamWaves];
-  __shared__ int found;
+  __shared__ int found[kBeamWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.parts;
   const int part = static_cast<int>(blockIdx.x - row * a.parts);
@@ -140,7 +140,6 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
         for (int e = 0; e < kPer; ++e) x[c][e] = -INFINITY;
       }
     }
-    if (tid == 0) found = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (base + c * kBeamChunk >= end) continue;
@@ -171,27 +170,36 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
     for (int j = 0; j < kWave; ++j) above += row_lane(mx, j) > mx ? 1 : 0;
     float reach = -wave_max(above < a.count ? -mx : -INFINITY);
     if (held == a.count) reach = fmaxf(reach, best[a.count - 1].value);
+    int mine_found = 0;  // (wave-uniform)
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       if (base + c * kBeamChunk >= end) continue;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int index = from + c * kBeamChunk + (e >> 2) * 4 * kWave + (e & 3);
-        const bool in = x[c][e] >= reach && index < end;
-        const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
-        if (who != 0ull) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(&found, __builtin_popcountll(who));
-          at = __builtin_amdgcn_readfirstlane(at) + __builtin_popcountll(who & ((1ull << lane) - 1));
-          if (in && at < kGathered) gathered[kMaxCount + at] = Entry{x[c][e], index};
+      for (int g = 0; g < kPer / 4; ++g) {  // (few groups of four values hold one that reaches it)
+        const float most = fmaxf(fmaxf(x[c][4 * g], x[c][4 * g + 1]), fmaxf(x[c][4 * g + 2], x[c][4 * g + 3]));
+        if (__builtin_amdgcn_ballot_w64(most >= reach) == 0ull) continue;
+#pragma unroll
+        for (int e = 4 * g; e < 4 * g + 4; ++e) {
+          const int index = from + c * kBeamChunk + g * 4 * kWave + (e & 3);
+          const bool in = x[c][e] >= reach && index < end;
+          const unsigned long long who = __builtin_amdgcn_ballot_w64(in);
+          const int at = mine_found + __builtin_popcountll(who & ((1ull << lane) - 1));
+          if (in && at < kGathered) gathered[wave][at] = Entry{x[c][e], index};
+          mine_found += __builtin_popcountll(who);
         }
       }
     }
-    if (tid < held) gathered[tid] = best[tid];
+    if (lane == 0) found[wave] = mine_found;
+    if (tid < held) earlier[tid] = best[tid];
     __syncthreads();
-    int fresh = found;
-    if (fresh > kGathered) {  // a sorted list a wave, entry `lane`, largest first
-      __syncthreads();        // (every wave has read `found`, and none writes to the list before)
+    int count[kBeamWaves], total = held, most = 0;
+#pragma unroll
+    for (int w = 0; w < kBeamWaves; ++w) {
+      count[w] = __builtin_amdgcn_readfirstlane(found[w]);
+      most = max(most, count[w]);
+    }
+    if (most > kGathered) {  // a sorted list a wave, entry `lane`, largest first
+      __syncthreads();       // (every wave has read the counts)
       float lv = -INFINITY, last_v = -INFINITY;
       int li = 0x7FFFFFFF, last_i = 0x7FFFFFFF;  // last: entry count - 1
 #pragma unroll
@@ -218,19 +226,28 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
         }
       }
       // (entries that no value took come last: their index is no value's)
-      gathered[kMaxCount + tid] = Entry{lv, li < 0x7FFFFFFF ? li : 0x7FFFFF00 + tid};
-      fresh = kBeamThreads;
+      gathered[wave][lane] = Entry{lv, li < 0x7FFFFFFF ? li : 0x7FFFFF00 + tid};
+#pragma unroll
+      for (int w = 0; w < kBeamWaves; ++w) count[w] = kWave;
       __syncthreads();
     }
     // an entry's place is the number of entries before it
-    const int total = held + fresh;
-    for (int i = tid; i < total; i += kBeamThreads) {
-      const Entry one = gathered[i < held ? i : kMaxCount + i - held];
+    const auto put = [&](Entry one) __attribute__((always_inline)) {
       int place = 0;
-      for (int j = 0; j < held; ++j) place += before(gathered[j].value, gathered[j].index, one.value, one.index) ? 1 : 0;
-      for (int j = 0; j < fresh; ++j)
-        place += before(gathered[kMaxCount + j].value, gathered[kMaxCount + j].index, one.value, one.index) ? 1 : 0;
+#pragma unroll 4
+      for (int j = 0; j < held; ++j) place += before(earlier[j].value, earlier[j].index, one.value, one.index) ? 1 : 0;
+#pragma unroll
+      for (int w = 0; w < kBeamWaves; ++w)
+#pragma unroll 4
+        for (int j = 0; j < count[w]; ++j) place += before(gathered[w][j].value, gathered[w][j].index, one.value, one.index) ? 1 : 0;
       if (place < a.count) best[place] = one;
+    };
+    if (tid < held) put(earlier[tid]);
+#pragma unroll
+    for (int w = 0; w < kBeamWaves; ++w) {
+      if (w == wave)
+        for (int i = lane; i < count[w]; i += kWave) put(gathered[w][i]);
+      total += count[w];
     }
     held = min(a.count, total);
     __syncthreads();
@@ -305,15 +322,13 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   float value = 0.0f;
   unsigned long long key = 0ull;  // of the list's next candidate; 0: none is left
   double total = 0.0;
+  Entry ahead = lists[lane * a.count];  // the entry that comes next (read while others win)
   const auto look = [&]() __attribute__((always_inline)) {
-    key = 0ull;
-    if (at < held) {
-      const Entry e = lists[lane * a.count + at];
-      token = dead ? at : e.index;  // (equal totals: the tokens in order)
-      value = dead ? 0.0f : e.value;
-      total = dead ? -INFINITY : shift + static_cast<double>(e.value);
-      key = image(total);
-    }
+    token = dead ? at : ahead.index;  // (equal totals: the tokens in order)
+    value = dead ? 0.0f : ahead.value;
+    total = dead ? -INFINITY : shift + static_cast<double>(ahead.value);
+    key = at < held ? image(total) : 0ull;
+    ahead = lists[lane * a.count + min(at + 1, a.count - 1)];
   };
   look();
   for (int n = 0; n < a.count; ++n) {
