@@ -135,7 +135,7 @@ __device__ __forceinline__ int scan_lanes(int v, int lane) {  // sum over the la
 }
 
 // index: this workgroup's number for its KV head.  ONE: items of more than ROWS queries are one, and never divided.
-template <int ROWS, int UNIT, int LEAST, bool ONE, bool FIT>
+template <int ROWS, int UNIT, int LEAST, bool ONE, bool SORT>
 __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int index, Work& w) {
   const int lane = threadIdx.x & 63;
   const auto look = [&](int s, int& items, int& steps, bool& whole) __attribute__((always_inline)) {
@@ -151,22 +151,36 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int inde
   look(lane, items, steps, whole);
   int most = 1 << 30;  // T
   if (a.aim > 0) {
-    float sum = wave_sum(static_cast<float>(items) * static_cast<float>(steps)), count = wave_sum(static_cast<float>(items));
+    float sum = wave_sum(static_cast<float>(items) * static_cast<float>(steps));
     for (int base = kWave; base < a.seqs; base += kWave) {
       int its, sts;
       bool all;
       look(base + lane, its, sts, all);
       sum += wave_sum(static_cast<float>(its) * static_cast<float>(sts));
-      count += wave_sum(static_cast<float>(its));
     }
     most = max(LEAST, static_cast<int>(fminf(ceilf(sum * a.kv / a.aim), 1e9f)));
-    // one round of workgroups, if there can be: ranges a little longer rather than some in a second round
-    if (FIT && a.seqs <= kWave && count * a.kv <= a.aim)
-      for (int i = 0; i < 24; ++i) {
-        const int groups = items * (whole ? 1 : min(max(1, (steps + most - 1) / most), a.ranges));
-        if (wave_sum(static_cast<float>(groups)) * a.kv <= a.aim) break;
-        most += max(1, most / 16);
-      }
+    if (SORT && a.seqs == 1) {  // one round of workgroups, if there can be: all ranges are alike
+      const int one = __builtin_amdgcn_readlane(items, 0), all = __builtin_amdgcn_readlane(steps, 0);
+      const int each = min(a.aim / max(one * a.kv, 1), a.ranges);
+      if (each > 0) most = max(LEAST, (all + each - 1) / each);
+    }
+  }
+  // The longest ranges first: lane l looks at sequence `seq`, the l-th by its ranges' length.  (More sequences than lanes
+  // stay as they are.)
+  int seq = lane;
+  if (SORT && a.aim > 0 && a.seqs > 1 && a.seqs <= kWave) {
+    const int cuts = max(1, (steps + most - 1) / most), each = items > 0 ? (steps + cuts - 1) / cuts : -1;
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < kWave; ++j) {
+      const int other = __builtin_amdgcn_readlane(each, j);
+      rank += other > each || (other == each && j < lane) ? 1 : 0;
+    }
+    const auto sorted = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_ds_permute(4 * rank, v); };
+    items = sorted(items);
+    steps = sorted(steps);
+    whole = sorted(whole ? 1 : 0) != 0;
+    seq = sorted(lane);
   }
   w.seq = -1;
   w.total = 0;
@@ -180,7 +194,7 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int inde
     if (w.seq < 0 && past != 0ull) {
       const int l = __builtin_ctzll(past);
       const int its = __builtin_amdgcn_readlane(items, l);
-      w.seq = base + l;
+      w.seq = base > 0 ? base + l : __builtin_amdgcn_readlane(seq, l);
       w.ranges = __builtin_amdgcn_readlane(ranges, l);
       const int local = index - (__builtin_amdgcn_readlane(to, l) - its * w.ranges);
       const int nth = local / w.ranges;  // (the last items first: they see more keys)
