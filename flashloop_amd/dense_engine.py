@@ -103,8 +103,11 @@ class DenseEngine:
         hidden = bb.norm.weight.numel()
         if hidden % 8 or hidden > 8192 or any(l.mlp.up_proj.weight.shape[0] % 8 for l in bb.layers):
             raise ValueError("DenseEngine needs a hidden width (up to 8192) and an MLP width that are multiples of 8")
-        if not _is_plain(bb.embed_tokens, torch.nn.Embedding) or not _is_plain(bb.rotary_emb, RotaryEmbedding):
-            raise ValueError("DenseEngine needs plain embedding and rotary modules")
+        emb, rot = bb.embed_tokens, bb.rotary_emb
+        if (not _is_plain(emb, torch.nn.Embedding) or not _is_plain(rot, RotaryEmbedding) or emb.max_norm is not None
+                or emb.weight.dtype != torch.bfloat16 or not emb.weight.is_contiguous() or emb.weight.data_ptr() % 16
+                or rot.inv_freq.dtype not in (torch.float32, torch.bfloat16)):
+            raise ValueError("DenseEngine needs plain embedding (bf16) and rotary modules")
         layers = []
         for layer in bb.layers:
             a, m = layer.self_attn, layer.mlp
@@ -129,7 +132,7 @@ class DenseEngine:
     def _release(self) -> None:
         if getattr(self, "_graph", None) is not None:
             self._graph.reset()
-        self._graph = self._tok = self._out = None
+        self._graph = self._tok = self._pos = self._out = None
 
     @property
     def positions(self) -> tuple[int, ...]:
@@ -160,16 +163,20 @@ class DenseEngine:
             hid, z = kernels.norm_chain(hid, x=y, w_a=w[10], w_f=final, w_b=nxt, eps=eps)
         return hid
 
-    def _step(self, hid: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-        """One token a sequence, at position lens - 1: logits into ``out``.  Up to 8 sequences of one KV head a query head
+    def _step(self, out: torch.Tensor) -> torch.Tensor:
+        """One token a sequence, at its next position: logits into ``out``.  Up to 8 sequences of one KV head a query head
         run on the fused GEMVs (norms, rotation and SwiGLU within them), as ``FlashLoopEngine``'s steps do."""
         c, (layers, _, head, eps) = self.cache, self._weights
-        rows = hid.shape[0]
+        c.lens.add_(1)
+        self._pos.add_(1)
+        bb = self.model.model
+        h, cos, sin = kernels.decode_inputs(self._tok, self._pos, bb.embed_tokens.weight, bb.rotary_emb.inv_freq)
+        rows = h.shape[0]
+        hid, rope = h.view(rows, -1), (cos.view(rows, -1), sin.view(rows, -1))
         cfg = self.config
         if rows > 8 or cfg.num_attention_heads != cfg.num_key_value_heads or hid.shape[1] > 4096:
             h = self._rows(hid, c.table, c.lens, None, 1, c.capacity)
             return out.copy_(F.linear(h, head))
-        rope = tuple(t.index_select(0, (c.lens - 1).clamp(min=0)) for t in self._rope)
         pending = dict(w_b=layers[0][7], want_h=False)
         for slot, w, nxt, final in self._layers():
             h, (q, k, v) = kernels.gemv_chain(hid, list(w[:3]), eps=eps, epilogue=kernels.EPI_ROPE, rope=rope, **pending)
@@ -225,8 +232,13 @@ class DenseEngine:
             if ends:
                 last[ends] = h[[starts[i + 1] - 1 for i in ends]]
             done = [d + r for d, r in zip(done, step)]
-        c.lens.copy_(torch.tensor(self._lens, dtype=torch.int32))
+        self._lengths_to_device()
         return F.linear(last, self._weights[2]).float()
+
+    def _lengths_to_device(self) -> None:
+        self.cache.lens.copy_(torch.tensor(self._lens, dtype=torch.int32))
+        if self._pos is not None:
+            self._pos.copy_(torch.tensor(self._lens)[:, None] - 1)
 
     def _begin(self, input_ids: torch.Tensor, counts: list[int], extra: int, beams: int) -> None:
         capacity = max(counts) + int(extra)
@@ -283,7 +295,8 @@ class DenseEngine:
     @torch.inference_mode()
     def decode(self, token_ids: torch.Tensor) -> DenseOutput:
         """One token for every sequence: ``token_ids`` [B, 1].  With graphs on, the returned logits live in the graph's
-        output buffer until the next step."""
+        output buffer until the next step.  A token outside the vocabulary gives its sequence NaN logits and rows
+        (``FlashLoopEngine.decode``)."""
         self._need()
         rows = len(self._lens)
         if tuple(token_ids.shape) != (rows, 1):
@@ -292,40 +305,35 @@ class DenseEngine:
         c = self.cache
         if self._out is None:
             self._out = torch.empty(rows, self.config.vocab_size, dtype=torch.float32, device=c.lens.device)
-            self._tok = torch.zeros(rows, dtype=torch.long, device=c.lens.device)
-        self._tok.copy_(token_ids[:, 0])
+            self._tok = torch.zeros(rows, 1, dtype=torch.long, device=c.lens.device)
+            self._pos = (c.lens - 1).long()[:, None]  # (of the last token: a step writes the next)
+        self._tok.copy_(token_ids)
         if self.use_graphs:
             if self._graph is None:
                 self._capture()
             self._graph.replay()
             logits = self._out
         else:
-            c.lens.add_(1)
-            logits = self._step(self.model.model.embed_tokens(self._tok), torch.empty_like(self._out))
+            logits = self._step(torch.empty_like(self._out))
         self._lens = [t + 1 for t in self._lens]
         return DenseOutput(logits, self.positions)
 
     def _capture(self) -> None:
         """Capture a step (lengths live on the device).  A warm-up on a side stream sizes workspaces and library
         handles; it writes the rows that the replay writes again."""
-        c, embed = self.cache, self.model.model.embed_tokens
-
-        def step():
-            c.lens.add_(1)
-            self._step(embed(self._tok), self._out)
-
         side = torch.cuda.Stream()  # default priority
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
-            step()
-            c.lens.sub_(1)
+            self._step(self._out)
+            self.cache.lens.sub_(1)
+            self._pos.sub_(1)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         was_enabled = gc.isenabled()
         gc.disable()  # (a graph destroyed by a collection during a capture aborts the process)
         try:
             with torch.cuda.graph(graph):
-                step()
+                self._step(self._out)
         finally:
             if was_enabled:
                 gc.enable()
@@ -381,7 +389,7 @@ class DenseEngine:
         self._begin(input_ids, counts, new, k)
         logits = self._feed(input_ids, counts, [b * k for b in range(bsz)]).repeat_interleave(k, dim=0)
         self._lens = [n for n in counts for _ in range(k)]
-        self.cache.lens.copy_(torch.tensor(self._lens, dtype=torch.int32))
+        self._lengths_to_device()
         scores = torch.full((bsz, k), -torch.inf, device=dev)  # (the beams are one until they part)
         scores[:, 0] = 0.0
         history = torch.zeros(bsz, k, new, dtype=torch.long, device=dev)

@@ -91,6 +91,22 @@ def test_many_sequences_and_graphs():
         assert engines[0].cache.lens.tolist() == [n + 66 for n in lengths] == list(engines[0].positions)
 
 
+def test_tokens_outside_the_vocabulary():
+    """NaN for its sequence, nothing for the others (captured and eager)."""
+    print("case: dense engine odd tokens", flush=True)
+    model = OuroForCausalLM.random_init(TINY, seed=3, device="cuda")
+    ids, mask = _ids([9, 20], extra=3)
+    for graphs in (True, False):
+        a, b = (DenseEngine(model, use_graphs=graphs) for _ in range(2))
+        for e in (a, b):
+            e.prefill(ids[:, :20], mask)
+        good = a.decode(ids[:, 20:21]).logits.clone()
+        bad = ids[:, 20:21].clone()
+        bad[0, 0] = TINY.vocab_size
+        got = b.decode(bad).logits
+        assert got[0].isnan().all() and torch.equal(got[1], good[1])
+
+
 def test_greedy_generation():
     print("case: dense engine greedy", flush=True)
     model = OuroForCausalLM.random_init(TINY, seed=4, device="cuda")

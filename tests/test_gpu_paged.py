@@ -83,6 +83,57 @@ def test_many_rows_in_one_call():
         assert attention_error(got, want, size, slack) <= 0
 
 
+@pytest.mark.parametrize("rows,kv,step", [(1, 1, 97), (2, 3, 41), (30, 1, 57), (300, 2, 31)])
+def test_many_sequences_of_unequal_lengths(rows, kv, step):
+    """More sequences than a wave has lanes (and fewer), keys divided by each sequence's own length."""
+    for seqs in (70, 9):
+        print(f"case: unequal lengths {rows} {kv} {seqs}", flush=True)
+        counts = [rows if s % 4 else 1 for s in range(seqs)]
+        lens = [r + (s * s * step) % 4001 if s % 3 else r + s % 5 for s, r in enumerate(counts)]
+        got, want, size, slack = _attend(10, counts, lens, 2 * kv, kv, 32)
+        assert attention_error(got, want, size, slack) <= 0
+
+
+def test_hints_have_no_part_in_the_result():
+    """max_q and max_kv that are too small or too large, and a call on one sequence of a batch."""
+    print("case: hints", flush=True)
+    g = _gen(11)
+    lens, rows = [2000, 37, 900], [40, 2, 1]
+    starts = _starts(rows)
+    (kp, vp), table, (keys, values) = make_pool(g, lens, 130, 16, 2, DEV)
+    q = torch.randn(starts[-1], 4, DIM, generator=g, device=DEV).bfloat16()
+    want = plain_attention(q, keys, values, lens, starts, SCALING)
+    for max_q, max_kv in ((1, 1), (1, 4000), (40, 1), (4000, 100_000), (3, 130), (None, None)):
+        got = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, _ints(starts), max_q=max_q, max_kv=max_kv)
+        assert attention_error(got, *want) <= 0, (max_q, max_kv)
+    one = kernels.paged_attention(q.flatten(1)[:40], kp, vp, table[:1].contiguous(), _ints(lens[:1]), SCALING, _ints([0, 40]))
+    assert attention_error(one, *(t[:40] for t in want)) <= 0
+
+
+@pytest.mark.parametrize("rows,before", [(1, 0), (2, 500), (100, 3000), (700, 100)])
+def test_two_calls_at_once(rows, before):
+    """Calls whose workspaces are theirs alone: the same on two streams at a time as one after the other."""
+    print(f"case: two calls at once {rows} {before}", flush=True)
+    g = _gen(12)
+    lens = [rows + before, rows + before // 2]
+    starts = _ints(_starts([rows, rows]))
+    sets = []
+    for _ in range(2):
+        (kp, vp), table, _ = make_pool(g, lens, 240, 16, 2, DEV)
+        sets.append((torch.randn(2 * rows, 4 * DIM, generator=g, device=DEV).bfloat16(), kp, vp, table, _ints(lens), SCALING, starts))
+    want = [kernels.paged_attention(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(kernels.paged_attention(*sets[i]))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w) for o in outs)
+
+
 @pytest.mark.parametrize("rows", [[3], [20, 3], [140]])
 def test_rows_before_the_first_key(rows):
     """A sequence shorter than its rows: the rows before its first key are zeros, the others see what there is."""
