@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   const auto look = [&]() __attribute__((always_inline)) {
     token = dead ? at : ahead.index;  // (equal totals: the tokens in order)
     value = dead ? 0.0f : ahead.value;
-    total = dead ? -INFINITY : shift + static_cast<double>(ahead.value);
+    total = dead ? -INFINITY : shift + static_cast<double>(ahead.value) + 0.0;  // (-0 becomes 0: they are equal, their images not)
     key = at < held ? image(total) : 0ull;
     ahead = lists[lane * a.count + min(at + 1, a.count - 1)];
   };

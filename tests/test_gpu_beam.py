@@ -82,6 +82,16 @@ def test_select_dead_beams_and_masked_tokens():
                     _check(x, s, count, (vocab, scores, name, count))
 
 
+def test_select_zeros_of_both_signs():
+    """-0 and 0 are equal: the lower beam and token come first."""
+    print("case: select zeros", flush=True)
+    inf = torch.inf
+    for first, score in ((-0.0, -0.0), (0.0, -0.0), (-0.0, 0.0)):
+        logits = torch.tensor([[first, -inf], [0.0, -inf]], device=DEV)
+        _check(logits, torch.tensor([[score, 0.0]], device=DEV), 4, (first, score))
+        _check(torch.tensor([[first], [0.0]], device=DEV), torch.tensor([[score, 0.0]], device=DEV), 2, (first, score, "one"))
+
+
 def test_select_layouts_streams_and_graphs():
     """Rows of a wider matrix at odd distances, another stream, replays over new logits."""
     print("case: select layouts", flush=True)
