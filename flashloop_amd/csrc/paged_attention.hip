@@ -184,7 +184,7 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int inde
   }
   w.seq = -1;
   w.total = 0;
-  int slots = 0, divided = 0;
+  int slots = 0, divided = 0, listed = 0;  // listed: divided items that all have their room and their workgroups
   for (int base = 0; base < a.seqs; base += kWave) {
     if (base > 0) look(base + lane, items, steps, whole);
     const int ranges = whole ? 1 : min(max(1, (steps + most - 1) / most), a.ranges);
@@ -212,11 +212,14 @@ __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int inde
       }
       if (index != 0) return true;
     }
+    // (all of them, unless the rows of q_starts overlap: the join must not read what no workgroup wrote)
+    const unsigned long long fit = __builtin_amdgcn_ballot_w64(slots_to <= a.slots && static_cast<int64_t>(to) * a.kv <= gridDim.x);
+    if (fit != 0ull) listed = __builtin_amdgcn_readlane(split_to, kWave - 1 - __builtin_clzll(fit));
     w.total = __builtin_amdgcn_readlane(to, kWave - 1);
     slots = __builtin_amdgcn_readlane(slots_to, kWave - 1);
     divided = __builtin_amdgcn_readlane(split_to, kWave - 1);
   }
-  if (a.aim > 0 && head == 0 && index == 0 && threadIdx.x == 0) *a.divided = min(divided, a.items);
+  if (a.aim > 0 && head == 0 && index == 0 && threadIdx.x == 0) *a.divided = min(listed, a.items);
   return w.seq >= 0;
 }
 

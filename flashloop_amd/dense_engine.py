@@ -426,8 +426,6 @@ class DenseEngine:
                 break
             self.cache.reorder(torch.gather(parents, 1, order).contiguous())
             logits = self.decode(torch.gather(tokens, 1, order).view(-1, 1)).logits
-        else:
-            step = new - 1
         if step + 1 == new:
             keep(scores[:, 0] / new**penalty, history[:, 0], torch.full_like(best_len, new))
         return [torch.cat([input_ids[b, :n], best_tokens[b, : int(l)]]) for b, (n, l) in enumerate(zip(counts, best_len.tolist()))]

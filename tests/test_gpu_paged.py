@@ -110,6 +110,23 @@ def test_hints_have_no_part_in_the_result():
     assert attention_error(one, *(t[:40] for t in want)) <= 0
 
 
+def test_starts_that_overlap():
+    """q_starts that fall: what the rows then hold is not specified, but only they are written, and only what was
+    written is joined (more tiles than the launch has, the divided ones the last)."""
+    print("case: starts that overlap", flush=True)
+    g = _gen(13)
+    n, seqs = 2000, 66
+    lens = [100] * (seqs - 2) + [3000, 1]
+    (kp, vp), table, _ = make_pool(g, lens, 190, 16, 2, DEV)
+    q = torch.randn(n, 4 * DIM, generator=g, device=DEV).bfloat16()
+    starts = _ints([0, n] * (seqs // 2) + [0])
+    held = [kp.clone(), vp.clone()]
+    got = kernels.paged_attention(q, kp, vp, table, _ints(lens), SCALING, starts, max_q=n, max_kv=500)
+    torch.cuda.synchronize()
+    assert got.shape == q.shape
+    assert torch.equal(kp.view(torch.int16), held[0].view(torch.int16)) and torch.equal(vp.view(torch.int16), held[1].view(torch.int16))
+
+
 @pytest.mark.parametrize("rows,before", [(1, 0), (2, 500), (100, 3000), (700, 100)])
 def test_two_calls_at_once(rows, before):
     """Calls whose workspaces are theirs alone: the same on two streams at a time as one after the other."""
