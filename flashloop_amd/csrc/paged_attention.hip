@@ -3,12 +3,16 @@
 // sees the keys up to its own position; the query heads of a group share one KV head, so a group's rows
 // (token i, head g of the group: row i * group + g) are the queries of that head's keys.
 //
-//  * chunk_kernel: the tiles of attention.hip (128 queries a workgroup, 64 keys a step through LDS, S^T and
-//    O^T on v_mfma_f32_32x32x16_bf16), the rows' sequence found by a scan of the sequences' tile counts.
+//  * chunk_kernel: chunks of new tokens.  A workgroup has 256 queries in eight waves, one workgroup a CU; S^T and O^T on
+//    v_mfma_f32_32x32x16_bf16, 64 keys a step, K and V through a ring of four tiles in LDS that transfers without registers
+//    fill.  A long prompt (8192 tokens, 16 heads) 259-265 us: 1040 TFLOP/s of the causal half, matrix cores busy 49%.  On the
+//    same transfers with no arithmetic between the products it runs at 1550 TFLOP/s of those it has (the card's power sets that
+//    rate); the rest are the exponentials and the roundings to bf16 in the products' shadow, one behind the other in a wave.
 //  * step_kernel: few queries a sequence (one decode step).  A wave owns steps of 32 keys and up to 16
 //    queries on v_mfma_f32_16x16x32_bf16: K goes from memory into the first product's operand, V through a
-//    part of LDS of the wave's own, the next step's loads in flight, no barrier until the waves' join.
-//  * merge_kernel joins the key ranges where a launch divides them.
+//    part of LDS of the wave's own, the next step's loads in flight, no barrier until the waves' join.  Bound by bytes: 32
+//    sequences of up to 8192 tokens, 16 heads, 183 us, 5.6 TB/s.  One sequence of 2048 tokens takes 8 us, five memory latencies.
+//  * join_kernel and join_slices_kernel join the parts where a launch divides keys.
 //
 // A key that a row does not see has no part in its result, whatever its K and V rows hold: scores are
 // replaced, V rows past a sequence's end are zeroed, and where some row of a tile does not see a key, the
@@ -31,9 +35,10 @@ constexpr int kChunkRows = 32 * kChunkWaves;  // its queries
 constexpr int kStepKeys = 32;            // keys of a wave's step in step_kernel
 constexpr int kStepRows = 16;            // its queries
 constexpr int kMaxRanges = kWave;        // ranges of an item's keys: the join has one a lane
-// Workgroups that a call aims at, and the least steps of a range
-constexpr int kStepAim = 1024, kStepLeast = kWaves;
-constexpr int kChunkAim = 256, kChunkLeast = 7;  // (one a CU)
+// Workgroups that a call aims at
+constexpr int kStepAim = 1024;
+constexpr int kChunkAim = 256;          // (one a CU: its LDS is theirs)
+constexpr int kStepLeast = kWaves;      // least steps of a range in step_kernel
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -55,9 +60,10 @@ struct PagedArgs {
   const int32_t* starts; // [seqs + 1], or null: row s is sequence s's
   int n, seqs, heads, kv, group, width, pages, page_log2;
   float scale;  // scaling * log2(e)
-  // Key ranges (Work): workgroups aimed at, or 0: every item is one; and the workspace for their outputs
+  // Divided keys.  aim: step_kernel's workgroups aimed at, chunk_kernel's slices a KV head; 0: nothing is divided.  And the
+  // workspace for their outputs
   int aim, ranges, slots, items;  // ranges of an item at most; ranges' outputs a KV head and divided items that there is room for
-  int32_t* divided;       // number of divided items
+  int32_t* divided;       // number of divided items (step_kernel)
   struct Divided* list;   // [items]
   float2* part_ml;        // [kv][slots][rows of an item]: maximum of q.k (kUnseen: no key) and sum
   float* part_o;          // [kv][slots][rows of an item][128]
@@ -112,123 +118,96 @@ __device__ __forceinline__ Pages pages_of(const PagedArgs& a, int s, int head, i
   return p;
 }
 
-// A workgroup's work.  An item is up to ROWS queries of a sequence, against its keys in UNIT-key steps; where the
-// items are too few for the chip, or too unequal, a sequence's are divided into ranges of about T steps, T such that the
-// call makes about `aim` workgroups.  Every workgroup finds this out for itself, sequences in lanes: the lengths are on
-// the device alone.  Since a divided item has more than T steps, there are at most 2 aim / kv ranges of divided ones.
-struct Work {
-  int seq, item, range, ranges;
-  int slot;     // of its first range's output (ranges > 1)
-  int total;    // workgroups that have work, a KV head
-};
+__device__ __forceinline__ int items_of(const PagedArgs& a, int rows, int each) { return (rows * a.group + each - 1) / each; }
 
-template <int ROWS>
-__device__ __forceinline__ int items_of(const PagedArgs& a, int rows) { return (rows * a.group + ROWS - 1) / ROWS; }
-
-__device__ __forceinline__ int scan_lanes(int v, int lane) {  // sum over the lanes up to this one
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const int u = __shfl_up(v, off, kWave);
-    v += lane >= off ? u : 0;
-  }
-  return v;
+// The keys of a sequence that its table row can name.
+__device__ __forceinline__ int keys_of(const PagedArgs& a, int len) {
+  return static_cast<int>(min(static_cast<int64_t>(max(len, 0)), static_cast<int64_t>(a.width) << a.page_log2));
 }
 
-// index: this workgroup's number for its KV head.  ONE: items of more than ROWS queries are one, and never divided.
-template <int ROWS, int UNIT, int LEAST, bool ONE, bool SORT>
+// v of the lane that CTRL names, in the rows of 16 lanes of MASK; elsewhere 0
+template <int CTRL, int MASK>
+__device__ __forceinline__ int from_lane(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, MASK, 0xF, false); }
+template <int CTRL, int MASK>
+__device__ __forceinline__ double from_lane(double v) {
+  const int64_t u = __double_as_longlong(v);
+  const int lo = from_lane<CTRL, MASK>(static_cast<int>(u)), hi = from_lane<CTRL, MASK>(static_cast<int>(u >> 32));
+  return __longlong_as_double((static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo));
+}
+// sum over the lanes up to this one: within rows of 16, then with the rows before
+template <class T>
+__device__ __forceinline__ T scan_lanes(T v) {
+  v += from_lane<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+  v += from_lane<0x112, 0xF>(v);
+  v += from_lane<0x114, 0xF>(v);
+  v += from_lane<0x118, 0xF>(v);
+  v += from_lane<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return v + from_lane<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+}
+
+// step_kernel's work.  An item is a sequence with up to 16 queries, against its keys in steps; where the items are too few
+// for the chip, or too unequal, a sequence's are divided into ranges of about T steps, T such that the call makes about `aim`
+// workgroups.  Every workgroup finds this out for itself, sequences in lanes: the lengths are on the device alone.  Since
+// a divided item has more than T steps, there are at most 2 aim / kv ranges of divided ones.
+struct Work {
+  int seq, range, ranges;
+  int slot;  // of its first range's output (ranges > 1)
+};
+
+// index: this workgroup's number for its KV head.  (Sequences of more than 16 queries are never divided.)
 __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int index, Work& w) {
   const int lane = threadIdx.x & 63;
   const auto look = [&](int s, int& items, int& steps, bool& whole) __attribute__((always_inline)) {
     const int2 rows = s < a.seqs ? rows_of(a, s) : make_int2(0, 0);
-    const int64_t keys = s < a.seqs ? min(static_cast<int64_t>(max(a.lens[s], 0)), static_cast<int64_t>(a.width) << a.page_log2) : 0;
-    items = items_of<ROWS>(a, rows.y);
-    whole = ONE && items > 1;
-    if (ONE) items = min(items, 1);
-    steps = static_cast<int>((keys + UNIT - 1) / UNIT);
+    const int keys = s < a.seqs ? keys_of(a, a.lens[s]) : 0;
+    items = min(rows.y, 1);
+    whole = items_of(a, rows.y, kStepRows) > 1;
+    steps = (keys + kStepKeys - 1) / kStepKeys;
   };
   int items, steps;
   bool whole;
   look(lane, items, steps, whole);
-  int most = 1 << 30;  // T
-  if (a.aim > 0) {
-    float sum = wave_sum(static_cast<float>(items) * static_cast<float>(steps));
-    for (int base = kWave; base < a.seqs; base += kWave) {
-      int its, sts;
-      bool all;
-      look(base + lane, its, sts, all);
-      sum += wave_sum(static_cast<float>(its) * static_cast<float>(sts));
-    }
-    most = max(LEAST, static_cast<int>(fminf(ceilf(sum * a.kv / a.aim), 1e9f)));
-    if (SORT && a.seqs == 1) {  // one round of workgroups, if there can be: all ranges are alike
-      const int one = __builtin_amdgcn_readlane(items, 0), all = __builtin_amdgcn_readlane(steps, 0);
-      const int each = min(a.aim / max(one * a.kv, 1), a.ranges);
-      if (each > 0) most = max(LEAST, (all + each - 1) / each);
-    }
+  float sum = wave_sum(static_cast<float>(items) * static_cast<float>(steps));
+  for (int base = kWave; base < a.seqs; base += kWave) {
+    int its, sts;
+    bool all;
+    look(base + lane, its, sts, all);
+    sum += wave_sum(static_cast<float>(its) * static_cast<float>(sts));
   }
-  // The longest ranges first: lane l looks at sequence `seq`, the l-th by its ranges' length.  (More sequences than lanes
-  // stay as they are.)
-  int seq = lane;
-  if (SORT && a.aim > 0 && a.seqs > 1 && a.seqs <= kWave) {
-    const int cuts = max(1, (steps + most - 1) / most), each = items > 0 ? (steps + cuts - 1) / cuts : -1;
-    int rank = 0;
-#pragma unroll
-    for (int j = 0; j < kWave; ++j) {
-      const int other = __builtin_amdgcn_readlane(each, j);
-      rank += other > each || (other == each && j < lane) ? 1 : 0;
-    }
-    const auto sorted = [&](int v) __attribute__((always_inline)) { return __builtin_amdgcn_ds_permute(4 * rank, v); };
-    items = sorted(items);
-    steps = sorted(steps);
-    whole = sorted(whole ? 1 : 0) != 0;
-    seq = sorted(lane);
-  }
+  const int most = max(kStepLeast, static_cast<int>(fminf(ceilf(sum * a.kv / a.aim), 1e9f)));  // T
   w.seq = -1;
-  w.total = 0;
-  int slots = 0, divided = 0, listed = 0;  // listed: divided items that all have their room and their workgroups
+  int total = 0, slots = 0, divided = 0;
   for (int base = 0; base < a.seqs; base += kWave) {
     if (base > 0) look(base + lane, items, steps, whole);
     const int ranges = whole ? 1 : min(max(1, (steps + most - 1) / most), a.ranges);
     const int groups = items * ranges, parts = ranges > 1 ? groups : 0, split = ranges > 1 ? items : 0;
-    const int to = w.total + scan_lanes(groups, lane), slots_to = slots + scan_lanes(parts, lane), split_to = divided + scan_lanes(split, lane);
+    const int to = total + scan_lanes(groups), slots_to = slots + scan_lanes(parts), split_to = divided + scan_lanes(split);
     const unsigned long long past = __builtin_amdgcn_ballot_w64(to > index);
     if (w.seq < 0 && past != 0ull) {
       const int l = __builtin_ctzll(past);
-      const int its = __builtin_amdgcn_readlane(items, l);
-      w.seq = base > 0 ? base + l : __builtin_amdgcn_readlane(seq, l);
+      w.seq = base + l;
       w.ranges = __builtin_amdgcn_readlane(ranges, l);
-      const int local = index - (__builtin_amdgcn_readlane(to, l) - its * w.ranges);
-      const int nth = local / w.ranges;  // (the last items first: they see more keys)
-      w.range = local - nth * w.ranges;
-      w.item = its - 1 - nth;
-      w.slot = __builtin_amdgcn_readlane(slots_to, l) - its * w.ranges + nth * w.ranges;
-      if (w.ranges > 1 && w.slot + w.ranges > a.slots) {  // (only where the rows of q_starts overlap)
-        w.seq = -1;
-        return false;
-      }
+      w.range = index - (__builtin_amdgcn_readlane(to, l) - w.ranges);
+      w.slot = __builtin_amdgcn_readlane(slots_to, l) - w.ranges;
       if (w.ranges > 1 && head == 0 && w.range == 0 && threadIdx.x == 0) {
-        const int at = __builtin_amdgcn_readlane(split_to, l) - its + nth;
         const int2 rows = rows_of_one(a, w.seq);
-        if (at < a.items) a.list[at] = Divided{rows.x, rows.y, w.item, w.ranges, w.slot};
+        a.list[__builtin_amdgcn_readlane(split_to, l) - 1] = Divided{rows.x, rows.y, 0, w.ranges, w.slot};
       }
       if (index != 0) return true;
     }
-    // (all of them, unless the rows of q_starts overlap: the join must not read what no workgroup wrote)
-    const unsigned long long fit = __builtin_amdgcn_ballot_w64(slots_to <= a.slots && static_cast<int64_t>(to) * a.kv <= gridDim.x);
-    if (fit != 0ull) listed = __builtin_amdgcn_readlane(split_to, kWave - 1 - __builtin_clzll(fit));
-    w.total = __builtin_amdgcn_readlane(to, kWave - 1);
+    total = __builtin_amdgcn_readlane(to, kWave - 1);
     slots = __builtin_amdgcn_readlane(slots_to, kWave - 1);
     divided = __builtin_amdgcn_readlane(split_to, kWave - 1);
   }
-  if (a.aim > 0 && head == 0 && index == 0 && threadIdx.x == 0) *a.divided = min(listed, a.items);
+  if (head == 0 && index == 0 && threadIdx.x == 0) *a.divided = divided;
   return w.seq >= 0;
 }
 
-// Rows that belong to no sequence: zeros, by the workgroups without work.
-__device__ __forceinline__ void clear_behind(const PagedArgs& a, int head, int index, int total, int threads) {
+// Rows that belong to no sequence: zeros, by all workgroups.
+__device__ __forceinline__ void clear_behind(const PagedArgs& a, int head, int index, int threads) {
   if (a.starts == nullptr) return;
-  const int behind = min(max(a.starts[a.seqs], 0), a.n);
-  const int spare = static_cast<int>(gridDim.x) / a.kv - total, width = a.group * kDim / 8;
-  for (int64_t row = behind + index - total; row < a.n; row += spare)
+  const int behind = min(max(uniform(a.starts)[a.seqs], 0), a.n), groups = static_cast<int>(gridDim.x) / a.kv, width = a.group * kDim / 8;
+  for (int64_t row = static_cast<int64_t>(behind) + index; row < a.n; row += groups)
     for (int c = threadIdx.x; c < width; c += threads)
       *reinterpret_cast<uint4*>(a.o + (row * a.heads + head * a.group) * kDim + 8 * c) = make_uint4(0, 0, 0, 0);
 }
@@ -279,417 +258,554 @@ __device__ __forceinline__ void slots(std::integer_sequence<int, I...>, F f) {
   (f(std::integral_constant<int, I>{}), ...);
 }
 
-__global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs a) {
+// chunk_kernel's work.  An item is up to 256 queries of a sequence against the keys up to its last one.  Where keys are
+// divided, a KV head's items lie one after another on a line, each as long as its keys (times `group`) and kApart steps of 64
+// more; the line is cut into `aim` equal slices, and a workgroup takes a slice: the end of one item, whole ones, the
+// beginning of another.  So the workgroups end at about the same time, however unequal the sequences are.  (20 sequences of
+// 1-700 new tokens over up to 3000, 16 heads on 4: 82-89 us with items divided by their own lengths, the longest ranges first,
+// 77-82 with slices; 8 of up to 300 over 6000, 16 heads: 105, 92.)  Else a workgroup takes one item, a sequence's last ones first:
+// they see more keys.  Every workgroup finds its work for itself, sequences in lanes: the lengths are on the device alone.
+// kApart: beginning a part costs some 10 us, finding it, first latencies and the stores (3, 5, 7, 10 steps: 84, 79, 78, 80 us).
+constexpr double kApart = 7.0;
+constexpr int kLeastSteps = 7;  // of a slice; a cut moves by less than 2
+
+// One sequence's items on the line.
+struct Line {
+  int q, items;   // queries, items
+  double before;  // of each item: keys before the call's, and kApart
+  __device__ __forceinline__ Line(const PagedArgs& a, int rows, int keys) {
+    q = rows * a.group;
+    items = items_of(a, rows, kChunkRows);
+    before = static_cast<double>(max(keys - rows, 0)) * a.group + kApart * kKeys * a.group;
+  }
+  // where item i begins (i = items: where the last one ends)
+  __device__ __forceinline__ double at(int i) const {
+#pragma clang fp contract(off)  // (all workgroups get the same, wherever this is inlined)
+    const double n = i;
+    return n * before + (i < items ? 0.5 * kChunkRows * n * (n + 1) : 0.5 * kChunkRows * n * (n - 1) + q);
+  }
+};
+
+// The step of the `all` of an item at begins .. ends that a cut falls on: none within two of the item's ends.
+__device__ __forceinline__ int cut_at(double cut, double begins, double ends, double apart, double scale, int all) {
+#pragma clang fp contract(off)
+  const double steps = (cut - begins - apart) * scale;
+  return cut >= ends || steps > all - 2 ? all : (steps < 2.0 ? 0 : static_cast<int>(steps));
+}
+
+__device__ __forceinline__ double lane_f64(double v, int l) {
+  const int64_t u = __double_as_longlong(v);
+  const int lo = __builtin_amdgcn_readlane(static_cast<int>(u), l), hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), l);
+  return __longlong_as_double((static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo));
+}
+
+// Where a wave is on the line.  (In LDS, each wave's its own: no register is held while it works on a part.)
+struct Walk {
+  double x, begin, end, slice;  // the next item; the workgroup's slice; a slice's length
+  double from;                  // where the sequences from `base` on begin
+  int base, opens;              // opens: the slice ends in an item that it begins
+};
+
+// chunk_kernel's arguments, read again where this stands: held all at once over its loop they leave no scalar register, and
+// from where the launch put them they take a microsecond.
+__device__ __forceinline__ PagedArgs args_again(const PagedArgs& lds) {
+  asm volatile("" ::: "memory");
+  constexpr int kWords = sizeof(PagedArgs) / 4;
+  int w[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) w[i] = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(&lds)[i]);
+  PagedArgs a;
+  __builtin_memcpy(&a, w, sizeof(a));
+  // (pointers to global memory: the compiler knows it of arguments only)
+  const auto global = [](auto*& p) __attribute__((always_inline)) {
+    typedef typename std::remove_reference<decltype(*p)>::type value_t;
+    p = (value_t*)(__attribute__((address_space(1))) value_t*)p;
+  };
+  global(a.q), global(a.k), global(a.v), global(a.o), global(a.table), global(a.lens), global(a.starts), global(a.list);
+  global(a.part_ml), global(a.part_o);
+  return a;
+}
+
+__global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs first_args) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds_all[2 * kRing * kTileBytes];
-  __shared__ int wave_pos[2][kChunkWaves];
   __shared__ unsigned long long odd_keys[4];  // by tile % 4: keys of a tile with infinite or NaN values
   __shared__ int no_page;                     // the first key without a page
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
-  Work w;
-  if (!find_work<kChunkRows, kKeys, kChunkLeast, false, true>(a, head, index, w)) {
-    clear_behind(a, head, index, w.total, kChunkThreads);
-    return;
-  }
-  const int seq = __builtin_amdgcn_readfirstlane(w.seq), ranges = __builtin_amdgcn_readfirstlane(w.ranges);
-  const int2 rows = rows_of_one(a, seq);
-  const int len = max(uniform(a.lens)[seq], 0);
-  const Pages pages = pages_of(a, seq, head, len);
-  // this lane's query: column lane % 32 of the wave's
-  const int r = __builtin_amdgcn_readfirstlane(w.item) * kChunkRows + wave * 32 + (lane & 31);
-  const bool valid = r < rows.y * a.group;
-  const int rc = valid ? r : rows.y * a.group - 1;
-  const int token = rc / a.group, out_head = head * a.group + rc - token * a.group;
-  const int pos = len - rows.y + token;
-  const int64_t out_at = (static_cast<int64_t>(rows.x + token) * a.heads + out_head) * kDim;  // elements of o
-  bf16x8_t q[8];
+  __shared__ Walk walk[kChunkWaves];
+  __shared__ PagedArgs args;
+  __shared__ int3 line_of[kChunkWaves][kWave];    // a lane's sequence: first row, rows, length
+  __shared__ double line_to[kChunkWaves][kWave];  // where the lane's sequence of the 64 from `base` on ends, from `from` on
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = static_cast<int>(blockIdx.x) % first_args.kv, mine_index = static_cast<int>(blockIdx.x) / first_args.kv;
+
+  // the lane's sequence of those from `base` on: into line_of, and where it ends into line_to
+  const auto look = [&](const PagedArgs& a, int s, double& to, double& most) __attribute__((always_inline)) {
+    const int known = min(s, a.seqs - 1);  // (the loads one beside the other)
+    const int given = a.lens[known];
+    int2 rows = rows_of(a, known);
+    rows.y = s < a.seqs ? rows.y : 0;
+    const int len = s < a.seqs ? max(given, 0) : 0;
+    const Line line(a, rows.y, keys_of(a, len));
+    to = scan_lanes(a.aim > 0 ? (line.items > 0 ? line.at(line.items) : 0.0) : static_cast<double>(line.items));
+    most = fmax(most, line.before + line.q);
+    line_to[wave][lane] = to;
+    line_of[wave][lane] = make_int3(rows.x, rows.y, len);
+  };
   {
-    const uint16_t* qp = a.q + (rows.x + token) * a.q_row + out_head * kDim + 8 * h;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
-  }
-  int wmin = pos, wmax = pos;
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) {
-    wmin = min(wmin, __shfl_xor(wmin, off, kWave));
-    wmax = max(wmax, __shfl_xor(wmax, off, kWave));
-  }
-  wmin = __builtin_amdgcn_readfirstlane(wmin);
-  wmax = __builtin_amdgcn_readfirstlane(wmax);
-  if (lane == 0) {
-    wave_pos[0][wave] = wmin;
-    wave_pos[1][wave] = wmax;
-  }
-  if (tid < 4) odd_keys[tid] = 0ull;
-  if (tid == 0) no_page = 0x7FFFFFFF;
-  lds_barrier();
-  int low = wave_pos[0][0], end = wave_pos[1][0];
-#pragma unroll
-  for (int w = 1; w < kChunkWaves; ++w) {
-    low = min(low, wave_pos[0][w]);
-    end = max(end, wave_pos[1][w]);
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-  end = __builtin_amdgcn_readfirstlane(min(end, pages.last));
-  int tiles = end >= 0 ? end / kKeys + 1 : 0, first = 0;
-  if (ranges > 1) {
-    const int range = __builtin_amdgcn_readfirstlane(w.range);
-    first = static_cast<int>(static_cast<int64_t>(tiles) * range / ranges);
-    tiles = static_cast<int>(static_cast<int64_t>(tiles) * (range + 1) / ranges);
-  }
-  const int mine = min(tiles, (wmax >> 6) + 1);  // tiles that some query of the wave sees (none: at most `first`)
-
-  f32x16_t o[4];
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-  // the reference of the running softmax (a score, and it scaled to base 2), this lane's parts of the sum
-  float raw = kNone, off = -scaled_max(kNone, a.scale), sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  // Scores may pass the reference by 2^8 before it moves: the probabilities are as exact in bf16 as under 1, and most tiles
-  // then leave the outputs alone.
-  const float slack = 8.0f / a.scale;
-  bool far = false;  // (wave-uniform) some query's reference lies past kFar
-
-  if (first < tiles) {
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds_all));
-    constexpr uint32_t kV = kRing * kTileBytes;  // V's tiles lie behind K's
-
-    // Transfers: a wave brings the 8 keys 8 w .. of a tile, which share a page: twice four rows.  Their places for 64
-    // tiles lie in the lanes of two registers (a scalar load among a tile's LDS reads would make their waits wait for all).
-    uint32_t kv[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) kv[i] = 1024 * i + 256 * (lane >> 4) + 16 * ((lane & 15) ^ (8 * (wave & 1) + 4 * i + (lane >> 4)));
-    const uint32_t vv = 256 * (lane >> 4) + 16 * ((lane & 15) ^ (4 * (lane >> 4)));
-    const auto block_key = [&](int tile) __attribute__((always_inline)) {
-      return min(min(tile, tiles - 1) * kKeys + 8 * (wave & ~1), pages.last & ~15);
-    };
-    uint32_t at_lo = 0, at_hi = 0;  // bytes from the pool's start
-    int at_from = 0, lost = 0x7FFFFFFF;  // lost: the first key of this wave's without a page
-    const auto look_up = [&](int tile) __attribute__((always_inline)) {
-      at_from = tile;
-      const int key = block_key(tile + lane);
-      const int id = *(a.table + static_cast<int64_t>(seq) * a.width + (key >> pages.log2));
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it, and q before the first, have arrived here, and no use waits for them
-      const uint64_t at = 2 * static_cast<uint64_t>(pages.at(id, key) + 8 * (wave & 1) * kDim);
-      at_lo = static_cast<uint32_t>(at);
-      at_hi = static_cast<uint32_t>(at >> 32);
-      const unsigned long long none = __builtin_amdgcn_ballot_w64(!pages.exists(id));
-      if (none != 0ull) lost = min(lost, __builtin_amdgcn_readlane(key, __builtin_ctzll(none)));
-    };
-    const auto place = [&](int tile) __attribute__((always_inline)) {  // of the wave's keys of a tile
-      return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_hi), tile - at_from))) << 32) |
-             static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_lo), tile - at_from));
-    };
-    const auto part_of = [&](const uint16_t* pool, uint64_t at) __attribute__((always_inline)) {
-      const uint64_t u = reinterpret_cast<uintptr_t>(pool) + at;
-      return lds_buffer_t{static_cast<int>(u), static_cast<int>(u >> 32), 8 * kDim * 2, 0x00020000};
-    };
-    const auto ring = [&](int tile) __attribute__((always_inline)) { return static_cast<uint32_t>((tile - first) % kRing) * kTileBytes; };
-    const auto bring_k = [&](int tile, uint64_t at) __attribute__((always_inline)) {
-      const lds_buffer_t r = part_of(a.k, at);
-      const uint32_t to = lds0 + ring(tile) + 2048u * wave;
-      to_lds<16>(r, kv[0], 0, to);
-      to_lds<16>(r, kv[1], 0, to + 1024u);
-    };
-    const auto bring_v = [&](int tile, uint64_t at) __attribute__((always_inline)) {
-      const lds_buffer_t r = part_of(a.v, at);
-      const uint32_t to = lds0 + kV + ring(tile) + 2048u * wave;
-      to_lds<16>(r, vv, 0, to);
-      to_lds<16>(r, vv, 1024u, to + 1024u);
-    };
-    // This wave's V rows of a tile, arrived: zeros past the sequence's end, and in the place of infinite and NaN values that
-    // some row does not see
-    const auto mend = [&](int tile) __attribute__((always_inline)) {
-      if (tile >= tiles || tile * kKeys + kKeys - 1 <= low) return;
-      uint32_t bits = 0;
-      uint8_t* const at = lds_all + kV + ring(tile) + 2048 * wave + 16 * lane;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = tile * kKeys + 8 * wave + 4 * i + (lane >> 4);
-        u32x4_t v = *reinterpret_cast<u32x4_t*>(at + 1024 * i);
-        bool any = false;
-        if (key > pages.last)
-          v = u32x4_t{0, 0, 0, 0};
-        else if (key > low)
-          any = drop_nonfinite(v);
-        if (any || key > pages.last) *reinterpret_cast<u32x4_t*>(at + 1024 * i) = v;
-        const unsigned long long lanes = __builtin_amdgcn_ballot_w64(any);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if ((lanes >> (16 * j)) & 0xFFFFull) bits |= 1u << (4 * i + j);
+    const PagedArgs a = first_args;
+    double to, most = 0.0, x = mine_index, x_end = mine_index + 1.0, slice = 1.0;
+    if (lane == 0) args = a;
+    if (a.aim > 0) {
+      double total = 0.0;
+      for (int base = (a.seqs - 1) / kWave * kWave; base >= 0; base -= kWave) {  // (the first ones last: they stay)
+        look(a, base + lane, to, most);
+        total += lane_f64(to, kWave - 1);
       }
-      if (bits != 0 && lane == 0) atomicOr(&odd_keys[tile & 3], static_cast<unsigned long long>(bits) << (8 * wave));
-    };
-
-    // Operands: K fragment i is rows lane % 32 of half i % 2 of the tile, channels 16 (i / 2) + 8 h ..; V fragment j rows
-    // 16 (j / 4) + 4 h .. (+ 8), channels 32 (j % 4) + ..
-    typedef const __attribute__((address_space(3))) uint8_t* lds_at;
-    uint32_t kx[8], vx[4];
-    const int i16 = lane & 15;
-#pragma unroll
-    for (int st = 0; st < 8; ++st) kx[st] = lds0 + 256 * (lane & 31) + (16 * (h ^ i16) ^ 32 * st);
-#pragma unroll
-    for (int d = 0; d < 4; ++d) vx[d] = lds0 + kV + 256 * (4 * h + (i16 >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3) + (64 * (i16 >> 2) ^ 64 * d);
-    const auto k_part = [&](uint32_t of, int i) __attribute__((always_inline)) {
-      return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(reinterpret_cast<lds_at>(kx[i >> 1] + of) + 8192 * (i & 1));
-    };
-    const auto v_part = [&](uint32_t of, int j) __attribute__((always_inline)) {
-      const lds_at at = reinterpret_cast<lds_at>(vx[j & 3] + of) + 4096 * (j >> 2);
-      const bf16x4_t lo = read_tr((lds_rows)at), hi = read_tr((lds_rows)(at + 2048));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    };
-    const auto scores_part = [&](int i, bf16x8_t k, f32x16_t (&s)[2]) __attribute__((always_inline)) {
-      f32x16_t zero;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
-      s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
-    };
-    // probabilities 2 k and 2 k + 1 of the tile's 32 a lane: words of the second product's operand
-    u32x4_t p[4];
-    const auto pair = [&](int k, const f32x16_t (&s)[2]) __attribute__((always_inline)) {
-      const int t = k >> 2, e = 8 * (t & 1) + 2 * (k & 3);
-      const float p0 = fast_exp2(fmaf(s[t >> 1][e], a.scale, off)), p1 = fast_exp2(fmaf(s[t >> 1][e + 1], a.scale, off));
-      p[t][k & 3] = attn_bf16_pair(p0, p1);
-      sum[k & 3] = add_pair(p[t][k & 3], sum[k & 3]);
-    };
-    const auto outputs_part = [&](int j, bf16x8_t v) __attribute__((always_inline)) {
-      o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8_t, p[j >> 2]), o[j & 3], 0, 0, 0);
-    };
-    const auto hide = [&](int tile, f32x16_t (&s)[2]) __attribute__((always_inline)) {
-      if (tile * kKeys + kKeys - 1 > wmin) {  // keys past a query's position
-        const int lim = pos - tile * kKeys - 4 * h;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * b + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
-      }
-    };
-    const auto largest = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
-      float m = s[0][0];
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
-      return m;
-    };
-    // the reference moves where a score passes it too far
-    const auto move_to = [&](float m, f32x16_t (&s)[2]) __attribute__((always_inline)) {
-      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-      m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-      if (__builtin_amdgcn_ballot_w64(m > raw + slack) != 0ull) {
-        const float top = fmaxf(raw, m), mn = scaled_max(top, a.scale);
-        const float alpha = exp2_between(raw, top, scaled_max(raw, a.scale), mn, a.scale);
-        raw = top;
-        off = -mn;
-        far = __builtin_amdgcn_ballot_w64(fabsf(mn) > kFar && top > kNone) != 0ull;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[i] *= alpha;
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-      }
-      if (far) {  // (differences before the scale)
-        off = 0.0f;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] -= raw;
-      }
-    };
-    const auto add_odd = [&](int tile) __attribute__((always_inline)) {
-      if (tile * kKeys + kKeys - 1 <= low) return;
-      for (unsigned long long odd = odd_keys[tile & 3]; odd != 0ull; odd &= odd - 1) {
-        // key j lies in result register 4 (j / 8) + j % 4 of lane half j / 4 % 2
-        const int j = __builtin_amdgcn_readfirstlane(__builtin_ctzll(odd)), e = 4 * (j >> 3) + (j & 3);
-        const int key = tile * kKeys + j;
-        const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * h;
-        float w = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (8 * t + i == e) w = static_cast<float>(__builtin_bit_cast(bf16x8_t, p[t])[i]);
-        w = __shfl(w, (lane & 31) + 32 * ((j >> 2) & 1), kWave);
-        if (key <= pos) {
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const uint2 v = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * g);
-              float x[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-              add_nonfinite(w, v, x[0], x[1], x[2], x[3]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[d][4 * g + i] = x[i];
-              __builtin_amdgcn_sched_barrier(0);  // (a piece at a time: this path must not set the kernel's registers)
-            }
-        }
-      }
-    };
-
-    look_up(first);
-    uint64_t at_v = 0;  // place of the tile whose V goes next
-    {
-      uint64_t at[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) at[i] = place(first + i);
-      bring_k(first, at[0]);
-      bring_v(first, at[0]);
-      bring_k(first + 1, at[1]);
-      bring_k(first + 2, at[2]);
-      bring_v(first + 1, at[1]);
-      bring_k(first + 3, at[3]);
-      bring_v(first + 2, at[2]);
-      at_v = at[3];
+      // (an item lies in at most 64 slices: the join has one a lane; `most` in 32 bits and a little more)
+      const double longest = 1.001 * wave_max(static_cast<float>(most));
+      slice = fmax(total / a.aim, fmax(static_cast<double>(kLeastSteps) * kKeys * a.group, longest * (1.0 / (kMaxRanges - 2))));
+      x = mine_index < a.aim ? mine_index * slice : 1e300;
+      x_end = mine_index + 1 < a.aim ? (mine_index + 1) * slice : 1e300;
+    } else {
+      look(a, lane, to, most);
     }
-    // All but K of the fourth tile and V of the third have arrived.
-    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-    lds_barrier();
-    f32x16_t sa[2], sb[2];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) scores_part(i, k_part(ring(first), i), sa);
-    hide(first, sa);
-    move_to(largest(sa), sa);
+    walk[wave] = Walk{x, x, x_end, slice, 0.0, 0, 0};
+  }
 
-    // One tile: the next one's scores (matrix slots 0-15) and this one's outputs (16-31), with this one's exponentials and
-    // then the next one's maximum spread over the slots, so that the vector unit works in the matrix core's shadow.
-    // Fragments are read four slots ahead, the first four of the tile after that before the barrier: K arrives two tiles
-    // before its scores, V one before its outputs.  EDGE: some row of the workgroup does not see some key of this tile or
-    // the next.  The order is kept by hand: left to it, the compiler computes all exponentials at once.
-    bf16x8_t ahead[4];
-    const auto flow = [&](int tile, uint32_t v_at, uint32_t k_at, uint32_t k_then, f32x16_t (&now)[2], f32x16_t (&next)[2],
-                          auto edge_tag) __attribute__((always_inline)) {
-      constexpr bool EDGE = decltype(edge_tag)::value;
-      bf16x8_t kf[16], vf[16];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) kf[i] = ahead[i];
-      float m = kNone;
-      uint64_t at = 0;
-      slots(std::make_integer_sequence<int, 32>{}, [&](auto slot) __attribute__((always_inline)) {
-        constexpr int i = decltype(slot)::value;
-        if constexpr (i < 12)
-          kf[i + 4] = k_part(k_at, i + 4);
-        else if constexpr (i < 28)
-          vf[i - 12] = v_part(v_at, i - 12);
+  while (true) {
+    const PagedArgs a = args_again(args);
+    int tid = threadIdx.x, index = mine_index;
+    asm volatile("" : "+v"(tid), "+s"(index));  // (nor is what depends on it held from part to part)
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+    double to = line_to[wave][lane];
+    int3 of = line_of[wave][lane];
+    const double x = walk[wave].x, x_begin = walk[wave].begin, x_end = walk[wave].end, slice = walk[wave].slice;
+    if (__builtin_amdgcn_readfirstlane(x >= x_end)) break;
+    double from = walk[wave].from;
+    int base = __builtin_amdgcn_readfirstlane(walk[wave].base);
+    unsigned long long past;
+    while ((past = __builtin_amdgcn_ballot_w64(from + to > x)) == 0ull) {
+      base += kWave;
+      if (base >= a.seqs) break;
+      from += lane_f64(to, kWave - 1);
+      double unused = 0.0;
+      look(a, base + lane, to, unused);
+      of = line_of[wave][lane];
+      walk[wave].from = from;
+      walk[wave].base = base;
+    }
+    if (past == 0ull) break;
+    const int who = __builtin_ctzll(past), seq = base + who;
+    const double start = from + (who > 0 ? lane_f64(to, who - 1) : 0.0), stop = from + lane_f64(to, who);
+    const int2 rows = make_int2(__builtin_amdgcn_readlane(of.x, who), __builtin_amdgcn_readlane(of.y, who));
+    const int len = __builtin_amdgcn_readlane(of.z, who);
+    const Pages pages = pages_of(a, seq, head, len);
+    const Line line(a, rows.y, pages.last + 1);
+    int item = 0;
+    double begins = 0.0, ends = 0.0;  // the item's place on the line
+    if (a.aim > 0) {
+      for (int high = line.items - 1; item < high;) {
+        const int mid = item + (high - item + 1) / 2;
+        if (__builtin_amdgcn_readfirstlane(start + line.at(mid) <= x))
+          item = mid;
         else
-          ahead[i - 28] = k_part(k_then, i - 28);
-        if constexpr (i < 16)
-          scores_part(i, kf[i], next);
-        else
-          outputs_part(i - 16, vf[i - 16]);
-        // 16 pairs over the slots 0-25 (operand t is complete well before slot 16 + 4 t)
-        constexpr int k = (3 * i + 2) / 5;
-        if constexpr (i < 26 && 5 * k / 3 == i) {
-          asm volatile("" : "+v"(off));  // (no pair is computed before its slot)
-          pair(k, now);
-        }
-        if constexpr (i == 2) bring_v(tile + 3, at_v);
-        if constexpr (i == 4) at = place(tile + 4);
-        if constexpr (i == 7) bring_k(tile + 4, at);
-        if constexpr (EDGE && (i == 17 || i == 18)) {  // keys past a query's position
-          const int lim = pos - (tile + 1) * kKeys - 4 * h;
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (32 * (i - 17) + 8 * (e >> 2) + (e & 3) > lim) next[i - 17][e] = -INFINITY;
-        }
-        if constexpr (i >= 26 || i == 19 || i == 24) {  // 4 scores a time
-          constexpr int e = i >= 26 ? 2 + (i - 26) : (i == 19 ? 0 : 1);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) m = fmaxf(m, next[e >> 2][4 * (e & 3) + x]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      at_v = at;
-      if (EDGE) add_odd(tile);
-      move_to(m, next);
-    };
-    const auto arrive = [&](int tile) __attribute__((always_inline)) {
-      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      __builtin_amdgcn_s_barrier();  // (this wave's reads of what the next transfers replace are done: their results were used)
-      asm volatile("" ::: "memory");
-      if (tile + 8 >= at_from + kWave) look_up(tile + 5);
-    };
-    int tile = first;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ahead[i] = k_part(ring(tile + 1), i);
-    // (four tiles at a time: their places in the ring are constants, and the scores change places)
-    for (; tile + 4 < tiles && (tile + 5) * kKeys - 1 <= low; tile += 4) {
-      constexpr uint32_t kT = kTileBytes;
-      flow(tile, 0 * kT, 1 * kT, 2 * kT, sa, sb, std::false_type{});
-      arrive(tile);
-      flow(tile + 1, 1 * kT, 2 * kT, 3 * kT, sb, sa, std::false_type{});
-      arrive(tile + 1);
-      flow(tile + 2, 2 * kT, 3 * kT, 0 * kT, sa, sb, std::false_type{});
-      arrive(tile + 2);
-      flow(tile + 3, 3 * kT, 0 * kT, 1 * kT, sb, sa, std::false_type{});
-      arrive(tile + 3);
-    }
-    // The last tiles, of which some row does not see some key
-    mend(tile);
-    lds_barrier();
-    for (; tile < tiles; ++tile) {
-      if (tid == 0) odd_keys[(tile + 2) & 3] = 0ull;
-      if (tile < mine) {
-        flow(tile, ring(tile), ring(tile + 1), ring(tile + 2), sa, sb, std::true_type{});
-#pragma unroll
-        for (int b = 0; b < 2; ++b) sa[b] = sb[b];
-      } else {
-        bring_v(tile + 3, at_v);
-        at_v = place(tile + 4);
-        bring_k(tile + 4, at_v);
+          high = mid - 1;
       }
-      asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-      mend(tile + 1);
-      lds_barrier();
-      if (tile + 8 >= at_from + kWave) look_up(tile + 5);
+      begins = start + line.at(item);
+      ends = item + 1 < line.items ? start + line.at(item + 1) : stop;
+    } else {
+      item = line.items - 1 - static_cast<int>(x - start);
+      ends = x + 1.0;
     }
-    if (lost != 0x7FFFFFFF && lane == 0) atomicMin(&no_page, lost);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into LDS when the workgroup ends)
-    lds_barrier();
-  }
+    item = __builtin_amdgcn_readfirstlane(item);
+    walk[wave].x = ends;
+    const auto position = [&](int query) __attribute__((always_inline)) { return len - rows.y + min(query, line.q - 1) / a.group; };
+    const int low = position(item * kChunkRows), end = min(position((item + 1) * kChunkRows - 1), pages.last);
+    const int all = end >= 0 ? end / kKeys + 1 : 0;
+    int tiles = all, first = 0, parts = 1;  // this slice's; slices of the item
+    if (a.aim > 0) {
+      const double apart = kApart * kKeys * a.group, scale = all / (ends - begins - apart);
+      const auto cut = [&](double at) __attribute__((always_inline)) { return cut_at(at, begins, ends, apart, scale, all); };
+      first = __builtin_amdgcn_readfirstlane(x_begin <= begins ? 0 : cut(x_begin));
+      tiles = __builtin_amdgcn_readfirstlane(cut(x_end));
+      if (__builtin_amdgcn_readfirstlane(all > 0 ? first >= tiles : x_begin > begins)) continue;  // (the next or the last slice has it)
+      if (first > 0 || tiles < all) parts = 2;
+      if (first == 0 && tiles < all) {
+        walk[wave].opens = 1;
+        if (head == 0 && tid == 0) {
+          int last = min(static_cast<int>(ends / slice), a.aim - 1);
+          while (last > index && (last * slice >= ends || cut(last * slice) >= all)) --last;
+          a.list[index] = Divided{rows.x, rows.y, item, last - index + 1, 2 * index + 1};
+        }
+      }
+    }
+    const int part_slot = 2 * index + (first == 0 ? 1 : 0);
+    // this lane's query: column lane % 32 of the wave's
+    const int pos = position(item * kChunkRows + wave * 32 + (lane & 31));
+    const int wmin = position(item * kChunkRows + wave * 32), wmax = position(item * kChunkRows + wave * 32 + 31);
+    if (tid < 4) odd_keys[tid] = 0ull;
+    if (tid == 0) no_page = 0x7FFFFFFF;
+    const int mine = min(tiles, (wmax >> 6) + 1);  // tiles that some query of the wave sees (none: at most `first`)
 
-  float l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-  // NaN: a sequence longer than its table row, a key without a page
-  l += swap_half(l) + (len - 1 > pages.last || pos >= no_page ? NAN : 0.0f);
-  if (!valid) return;
-  if (ranges > 1) {
-    const int64_t part = (static_cast<int64_t>(head) * a.slots + w.slot + w.range) * kChunkRows + wave * 32 + (lane & 31);
-    float* op = a.part_o + part * kDim + 4 * h;
+    f32x16_t o[4];
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<float4*>(op + 32 * d + 8 * g) =
-            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
-    const bool seen = pos >= first * kKeys && first < tiles;
-    if (h == 0) a.part_ml[part] = make_float2(seen ? raw : kUnseen, l);
-    return;
-  }
-  const float inv = pos >= 0 ? 1.0f / l : 0.0f;
-  uint16_t* op = a.o + out_at + 4 * h;
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    // the reference of the running softmax (a score, and it scaled to base 2), this lane's parts of the sum
+    float raw = kNone, off = -scaled_max(kNone, a.scale), sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // Scores may pass the reference by 2^8 before it moves: the probabilities are as exact in bf16 as under 1, and most tiles
+    // then leave the outputs alone.
+    const float slack = 8.0f / a.scale;
+    bool far = false;  // (wave-uniform) some query's reference lies past kFar
+
+    if (first < tiles) {
+      bf16x8_t q[8];
+      const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)lds_all));
+      constexpr uint32_t kV = kRing * kTileBytes;  // V's tiles lie behind K's
+
+      // Transfers: a wave brings the 8 keys 8 w .. of a tile, which share a page: twice four rows.  Their places for 64
+      // tiles lie in the lanes of two registers (a scalar load among a tile's LDS reads would make their waits wait for all).
+      uint32_t kv[2];
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
+      for (int i = 0; i < 2; ++i) kv[i] = 1024 * i + 256 * (lane >> 4) + 16 * ((lane & 15) ^ (8 * (wave & 1) + 4 * i + (lane >> 4)));
+      const uint32_t vv = 256 * (lane >> 4) + 16 * ((lane & 15) ^ (4 * (lane >> 4)));
+      const auto block_key = [&](int tile) __attribute__((always_inline)) {
+        return min(min(tile, tiles - 1) * kKeys + 8 * (wave & ~1), pages.last & ~15);
+      };
+      uint32_t at_lo = 0, at_hi = 0;  // bytes from the pool's start
+      int at_from = 0, lost = 0x7FFFFFFF;  // lost: the first key of this wave's without a page
+      const auto look_up = [&](int tile) __attribute__((always_inline)) {
+        at_from = tile;
+        const int key = block_key(tile + lane);
+        const int id = *(a.table + static_cast<int64_t>(seq) * a.width + (key >> pages.log2));
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): it, and q before the first, have arrived here, and no use waits for them
+        const uint64_t at = 2 * static_cast<uint64_t>(pages.at(id, key) + 8 * (wave & 1) * kDim);
+        at_lo = static_cast<uint32_t>(at);
+        at_hi = static_cast<uint32_t>(at >> 32);
+        const unsigned long long none = __builtin_amdgcn_ballot_w64(!pages.exists(id));
+        if (none != 0ull) lost = min(lost, __builtin_amdgcn_readlane(key, __builtin_ctzll(none)));
+      };
+      const auto place = [&](int tile) __attribute__((always_inline)) {  // of the wave's keys of a tile
+        return (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_hi), tile - at_from))) << 32) |
+               static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at_lo), tile - at_from));
+      };
+      // (past the last tile: of no bytes, so that it moves none, and the number of transfers in flight is the same)
+      const auto part_of = [&](const uint16_t* pool, int tile, uint64_t at) __attribute__((always_inline)) {
+        const uint64_t u = reinterpret_cast<uintptr_t>(pool) + at;
+        return lds_buffer_t{static_cast<int>(u), static_cast<int>(u >> 32), tile < tiles ? 8 * kDim * 2 : 0, 0x00020000};
+      };
+      const auto ring = [&](int tile) __attribute__((always_inline)) { return static_cast<uint32_t>((tile - first) % kRing) * kTileBytes; };
+      const auto bring_k = [&](int tile, uint64_t at) __attribute__((always_inline)) {
+        const lds_buffer_t r = part_of(a.k, tile, at);
+        const uint32_t to = lds0 + ring(tile) + 2048u * wave;
+        to_lds<16>(r, kv[0], 0, to);
+        to_lds<16>(r, kv[1], 0, to + 1024u);
+      };
+      const auto bring_v = [&](int tile, uint64_t at) __attribute__((always_inline)) {
+        const lds_buffer_t r = part_of(a.v, tile, at);
+        const uint32_t to = lds0 + kV + ring(tile) + 2048u * wave;
+        to_lds<16>(r, vv, 0, to);
+        to_lds<16>(r, vv, 1024u, to + 1024u);
+      };
+      // This wave's V rows of a tile, arrived: zeros past the sequence's end, and in the place of infinite and NaN values that
+      // some row does not see
+      const auto mend = [&](int tile) __attribute__((always_inline)) {
+        if (tile >= tiles || tile * kKeys + kKeys - 1 <= low) return;
+        uint32_t bits = 0;
+        uint8_t* const at = lds_all + kV + ring(tile) + 2048 * wave + 16 * lane;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const float x[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-      *reinterpret_cast<uint2*>(op + 32 * d + 8 * g) = pair4(x, inv);
+        for (int i = 0; i < 2; ++i) {
+          const int key = tile * kKeys + 8 * wave + 4 * i + (lane >> 4);
+          u32x4_t v = *reinterpret_cast<u32x4_t*>(at + 1024 * i);
+          bool any = false;
+          if (key > pages.last)
+            v = u32x4_t{0, 0, 0, 0};
+          else if (key > low)
+            any = drop_nonfinite(v);
+          if (any || key > pages.last) *reinterpret_cast<u32x4_t*>(at + 1024 * i) = v;
+          const unsigned long long lanes = __builtin_amdgcn_ballot_w64(any);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((lanes >> (16 * j)) & 0xFFFFull) bits |= 1u << (4 * i + j);
+        }
+        if (bits != 0 && lane == 0) atomicOr(&odd_keys[tile & 3], static_cast<unsigned long long>(bits) << (8 * wave));
+      };
+
+      // Operands: K fragment i is rows lane % 32 of half i % 2 of the tile, channels 16 (i / 2) + 8 h ..; V fragment j rows
+      // 16 (j / 4) + 4 h .. (+ 8), channels 32 (j % 4) + ..
+      typedef const __attribute__((address_space(3))) uint8_t* lds_at;
+      uint32_t kx[8], vx[4];
+      const int i16 = lane & 15;
+#pragma unroll
+      for (int st = 0; st < 8; ++st) kx[st] = lds0 + 256 * (lane & 31) + (16 * (h ^ i16) ^ 32 * st);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) vx[d] = lds0 + kV + 256 * (4 * h + (i16 >> 2)) + 32 * ((lane >> 4) & 1) + 8 * (i16 & 3) + (64 * (i16 >> 2) ^ 64 * d);
+      const auto k_part = [&](uint32_t of, int i) __attribute__((always_inline)) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(reinterpret_cast<lds_at>(kx[i >> 1] + of) + 8192 * (i & 1));
+      };
+      const auto v_part = [&](uint32_t of, int j) __attribute__((always_inline)) {
+        const lds_at at = reinterpret_cast<lds_at>(vx[j & 3] + of) + 4096 * (j >> 2);
+        const bf16x4_t lo = read_tr((lds_rows)at), hi = read_tr((lds_rows)(at + 2048));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      const auto scores_part = [&](int i, bf16x8_t k, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        f32x16_t zero;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zero[e] = 0.0f;
+        s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[i >> 1], i < 2 ? zero : s[i & 1], 0, 0, 0);
+      };
+      // probabilities 2 k and 2 k + 1 of the tile's 32 a lane: words of the second product's operand
+      u32x4_t p[4];
+      const auto pair = [&](int k, const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        const int t = k >> 2, e = 8 * (t & 1) + 2 * (k & 3);
+        const float p0 = fast_exp2(fmaf(s[t >> 1][e], a.scale, off)), p1 = fast_exp2(fmaf(s[t >> 1][e + 1], a.scale, off));
+        p[t][k & 3] = attn_bf16_pair(p0, p1);
+        sum[k & 3] = add_pair(p[t][k & 3], sum[k & 3]);
+      };
+      const auto outputs_part = [&](int j, bf16x8_t v) __attribute__((always_inline)) {
+        o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8_t, p[j >> 2]), o[j & 3], 0, 0, 0);
+      };
+      const auto hide = [&](int tile, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        if (tile * kKeys + kKeys - 1 > wmin) {  // keys past a query's position
+          const int lim = pos - tile * kKeys - 4 * h;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * b + 8 * (i >> 2) + (i & 3) > lim) s[b][i] = -INFINITY;
+        }
+      };
+      const auto largest = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        float m = s[0][0];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
+        return m;
+      };
+      // the reference moves where a score passes it too far
+      const auto move_to = [&](float m, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+        if (__builtin_amdgcn_ballot_w64(m > raw + slack) != 0ull) {
+          const float top = fmaxf(raw, m), mn = scaled_max(top, a.scale);
+          const float alpha = exp2_between(raw, top, scaled_max(raw, a.scale), mn, a.scale);
+          raw = top;
+          off = -mn;
+          far = __builtin_amdgcn_ballot_w64(fabsf(mn) > kFar && top > kNone) != 0ull;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] *= alpha;
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        }
+        if (far) {  // (differences before the scale)
+          off = 0.0f;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][i] -= raw;
+        }
+      };
+      const auto add_odd = [&](int tile) __attribute__((always_inline)) {
+        if (tile * kKeys + kKeys - 1 <= low) return;
+        for (unsigned long long odd = odd_keys[tile & 3]; odd != 0ull; odd &= odd - 1) {
+          // key j lies in result register 4 (j / 8) + j % 4 of lane half j / 4 % 2
+          const int j = __builtin_amdgcn_readfirstlane(__builtin_ctzll(odd)), e = 4 * (j >> 3) + (j & 3);
+          const int key = tile * kKeys + j;
+          const uint16_t* vp = a.v + pages.at(pages.page(key & ~15), key & ~15) + (key & 15) * kDim + 4 * h;
+          float w = 0.0f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (8 * t + i == e) w = static_cast<float>(__builtin_bit_cast(bf16x8_t, p[t])[i]);
+          w = __shfl(w, (lane & 31) + 32 * ((j >> 2) & 1), kWave);
+          if (key <= pos) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const uint2 v = *reinterpret_cast<const uint2*>(vp + 32 * d + 8 * g);
+                float x[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                add_nonfinite(w, v, x[0], x[1], x[2], x[3]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[d][4 * g + i] = x[i];
+                __builtin_amdgcn_sched_barrier(0);  // (a piece at a time: this path must not set the kernel's registers)
+              }
+          }
+        }
+      };
+
+      const int token = pos - len + rows.y, out_head = head * a.group + min(item * kChunkRows + wave * 32 + (lane & 31), line.q - 1) - token * a.group;
+      const uint16_t* qp = a.q + (rows.x + token) * a.q_row + out_head * kDim + 8 * h;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) q[s] = *reinterpret_cast<const bf16x8_t*>(qp + 16 * s);
+      look_up(first);
+      uint64_t at_v = 0;  // place of the tile whose V goes next
+      {
+        uint64_t at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at[i] = place(first + i);
+        bring_k(first, at[0]);
+        bring_v(first, at[0]);
+        bring_k(first + 1, at[1]);
+        bring_k(first + 2, at[2]);
+        bring_v(first + 1, at[1]);
+        bring_k(first + 3, at[3]);
+        bring_v(first + 2, at[2]);
+        at_v = at[3];
+      }
+      asm volatile("s_waitcnt vmcnt(12)" ::: "memory");  // K of the first tile
+      lds_barrier();
+      f32x16_t sa[2], sb[2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) scores_part(i, k_part(ring(first), i), sa);
+      hide(first, sa);
+      move_to(largest(sa), sa);
+      asm volatile("s_waitcnt vmcnt(6)" ::: "memory");  // all but V of the second and third, K of the fourth
+      lds_barrier();
+
+      // One tile: the next one's scores (matrix slots 0-15) and this one's outputs (16-31), with this one's exponentials and
+      // then the next one's maximum spread over the slots, so that the vector unit works in the matrix core's shadow.
+      // Fragments are read four slots ahead, the first four of the tile after that before the barrier: K arrives two tiles
+      // before its scores, V one before its outputs.  EDGE: some row of the workgroup does not see some key of this tile or
+      // the next.  The order is kept by hand: left to it, the compiler computes all exponentials at once.
+      bf16x8_t ahead[4];
+      const auto flow = [&](int tile, uint32_t v_at, uint32_t k_at, uint32_t k_then, f32x16_t (&now)[2], f32x16_t (&next)[2],
+                            auto edge_tag) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        bf16x8_t kf[16], vf[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kf[i] = ahead[i];
+        float m = kNone;
+        uint64_t at = 0;
+        slots(std::make_integer_sequence<int, 32>{}, [&](auto slot) __attribute__((always_inline)) {
+          constexpr int i = decltype(slot)::value;
+          if constexpr (i < 12)
+            kf[i + 4] = k_part(k_at, i + 4);
+          else if constexpr (i < 28)
+            vf[i - 12] = v_part(v_at, i - 12);
+          else
+            ahead[i - 28] = k_part(k_then, i - 28);
+          if constexpr (i < 16)
+            scores_part(i, kf[i], next);
+          else
+            outputs_part(i - 16, vf[i - 16]);
+          // 16 pairs over the slots 0-25 (operand t is complete well before slot 16 + 4 t)
+          constexpr int k = (3 * i + 2) / 5;
+          if constexpr (i < 26 && 5 * k / 3 == i) {
+            asm volatile("" : "+v"(off));  // (no pair is computed before its slot)
+            pair(k, now);
+          }
+          if constexpr (i == 2) bring_v(tile + 3, at_v);
+          if constexpr (i == 4) at = place(tile + 4);
+          if constexpr (i == 7) bring_k(tile + 4, at);
+          if constexpr (EDGE && i == 18) hide(tile + 1, next);
+          if constexpr (i >= 26 || i == 19 || i == 24) {  // 4 scores a time
+            constexpr int e = i >= 26 ? 2 + (i - 26) : (i == 19 ? 0 : 1);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) m = fmaxf(m, next[e >> 2][4 * (e & 3) + x]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        at_v = at;
+        if (EDGE) add_odd(tile);
+        if (tile + 1 < tiles) move_to(m, next);
+      };
+      const auto arrive = [&](int tile) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // (this wave's reads of what the next transfers replace are done: their results were used)
+        asm volatile("" ::: "memory");
+        if (tile + 8 >= at_from + kWave) look_up(tile + 5);
+      };
+      int tile = first;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ahead[i] = k_part(ring(tile + 1), i);
+      // (four tiles at a time: their places in the ring are constants, and the scores change places)
+      for (; tile + 4 <= tiles && min(tile + 5, tiles) * kKeys - 1 <= low; tile += 4) {
+        constexpr uint32_t kT = kTileBytes;
+        flow(tile, 0 * kT, 1 * kT, 2 * kT, sa, sb, std::false_type{});
+        arrive(tile);
+        flow(tile + 1, 1 * kT, 2 * kT, 3 * kT, sb, sa, std::false_type{});
+        arrive(tile + 1);
+        flow(tile + 2, 2 * kT, 3 * kT, 0 * kT, sa, sb, std::false_type{});
+        arrive(tile + 2);
+        flow(tile + 3, 3 * kT, 0 * kT, 1 * kT, sb, sa, std::false_type{});
+        arrive(tile + 3);
+      }
+      // The last tiles, of which some row does not see some key
+      mend(tile);
+      lds_barrier();
+      const auto last = [&](f32x16_t (&now)[2], f32x16_t (&next)[2]) __attribute__((always_inline)) {
+        if (tid == 0) odd_keys[(tile + 2) & 3] = 0ull;
+        if (tile < mine) {
+          flow(tile, ring(tile), ring(tile + 1), ring(tile + 2), now, next, std::true_type{});
+        } else {
+          bring_v(tile + 3, at_v);
+          at_v = place(tile + 4);
+          bring_k(tile + 4, at_v);
+        }
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        mend(tile + 1);
+        lds_barrier();
+        if (tile + 8 >= at_from + kWave) look_up(tile + 5);
+        ++tile;
+      };
+      while (tile < tiles) {
+        last(sa, sb);
+        if (tile < tiles) last(sb, sa);
+      }
+      if (lost != 0x7FFFFFFF && lane == 0) atomicMin(&no_page, lost);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is on its way into LDS when the workgroup ends)
+      lds_barrier();
     }
+
+    float l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    // NaN: a sequence longer than its table row, a key without a page
+    l += swap_half(l) + (len - 1 > pages.last || pos >= no_page ? NAN : 0.0f);
+    const PagedArgs e = args_again(args);
+    const int r = item * kChunkRows + wave * 32 + (lane & 31), token = pos - len + rows.y;
+    const bool valid = r < rows.y * e.group;
+    if (parts > 1) {
+      const int64_t part = static_cast<int64_t>(head) * e.slots + part_slot;
+      float* const op = e.part_o + ((part * kChunkWaves + wave) * 16 * kWave + lane) * 4;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(op + (4 * d + g) * kWave * 4) =
+              make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+      if (h == 0) e.part_ml[part * kChunkRows + wave * 32 + lane] = make_float2(pos >= first * kKeys ? raw : kUnseen, l);
+    } else if (valid) {
+      const float inv = pos >= 0 ? 1.0f / l : 0.0f;
+      uint16_t* op = e.o + (static_cast<int64_t>(rows.x + token) * e.heads + head * e.group + r - token * e.group) * kDim + 4 * h;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float y[4] = {o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+          *reinterpret_cast<uint2*>(op + 32 * d + 8 * g) = pair4(y, inv);
+        }
+    }
+    lds_barrier();  // (no_page and the tiles are the next part's)
+  }
+  const PagedArgs a = args_again(args);
+  if (a.aim > 0 && walk[wave].opens == 0 && head == 0 && tid == 0 && mine_index < a.aim) a.list[mine_index].ranges = 0;
+  clear_behind(a, head, mine_index, kChunkThreads);
 }
 
 __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
   // a wave's V rows of 256 bytes; 32-byte piece d of row r lies at d ^ (r % 8), so that the 16 rows of a transposed
-  // read cover all banks without padding 
+  // read cover all banks without padding
   __shared__ __attribute__((aligned(16))) uint16_t lds[kWaves][kStepKeys * kDim];
   __shared__ float2 wave_ml[kWaves][kStepRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
   const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
-  Work w{index, 0, 0, 1, 0, a.seqs};
-  if (a.aim > 0 ? !find_work<kStepRows, kStepKeys, kStepLeast, true, false>(a, head, index, w) : index >= a.seqs) {
-    clear_behind(a, head, index, w.total, kThreads);
-    return;
-  }
+  clear_behind(a, head, index, kThreads);
+  Work w{index, 0, 1, 0};
+  if (a.aim > 0 ? !find_work(a, head, index, w) : index >= a.seqs) return;
   const int seq = __builtin_amdgcn_readfirstlane(w.seq), ranges = __builtin_amdgcn_readfirstlane(w.ranges);
   const int2 rows = rows_of_one(a, seq);
   const int len = max(uniform(a.lens)[seq], 0);
@@ -912,46 +1028,97 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
   }
 }
 
-// Joins the key ranges of divided items of ROWS queries: a wave takes ROWS / gridDim.y / 4 rows of one KV head, 2 channels a
-// lane.  Range r's maximum and sum come to lane r in one load, and the ranges' rows are loaded eight at a time, so that a
+// Joins the key ranges of step_kernel's divided items: a wave takes a row of one KV head, 2 channels a lane.  Range r's maximum and sum come to lane r in one load, and the ranges' rows are loaded eight at a time, so that a
 // join costs two or three memory latencies (one load after another: 13 us for one row of 16 ranges).
-template <int ROWS>
 __global__ __launch_bounds__(kThreads) void join_kernel(PagedArgs a) {
   const int head = static_cast<int>(blockIdx.x) % a.kv, nth = static_cast<int>(blockIdx.x) / a.kv;
   if (nth >= *a.divided) return;
   const Divided d = a.list[nth];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int each = ROWS / kWaves / static_cast<int>(gridDim.y);
   const int64_t slot = static_cast<int64_t>(head) * a.slots + d.slot;
-  for (int i = 0; i < each; ++i) {
-    const int r = (static_cast<int>(blockIdx.y) * each + i) * kWaves + wave, q = d.item * ROWS + r;
-    if (q >= d.rows * a.group) return;
-    const int token = q / a.group;
-    const int64_t out = (static_cast<int64_t>(d.first + token) * a.heads + head * a.group + q - token * a.group) * kDim + 2 * lane;
-    const float2 ml = lane < d.ranges ? a.part_ml[(slot + lane) * ROWS + r] : make_float2(kUnseen, 0.0f);
-    const float* const part = a.part_o + (slot * ROWS + r) * kDim + 2 * lane;
-    const float top = wave_max(ml.x);
-    const bool seen = ml.x != kUnseen;
-    const float w = seen ? exp2_between(ml.x, top, scaled_max(ml.x, a.scale), scaled_max(top, a.scale), a.scale) : 0.0f;
-    const float l = wave_sum(seen ? w * ml.y : (ml.y != ml.y ? ml.y : 0.0f));
-    const unsigned long long parts = __builtin_amdgcn_ballot_w64(seen);
-    float o0 = 0.0f, o1 = 0.0f;
-    for (int base = 0; base < d.ranges; base += 8) {
-      float2 v[8];
+  const int r = static_cast<int>(blockIdx.y) * kWaves + wave;
+  if (r >= d.rows * a.group) return;
+  const int token = r / a.group;
+  const int64_t out = (static_cast<int64_t>(d.first + token) * a.heads + head * a.group + r - token * a.group) * kDim + 2 * lane;
+  const float2 ml = lane < d.ranges ? a.part_ml[(slot + lane) * kStepRows + r] : make_float2(kUnseen, 0.0f);
+  const float* const part = a.part_o + (slot * kStepRows + r) * kDim + 2 * lane;
+  const float top = wave_max(ml.x);
+  const bool seen = ml.x != kUnseen;
+  const float w = seen ? exp2_between(ml.x, top, scaled_max(ml.x, a.scale), scaled_max(top, a.scale), a.scale) : 0.0f;
+  const float l = wave_sum(seen ? w * ml.y : (ml.y != ml.y ? ml.y : 0.0f));
+  const unsigned long long parts = __builtin_amdgcn_ballot_w64(seen);
+  float o0 = 0.0f, o1 = 0.0f;
+  for (int base = 0; base < d.ranges; base += 8) {
+    float2 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        v[k] = (parts >> (base + k)) & 1 ? *reinterpret_cast<const float2*>(part + static_cast<int64_t>(base + k) * ROWS * kDim)
-                                         : make_float2(0.0f, 0.0f);
+    for (int k = 0; k < 8; ++k)
+      v[k] = (parts >> (base + k)) & 1 ? *reinterpret_cast<const float2*>(part + static_cast<int64_t>(base + k) * kStepRows * kDim)
+                                       : make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = row_lane(w, base + k);
-        o0 = fmaf(f, v[k].x, o0);
-        o1 = fmaf(f, v[k].y, o1);
-      }
+    for (int k = 0; k < 8; ++k) {
+      const float f = row_lane(w, base + k);
+      o0 = fmaf(f, v[k].x, o0);
+      o1 = fmaf(f, v[k].y, o1);
     }
-    const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
-    *reinterpret_cast<uint32_t*>(a.o + out) = attn_bf16_pair(o0 * inv, o1 * inv);
   }
+  const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint32_t*>(a.o + out) = attn_bf16_pair(o0 * inv, o1 * inv);
+}
+
+// Joins chunk_kernel's parts of the item that a slice opens: its slots are 2 i + 1, 2 (i + 1), 2 (i + 2) ..  A wave takes the
+// 32 queries of a wave of that kernel and 32 channels (blockIdx.y, wave), in its registers' order, so that all loads are of
+// whole kilobytes; four parts' at a time, under a running maximum.
+__global__ __launch_bounds__(kThreads) void join_slices_kernel(PagedArgs a) {
+  const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
+  const Divided item = a.list[index];
+  const int lane = threadIdx.x & 63, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, block = blockIdx.y;
+  const int r = item.item * kChunkRows + 32 * block + (lane & 31);
+  if (item.item * kChunkRows + 32 * block >= item.rows * a.group || item.ranges == 0) return;
+  constexpr int kAhead = 4;
+  float top = kUnseen, l = 0.0f, bad = 0.0f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+  for (int base = 0; base < item.ranges; base += kAhead) {
+    float2 ml[kAhead];
+    f32x4_t v[kAhead][4];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int range = min(base + k, item.ranges - 1);
+      const int64_t part = static_cast<int64_t>(head) * a.slots + item.slot + (range > 0 ? 2 * range - 1 : 0);
+      ml[k] = a.part_ml[part * kChunkRows + 32 * block + (lane & 31)];
+      const float* const p = a.part_o + (((part * kChunkWaves + block) * 16 + 4 * d) * kWave + lane) * 4;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) v[k][g] = *reinterpret_cast<const f32x4_t*>(p + g * kWave * 4);
+    }
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (base + k >= item.ranges) ml[k] = make_float2(kUnseen, 0.0f);
+      most = fmaxf(most, ml[k].x);
+    }
+    const float sm = scaled_max(most, a.scale);
+    const float keep = top == kUnseen ? 0.0f : exp2_between(top, most, scaled_max(top, a.scale), sm, a.scale);
+    l *= keep;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] *= keep;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const bool seen = ml[k].x != kUnseen;
+      if (!seen && ml[k].y != ml[k].y) bad = ml[k].y;
+      const float w = seen ? exp2_between(ml[k].x, most, scaled_max(ml[k].x, a.scale), sm, a.scale) : 0.0f;
+      l = seen ? fmaf(w, ml[k].y, l) : l;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = seen ? fmaf(w, v[k][i >> 2][i & 3], o[i]) : o[i];
+    }
+    top = most;
+  }
+  if (r >= item.rows * a.group) return;
+  l += bad;
+  const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
+  const int token = r / a.group;
+  uint16_t* const out = a.o + (static_cast<int64_t>(item.first + token) * a.heads + head * a.group + r - token * a.group) * kDim + 32 * d + 4 * h;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) *reinterpret_cast<uint2*>(out + 8 * g) = pair4(o + 4 * g, inv);
 }
 
 // How a call is launched: which kernel, and the room for divided items.
@@ -966,20 +1133,29 @@ Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t m
   Launch p{};
   // up to 16 queries of a KV head are one pass over its keys in step_kernel
   p.step = !starts || max_q * group <= kStepRows;
-  const int rows = p.step ? kStepRows : kChunkRows, unit = p.step ? kStepKeys : kKeys, least = p.step ? kStepLeast : kChunkLeast;
+  const int rows = p.step ? kStepRows : kChunkRows, unit = p.step ? kStepKeys : kKeys;
   const int64_t items = p.step ? seqs : (n * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs : 0);
-  p.aim = p.step ? kStepAim : kChunkAim;
-  // nothing is divided where the longest sequence is one range, or (one sequence, or single rows) items alone make as many
-  // workgroups as ranges would
   const int64_t steps = (max_kv + unit - 1) / unit;
-  if (steps <= least || ((p.step || seqs == 1) && items * kv >= p.aim)) p.aim = 0;
-  p.groups = items + (starts ? 1 : 0);
+  p.groups = items;
   p.ranges = 1;
-  if (p.aim == 0) return p;
-  p.ranges = static_cast<int>(std::min<int64_t>(kMaxRanges, (steps + least - 1) / least));
-  p.slots = static_cast<int>(std::min<int64_t>(2 * (p.aim / kv) + 8, items * p.ranges));
-  p.items = static_cast<int>(std::min<int64_t>(p.aim / kv + 8, items));
-  p.groups += p.slots;
+  if (p.step) {
+    // nothing is divided where the longest sequence is one range, or the sequences alone make as many workgroups as ranges would
+    if (steps <= kStepLeast || items * kv >= kStepAim) return p;
+    p.aim = kStepAim;
+    p.ranges = static_cast<int>(std::min<int64_t>(kMaxRanges, (steps + kStepLeast - 1) / kStepLeast));
+    p.slots = static_cast<int>(std::min<int64_t>(2 * (p.aim / kv) + 8, items * p.ranges));
+    p.items = static_cast<int>(std::min<int64_t>(p.aim / kv + 8, items));
+    p.groups += p.slots;
+  } else {
+    // One sequence's items are divided where they are fewer than the CUs.  Several sequences' always, as their lengths are not
+    // known here: whole items would be 5% faster where there are many of about one length (12 sequences of up to 2000 tokens
+    // over 8000, 8 query heads a KV head, 4 of these: 435 and 457 us), and as long as the longest where one is long.
+    const int64_t slices = std::min<int64_t>(kChunkAim / kv, (items * (steps + static_cast<int>(kApart)) + kLeastSteps - 1) / kLeastSteps);
+    if (slices < 2 || steps <= kLeastSteps || (seqs == 1 && items * kv >= kChunkAim)) return p;
+    p.aim = p.items = static_cast<int>(slices);
+    p.groups = p.aim;
+    p.slots = 2 * p.aim;
+  }
   p.list_at = 16;
   p.ml_at = (p.list_at + p.items * sizeof(Divided) + 15) / 16 * 16;
   p.o_at = p.ml_at + static_cast<size_t>(kv) * p.slots * rows * sizeof(float2);
@@ -1025,9 +1201,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   FL_REQUIRE(seqs > 0, "fl_paged_attention: rows without a sequence");
   Launch p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, max_kv, q_starts != nullptr);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < p.bytes) {
-    p.aim = 0;  // (no room for divided items: none is divided)
-    p.groups -= p.slots;
-    p.ranges = 1;
+    p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, 1, q_starts != nullptr);  // (no room for divided items: none is)
   }
   FL_REQUIRE(p.groups * kv_heads <= 0x7FFFFFFF / kChunkThreads, "fl_paged_attention: grid too large");
   uint8_t* const ws = static_cast<uint8_t*>(workspace);
@@ -1045,9 +1219,9 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   if (p.aim == 0) return FL_OK;
   const unsigned items = static_cast<unsigned>(p.items * kv_heads);
   if (p.step)
-    hipLaunchKernelGGL(join_kernel<kStepRows>, dim3(items, kStepRows / kWaves), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(join_kernel, dim3(items, kStepRows / kWaves), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL(join_kernel<kChunkRows>, dim3(items, 16), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(join_slices_kernel, dim3(items, kChunkWaves), dim3(kThreads), 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention(join)");
   return FL_OK;
 }

@@ -94,6 +94,22 @@ def test_many_sequences_of_unequal_lengths(rows, kv, step):
         assert attention_error(got, want, size, slack) <= 0
 
 
+@pytest.mark.parametrize("rows,before,heads,kv,page", [
+    ([20], [40000], 1, 1, 64),                                       # one item in as many parts as there may be
+    ([300, 1, 20, 700] * 20, [0, 2500, 31, 64] * 20, 2, 1, 32),      # more sequences than lanes, whole items and parts of them
+    ([1000, 3, 500], [0, 0, 60], 4, 4, 64),                          # items that see little in front of ones that see all
+    ([5] * 66 + [400], [0] * 66 + [7000], 3, 1, 128),                # almost all of the work behind the first 64 sequences
+    ([60, 0, 0, 61], [5000, 0, 17, 4999], 16, 2, 16),
+])
+def test_slices(rows, before, heads, kv, page):
+    print(f"case: slices {rows[:5]} {before[:5]} {heads}/{kv}", flush=True)
+    lens = [r + b for r, b in zip(rows, before)]
+    for behind in (0, 3):
+        got, want, size, slack = _attend(14, rows, lens, heads, kv, page, behind=behind)
+        assert attention_error(got, want, size, slack) <= 0
+        assert not got[sum(rows):].any()
+
+
 def test_hints_have_no_part_in_the_result():
     """max_q and max_kv that are too small or too large, and a call on one sequence of a batch."""
     print("case: hints", flush=True)
