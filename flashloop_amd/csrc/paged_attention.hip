@@ -1066,41 +1066,42 @@ __global__ __launch_bounds__(kThreads) void join_kernel(PagedArgs a) {
 }
 
 // Joins chunk_kernel's parts of the item that a slice opens: its slots are 2 i + 1, 2 (i + 1), 2 (i + 2) ..  A wave takes the
-// 32 queries of a wave of that kernel and 32 channels (blockIdx.y, wave), in its registers' order, so that all loads are of
-// whole kilobytes; four parts' at a time, under a running maximum.
+// 32 queries of a wave of that kernel and 16 channels, in its registers' order, so that all loads are of whole kilobytes; eight
+// parts' at a time, under a running maximum.
 __global__ __launch_bounds__(kThreads) void join_slices_kernel(PagedArgs a) {
   const int head = static_cast<int>(blockIdx.x) % a.kv, index = static_cast<int>(blockIdx.x) / a.kv;
   const Divided item = a.list[index];
-  const int lane = threadIdx.x & 63, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, block = blockIdx.y;
+  const int lane = threadIdx.x & 63, h = lane >> 5, block = blockIdx.y >> 1;
+  const int piece = (blockIdx.y & 1) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // of 16 channels
   const int r = item.item * kChunkRows + 32 * block + (lane & 31);
   if (item.item * kChunkRows + 32 * block >= item.rows * a.group || item.ranges == 0) return;
-  constexpr int kAhead = 4;
-  float top = kUnseen, l = 0.0f, bad = 0.0f, o[16];
+  constexpr int kAhead = 8;
+  float top = kUnseen, l = 0.0f, bad = 0.0f, o[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) o[i] = 0.0f;
+  for (int i = 0; i < 8; ++i) o[i] = 0.0f;
   for (int base = 0; base < item.ranges; base += kAhead) {
     float2 ml[kAhead];
-    f32x4_t v[kAhead][4];
+    f32x4_t v[kAhead][2];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      const int range = min(base + k, item.ranges - 1);
+      ml[k] = make_float2(kUnseen, 0.0f);
+      v[k][0] = v[k][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      const int range = base + k;
+      if (range >= item.ranges) continue;
       const int64_t part = static_cast<int64_t>(head) * a.slots + item.slot + (range > 0 ? 2 * range - 1 : 0);
       ml[k] = a.part_ml[part * kChunkRows + 32 * block + (lane & 31)];
-      const float* const p = a.part_o + (((part * kChunkWaves + block) * 16 + 4 * d) * kWave + lane) * 4;
+      const float* const p = a.part_o + (((part * kChunkWaves + block) * 16 + 2 * piece) * kWave + lane) * 4;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) v[k][g] = *reinterpret_cast<const f32x4_t*>(p + g * kWave * 4);
+      for (int g = 0; g < 2; ++g) v[k][g] = *reinterpret_cast<const f32x4_t*>(p + g * kWave * 4);
     }
     float most = top;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (base + k >= item.ranges) ml[k] = make_float2(kUnseen, 0.0f);
-      most = fmaxf(most, ml[k].x);
-    }
+    for (int k = 0; k < kAhead; ++k) most = fmaxf(most, ml[k].x);
     const float sm = scaled_max(most, a.scale);
     const float keep = top == kUnseen ? 0.0f : exp2_between(top, most, scaled_max(top, a.scale), sm, a.scale);
     l *= keep;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] *= keep;
+    for (int i = 0; i < 8; ++i) o[i] *= keep;
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const bool seen = ml[k].x != kUnseen;
@@ -1108,7 +1109,7 @@ __global__ __launch_bounds__(kThreads) void join_slices_kernel(PagedArgs a) {
       const float w = seen ? exp2_between(ml[k].x, most, scaled_max(ml[k].x, a.scale), sm, a.scale) : 0.0f;
       l = seen ? fmaf(w, ml[k].y, l) : l;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[i] = seen ? fmaf(w, v[k][i >> 2][i & 3], o[i]) : o[i];
+      for (int i = 0; i < 8; ++i) o[i] = seen ? fmaf(w, v[k][i >> 2][i & 3], o[i]) : o[i];
     }
     top = most;
   }
@@ -1116,9 +1117,9 @@ __global__ __launch_bounds__(kThreads) void join_slices_kernel(PagedArgs a) {
   l += bad;
   const float inv = top != kUnseen || l != l ? 1.0f / l : 0.0f;
   const int token = r / a.group;
-  uint16_t* const out = a.o + (static_cast<int64_t>(item.first + token) * a.heads + head * a.group + r - token * a.group) * kDim + 32 * d + 4 * h;
+  uint16_t* const out = a.o + (static_cast<int64_t>(item.first + token) * a.heads + head * a.group + r - token * a.group) * kDim + 16 * piece + 4 * h;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) *reinterpret_cast<uint2*>(out + 8 * g) = pair4(o + 4 * g, inv);
+  for (int g = 0; g < 2; ++g) *reinterpret_cast<uint2*>(out + 8 * g) = pair4(o + 4 * g, inv);
 }
 
 // How a call is launched: which kernel, and the room for divided items.
@@ -1221,7 +1222,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   if (p.step)
     hipLaunchKernelGGL(join_kernel, dim3(items, kStepRows / kWaves), dim3(kThreads), 0, st, a);
   else
-    hipLaunchKernelGGL(join_slices_kernel, dim3(items, kChunkWaves), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(join_slices_kernel, dim3(items, 2 * kChunkWaves), dim3(kThreads), 0, st, a);
   FL_LAUNCH_CHECK("fl_paged_attention(join)");
   return FL_OK;
 }
