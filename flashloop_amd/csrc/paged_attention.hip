@@ -989,7 +989,7 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
     float* const wo = reinterpret_cast<float*>(vl);
     static_assert(kStepRows * kDim * sizeof(float) <= kStepKeys * kDim * sizeof(uint16_t), "a wave's outputs fit its V rows");
 #pragma unroll
-    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&wo[c * kDim + 16 * d + 4 * g]) = o[d];
+    for (int d = 0; d < 8; ++d) *reinterpret_cast<f32x4_t*>(&wo[c * kDim + 4 * ((4 * d + g) ^ c)]) = o[d];  // (16-byte piece p at p ^ c)
     lds_barrier();
     const int jr = tid >> 4, ch = 8 * (tid & 15);
     if (base + jr < rows.y * a.group) {
@@ -1004,9 +1004,10 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
         if (ml.x == kUnseen) continue;
         const float f = exp2_between(ml.x, top, scaled_max(ml.x, a.scale), st, a.scale);
         sum = fmaf(f, ml.y, sum);
-        const float* src = reinterpret_cast<const float*>(lds[w]) + jr * kDim + ch;
+        const float* src = reinterpret_cast<const float*>(lds[w]) + jr * kDim;
+        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(src + 4 * (ch / 4 ^ jr)), hi = *reinterpret_cast<const f32x4_t*>(src + 4 * ((ch / 4 + 1) ^ jr));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, i < 4 ? lo[i & 3] : hi[i & 3], acc[i]);
       }
       const int tok = (base + jr) / a.group, oh = head * a.group + base + jr - tok * a.group;
       const int64_t orow = static_cast<int64_t>(rows.x + tok) * a.heads + oh;

@@ -17,7 +17,8 @@
  * replaces.
  *
  * Fixed geometry (flashloop/config.py:18-65, 92-134): head_dim 128, 4-bit codes,
- * group 64, multi-head attention (query heads == KV heads), at most 4 loops.
+ * group 64, multi-head attention (query heads == KV heads), at most 4 loops.  (K/V pages, at the end of this
+ * file, take grouped heads and any number of loops.)
  */
 #ifndef FLASHLOOP_AMD_H
 #define FLASHLOOP_AMD_H
@@ -613,9 +614,10 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  * from 16 to 1024.  page_table i32 [seqs, table_width] names the pages of each sequence in order (entries
  * past its last page are not read), kv_lens i32 [seqs] counts its tokens, those of the call among them.  A
  * call's rows are tokens of several sequences one after another: q_starts i32 [seqs + 1] is non-decreasing
- * from 0, rows q_starts[s] .. q_starts[s + 1] - 1 are the last tokens of sequence s (q_starts NULL: one row a
- * sequence); rows from q_starts[seqs] on belong to none.  All of these lie in device memory.  A page that
- * several sequences name (a common prompt) is read by all of them; only one may append to it.
+ * from 0 (else what is stored and returned is unspecified), rows q_starts[s] .. q_starts[s + 1] - 1 are the last
+ * tokens of sequence s (q_starts NULL: one row a sequence); rows from q_starts[seqs] on belong to none.  All of
+ * these lie in device memory.  A page that several sequences name (a common prompt) is read by all of them; only
+ * one may append to it.
  *
  * fl_paged_append: rotate-half rotary embedding of the rows of q (to q_out, which may be q) and k with row p
  * of rope_cos / rope_sin ([rope_positions, 128], bf16 or f32, both halves of a row alike or not) at position
@@ -631,8 +633,8 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  * position is negative) and rows that belong to no sequence are zeros; a row that sees a key without a page
  * is NaN.  max_q and max_kv, the most rows and tokens of a sequence, choose how the work is divided and change
  * no result beyond rounding; larger ones than there are only cost time, and so do smaller ones.  With a
- * workspace (16-byte aligned, of fl_paged_attention_workspace bytes; nullable) calls of few rows divide the
- * keys over several workgroups and join them; a smaller one divides them less.
+ * workspace (16-byte aligned, of fl_paged_attention_workspace bytes; nullable) calls whose rows are too few or too
+ * unequal for the chip divide the keys over several workgroups and join them; with none or a smaller one they do not.
  *
  * fl_beam_select: the `count` (at most 64) best continuations of each sequence's beams (at most 64):
  *   total[k, t] = scores[s, k] + x[k, t] - log(sum_t exp(x[k, t])),  x = logits[s * beams + k] (f32 or bf16)
