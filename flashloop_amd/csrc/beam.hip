@@ -280,24 +280,24 @@ __device__ __forceinline__ unsigned long long image(double v) {
 }
 
 template <int CTRL>
-__device__ __forceinline__ unsigned long long dpp_max(unsigned long long v) {
-  const unsigned lo = static_cast<unsigned>(dpp_i<CTRL>(static_cast<int>(v)));
-  const unsigned hi = static_cast<unsigned>(dpp_i<CTRL>(static_cast<int>(v >> 32)));
-  const unsigned long long u = (static_cast<unsigned long long>(hi) << 32) | lo;
-  return u > v ? u : v;
-}
-__device__ __forceinline__ unsigned long long lane_of(unsigned long long v, int l) {
-  return (static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), l))) << 32) |
-         static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), l));
-}
-__device__ __forceinline__ unsigned long long wave_max64(unsigned long long v) {
+__device__ __forceinline__ unsigned dpp_max(unsigned v) { return max(v, static_cast<unsigned>(dpp_i<CTRL>(static_cast<int>(v)))); }
+__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
   v = dpp_max<kDppXor1>(v);
   v = dpp_max<kDppXor2>(v);
   v = dpp_max<kDppHalfMirror>(v);
   v = dpp_max<kDppMirror>(v);
-  const unsigned long long a = lane_of(v, 0), b = lane_of(v, 16), c = lane_of(v, 32), d = lane_of(v, 48);
-  const unsigned long long e = a > b ? a : b, f = c > d ? c : d;
-  return e > f ? e : f;
+  const auto row = [&](int l) __attribute__((always_inline)) { return static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(v), l)); };
+  return max(max(row(0), row(16)), max(row(32), row(48)));
+}
+// lanes with the largest key; none where all are 0
+__device__ __forceinline__ unsigned long long lanes_of_max(unsigned long long key) {
+  const unsigned hi = static_cast<unsigned>(key >> 32), lo = static_cast<unsigned>(key);
+  const unsigned top = wave_max_u32(hi);
+  const bool first = hi == top && key != 0ull;
+  const unsigned long long who = __builtin_amdgcn_ballot_w64(first);
+  if ((who & (who - 1)) == 0ull) return who;
+  const unsigned rest = first ? lo : 0u, most = wave_max_u32(rest);  // (by all lanes)
+  return __builtin_amdgcn_ballot_w64(first && rest == most);
 }
 
 // One sequence: list `lane` is part lane % parts of beam lane / parts, so equal candidates go to the lower lane.
@@ -337,8 +337,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamArgs a) {
   };
   look();
   for (int n = 0; n < a.count; ++n) {
-    const unsigned long long best = wave_max64(key);
-    const unsigned long long who = __builtin_amdgcn_ballot_w64(key == best && key != 0ull);
+    const unsigned long long who = lanes_of_max(key);
     if (who == 0ull) break;
     int winner = __builtin_ctzll(who);
     // totals of one beam may be equal in 64 bits where its logits are not: the logits decide
