@@ -89,28 +89,29 @@ __device__ __forceinline__ double scale_to(float shift, float top) {
 // a comes before b
 __device__ __forceinline__ bool before(float av, int ai, float bv, int bi) { return av > bv || (av == bv && ai < bi); }
 
-// x[kPer] <- values at index .. of the row; past `end`: -inf.  Four neighbouring values a lane and load.
-template <bool F32, bool ALIGNED>
+// x[kPer] <- values at index `from` .. of the row, four neighbouring ones a lane and load.  WHOLE: all of the chunk lie before
+// `end`; else those past it are -inf.
+template <bool F32, bool ALIGNED, bool WHOLE>
 __device__ __forceinline__ void load_values(const BeamArgs& a, int64_t row, int from, int end, float* x) {
+  const float* const wide = static_cast<const float*>(a.logits) + row * a.row_stride;
+  const uint16_t* const half = static_cast<const uint16_t*>(a.logits) + row * a.row_stride;
 #pragma unroll
   for (int j = 0; j < kPer / 4; ++j) {
     const int at = from + j * 4 * kWave;
-    const int64_t p = row * a.row_stride + at;
-    if (ALIGNED && at + 3 < end) {
-      if (F32) {
-        const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.logits) + p);
-        x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.logits) + p);
-        x[4 * j] = bf16lo_to_f32(v.x), x[4 * j + 1] = bf16hi_to_f32(v.x);
-        x[4 * j + 2] = bf16lo_to_f32(v.y), x[4 * j + 3] = bf16hi_to_f32(v.y);
-      }
+    if (ALIGNED && WHOLE && F32) {
+      const float4 v = *reinterpret_cast<const float4*>(wide + at);
+      x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
+    } else if (ALIGNED && WHOLE) {
+      const uint2 v = *reinterpret_cast<const uint2*>(half + at);
+      x[4 * j] = bf16lo_to_f32(v.x), x[4 * j + 1] = bf16hi_to_f32(v.x);
+      x[4 * j + 2] = bf16lo_to_f32(v.y), x[4 * j + 3] = bf16hi_to_f32(v.y);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[4 * j + i] = at + i >= end ? -INFINITY
-                       : F32         ? static_cast<const float*>(a.logits)[p + i]
-                                     : bf16_to_f32(static_cast<const uint16_t*>(a.logits)[p + i]);
+      for (int i = 0; i < 4; ++i) {
+        const int one = WHOLE ? at + i : min(at + i, end - 1);
+        const float v = F32 ? wide[one] : bf16_to_f32(half[one]);
+        x[4 * j + i] = WHOLE || at + i < end ? v : -INFINITY;
+      }
     }
   }
 }
@@ -138,8 +139,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
     float x[kChunks][kPer], mx = -INFINITY;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
-      if (base + c * kBeamChunk < end) {
-        load_values<F32, ALIGNED>(a, row, from + c * kBeamChunk, end, x[c]);
+      if (base + (c + 1) * kBeamChunk <= end) {
+        load_values<F32, ALIGNED, true>(a, row, from + c * kBeamChunk, end, x[c]);
+      } else if (base + c * kBeamChunk < end) {
+        load_values<F32, ALIGNED, false>(a, row, from + c * kBeamChunk, end, x[c]);
       } else {
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[c][e] = -INFINITY;
@@ -237,22 +240,39 @@ __global__ __launch_bounds__(kBeamThreads) void beam_part_kernel(BeamArgs a) {
       __syncthreads();
     }
     // an entry's place is the number of entries before it
-    const auto put = [&](Entry one) __attribute__((always_inline)) {
-      int place = 0;
+#pragma unroll
+    for (int w = 0; w < kBeamWaves; ++w) total += count[w];
+    if (total <= kWave) {  // an entry a lane (what LDS would give one after the other comes from the lanes: 2.4 -> 0.5 us)
+      if (wave == 0) {
+        Entry one = earlier[min(lane, kMaxCount - 1)];
+        int at = lane - held;
+#pragma unroll
+        for (int w = 0; w < kBeamWaves; ++w) {
+          if (at >= 0 && at < count[w]) one = gathered[w][at];
+          at -= count[w];
+        }
+        int place = 0;
 #pragma unroll 4
-      for (int j = 0; j < held; ++j) place += before(earlier[j].value, earlier[j].index, one.value, one.index) ? 1 : 0;
+        for (int l = 0; l < total; ++l)
+          place += before(row_lane(one.value, l), __builtin_amdgcn_readlane(one.index, l), one.value, one.index) ? 1 : 0;
+        if (lane < total && place < a.count) best[place] = one;
+      }
+    } else {
+      const auto put = [&](Entry one) __attribute__((always_inline)) {
+        int place = 0;
+#pragma unroll 4
+        for (int l = 0; l < held; ++l) place += before(earlier[l].value, earlier[l].index, one.value, one.index) ? 1 : 0;
+#pragma unroll
+        for (int w = 0; w < kBeamWaves; ++w)
+#pragma unroll 4
+          for (int l = 0; l < count[w]; ++l) place += before(gathered[w][l].value, gathered[w][l].index, one.value, one.index) ? 1 : 0;
+        if (place < a.count) best[place] = one;
+      };
+      if (tid < held) put(earlier[tid]);
 #pragma unroll
       for (int w = 0; w < kBeamWaves; ++w)
-#pragma unroll 4
-        for (int j = 0; j < count[w]; ++j) place += before(gathered[w][j].value, gathered[w][j].index, one.value, one.index) ? 1 : 0;
-      if (place < a.count) best[place] = one;
-    };
-    if (tid < held) put(earlier[tid]);
-#pragma unroll
-    for (int w = 0; w < kBeamWaves; ++w) {
-      if (w == wave)
-        for (int i = lane; i < count[w]; i += kWave) put(gathered[w][i]);
-      total += count[w];
+        if (w == wave)
+          for (int l = lane; l < count[w]; l += kWave) put(gathered[w][l]);
     }
     held = min(a.count, total);
     __syncthreads();
