@@ -8,11 +8,11 @@
 // reach it can be among the largest: 18 of 12288 normal values for 16.  They are gathered in LDS and placed by
 // counting.  Rows in which more values reach it than LDS holds (equal ones, masked ones) are inserted one by one
 // into sorted lists, an entry a lane.  A second launch joins the parts of a sequence's beams, one list a lane.
-// 256 rows of 49152 f32 values (50 MB), 16 results of each eight: 24.5 + 7.5 us.  The bytes are 10 us of them, the
-// exponentials in 64 bits 6, the values to reach and the gathering 5; the workgroups all pass these one after the other, as
-// they are on the chip together.  One sequence of four beams: 7.7 + 5.0 us, latencies; the join compares the
-// lists' heads once a result, 0.3 us each (gathering what reaches the count-th largest head and counting places: 20 us
-// slower, as the lists of a beam that leads hold most of their entries past it).
+// 256 rows of 49152 f32 values (50 MB), 16 results of each eight: 21.9 + 6.6 us (bf16: as long; 512 rows of bf16 45).  The
+// bytes are 10 us of it, the exponentials in 64 bits 6, what follows a workgroup's last value 4 (what to reach 0.7, gathering
+// 1.5, placing 1.2 in four barriers).  One sequence of four beams: 7.5 + 4.5 us, latencies; the join compares the lists'
+// heads once a result, 0.2 us each (gathering what reaches the count-th largest head and counting places: 20 us slower, as
+// the lists of a beam that leads hold most of their entries past it).
 //
 // The sums and totals are in 64 bits: totals of different beams decide the order among nearly equal
 // candidates, and 32 bits would leave it to the order of the sum.  Within a beam the logits decide.
@@ -56,22 +56,20 @@ struct BeamArgs {
   int64_t* out_tokens;
 };
 
-// exp(t), t <= 600, to 1e-11 of it: t = k ln 2 + r, |r| <= ln 2 / 2, and the series of exp(r) up to r^9.
+// exp(t), t <= 600, to 2e-12 of it: t log2(e) = k + f, |f| <= 1/2, and the polynomial through 2^f at the nine Chebyshev
+// points of [-1/2, 1/2] (1.1e-12; the series takes a degree more and a step more to its argument).
 __device__ __forceinline__ double exp64(double t) {
-  t = fmax(t, -800.0);
-  const double k = rint(t * 1.4426950408889634);
-  double r = fma(k, -0.69314718055994529, t);
-  r = fma(k, -2.3190468138462996e-17, r);
-  double p = 1.0 / 362880;
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
+  t = fmax(t, -800.0) * 1.4426950408889634;
+  const double k = rint(t), f = t - k;
+  double p = 1.325497460306718e-06;
+  p = fma(p, f, 1.531007807039615e-05);
+  p = fma(p, f, 0.00015403457039410448);
+  p = fma(p, f, 0.0013333450573018062);
+  p = fma(p, f, 0.009618129157656703);
+  p = fma(p, f, 0.055504109412010456);
+  p = fma(p, f, 0.24022650695821055);
+  p = fma(p, f, 0.6931471805459343);
+  p = fma(p, f, 1.0);  // (as exp(0) should be)
   return ldexp(p, static_cast<int>(k));
 }
 
