@@ -5,13 +5,13 @@
 //
 //  * chunk_kernel: chunks of new tokens.  A workgroup has 256 queries in eight waves, one workgroup a CU; S^T and O^T on
 //    v_mfma_f32_32x32x16_bf16, 64 keys a step, K and V through a ring of four tiles in LDS that transfers without registers
-//    fill.  A long prompt (8192 tokens, 16 heads) 259-265 us: 1040 TFLOP/s of the causal half, matrix cores busy 49%.  On the
+//    fill.  A long prompt (8192 tokens, 16 heads) 258-279 us by the card: 990-1070 TFLOP/s of the causal half, matrix cores busy 49%.  On the
 //    same transfers with no arithmetic between the products it runs at 1550 TFLOP/s of those it has (the card's power sets that
 //    rate); the rest are the exponentials and the roundings to bf16 in the products' shadow, one behind the other in a wave.
 //  * step_kernel: few queries a sequence (one decode step).  A wave owns steps of 32 keys and up to 16
 //    queries on v_mfma_f32_16x16x32_bf16: K goes from memory into the first product's operand, V through a
 //    part of LDS of the wave's own, the next step's loads in flight, no barrier until the waves' join.  Bound by bytes: 32
-//    sequences of up to 8192 tokens, 16 heads, 183 us, 5.6 TB/s.  One sequence of 2048 tokens takes 8 us, five memory latencies.
+//    sequences of up to 8192 tokens, 16 heads, 185 us, 5.6 TB/s.  One sequence of 2048 tokens takes 7 us, five memory latencies.
 //  * join_kernel and join_slices_kernel join the parts where a launch divides keys.
 //
 // A key that a row does not see has no part in its result, whatever its K and V rows hold: scores are
