@@ -639,9 +639,10 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  * fl_beam_select: the `count` (at most 64) best continuations of each sequence's beams (at most 64):
  *   total[k, t] = scores[s, k] + x[k, t] - log(sum_t exp(x[k, t])),  x = logits[s * beams + k] (f32 or bf16)
  * in descending order, ties to the lower beam, then the lower token.  Sums and totals are in 64 bits (out_scores:
- * rounded to f32); where totals of one beam are equal in 64 bits and its logits are not, the logits decide.  A
- * beam whose score is not finite, or whose row holds a NaN or +inf or nothing but -inf, has totals of -inf: its
- * tokens come after all others, in order.  out_scores f32, out_beams i32, out_tokens i64: [seqs, count].
+ * rounded to f32; the sums to 1e-11, so that totals of two beams closer than that may come in either order); where
+ * totals of one beam are equal in 64 bits and its logits are not, the logits decide.  A beam whose score is not
+ * finite, or whose row holds a NaN or +inf or nothing but -inf, has totals of -inf: its tokens come after all
+ * others, in order.  out_scores f32, out_beams i32, out_tokens i64: [seqs, count].
  *
  * fl_paged_reorder: beam k of each sequence takes over the state of beam parents[s, k] (i32, 0 .. beams - 1;
  * at most 64 beams) before its next token.  k_pages / v_pages are those of `layers` layers, [layers, pages,
