@@ -430,7 +430,10 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs first
     const int all = end >= 0 ? end / kKeys + 1 : 0;
     int tiles = all, first = 0, parts = 1;  // this slice's; slices of the item
     if (a.aim > 0) {
-      const double apart = kApart * kKeys * a.group, scale = all / (ends - begins - apart);
+      // scale: steps a unit of the line, never less than a step for each 64 keys of it.  An item that sees fewer keys than its
+      // length stands for (rows in front of the sequence's first key, a length past the table) would else be spread so thin
+      // that a slice in its middle gets no step, and the join would read a part that no workgroup has written.
+      const double apart = kApart * kKeys * a.group, scale = fmax(all / (ends - begins - apart), 1.0 / (kKeys * a.group));
       const auto cut = [&](double at) __attribute__((always_inline)) { return cut_at(at, begins, ends, apart, scale, all); };
       first = __builtin_amdgcn_readfirstlane(x_begin <= begins ? 0 : cut(x_begin));
       tiles = __builtin_amdgcn_readfirstlane(cut(x_end));

@@ -1,0 +1,64 @@
+"""Attention over K/V pages where its work is divided in unusual ways, against 64 bits."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from flashloop_amd import _lib, kernels  # noqa: E402
+from paged_util import DIM, attention_error, make_pool, plain_attention  # noqa: E402
+
+DEV = "cuda"
+SCALING = DIM**-0.5
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _starts(rows):
+    out = [0]
+    for r in rows:
+        out.append(out[-1] + r)
+    return out
+
+
+def _on_workspace(fill, q, kp, vp, table, lens, starts, max_q, max_kv):
+    """The C call on a workspace whose bytes are ``fill`` before it."""
+    lib = _lib.load()
+    (n, cols), (pages, kv, page, _), (seqs, width) = q.shape, kp.shape, table.shape
+    heads = cols // DIM
+    size = lib.fl_paged_attention_workspace(n, seqs, heads, kv, max_q, max_kv)
+    assert size > 0  # (keys are divided)
+    ws = torch.full((size,), fill, dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(q)
+    rc = lib.fl_paged_attention(q.data_ptr(), q.stride(0), kp.data_ptr(), vp.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
+                                starts.data_ptr(), n, seqs, heads, kv, width, pages, page, max_q, max_kv, SCALING, ws.data_ptr(), size,
+                                torch.cuda.current_stream().cuda_stream)
+    _lib.check(rc, "fl_paged_attention")
+    torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("rows,lens,heads,kv", [
+    ([2951, 1605], [402, 2107], 1, 1),
+    ([5, 1, 2844], [686, 1966, 284], 4, 2),
+    ([4324, 4544, 1, 5], [3216, 854, 1, 2], 1, 1),
+])
+def test_divided_items_of_sequences_shorter_than_their_rows(rows, lens, heads, kv):
+    """Many rows in front of a sequence's first key, in a call whose keys are divided: every part that is joined was
+    written by the same call, whatever the workspace held."""
+    print(f"case: divided, short lens {rows} {lens} {heads}/{kv}", flush=True)
+    g = _gen(1)
+    starts = _starts(rows)
+    (kp, vp), table, (keys, values) = make_pool(g, lens, -(-max(lens) // 64) + 1, 64, kv, DEV)
+    q = torch.randn(starts[-1], heads, DIM, generator=g, device=DEV).bfloat16()
+    want, size, slack = plain_attention(q, keys, values, lens, starts, SCALING)
+    for fill in (255, 0, 64):  # NaN, zeros, finite values
+        got = _on_workspace(fill, q.flatten(1), kp, vp, table, _ints(lens), _ints(starts), max(rows), max(lens)).view_as(q)
+        assert got.isfinite().all(), fill
+        assert attention_error(got, want, size, slack) <= 0, fill
