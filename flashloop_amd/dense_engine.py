@@ -186,6 +186,8 @@ class DenseEngine:
             hid, act = kernels.gemv_chain(hid, list(w[4:6]), x=kernels.gemv(o, [w[3]]), w_a=w[8], w_b=w[9], eps=eps,
                                           epilogue=kernels.EPI_SWIGLU)
             pending = dict(x=kernels.gemv(act, [w[6]]), w_a=w[10], w_f=final, w_b=nxt)
+        if head.shape[0] % 4:  # (the fused product takes multiples of 4 outputs)
+            return out.copy_(F.linear(kernels.norm_chain(hid, eps=eps, **pending)[0], head))
         _, logits = kernels.gemv_chain(hid, [head], eps=eps, epilogue=kernels.EPI_F32, out=out, **pending)
         return logits
 
