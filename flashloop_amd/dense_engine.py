@@ -267,9 +267,17 @@ class DenseEngine:
             raise ValueError(f"sequence {counts.index(min(counts))} has no tokens")
         if decode_capacity < 0:
             raise ValueError(f"decode_capacity={decode_capacity} is negative")
-        self._begin(input_ids, counts, decode_capacity, 1)
-        logits = self._feed(input_ids, counts, list(range(len(counts))))
+        logits = self._first(input_ids, counts, decode_capacity, 1)
         return DenseOutput(logits, self.positions)
+
+    def _first(self, input_ids: torch.Tensor, counts: list[int], extra: int, beams: int) -> torch.Tensor:
+        """Prompts into a new cache, each on the first of its beams' rows; no cache is left if that fails."""
+        try:
+            self._begin(input_ids, counts, extra, beams)
+            return self._feed(input_ids, counts, list(range(0, len(counts) * beams, beams)))
+        except BaseException:
+            self.reset()
+            raise
 
     @torch.inference_mode()
     def extend(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None) -> DenseOutput:
@@ -281,7 +289,13 @@ class DenseEngine:
         if min(counts) < 1:
             raise ValueError(f"sequence {counts.index(min(counts))} has no tokens")
         self._room(counts)
-        logits = self._feed(input_ids, counts, list(range(len(counts))))
+        before = list(self._lens)
+        try:
+            logits = self._feed(input_ids, counts, list(range(len(counts))))
+        except BaseException:  # (what was fed lies behind the sequences' ends, where the next call writes)
+            self._lens = before
+            self._lengths_to_device()
+            raise
         return DenseOutput(logits, self.positions)
 
     def _need(self) -> None:
@@ -304,38 +318,50 @@ class DenseEngine:
         if tuple(token_ids.shape) != (rows, 1):
             raise ValueError(f"decode requires token_ids of shape ({rows}, 1)")
         self._room([1] * rows)
-        c = self.cache
-        if self._out is None:
-            self._out = torch.empty(rows, self.config.vocab_size, dtype=torch.float32, device=c.lens.device)
-            self._tok = torch.zeros(rows, 1, dtype=torch.long, device=c.lens.device)
-            self._pos = (c.lens - 1).long()[:, None]  # (of the last token: a step writes the next)
-        self._tok.copy_(token_ids)
-        if self.use_graphs:
-            if self._graph is None:
-                self._capture()
-            self._graph.replay()
-            logits = self._out
-        else:
-            logits = self._step(torch.empty_like(self._out))
+        try:
+            logits = self._advance(token_ids)
+        except BaseException:  # (a step counts its token before it runs)
+            self._release()
+            self._lengths_to_device()
+            raise
         self._lens = [t + 1 for t in self._lens]
         return DenseOutput(logits, self.positions)
+
+    def _advance(self, token_ids: torch.Tensor) -> torch.Tensor:
+        rows, dev = len(self._lens), self.cache.lens.device
+        if self._out is None:
+            self._out = torch.empty(rows, self.config.vocab_size, dtype=torch.float32, device=dev)
+            self._tok = torch.zeros(rows, 1, dtype=torch.long, device=dev)
+            self._pos = (self.cache.lens - 1).long()[:, None]  # (of the last token: a step writes the next)
+        self._tok.copy_(token_ids)
+        if not self.use_graphs:
+            return self._step(torch.empty_like(self._out))
+        if self._graph is None:
+            self._capture()
+        self._graph.replay()
+        return self._out
 
     def _capture(self) -> None:
         """Capture a step (lengths live on the device).  A warm-up on a side stream sizes workspaces and library
         handles; it writes the rows that the replay writes again."""
         side = torch.cuda.Stream()  # default priority
         side.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(side):
-            self._step(self._out)
-            self.cache.lens.sub_(1)
-            self._pos.sub_(1)
-        torch.cuda.current_stream().wait_stream(side)
+        try:
+            with torch.cuda.stream(side):
+                self._step(self._out)
+                self.cache.lens.sub_(1)
+                self._pos.sub_(1)
+        finally:
+            torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         was_enabled = gc.isenabled()
         gc.disable()  # (a graph destroyed by a collection during a capture aborts the process)
         try:
             with torch.cuda.graph(graph):
                 self._step(self._out)
+        except BaseException:
+            graph.reset()
+            raise
         finally:
             if was_enabled:
                 gc.enable()
@@ -388,8 +414,7 @@ class DenseEngine:
         if min(counts) < 1:
             raise ValueError(f"sequence {counts.index(min(counts))} has no tokens")
         bsz, dev = len(counts), input_ids.device
-        self._begin(input_ids, counts, new, k)
-        logits = self._feed(input_ids, counts, [b * k for b in range(bsz)]).repeat_interleave(k, dim=0)
+        logits = self._first(input_ids, counts, new, k).repeat_interleave(k, dim=0)
         self._lens = [n for n in counts for _ in range(k)]
         self._lengths_to_device()
         scores = torch.full((bsz, k), -torch.inf, device=dev)  # (the beams are one until they part)

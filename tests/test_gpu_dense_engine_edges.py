@@ -42,3 +42,67 @@ def test_vocabularies_of_any_size(vocab, rows):
                 _near(out.logits[b], model.dense_forward(ids[b: b + 1, : t + 1])[0], (graphs, t, b))
     engine.reset()
     assert [len(o) for o in engine.generate(ids, max_new_tokens=4, num_beams=2)] == [16] * rows
+
+
+class _Stop(Exception):
+    pass
+
+
+def _stops_at(monkeypatch, name, calls):
+    """kernels.<name> raises at its ``calls``-th call from now on, once."""
+    from flashloop_amd import kernels
+
+    plain, left = getattr(kernels, name), [calls]
+
+    def call(*a, **kw):
+        left[0] -= 1
+        if left[0] == 0:
+            raise _Stop(name)
+        return plain(*a, **kw)
+
+    monkeypatch.setattr(kernels, name, call)
+
+
+@pytest.mark.parametrize("rows", [2, 9])
+@pytest.mark.parametrize("graphs,calls", [(False, 3), (True, 3), (True, 11)])
+def test_steps_that_fail_leave_the_sequences_as_they_were(monkeypatch, rows, graphs, calls):
+    """A step that raises half-way, in its warm-up and in its capture (8 layers and loops): positions, lengths on the
+    device and the cache are those before it, and the next steps are the same as without it."""
+    print(f"case: dense engine failing step rows {rows} graphs {graphs} calls {calls}", flush=True)
+    model = OuroForCausalLM.random_init(TINY, seed=12, device="cuda")
+    ids = _ids(rows, 20, TINY.vocab_size)
+    engine, plain = (DenseEngine(model, use_graphs=graphs, page_size=16) for _ in range(2))
+    for e in (engine, plain):
+        e.prefill(ids[:, :14], decode_capacity=8)
+    with monkeypatch.context() as m:
+        _stops_at(m, "paged_attention", calls)
+        with pytest.raises(_Stop):
+            engine.decode(ids[:, 14:15])
+    assert engine.positions == (14,) * rows and engine.cache.lens.tolist() == [14] * rows
+    for t in range(14, 17):
+        assert torch.equal(engine.decode(ids[:, t: t + 1]).logits, plain.decode(ids[:, t: t + 1]).logits), t
+    # more tokens that stop in their second chunk
+    engine.chunk = 2 * rows - 1
+    with monkeypatch.context() as m:
+        _stops_at(m, "paged_attention", 8 + 3)
+        with pytest.raises(_Stop):
+            engine.extend(ids[:, 17:19])
+    assert engine.positions == (17,) * rows and engine.cache.lens.tolist() == [17] * rows
+    engine.chunk = plain.chunk
+    assert torch.equal(engine.extend(ids[:, 17:19]).logits, plain.extend(ids[:, 17:19]).logits)
+    assert torch.equal(engine.decode(ids[:, 19:20]).logits, plain.decode(ids[:, 19:20]).logits)
+
+
+def test_prompts_that_fail_leave_no_cache(monkeypatch):
+    print("case: dense engine failing prompt", flush=True)
+    model = OuroForCausalLM.random_init(TINY, seed=13, device="cuda")
+    ids = _ids(2, 9, TINY.vocab_size)
+    engine = DenseEngine(model)
+    for call in (lambda: engine.prefill(ids), lambda: engine.generate(ids, max_new_tokens=3),
+                 lambda: engine.generate(ids, max_new_tokens=3, num_beams=2)):
+        with monkeypatch.context() as m:
+            _stops_at(m, "paged_attention", 5)
+            with pytest.raises(_Stop):
+                call()
+        assert engine.cache is None and engine.positions == ()
+    assert torch.equal(engine.prefill(ids).logits, DenseEngine(model).prefill(ids).logits)
