@@ -156,7 +156,8 @@ struct Work {
   int slot;  // of its first range's output (ranges > 1)
 };
 
-// index: this workgroup's number for its KV head.  (Sequences of more than 16 queries are never divided.)
+// index: this workgroup's number for its KV head.  (Sequences of more than 16 queries, which a call has here where
+// max_q is less than there is, are never divided.)
 __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int index, Work& w) {
   const int lane = threadIdx.x & 63;
   const auto look = [&](int s, int& items, int& steps, bool& whole) __attribute__((always_inline)) {
@@ -1141,10 +1142,13 @@ struct Launch {
   size_t list_at, ml_at, o_at, bytes;
 };
 
-Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t max_kv, bool starts) {
+// (max_q: 1 without q_starts)
+Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t max_kv) {
   Launch p{};
-  // up to 16 queries of a KV head are one pass over its keys in step_kernel
-  p.step = !starts || max_q * group <= kStepRows;
+  // Up to 16 queries of a KV head are one pass over its keys in step_kernel; more would be several there, of one workgroup,
+  // for which the keys are not divided (32 heads on one KV head, a token over 512, 8192, 32768 tokens: 15.5, 147, 558 us there and
+  // 19.7, 26.8, 38 in chunk_kernel; of 32 sequences of 4096 78 and 37, of 64 of 200 12.4 and 13.7).
+  p.step = max_q * group <= kStepRows;
   const int rows = p.step ? kStepRows : kChunkRows, unit = p.step ? kStepKeys : kKeys;
   const int64_t items = p.step ? seqs : (n * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs : 0);
   const int64_t steps = (max_kv + unit - 1) / unit;
@@ -1183,8 +1187,8 @@ extern "C" size_t fl_paged_attention_workspace(int32_t rows, int32_t seqs, int32
   using namespace fl;
   if (rows <= 0 || seqs <= 0 || kv_heads <= 0 || heads < kv_heads || heads % kv_heads || max_q <= 0 || max_kv <= 0) return 0;
   // (with or without q_starts: what both may take)
-  const size_t a = plan(rows, seqs, kv_heads, heads / kv_heads, max_q, max_kv, true).bytes;
-  return rows == seqs ? std::max(a, plan(rows, seqs, kv_heads, heads / kv_heads, 1, max_kv, false).bytes) : a;
+  const size_t a = plan(rows, seqs, kv_heads, heads / kv_heads, max_q, max_kv).bytes;
+  return rows == seqs ? std::max(a, plan(rows, seqs, kv_heads, heads / kv_heads, 1, max_kv).bytes) : a;
 }
 
 extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, const uint16_t* k_pages, const uint16_t* v_pages,
@@ -1211,9 +1215,9 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
     FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_paged_attention: every tensor must be 16-byte aligned");
   if (rows == 0) return FL_OK;
   FL_REQUIRE(seqs > 0, "fl_paged_attention: rows without a sequence");
-  Launch p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, max_kv, q_starts != nullptr);
+  Launch p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, max_kv);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < p.bytes) {
-    p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, 1, q_starts != nullptr);  // (no room for divided items: none is)
+    p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, 1);  // (no room for divided items: none is)
   }
   FL_REQUIRE(p.groups * kv_heads <= 0x7FFFFFFF / kChunkThreads, "fl_paged_attention: grid too large");
   uint8_t* const ws = static_cast<uint8_t*>(workspace);

@@ -62,3 +62,20 @@ def test_divided_items_of_sequences_shorter_than_their_rows(rows, lens, heads, k
         got = _on_workspace(fill, q.flatten(1), kp, vp, table, _ints(lens), _ints(starts), max(rows), max(lens)).view_as(q)
         assert got.isfinite().all(), fill
         assert attention_error(got, want, size, slack) <= 0, fill
+
+
+@pytest.mark.parametrize("heads,kv,lens", [(32, 1, [20000]), (34, 2, [3000, 1, 0, 700]), (20, 1, [900] * 5), (300, 1, [500, 64])])
+def test_single_tokens_of_wide_groups(heads, kv, lens):
+    """More than 16 query heads on a KV head: a step without q_starts is divided over the chip as one with them is, with
+    the same bits."""
+    print(f"case: wide groups {heads}/{kv} {lens}", flush=True)
+    g = _gen(2)
+    (kp, vp), table, (keys, values) = make_pool(g, lens, -(-max(lens) // 64) + 1, 64, kv, DEV)
+    n = len(lens)
+    q = torch.randn(n, heads, DIM, generator=g, device=DEV).bfloat16()
+    want, size, slack = plain_attention(q, keys, values, lens, _starts([1] * n), SCALING)
+    for hint in ({}, {"max_kv": max(lens)}, {"max_kv": 1}):
+        got = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, **hint)
+        assert attention_error(got.view_as(q), want, size, slack) <= 0
+        other = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, _ints(_starts([1] * n)), max_q=1, **hint)
+        assert torch.equal(got, other)
