@@ -976,8 +976,8 @@ def _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, rows):
 
 
 def _head_rows(x: torch.Tensor, name: str, device):
-    """(rows, their distance, their number, their width) of bf16 rows [n, heads * 128]: at any distance that is a multiple
-    of 8 values, else as contiguous ones."""
+    """(rows, their distance, their number, their width) of bf16 rows [n, heads * 128]: where they are, if 16-byte aligned and at a
+    distance that is a multiple of 8 values, else a contiguous copy."""
     shape = x.shape
     if len(shape) != 2 or x.dtype is not torch.bfloat16 or shape[1] == 0 or shape[1] % HEAD_DIM or x.device != device:
         raise ValueError(f"{name} must be bfloat16 [rows, heads * {HEAD_DIM}] on {device}")
@@ -986,7 +986,7 @@ def _head_rows(x: torch.Tensor, name: str, device):
     if n == 1 and step == 1:
         stride = cols  # (one row lies at no distance)
     if step != 1 or stride % 8 or stride < cols or x.data_ptr() % 16:
-        return x.contiguous(), cols, n, cols
+        return x.clone(memory_format=torch.contiguous_format), cols, n, cols  # (rows off their alignment may be contiguous)
     return x, stride, n, cols
 
 

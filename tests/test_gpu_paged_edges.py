@@ -79,3 +79,26 @@ def test_single_tokens_of_wide_groups(heads, kv, lens):
         assert attention_error(got.view_as(q), want, size, slack) <= 0
         other = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, _ints(_starts([1] * n)), max_q=1, **hint)
         assert torch.equal(got, other)
+
+
+@pytest.mark.parametrize("off", [1, 4, 7])
+def test_contiguous_rows_off_their_alignment(off):
+    """Rows that begin anywhere in a buffer: what rows of their own give."""
+    print(f"case: misaligned rows {off}", flush=True)
+    g = _gen(3)
+    lens, kv, heads, page = [40, 7], 2, 4, 16
+    (kp, vp), table, _ = make_pool(g, lens, 4, page, kv, DEV, fill=0.0)
+    rope = tuple(torch.randn(64, DIM, generator=g, device=DEV) for _ in range(2))
+
+    def rows(width):
+        x = torch.randn(off + 2 * width * DIM, generator=g, device=DEV).bfloat16()[off:].view(2, width * DIM)
+        assert x.is_contiguous() and x.data_ptr() % 16
+        return x
+
+    q, k, v = rows(heads), rows(kv), rows(kv)
+    pools = [(kp.clone(), vp.clone()) for _ in range(2)]
+    got = kernels.paged_append(q, k, v, rope, *pools[0], table, _ints(lens))
+    want = kernels.paged_append(q.clone(), k.clone(), v.clone(), rope, *pools[1], table, _ints(lens))
+    assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(*pools))
+    assert torch.equal(kernels.paged_attention(q, *pools[0], table, _ints(lens), SCALING),
+                       kernels.paged_attention(q.clone(), *pools[0], table, _ints(lens), SCALING))
