@@ -38,6 +38,20 @@ void clear_error();
     }                                                                           \
   } while (0)
 
+// ---------------------------------------------------------------- host checks
+// Rows of `cols` elements, `stride` apart, at p and at q share no memory: one lies behind the other, or both are
+// columns of one wider matrix.
+inline bool apart(const void* p, int64_t p_stride, int64_t p_cols, int p_size, const void* q, int64_t q_stride, int64_t q_cols, int q_size,
+                  int rows) {
+  const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
+  if (a == 0 || b == 0 || a + ((rows - 1) * p_stride + p_cols) * p_size <= b || b + ((rows - 1) * q_stride + q_cols) * q_size <= a)
+    return true;
+  const int64_t step = p_stride * p_size;
+  if (step == 0 || step != q_stride * q_size) return false;
+  const int64_t at = ((b - a) % step + step) % step;  // q's columns from p's first
+  return p_cols * p_size <= at && at + q_cols * q_size <= step;
+}
+
 // ---------------------------------------------------------------- bf16
 // bf16 is carried as its 16-bit pattern.  Widening is exact; narrowing rounds to
 // nearest even (the rounding of torch's .to(torch.bfloat16)).

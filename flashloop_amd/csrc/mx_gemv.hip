@@ -544,19 +544,6 @@ void mx_launch_epi(int epilogue, const MxGemvArgs& a, const NormArgs& c, hipStre
   }
 }
 
-// Rows of `cols` elements, `stride` apart, at p and at q share no memory: one lies behind the other, or both are
-// columns of one wider matrix.
-bool apart(const void* p, int64_t p_stride, int64_t p_cols, int p_size, const void* q, int64_t q_stride, int64_t q_cols, int q_size,
-           int rows) {
-  const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p)), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(q));
-  if (a == 0 || b == 0 || a + ((rows - 1) * p_stride + p_cols) * p_size <= b || b + ((rows - 1) * q_stride + q_cols) * q_size <= a)
-    return true;
-  const int64_t step = p_stride * p_size;
-  if (step == 0 || step != q_stride * q_size) return false;
-  const int64_t at = ((b - a) % step + step) % step;  // q's columns from p's first
-  return p_cols * p_size <= at && at + q_cols * q_size <= step;
-}
-
 int32_t make_mx_args(MxGemvArgs& a, const void* x, int32_t x_is_f32, int64_t x_stride, int32_t m, int32_t k,
                      const uint8_t* const* codes, const uint8_t* const* scales, int32_t n, int32_t epilogue,
                      void* const* outputs, int64_t out_stride, const uint16_t* addend, int64_t addend_stride,

@@ -202,6 +202,26 @@ extern "C" int32_t fl_paged_append(const uint16_t* q, int64_t q_row_stride, cons
              "fl_paged_append: every tensor must be 16-byte aligned");
   if (rows == 0) return FL_OK;
   FL_REQUIRE(seqs > 0, "fl_paged_append: rows without a sequence");
+  // (a wave writes its heads of a row while others read theirs)
+  const auto outside = [&](const uint16_t* x, int64_t stride, int64_t cols, const void* block, int64_t bytes) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(x), from = reinterpret_cast<uintptr_t>(block);
+    return at + 2 * ((rows - 1) * stride + cols) <= from || from + bytes <= at;
+  };
+  const int64_t pool = 2 * static_cast<int64_t>(pages) * kv_heads * page_size * kDim;
+  for (const uint16_t* p : {k_pages, v_pages})
+    FL_REQUIRE(outside(k, k_row_stride, kv_cols, p, pool) && outside(v, v_row_stride, kv_cols, p, pool) &&
+                   (!turn || (outside(q, q_row_stride, q_cols, p, pool) && outside(q_out, q_out_row_stride, q_cols, p, pool))),
+               "fl_paged_append: rows lie on the pages");
+  if (turn) {
+    FL_REQUIRE((q_out == q && q_out_row_stride == q_row_stride) || apart(q_out, q_out_row_stride, q_cols, 2, q, q_row_stride, q_cols, 2, rows),
+               "fl_paged_append: q_out lies on other values of q");
+    FL_REQUIRE(apart(q_out, q_out_row_stride, q_cols, 2, k, k_row_stride, kv_cols, 2, rows) &&
+                   apart(q_out, q_out_row_stride, q_cols, 2, v, v_row_stride, kv_cols, 2, rows),
+               "fl_paged_append: q_out lies on k or v");
+    const int64_t table = static_cast<int64_t>(rope_positions) * kDim * (rope_is_f32 ? 4 : 2);
+    FL_REQUIRE(outside(q_out, q_out_row_stride, q_cols, rope_cos, table) && outside(q_out, q_out_row_stride, q_cols, rope_sin, table),
+               "fl_paged_append: q_out lies on a rope table");
+  }
   const int units = (heads + 2 * kv_heads + 7) / 8;
   const int64_t blocks = (static_cast<int64_t>(rows) * units + 3) / 4;
   FL_REQUIRE(blocks <= 0xFFFFFFFFll / 256, "fl_paged_append: grid too large");

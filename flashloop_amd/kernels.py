@@ -999,7 +999,7 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, rope:
     ``k_pages`` / ``v_pages`` bf16 [pages, KV, page, 128], written in place; ``page_table`` i32 [S, W]; ``kv_lens`` i32
     [S], with the call's rows counted; ``q_starts`` i32 [S + 1]: rows q_starts[s] .. q_starts[s + 1] - 1 are
     the last tokens of sequence s (None: one row a sequence).  Returns the rotated rows of ``q``, in ``out``
-    (``q`` itself, or rows that do not lie on it) if given; rows behind the last sequence as they are."""
+    (``q`` itself, or rows that lie on none of the operands) if given; rows behind the last sequence as they are."""
     device = k_pages.device
     k, k_stride, n, cols = _head_rows(k, "k", device)
     v, v_stride, n_v, cols_v = _head_rows(v, "v", device)

@@ -624,7 +624,8 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  * p, in fp32 and rounded once; k and the plain v to their pages.  Without rope tables k is stored as it is and
  * q is neither read nor written.  A row whose page or rope row does not exist is stored nowhere and its q_out
  * is NaN; rows that belong to no sequence are copied to q_out as they are.  Row strides in elements, multiples
- * of 8; tensors 16-byte aligned.
+ * of 8; tensors 16-byte aligned.  No rows may lie on the pages, nor q_out on k, v, the rope tables or other values of q
+ * (columns of one wider matrix do not lie on each other).
  *
  * fl_paged_attention: out[i, h, :] = sum_j softmax_j(scaling * q[i, h] . K[j]) V[j] over the keys j of the
  * row's sequence up to its own position, query heads h * kv_heads / heads sharing a KV head; out bf16 [rows,

@@ -102,3 +102,22 @@ def test_contiguous_rows_off_their_alignment(off):
     assert torch.equal(got, want) and all(torch.equal(a, b) for a, b in zip(*pools))
     assert torch.equal(kernels.paged_attention(q, *pools[0], table, _ints(lens), SCALING),
                        kernels.paged_attention(q.clone(), *pools[0], table, _ints(lens), SCALING))
+
+
+def test_rotated_rows_beside_others():
+    """``out`` in other columns of the matrix that holds q, k and v, and in rows behind them; on k it is refused."""
+    print("case: append out beside", flush=True)
+    g = _gen(4)
+    (kp, vp), table, _ = make_pool(g, [20, 5, 33], 4, 16, 2, DEV, fill=0.0)
+    lens = _ints([20, 5, 33])
+    wide = torch.randn(6, 12 * DIM, generator=g, device=DEV).bfloat16()
+    q, k, v, beside = wide[:3].split([4 * DIM, 2 * DIM, 2 * DIM, 4 * DIM], 1)
+    rope = tuple(torch.randn(64, DIM, generator=g, device=DEV) for _ in range(2))
+    want = kernels.paged_append(q, k, v, rope, kp, vp, table, lens)
+    with pytest.raises(RuntimeError, match="k or v"):
+        kernels.paged_append(q, k, v, rope, kp, vp, table, lens, out=wide[:3, 4 * DIM: 8 * DIM])
+    with pytest.raises(RuntimeError, match="other values of q"):
+        kernels.paged_append(q, k, v, rope, kp, vp, table, lens, out=wide[1:4, : 4 * DIM])
+    for out in (beside, wide[3:, : 4 * DIM], wide[3:].view(-1)[: 12 * DIM].view(3, 4 * DIM), q):
+        assert kernels.paged_append(q, k, v, rope, kp, vp, table, lens, out=out) is out
+        assert torch.equal(out, want)
