@@ -23,7 +23,7 @@ import torch.nn.functional as F
 
 from . import kernels
 from ._lib import HEAD_DIM, MAX_BEAMS
-from .engine import _is_plain
+from .engine import _calls_are_plain, _is_plain
 from .model import MLP, OuroConfig, OuroForCausalLM, RMSNorm, RotaryEmbedding
 
 
@@ -66,7 +66,11 @@ class DenseOutput:
 
 
 class DenseEngine:
-    """Prefill, decode and generate of a ragged batch (right-padded prompts) with every loop dense."""
+    """Prefill, decode and generate of a ragged batch (right-padded prompts) with every loop dense.
+
+    The kernels take the modules' weights.  A prompt takes the modules as they are then (in-place changes of a weight
+    are seen at any time); where a module was replaced or hooked or has another weight since, ``extend`` and ``decode``
+    raise."""
 
     def __init__(self, model: OuroForCausalLM, *, page_size: int = 64, chunk: int = 2048, use_graphs: bool = True) -> None:
         cfg = model.config
@@ -91,8 +95,15 @@ class DenseEngine:
         weights, not the modules, so modules that do more than multiply by them are refused."""
         bb = self.model.model
         eps = {float(bb.norm.eps)}
+        seen = []  # (the table that a module is in, its name there, the module, its class, its tensor's name and address)
 
-        def weight(m, kind):
+        def child(owner, name, kind, tensor=None):
+            m = getattr(owner, name)
+            seen.append((owner._modules, name, m, kind, tensor, getattr(m, tensor).data_ptr() if tensor and _is_plain(m, kind) else None))
+            return m
+
+        def weight(owner, name, kind=torch.nn.Linear):
+            m = child(owner, name, kind, "weight")
             w = m.weight if _is_plain(m, kind) else None
             if w is None or w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16 or getattr(m, "bias", None) is not None:
                 raise ValueError("DenseEngine needs plain bf16 Linear and RMSNorm layers without a bias")
@@ -103,24 +114,52 @@ class DenseEngine:
         hidden = bb.norm.weight.numel()
         if hidden % 8 or hidden > 8192 or any(l.mlp.up_proj.weight.shape[0] % 8 for l in bb.layers):
             raise ValueError("DenseEngine needs a hidden width (up to 8192) and an MLP width that are multiples of 8")
-        emb, rot = bb.embed_tokens, bb.rotary_emb
+        emb, rot = child(bb, "embed_tokens", torch.nn.Embedding, "weight"), child(bb, "rotary_emb", RotaryEmbedding, "inv_freq")
         if (not _is_plain(emb, torch.nn.Embedding) or not _is_plain(rot, RotaryEmbedding) or emb.max_norm is not None
                 or emb.weight.dtype != torch.bfloat16 or not emb.weight.is_contiguous() or emb.weight.data_ptr() % 16
                 or rot.inv_freq.dtype not in (torch.float32, torch.bfloat16)):
             raise ValueError("DenseEngine needs plain embedding (bf16) and rotary modules")
         layers = []
-        for layer in bb.layers:
-            a, m = layer.self_attn, layer.mlp
+        for i, layer in enumerate(bb.layers):
+            seen.append((bb.layers._modules, str(i), layer, None, None, None))
+            a, m = child(layer, "self_attn", None), child(layer, "mlp", MLP)
             if not _is_plain(m, MLP):
                 raise ValueError("DenseEngine needs plain MLP modules")
-            layers.append((*(weight(x, torch.nn.Linear) for x in (a.q_proj, a.k_proj, a.v_proj, a.o_proj, m.gate_proj, m.up_proj,
-                                                                  m.down_proj)),
-                           *(weight(x, RMSNorm) for x in (layer.input_layernorm, layer.input_layernorm_2,
-                                                          layer.post_attention_layernorm, layer.post_attention_layernorm_2))))
-        final, head = weight(bb.norm, RMSNorm), weight(self.model.lm_head, torch.nn.Linear)
+            layers.append((*(weight(a, n) for n in ("q_proj", "k_proj", "v_proj", "o_proj")),
+                           *(weight(m, n) for n in ("gate_proj", "up_proj", "down_proj")),
+                           *(weight(layer, n, RMSNorm) for n in ("input_layernorm", "input_layernorm_2", "post_attention_layernorm",
+                                                                 "post_attention_layernorm_2"))))
+        final, head = weight(bb, "norm", RMSNorm), weight(self.model, "lm_head")
         if len(eps) != 1:
             raise ValueError("DenseEngine needs RMSNorm layers of one eps")
+        self._seen, self._held = seen, (emb.weight.detach(), rot.inv_freq)  # (held: no other tensor gets these addresses)
         return layers, final, head, eps.pop()
+
+    def _same_modules(self) -> bool:
+        """Whether the modules are those, plain and with the tensors, that ``_weights`` were taken from."""
+        bb, eps = self.model.model, self._weights[3]
+        if not _calls_are_plain() or len(bb.layers) != len(self._weights[0]) or bb.embed_tokens.max_norm is not None:
+            return False
+        for table, name, m, kind, tensor, at in self._seen:  # (340 modules of 24 layers in 0.1 ms)
+            if table.get(name) is not m:
+                return False
+            if kind is None:
+                continue
+            own = m.__dict__
+            if type(m) is not kind or own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own:
+                return False
+            if at is not None:
+                t = own["_buffers" if kind is RotaryEmbedding else "_parameters"].get(tensor)
+                if t is None or t.data_ptr() != at or own["_parameters"].get("bias") is not None or "bias" in own:
+                    return False
+                if kind is RMSNorm and m.eps != eps:
+                    return False
+        return True
+
+    def _check_modules(self) -> None:
+        if not self._same_modules():
+            raise RuntimeError("a module of the model was replaced or hooked, or has another weight, since these sequences' prompts; call "
+                               "reset(): the next prompt takes the modules as they are then")
 
     def reset(self) -> None:
         """Drop the cache and the captured step."""
@@ -243,6 +282,8 @@ class DenseEngine:
             self._pos.copy_(torch.tensor(self._lens)[:, None] - 1)
 
     def _begin(self, input_ids: torch.Tensor, counts: list[int], extra: int, beams: int) -> None:
+        if not self._same_modules():
+            self._weights = self._plain_weights()
         capacity = max(counts) + int(extra)
         cfg, dev = self.config, input_ids.device
         shared = None
@@ -289,6 +330,7 @@ class DenseEngine:
         if min(counts) < 1:
             raise ValueError(f"sequence {counts.index(min(counts))} has no tokens")
         self._room(counts)
+        self._check_modules()
         before = list(self._lens)
         try:
             logits = self._feed(input_ids, counts, list(range(len(counts))))
@@ -320,6 +362,7 @@ class DenseEngine:
         self._room([1] * rows)
         try:
             logits = self._advance(token_ids)
+            self._check_modules()  # (while the GPU runs the step)
         except BaseException:  # (a step counts its token before it runs)
             self._release()
             self._lengths_to_device()
