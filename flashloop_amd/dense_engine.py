@@ -15,6 +15,8 @@ number of loops).  Every loop of every layer has its own keys and values
 
 from __future__ import annotations
 
+import contextlib
+import functools
 import gc
 from dataclasses import dataclass
 
@@ -57,6 +59,19 @@ class PagedKVCache:
     def reorder(self, parents: torch.Tensor) -> None:
         """Row s * K + k takes over the state of row s * K + parents[s, k] (i32 [S, K])."""
         self.table.copy_(kernels.paged_reorder(self.k_pages, self.v_pages, self.table, self.lens, parents))
+
+
+def _on_its_device(method):
+    """A method of an engine with its model's device as the current one (kernels and captures take the current device's
+    streams)."""
+
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        device = self.device
+        with torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext():
+            return method(self, *args, **kw)
+
+    return call
 
 
 @dataclass(frozen=True)
@@ -174,6 +189,10 @@ class DenseEngine:
         self._graph = self._tok = self._pos = self._out = None
 
     @property
+    def device(self) -> torch.device:
+        return next(self.model.parameters()).device
+
+    @property
     def positions(self) -> tuple[int, ...]:
         return tuple(self._lens)
 
@@ -231,10 +250,11 @@ class DenseEngine:
         return logits
 
     # ------------------------------------------------------------------ prompts
-    @staticmethod
-    def _lengths(input_ids: torch.Tensor, attention_mask: torch.Tensor | None) -> list[int]:
+    def _lengths(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None) -> list[int]:
         if input_ids.ndim != 2 or input_ids.shape[0] < 1 or input_ids.shape[1] < 1:
             raise ValueError("input_ids must be [B, T] with B, T >= 1")
+        if input_ids.device != self.device:
+            raise ValueError(f"input_ids lie on {input_ids.device}, the model on {self.device}")
         if attention_mask is None:
             return [input_ids.shape[1]] * input_ids.shape[0]
         if tuple(attention_mask.shape) != tuple(input_ids.shape):
@@ -296,6 +316,7 @@ class DenseEngine:
         self._rope = tuple(t[0].contiguous() for t in
                            self.model.model.rotary_emb(probe, torch.arange(self.cache.capacity, device=dev)[None]))
 
+    @_on_its_device
     @torch.inference_mode()
     def prefill(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, *,
                 decode_capacity: int = 4096) -> DenseOutput:
@@ -320,6 +341,7 @@ class DenseEngine:
             self.reset()
             raise
 
+    @_on_its_device
     @torch.inference_mode()
     def extend(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None) -> DenseOutput:
         """More tokens [B, T] (right-padded, at least one a sequence) onto the cached sequences: the logits of the last."""
@@ -350,6 +372,7 @@ class DenseEngine:
                 raise ValueError(f"sequence {b} has {t} tokens: the cache has room for {self.cache.capacity} (decode_capacity)")
 
     # ------------------------------------------------------------------ decode
+    @_on_its_device
     @torch.inference_mode()
     def decode(self, token_ids: torch.Tensor) -> DenseOutput:
         """One token for every sequence: ``token_ids`` [B, 1].  With graphs on, the returned logits live in the graph's
@@ -411,6 +434,7 @@ class DenseEngine:
         self._graph = graph
 
     # ------------------------------------------------------------------ generate
+    @_on_its_device
     @torch.inference_mode()
     def generate(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None, *, max_new_tokens: int,
                  eos_token_id: int | None = None, num_beams: int = 1, length_penalty: float = 1.0) -> list[torch.Tensor]:

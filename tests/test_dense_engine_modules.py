@@ -126,3 +126,36 @@ def test_weights_changed_in_place():
     engine.model.model.layers[0].register_forward_hook(lambda *a: None)  # (a layer is never called)
     engine.decode(IDS[:, :1])
     assert engine.positions == (8,)
+
+
+def test_calls_run_on_the_models_device(monkeypatch):
+    """With another device current, the model's is made the current one for a call; prompts on another device are refused."""
+    entered = []
+
+    class Current:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            entered.append(self.device)
+
+        def __exit__(self, *exc):
+            entered.append(None)
+
+    engine = _engine()
+    for call in (lambda: engine.extend(IDS), lambda: engine.decode(IDS[:, :1])):
+        call()
+    assert entered == []  # (a model on the CPU)
+    far = torch.device("cuda", 1)
+    monkeypatch.setattr(torch.cuda, "device", Current)
+    monkeypatch.setattr(DenseEngine, "device", far)
+    engine.decode(IDS[:, :1])
+    assert entered == [far, None]
+    held = engine.cache
+    for cache, call in ((held, lambda: engine.extend(IDS)), (None, lambda: engine.prefill(IDS)), (None, lambda: engine.generate(IDS, max_new_tokens=1)),
+                        (None, lambda: engine.generate(IDS, max_new_tokens=1, num_beams=2))):
+        engine.cache = cache
+        entered.clear()
+        with pytest.raises(ValueError, match="input_ids lie on cpu, the model on cuda:1"):
+            call()
+        assert entered[0] == far and entered[-1] is None
