@@ -775,7 +775,7 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs first
 
     float l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     // NaN: a sequence longer than its table row, a key without a page
-    l += swap_half(l) + (len - 1 > pages.last || pos >= no_page ? NAN : 0.0f);
+    l += swap_half(l) + ((len - 1 > pages.last && pos >= 0) || pos >= no_page ? NAN : 0.0f);
     const PagedArgs e = args_again(args);
     const int r = item * kChunkRows + wave * 32 + (lane & 31), token = pos - len + rows.y;
     const bool valid = r < rows.y * e.group;
@@ -845,7 +845,7 @@ __global__ __launch_bounds__(kThreads, 2) void step_kernel(PagedArgs a) {
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float raw = kNone, m = scaled_max(kNone, a.scale), l = 0.0f;
-    float poison = len - 1 > pages.last ? NAN : 0.0f;
+    float poison = len - 1 > pages.last && pos >= 0 ? NAN : 0.0f;
     bool far = false;
 
     bf16x8_t kr[2][4];

@@ -1062,7 +1062,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     keys up to its own position; H a multiple of the pages' KV heads.  The other arguments as in ``paged_append``.
     ``max_q`` and ``max_kv``: the most rows and tokens of a sequence, if known (by default the call's rows and the
     table's capacity): they divide the work and have no part in the result.  Returns bf16 [n, H*128]: zeros for
-    rows that see no key or belong to no sequence, NaN for rows that see a key without a page."""
+    rows that see no key or belong to no sequence, NaN for rows that see a key without a page and for all that see one
+    in a sequence longer than its row of ``page_table``."""
     device = k_pages.device
     q, q_stride, n, cols = _head_rows(q, "q", device)
     pages, kv, page, seqs, width = _paged_operands(k_pages, v_pages, page_table, kv_lens, q_starts, n)

@@ -632,7 +632,7 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  * heads * 128].  Scores, softmax and sums are fp32, probabilities are rounded to bf16 for the second product.
  * Keys that a row does not see have no part in its result, whatever their rows hold.  A row with no key (its
  * position is negative) and rows that belong to no sequence are zeros; a row that sees a key without a page
- * is NaN.  max_q and max_kv, the most rows and tokens of a sequence, choose how the work is divided and change
+ * is NaN, and so is every row with a key of a sequence that is longer than its table row.  max_q and max_kv, the most rows and tokens of a sequence, choose how the work is divided and change
  * no result beyond rounding; larger ones than there are only cost time, and so do smaller ones.  With a
  * workspace (16-byte aligned, of fl_paged_attention_workspace bytes; nullable) calls whose rows are too few or too
  * unequal for the chip divide the keys over several workgroups and join them; with none or a smaller one they do not.

@@ -121,3 +121,21 @@ def test_rotated_rows_beside_others():
     for out in (beside, wide[3:, : 4 * DIM], wide[3:].view(-1)[: 12 * DIM].view(3, 4 * DIM), q):
         assert kernels.paged_append(q, k, v, rope, kp, vp, table, lens, out=out) is out
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("rows,length,capacity,max_q,heads", [
+    (40, 33, 32, None, 2),    # chunk_kernel, an item alone
+    (40, 33, 32, 1, 2),       # step_kernel, its rows in passes of 16 queries
+    (600, 550, 512, None, 1),  # chunk_kernel, divided keys
+    (17, 16, 16, None, 1),    # as long as the table: no NaN
+])
+def test_rows_without_a_key_of_a_sequence_past_its_table(rows, length, capacity, max_q, heads):
+    """Zeros for the rows in front of the first key, NaN for the others of a sequence that its table row cannot hold."""
+    print(f"case: past the table {rows} {length} {capacity} {max_q}", flush=True)
+    g = _gen(5)
+    (kp, vp), table, _ = make_pool(g, [capacity], capacity // 16, 16, 1, DEV)
+    q = torch.randn(rows, heads * DIM, generator=g, device=DEV).bfloat16()
+    got = kernels.paged_attention(q, kp, vp, table, _ints([length]), SCALING, _ints([0, rows]), max_q=max_q)
+    assert not got[: rows - length].any()
+    rest = got[rows - length:]
+    assert rest.isnan().all() if length > capacity else rest.isfinite().all()
