@@ -5,9 +5,10 @@
 //
 //  * chunk_kernel: chunks of new tokens.  A workgroup has 256 queries in eight waves, one workgroup a CU; S^T and O^T on
 //    v_mfma_f32_32x32x16_bf16, 64 keys a step, K and V through a ring of four tiles in LDS that transfers without registers
-//    fill.  A long prompt (8192 tokens, 16 heads) 258-279 us by the card: 990-1070 TFLOP/s of the causal half, matrix cores busy 49%.  On the
-//    same transfers with no arithmetic between the products it runs at 1550 TFLOP/s of those it has (the card's power sets that
-//    rate); the rest are the exponentials and the roundings to bf16 in the products' shadow, one behind the other in a wave.
+//    fill.  A long prompt (8192 tokens, 16 heads) 285-290 us: 950-970 TFLOP/s of the causal half.  On the same transfers with no
+//    arithmetic between the products it runs at 1550 TFLOP/s of those it has (the card's power sets that rate); the rest are the
+//    exponentials, the roundings to bf16 and the moves of the softmax's reference in the products' shadow, one behind the other in
+//    a wave.
 //  * step_kernel: few queries a sequence (one decode step).  A wave owns steps of 32 keys and up to 16
 //    queries on v_mfma_f32_16x16x32_bf16: K goes from memory into the first product's operand, V through a
 //    part of LDS of the wave's own, the next step's loads in flight, no barrier until the waves' join.  Bound by bytes: 32
@@ -271,7 +272,7 @@ __device__ __forceinline__ void slots(std::integer_sequence<int, I...>, F f) {
 // more; the line is cut into `aim` equal slices, and a workgroup takes a slice: the end of one item, whole ones, the
 // beginning of another.  So the workgroups end at about the same time, however unequal the sequences are.  (20 sequences of
 // 1-700 new tokens over up to 3000, 16 heads on 4: 82-89 us with items divided by their own lengths, the longest ranges first,
-// 77-82 with slices; 8 of up to 300 over 6000, 16 heads: 105, 92.)  Else a workgroup takes one item, a sequence's last ones first:
+// 77-82 with slices, both with the softmax's reference moved less often; 8 of up to 300 over 6000, 16 heads: 105, 92.)  Else a workgroup takes one item, a sequence's last ones first:
 // they see more keys.  Every workgroup finds its work for itself, sequences in lanes: the lengths are on the device alone.
 // kApart: beginning a part costs some 10 us, finding it, first latencies and the stores (3, 5, 7, 10 steps: 84, 79, 78, 80 us).
 constexpr double kApart = 7.0;
@@ -464,9 +465,6 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs first
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     // the reference of the running softmax (a score, and it scaled to base 2), this lane's parts of the sum
     float raw = kNone, off = -scaled_max(kNone, a.scale), sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    // Scores may pass the reference by 2^8 before it moves: the probabilities are as exact in bf16 as under 1, and most tiles
-    // then leave the outputs alone.
-    const float slack = 8.0f / a.scale;
     bool far = false;  // (wave-uniform) some query's reference lies past kFar
 
     if (first < tiles) {
@@ -594,11 +592,13 @@ __global__ __launch_bounds__(kChunkThreads, 2) void chunk_kernel(PagedArgs first
           for (int i = 0; i < 16; ++i) m = fmaxf(m, s[b][i]);
         return m;
       };
-      // the reference moves where a score passes it too far
+      // The reference is the largest score so far, so that the largest probability is 1 and has no rounding: it carries much of a
+      // row.  (Moved only where a score passes it by 2^8, most tiles leave the outputs alone, 8192 prompt rows 289 -> 270 us, and the
+      // result is off by 2.10e-3 of its norm instead of 1.87e-3, of which its own rounding is 1.65e-3.)
       const auto move_to = [&](float m, f32x16_t (&s)[2]) __attribute__((always_inline)) {
         const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
         m = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-        if (__builtin_amdgcn_ballot_w64(m > raw + slack) != 0ull) {
+        if (__builtin_amdgcn_ballot_w64(m > raw) != 0ull) {
           const float top = fmaxf(raw, m), mn = scaled_max(top, a.scale);
           const float alpha = exp2_between(raw, top, scaled_max(raw, a.scale), mn, a.scale);
           raw = top;

@@ -139,3 +139,45 @@ def test_rows_without_a_key_of_a_sequence_past_its_table(rows, length, capacity,
     assert not got[: rows - length].any()
     rest = got[rows - length:]
     assert rest.isnan().all() if length > capacity else rest.isfinite().all()
+
+
+@pytest.mark.parametrize("rows,tokens,heads,kv", [
+    ([1] * 40, 250, 8, 8),       # step_kernel
+    ([100], 200, 4, 2),          # chunk_kernel, items alone
+    ([100, 2, 90, 77], 190, 16, 8),  # chunk_kernel, the items of several sequences on a line
+])
+def test_a_late_key_that_carries_half_of_a_row(rows, tokens, heads, kv):
+    """A key behind a hundred others that gets half of a row's weight: its value is 1, theirs are -1, so the result, about 0,
+    shows the rounding of its probability.  As the largest score it has none (2^0); the others' (at most 2^-8 of each, of
+    either sign) leave 2^-8 / sqrt(3) of the root of the sum of their squares, halved by the quotient: 1e-4 for the 140
+    or more keys that count (weights exp(N(0, 1/2)) of 180).  3e-4 is three times that; a probability with a rounding of its own
+    has 1.66e-3 / 2 in the mean square.  (The scores of a wave's rows lie within 8 bits of the first tile's largest.)"""
+    print(f"case: late key {rows[:3]} {tokens} {heads}/{kv}", flush=True)
+    g = _gen(6)
+    lens, starts, late = [r + tokens for r in rows], _starts(rows), tokens - 50
+    n, seqs, page = starts[-1], len(rows), 64
+    (kp, vp), table, (keys, values) = make_pool(g, lens, -(-max(lens) // page), page, kv, DEV)
+    q = (0.5 * torch.randn(n, heads, DIM, generator=g, device=DEV)).bfloat16()
+    q[..., 0] = 0
+    for s in range(seqs):
+        keys[s][..., 0] = 0
+        keys[s][:, late] = 0
+        keys[s][:, late, 0] = 16
+        values[s].fill_(-1)
+        values[s][:, late] = 1
+        # the late key's score: the others' logsumexp
+        pos = lens[s] - rows[s] + torch.arange(rows[s], device=DEV)
+        at = torch.arange(lens[s], device=DEV)
+        seen = (at <= pos[:, None]) & (at != late)
+        for h in range(heads):
+            logits = (q[starts[s]: starts[s + 1], h].double() @ keys[s][h // (heads // kv)].double().t().contiguous()) * SCALING
+            q[starts[s]: starts[s + 1], h, 0] = (torch.logsumexp(torch.where(seen, logits, -torch.inf), 1) / (16 * SCALING)).bfloat16()
+        for pool, x in ((kp, keys[s]), (vp, values[s])):
+            pool[table[s].long()[at // page], :, at % page] = x.transpose(0, 1)
+    want = plain_attention(q, keys, values, lens, starts, SCALING)[0]
+    assert want.abs().max() < 0.05
+    got = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, None if rows[0] == 1 else _ints(starts),
+                                  max_q=max(rows), max_kv=4000).view_as(q)
+    error = (got.double() - want).square().mean().sqrt().item()
+    print("error", error, flush=True)
+    assert error < 3e-4
