@@ -442,7 +442,8 @@ class DenseEngine:
 
         Beam search returns the completion with the largest sum of log-probabilities divided by
         length ** ``length_penalty`` (tokens of the completion, the EOS among them) of those that ended and those still running
-        at the end.  A sequence's search ends when none of its running beams can pass the best one that ended."""
+        at the end.  Of a step's 2 * ``num_beams`` best continuations an EOS ends those among the first ``num_beams``; the best others go
+        on.  A sequence's search ends when none of its running beams can pass the best one that ended."""
         if int(max_new_tokens) <= 0:
             raise ValueError("max_new_tokens must be positive")
         if not 1 <= num_beams <= MAX_BEAMS // 2:

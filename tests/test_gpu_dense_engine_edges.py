@@ -7,6 +7,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+from beam_util import CASES, plain_search, table_engine, tables_of  # noqa: E402
 from flashloop_amd import DenseEngine  # noqa: E402
 from flashloop_amd.model import OuroConfig, OuroForCausalLM  # noqa: E402
 
@@ -106,3 +107,18 @@ def test_prompts_that_fail_leave_no_cache(monkeypatch):
                 call()
         assert engine.cache is None and engine.positions == ()
     assert torch.equal(engine.prefill(ids).logits, DenseEngine(model).prefill(ids).logits)
+
+
+@pytest.mark.parametrize("beams,new,eos,penalty,kind", CASES)
+def test_beam_search_on_tables(beams, new, eos, penalty, kind):
+    """The search with the selection's kernel against a plain one, on logits from tables."""
+    print(f"case: beams on tables {beams} {new} {eos} {penalty} {kind}", flush=True)
+    model = OuroForCausalLM.random_init(dataclasses.replace(TINY, vocab_size=24, num_hidden_layers=1), seed=1, device="cuda")
+    prompts = _ids(5, 3, 24)
+    for seed in range(3):
+        first, tables = tables_of(kind, 5, new, eos, 24, 10 + seed)
+        got = table_engine(model, first, tables, "cuda").generate(prompts, max_new_tokens=new, eos_token_id=eos, num_beams=beams,
+                                                                   length_penalty=penalty)
+        for b in range(5):
+            want = plain_search(first[b], tables[b], beams, new, eos, penalty)
+            assert got[b].tolist() == prompts[b].tolist() + want[1], (seed, b, want)
