@@ -157,8 +157,8 @@ struct Work {
   int slot;  // of its first range's output (ranges > 1)
 };
 
-// index: this workgroup's number for its KV head.  (Sequences of more than 16 queries, which a call has here where
-// max_q is less than there is, are never divided.)
+// index: this workgroup's number for its KV head.  (Sequences of more than 16 queries -- short
+// ones of wide groups, or more rows than max_q says -- are never divided.)
 __device__ __forceinline__ bool find_work(const PagedArgs& a, int head, int index, Work& w) {
   const int lane = threadIdx.x & 63;
   const auto look = [&](int s, int& items, int& steps, bool& whole) __attribute__((always_inline)) {
@@ -1147,10 +1147,12 @@ struct Launch {
 // (max_q: 1 without q_starts)
 Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t max_kv) {
   Launch p{};
-  // Up to 16 queries of a KV head are one pass over its keys in step_kernel; more would be several there, of one workgroup,
-  // for which the keys are not divided (32 heads on one KV head, a token over 512, 8192, 32768 tokens: 15.5, 147, 558 us there and
-  // 19.7, 26.8, 38 in chunk_kernel; of 32 sequences of 4096 78 and 37, of 64 of 200 12.4 and 13.7).
-  p.step = max_q * group <= kStepRows;
+  // Up to 16 queries of a KV head are one pass over its keys in step_kernel.  More would be several there, by one workgroup for
+  // which the keys are not divided (32 heads on one KV head, a token over 8192, 32768 tokens: 147, 558 us there and 26.8, 38 in
+  // chunk_kernel; of 32 sequences of 4096 78 and 37), so they go there only as single tokens over keys that are one range anyway
+  // (a token over 512: 15.5 there, 19.7 in chunk_kernel, of 1024 sequences 80 and 104, 4096 of 100 93 and 343), in up to four
+  // passes (128 heads on one, 64 sequences of 500: 61 there, 29).
+  p.step = max_q * group <= kStepRows || (max_q == 1 && group <= 4 * kStepRows && max_kv <= kStepWhole * kStepKeys);
   const int rows = p.step ? kStepRows : kChunkRows, unit = p.step ? kStepKeys : kKeys;
   const int64_t items = p.step ? seqs : (n * group + kChunkRows - 1) / kChunkRows + (seqs > 1 ? seqs : 0);
   const int64_t steps = (max_kv + unit - 1) / unit;

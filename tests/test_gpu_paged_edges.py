@@ -64,7 +64,8 @@ def test_divided_items_of_sequences_shorter_than_their_rows(rows, lens, heads, k
         assert attention_error(got, want, size, slack) <= 0, fill
 
 
-@pytest.mark.parametrize("heads,kv,lens", [(32, 1, [20000]), (34, 2, [3000, 1, 0, 700]), (20, 1, [900] * 5), (300, 1, [500, 64])])
+@pytest.mark.parametrize("heads,kv,lens", [(32, 1, [20000]), (34, 2, [3000, 1, 0, 700]), (20, 1, [900] * 5), (300, 1, [500, 64]), (64, 1, [512, 0, 1, 33] * 20),
+                                           (65, 1, [512, 100]), (34, 2, [513, 16])])
 def test_single_tokens_of_wide_groups(heads, kv, lens):
     """More than 16 query heads on a KV head: a step without q_starts is divided over the chip as one with them is, with
     the same bits."""
