@@ -18,6 +18,7 @@ from __future__ import annotations
 import contextlib
 import functools
 import gc
+import math
 from dataclasses import dataclass
 
 import torch
@@ -448,8 +449,11 @@ class DenseEngine:
             raise ValueError("max_new_tokens must be positive")
         if not 1 <= num_beams <= MAX_BEAMS // 2:
             raise ValueError(f"num_beams must be 1..{MAX_BEAMS // 2}, got {num_beams}")
-        if length_penalty < 0:
+        if not length_penalty >= 0:
             raise ValueError(f"length_penalty={length_penalty} is negative")
+        # (sums of log-probabilities are fp32, and so are their quotients)
+        if num_beams > 1 and not length_penalty * math.log(int(max_new_tokens)) < 80:
+            raise ValueError(f"length_penalty={length_penalty}: {max_new_tokens} ** length_penalty is past fp32's range")
         if 2 * num_beams > self.config.vocab_size:
             raise ValueError(f"num_beams={num_beams} needs a vocabulary of {2 * num_beams}")
         if self.cache is not None:

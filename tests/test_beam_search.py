@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from beam_util import CASES, plain_search, table_engine, tables_of
-from flashloop_amd import kernels
+from flashloop_amd import DenseEngine, kernels
 from flashloop_amd.model import OuroConfig, OuroForCausalLM
 from paged_util import plain_select
 
@@ -38,3 +38,25 @@ def test_plain_search():
         assert got == tokens
         p = {1: 0.4, 3: 0.216}[len(tokens)]
         assert abs(score - float(torch.log(torch.tensor(p, dtype=torch.float64))) / len(tokens) ** penalty) < 1e-6
+
+
+def test_penalties_out_of_range():
+    """Quotients that fp32 cannot hold apart are refused before anything runs; the largest that is taken still tells
+    completions apart."""
+    model = OuroForCausalLM.random_init(TINY, seed=1)
+    engine, ids = DenseEngine(model), torch.zeros(1, 3, dtype=torch.long)
+    for penalty, new in ((-0.1, 4), (float("nan"), 4), (float("inf"), 4), (float("inf"), 1), (60.0, 4), (400.0, 12), (20.0, 100)):
+        with pytest.raises(ValueError, match="length_penalty"):
+            engine.generate(ids, max_new_tokens=new, num_beams=2, length_penalty=penalty)
+    assert engine.cache is None
+
+
+@pytest.mark.parametrize("penalty", [30.0, 57.0])
+def test_large_penalties(monkeypatch, penalty):
+    monkeypatch.setattr(kernels, "beam_select", lambda x, s, n: (lambda t, b, k: (t.float(), b, k))(*plain_select(x, s, n)))
+    model = OuroForCausalLM.random_init(TINY, seed=1)
+    first, tables = tables_of("ends", 2, 4, 3, 24, 1)
+    got = table_engine(model, first, tables, "cpu").generate(torch.zeros(2, 1, dtype=torch.long), max_new_tokens=4, eos_token_id=3, num_beams=3,
+                                                             length_penalty=penalty)
+    for b in range(2):
+        assert got[b].tolist()[1:] == plain_search(first[b], tables[b], 3, 4, 3, penalty)[1]
