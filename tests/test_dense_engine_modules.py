@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from flashloop_amd import DenseEngine
+from flashloop_amd import DenseEngine, PagedKVCache
 from flashloop_amd.model import OuroConfig, OuroForCausalLM, RMSNorm, RotaryEmbedding
 
 TINY = OuroConfig(vocab_size=64, hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2, num_key_value_heads=1)
@@ -159,3 +159,16 @@ def test_calls_run_on_the_models_device(monkeypatch):
         with pytest.raises(ValueError, match="input_ids lie on cpu, the model on cuda:1"):
             call()
         assert entered[0] == far and entered[-1] is None
+
+
+def test_cache_refusals():
+    """Sizes that hold nothing, and shared pages of rows that come later or are not there (a row before the first is the last one
+    of a list)."""
+    for sizes in ((0, 2, 1, 20), (1, 0, 1, 20), (1, 2, 0, 20), (1, 2, 1, 0), (1, 2, 1, -5)):
+        with pytest.raises(ValueError, match="positive"):
+            PagedKVCache(*sizes, "cpu", page_size=16)
+    for shared in ([(0, 0)], [(0, 0), (-1, 1)], [(1, 1), (1, 1)], [(0, 0), (0, -1)], [(0, 0), (2, 1)], []):
+        with pytest.raises(ValueError, match="shared"):
+            PagedKVCache(1, 2, 1, 40, "cpu", page_size=16, shared=shared)
+    cache = PagedKVCache(1, 2, 1, 40, "cpu", page_size=16, shared=[(0, 5), (0, 1)])
+    assert cache.table.tolist() == [[0, 1, 2], [0, 3, 4]] and cache.k_pages.shape[1] == 5
