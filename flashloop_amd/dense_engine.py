@@ -42,7 +42,7 @@ class PagedKVCache:
             raise ValueError(f"page_size must be a power of two from 16 to 1024, got {page_size}")
         if slots < 1 or rows < 1 or kv_heads < 1 or capacity < 1:
             raise ValueError(f"slots, rows, KV heads and capacity must be positive, got {slots}, {rows}, {kv_heads} and {capacity}")
-        if shared is not None and (len(shared) != rows or any(not 0 <= src <= r or pages < 0 for r, (src, pages) in enumerate(shared))):
+        if shared and (len(shared) != rows or any(not 0 <= src <= r or pages < 0 for r, (src, pages) in enumerate(shared))):
             raise ValueError("shared must name, for every row, that row or an earlier one and how many of its pages it shares")
         width = -(-capacity // page_size)
         table, used = [], 0

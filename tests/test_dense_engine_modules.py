@@ -167,8 +167,9 @@ def test_cache_refusals():
     for sizes in ((0, 2, 1, 20), (1, 0, 1, 20), (1, 2, 0, 20), (1, 2, 1, 0), (1, 2, 1, -5)):
         with pytest.raises(ValueError, match="positive"):
             PagedKVCache(*sizes, "cpu", page_size=16)
-    for shared in ([(0, 0)], [(0, 0), (-1, 1)], [(1, 1), (1, 1)], [(0, 0), (0, -1)], [(0, 0), (2, 1)], []):
+    for shared in ([(0, 0)], [(0, 0), (-1, 1)], [(1, 1), (1, 1)], [(0, 0), (0, -1)], [(0, 0), (2, 1)]):
         with pytest.raises(ValueError, match="shared"):
             PagedKVCache(1, 2, 1, 40, "cpu", page_size=16, shared=shared)
+    assert PagedKVCache(1, 2, 1, 40, "cpu", page_size=16, shared=[]).table.tolist() == [[0, 1, 2], [3, 4, 5]]
     cache = PagedKVCache(1, 2, 1, 40, "cpu", page_size=16, shared=[(0, 5), (0, 1)])
     assert cache.table.tolist() == [[0, 1, 2], [0, 3, 4]] and cache.k_pages.shape[1] == 5
