@@ -1219,6 +1219,12 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
     FL_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "fl_paged_attention: every tensor must be 16-byte aligned");
   if (rows == 0) return FL_OK;
   FL_REQUIRE(seqs > 0, "fl_paged_attention: rows without a sequence");
+  // (in q's place is fine: who writes a row's head has read it, or runs after all who do)
+  const int64_t cols = static_cast<int64_t>(heads) * kDim, pool = static_cast<int64_t>(pages) * kv_heads * page_size * kDim;
+  FL_REQUIRE((out == q && q_row_stride == cols) || apart(out, cols, cols, 2, q, q_row_stride, cols, 2, rows),
+             "fl_paged_attention: out lies on other values of q");
+  for (const uint16_t* p : {k_pages, v_pages})
+    FL_REQUIRE(apart(out, rows * cols, rows * cols, 2, p, pool, pool, 2, 1), "fl_paged_attention: out lies on the pages");
   Launch p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, max_kv);
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < p.bytes) {
     p = plan(rows, seqs, kv_heads, group, q_starts ? max_q : 1, 1);  // (no room for divided items: none is)

@@ -629,7 +629,7 @@ int32_t fl_mx_matmul(const uint8_t* x_codes, const uint8_t* x_scales, int64_t m,
  *
  * fl_paged_attention: out[i, h, :] = sum_j softmax_j(scaling * q[i, h] . K[j]) V[j] over the keys j of the
  * row's sequence up to its own position, query heads h * kv_heads / heads sharing a KV head; out bf16 [rows,
- * heads * 128].  Scores, softmax and sums are fp32, probabilities are rounded to bf16 for the second product.
+ * heads * 128], which may be q but may not lie on other values of it, nor on the pages.  Scores, softmax and sums are fp32, probabilities are rounded to bf16 for the second product.
  * Keys that a row does not see have no part in its result, whatever their rows hold.  A row with no key (its
  * position is negative) and rows that belong to no sequence are zeros; a row that sees a key without a page
  * is NaN, and so is every row with a key of a sequence that is longer than its table row.  max_q and max_kv, the most rows and tokens of a sequence, choose how the work is divided and change

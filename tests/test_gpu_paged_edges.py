@@ -245,3 +245,27 @@ def test_large_scores_pick_their_keys(rows, lens):
         want, weight, _ = plain_attention(q, keys, values, lens, starts, SCALING)
         got = kernels.paged_attention(q.flatten(1), kp, vp, table, _ints(lens), SCALING, _ints(starts), max_q=max(rows)).view_as(q)
         assert attention_error(got, want, weight, torch.zeros_like(weight[..., :1])) <= 0
+
+
+@pytest.mark.parametrize("rows,lens,heads,kv", [([1, 1, 1], [100, 3000, 0], 4, 4), ([1, 1], [900, 12], 40, 2), ([300, 20], [1000, 2000], 4, 2),
+                                                ([4000, 7], [4100, 7], 16, 16)])
+def test_results_in_the_place_of_q(rows, lens, heads, kv):
+    """The C call with out = q, keys divided or not: the same bits as beside it."""
+    print(f"case: in place {rows} {lens} {heads}/{kv}", flush=True)
+    g = _gen(9)
+    starts, page = _starts(rows), 64
+    (kp, vp), table, _ = make_pool(g, lens, -(-max(lens) // page), page, kv, DEV)
+    q = torch.randn(starts[-1], heads * DIM, generator=g, device=DEV).bfloat16()
+    lib, width, st = _lib.load(), table.shape[1], _ints(starts)
+    for max_kv in (max(lens), 1):
+        want = kernels.paged_attention(q, kp, vp, table, _ints(lens), SCALING, st, max_q=max(rows), max_kv=max_kv)
+        for _ in range(3):
+            x = q.clone()
+            size = lib.fl_paged_attention_workspace(starts[-1], len(rows), heads, kv, max(rows), max_kv)
+            ws = torch.empty(max(size, 16), dtype=torch.uint8, device=DEV)
+            held = _ints(lens)
+            _lib.check(lib.fl_paged_attention(x.data_ptr(), heads * DIM, kp.data_ptr(), vp.data_ptr(), x.data_ptr(), table.data_ptr(),
+                                              held.data_ptr(), st.data_ptr(), starts[-1], len(rows), heads, kv, width, kp.shape[0], page,
+                                              max(rows), max_kv, SCALING, ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream), "in place")
+            torch.cuda.synchronize()
+            assert torch.equal(x, want)

@@ -46,3 +46,20 @@ def test_rows_that_lie_on_something():
             refused(dict(fine, **{name: fine[pool] + POOL - 16}), b"pages")
             refused(dict(fine, **{name: fine[pool] - last + 16}), b"pages")
     refused(dict(fine, k=at(7)), b"pages", turn=False)
+
+
+@needs_library
+def test_attention_that_lies_on_something():
+    lib = _lib.load()
+    at = lambda i: BASE + i * (1 << 20)
+
+    def refused(text, q=at(1), stride=512, out=at(2), k=at(3), v=at(4)):
+        rc = lib.fl_paged_attention(q, stride, k, v, out, BASE, BASE, None, ROWS, ROWS, HEADS, KV, 2, PAGES, PAGE, 1, 32, 0.1, None, 0, None)
+        assert rc == _lib.FL_E_INVALID and text in lib.fl_last_error(), (rc, lib.fl_last_error())
+
+    refused(b"other values of q", out=at(1) + 16)
+    refused(b"other values of q", out=at(1) - 1024)
+    refused(b"other values of q", out=at(1), stride=520)
+    for pool in (3, 4):
+        refused(b"on the pages", out=at(pool) + POOL - 16)
+        refused(b"on the pages", out=at(pool) - ROWS * 1024 + 16)
