@@ -271,10 +271,11 @@ __device__ __forceinline__ void slots(std::integer_sequence<int, I...>, F f) {
 // divided, a KV head's items lie one after another on a line, each as long as its keys (times `group`) and kApart steps of 64
 // more; the line is cut into `aim` equal slices, and a workgroup takes a slice: the end of one item, whole ones, the
 // beginning of another.  So the workgroups end at about the same time, however unequal the sequences are.  (20 sequences of
-// 1-700 new tokens over up to 3000, 16 heads on 4: 82-89 us with items divided by their own lengths, the longest ranges first,
-// 77-82 with slices, both with the softmax's reference moved less often; 8 of up to 300 over 6000, 16 heads: 105, 92.)  Else a workgroup takes one item, a sequence's last ones first:
-// they see more keys.  Every workgroup finds its work for itself, sequences in lanes: the lengths are on the device alone.
-// kApart: beginning a part costs some 10 us, finding it, first latencies and the stores (3, 5, 7, 10 steps: 84, 79, 78, 80 us).
+// 1-700 new tokens over up to 3000, 16 heads on 4: 112 us as whole items, 88 in slices; 8 of up to 300 over 6000, 16 heads:
+// 170, 98; four of 40 over 9000: 209, 59.)  Else a workgroup takes one item, a sequence's last ones first: they see more
+// keys.  Every workgroup finds its work for itself, sequences in lanes: the lengths are on the device alone.
+// kApart: beginning a part costs some 10 us, finding it, first latencies and the stores (3, 5, 7, 10 steps: these 20 sequences
+// 95, 90, 88, 92 us; 12 of up to 2000 over 8000, 32 heads on 4, 540, 523, 514, 511).
 constexpr double kApart = 7.0;
 constexpr int kLeastSteps = 7;  // of a slice; a cut moves by less than 2
 
@@ -1169,7 +1170,7 @@ Launch plan(int64_t n, int64_t seqs, int kv, int group, int64_t max_q, int64_t m
   } else {
     // One sequence's items are divided where they are fewer than the CUs.  Several sequences' always, as their lengths are not
     // known here: whole items would be 5% faster where there are many of about one length (12 sequences of up to 2000 tokens
-    // over 8000, 8 query heads a KV head, 4 of these: 435 and 457 us), and as long as the longest where one is long.
+    // over 8000, 8 query heads a KV head, 4 of these: 487 and 514 us), and as long as the longest where one is long.
     const int64_t slices = std::min<int64_t>(kChunkAim / kv, (items * (steps + static_cast<int>(kApart)) + kLeastSteps - 1) / kLeastSteps);
     if (slices < 2 || steps <= kLeastSteps || (seqs == 1 && items * kv >= kChunkAim)) return p;
     p.aim = p.items = static_cast<int>(slices);
