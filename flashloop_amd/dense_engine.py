@@ -464,9 +464,13 @@ class DenseEngine:
             raise RuntimeError("engine cache is already initialized; call reset()")
         if eos_token_id is None:
             eos_token_id = getattr(self.config, "eos_token_id", None)
-        if num_beams == 1:
-            return self._greedy(input_ids, attention_mask, int(max_new_tokens), eos_token_id)
-        return self._beams(input_ids, attention_mask, int(max_new_tokens), eos_token_id, num_beams, float(length_penalty))
+        try:
+            if num_beams == 1:
+                return self._greedy(input_ids, attention_mask, int(max_new_tokens), eos_token_id)
+            return self._beams(input_ids, attention_mask, int(max_new_tokens), eos_token_id, num_beams, float(length_penalty))
+        except BaseException:
+            self.reset()
+            raise
 
     def _greedy(self, input_ids, attention_mask, new, eos) -> list[torch.Tensor]:
         counts = self._lengths(input_ids, attention_mask)

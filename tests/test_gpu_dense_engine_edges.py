@@ -109,6 +109,24 @@ def test_prompts_that_fail_leave_no_cache(monkeypatch):
     assert torch.equal(engine.prefill(ids).logits, DenseEngine(model).prefill(ids).logits)
 
 
+def test_generation_that_fails_can_begin_again(monkeypatch):
+    """A step or a rearrangement that raises on the way: no cache is left, and the same call then gives what it gives without."""
+    print("case: dense engine failing generation", flush=True)
+    model = OuroForCausalLM.random_init(TINY, seed=14, device="cuda")
+    ids = _ids(2, 20, TINY.vocab_size)
+    engine = DenseEngine(model, page_size=16)
+    for beams, name, calls in ((1, "paged_attention", 8 + 3), (3, "paged_attention", 8 + 8 + 5), (3, "paged_reorder", 2), (3, "beam_select", 3)):
+        want = DenseEngine(model, page_size=16).generate(ids, max_new_tokens=6, num_beams=beams)
+        with monkeypatch.context() as m:
+            _stops_at(m, name, calls)
+            with pytest.raises(_Stop):
+                engine.generate(ids, max_new_tokens=6, num_beams=beams)
+        assert engine.cache is None and engine.positions == ()
+        got = engine.generate(ids, max_new_tokens=6, num_beams=beams)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        engine.reset()
+
+
 @pytest.mark.parametrize("beams,new,eos,penalty,kind", CASES)
 def test_beam_search_on_tables(beams, new, eos, penalty, kind):
     """The search with the selection's kernel against a plain one, on logits from tables."""
