@@ -1211,7 +1211,7 @@ extern "C" int32_t fl_paged_attention(const uint16_t* q, int64_t q_row_stride, c
   FL_REQUIRE(q_row_stride >= static_cast<int64_t>(heads) * kDim && q_row_stride % 8 == 0, "fl_paged_attention: bad row stride");
   FL_REQUIRE(q_starts != nullptr || rows == seqs, "fl_paged_attention: one row a sequence without q_starts");
   FL_REQUIRE(max_q > 0 && max_kv > 0, "fl_paged_attention: max_q and max_kv must be positive");
-  FL_REQUIRE(scaling > 0.0f && std::isfinite(scaling), "fl_paged_attention: scaling must be positive and finite");
+  FL_REQUIRE(scaling > 0.0f && std::isfinite(scaling * kLog2e), "fl_paged_attention: scaling must be positive and finite");
   FL_REQUIRE(static_cast<int64_t>(table_width) * page_size <= 0x7FFFFFFF - 4096, "fl_paged_attention: a sequence's pages hold too many tokens");
   const int group = heads / kv_heads;
   FL_REQUIRE(static_cast<int64_t>(rows) * group <= 0x7FFFFFFF - 4096, "fl_paged_attention: too many rows");

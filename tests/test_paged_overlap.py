@@ -1,4 +1,4 @@
-"""Rows that lie on what fl_paged_append reads or writes elsewhere are refused (checked before a launch: no GPU)."""
+"""Rows that lie on what the K/V page operators read or write elsewhere are refused (checked before a launch: no GPU)."""
 
 import pytest
 
@@ -53,10 +53,12 @@ def test_attention_that_lies_on_something():
     lib = _lib.load()
     at = lambda i: BASE + i * (1 << 20)
 
-    def refused(text, q=at(1), stride=512, out=at(2), k=at(3), v=at(4)):
-        rc = lib.fl_paged_attention(q, stride, k, v, out, BASE, BASE, None, ROWS, ROWS, HEADS, KV, 2, PAGES, PAGE, 1, 32, 0.1, None, 0, None)
+    def refused(text, q=at(1), stride=512, out=at(2), k=at(3), v=at(4), scaling=0.1):
+        rc = lib.fl_paged_attention(q, stride, k, v, out, BASE, BASE, None, ROWS, ROWS, HEADS, KV, 2, PAGES, PAGE, 1, 32, scaling, None, 0, None)
         assert rc == _lib.FL_E_INVALID and text in lib.fl_last_error(), (rc, lib.fl_last_error())
 
+    for scaling in (2.4e38, 3e38):  # (finite, but not in base 2)
+        refused(b"scaling", scaling=scaling)
     refused(b"other values of q", out=at(1) + 16)
     refused(b"other values of q", out=at(1) - 1024)
     refused(b"other values of q", out=at(1), stride=520)
